@@ -65,6 +65,18 @@ _SIGNATURES = {
     "bp_mlstm_accept": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "bp_mlstm_commit_state": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong,
                                       c_longlong, c_longlong, c_void_p, c_int, c_int, c_void_p]),
+    "bp_paged_append": (c_int, [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_longlong,
+                                c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                                c_int, c_float, c_void_p, c_longlong, c_void_p]),
+    "bp_paged_attention_workspace_bytes": (c_size_t, [c_int] * 5),
+    "bp_paged_attention": (c_int, [c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_void_p, c_longlong, c_int,
+                                   c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_longlong,
+                                   c_void_p, c_size_t, c_void_p]),
+    "bp_quantize_rows_int8": (c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p]),
+    "bp_int8_mm": (c_int, [c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_void_p,
+                           c_longlong, c_int, c_int, c_int, c_int, c_void_p]),
+    "bp_token_logprobs": (c_int, [c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                  c_int, c_int, c_void_p]),
     "bp_device_errors": (c_int, [ctypes.POINTER(ctypes.c_uint)]),
 }
 

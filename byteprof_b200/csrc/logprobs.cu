@@ -1,0 +1,385 @@
+// Log probabilities of given tokens with the entropy of each row and its top alternatives, in one pass over
+// the logits (bp_token_logprobs).
+//
+// Reference: byteprof's bits-per-byte evaluation takes log_softmax of every row and gathers the given byte
+// (byteprof/evaluate.py:122-166), several passes over [rows, vocab].
+//
+//   m = max x, R = sum over all but one instance of the maximum of exp(x - m), T = sum exp(x - m) (m - x):
+//   lse = m + log1p(R), logprob = x_id - lse, entropy = log1p(R) + T / (1 + R).
+// R leaves the maximum's own term (1) out, so a row whose probability is all on one token keeps the small
+// rest that 1 + R would round away. Two parts merge as (m1 >= m2, f = exp(m2 - m1)):
+//   R = R1 + f (1 + R2), T = T1 + f (T2 + (m1 - m2)(1 + R2)).
+// An empty part is m = -FLT_MAX, R = -1 (a total of 0). All of it in fp32, over short chains (a thread's share).
+//
+// Top alternatives: each warp keeps its best `top` (value, index) sorted across its lanes; a vector of logits
+// is looked at only when its maximum reaches the warp's last entry, so after the first few hundred values
+// almost none are. Order: larger value first, NaN as the largest, the lower index among equals.
+//
+// Memory bound: rows * vocab values read once. One warp per row for short rows, one CTA or a cluster of up
+// to 8 CTAs for long ones, merged in rank order (deterministic).
+#include <float.h>
+
+#include "bp_common.cuh"
+#include "skinny_internal.h"
+#include "sm100.cuh"
+
+namespace bp {
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxTop = 32;
+constexpr int kWarpRowThreads = 256;  // 8 rows per CTA
+constexpr int kRowThreads = 512;
+constexpr int kMaxCluster = 8;
+
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+struct Stat {
+  float m, r, t;
+  __device__ __forceinline__ void init() { m = -FLT_MAX, r = -1.0f, t = 0.0f; }
+  // adds one value that is not the implicit maximum (x <= m, or NaN)
+  __device__ __forceinline__ void add(float x) {
+    const float d = m - x;
+    const float e = ex2(d * -kLog2e);
+    r += e;
+    t = fmaf(e, fminf(d, 1e30f), t);  // -inf: e = 0, and 0 * inf would be NaN
+  }
+  // raises the maximum to vm > m: the old part joins the rest
+  __device__ __forceinline__ void raise(float vm) {
+    const float n = r + 1.0f, f = ex2((m - vm) * kLog2e);
+    if (n == 0.0f || f == 0.0f) {
+      r = isnan(n) ? n : 0.0f;
+      t = 0.0f;
+    } else {
+      r = n * f;
+      t = (t + n * (vm - m)) * f;
+    }
+    m = vm;
+  }
+  __device__ __forceinline__ void merge(float m2, float r2, float t2) {
+    if (m2 > m) {
+      const float a = m, b = r, c = t;
+      m = m2, r = r2, t = t2;
+      m2 = a, r2 = b, t2 = c;
+    }
+    const float n = r2 + 1.0f, f = m2 == m ? 1.0f : ex2((m2 - m) * kLog2e);
+    if (n == 0.0f) return;
+    if (f == 0.0f) {
+      if (isnan(n)) r = n;
+      return;
+    }
+    r += f * n;
+    t += f * (t2 + (m - m2) * n);
+  }
+};
+
+// torch order: NaN is the largest value; the lower index wins among equals.
+__device__ __forceinline__ bool better(float a, int ia, float b, int ib) {
+  const bool na = isnan(a), nb = isnan(b);
+  if (na || nb) return na && (!nb || ia < ib);
+  return a > b || (a == b && ia < ib);
+}
+
+// A warp's sorted list: lane l holds the l-th best so far (index INT_MAX: none).
+struct TopList {
+  float v;
+  int i;
+  float thr;  // the last wanted entry
+  int thr_i;
+  __device__ __forceinline__ void init() { v = -INFINITY, i = 0x7fffffff, thr = -INFINITY, thr_i = 0x7fffffff; }
+  __device__ __forceinline__ void insert(float x, int ix, int top, int lane) {
+    const int pos = __popc(__ballot_sync(kFull, lane < top && better(v, i, x, ix)));
+    const float pv = __shfl_up_sync(kFull, v, 1);
+    const int pi = __shfl_up_sync(kFull, i, 1);
+    if (lane > pos) v = pv, i = pi;
+    if (lane == pos) v = x, i = ix;
+    thr = __shfl_sync(kFull, v, top - 1);
+    thr_i = __shfl_sync(kFull, i, top - 1);
+  }
+  // every lane offers one value (or none)
+  __device__ __forceinline__ void offer(float x, int ix, bool valid, int top, int lane) {
+    unsigned mask = __ballot_sync(kFull, valid && better(x, ix, thr, thr_i));
+    while (mask != 0) {
+      const int src = __ffs(mask) - 1;
+      mask &= mask - 1;
+      const float bx = __shfl_sync(kFull, x, src);
+      const int bi = __shfl_sync(kFull, ix, src);
+      if (better(bx, bi, thr, thr_i)) insert(bx, bi, top, lane);
+    }
+  }
+};
+
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static constexpr int N = 4;
+  __device__ static __forceinline__ void load(const float* p, float (&f)[4]) {
+    const float4 v = __ldcs(reinterpret_cast<const float4*>(p));
+    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+  }
+  __device__ static __forceinline__ float one(const float* p) { return *p; }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  __device__ static __forceinline__ void load(const __nv_bfloat16* p, float (&f)[8]) {
+    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
+    f[0] = bf16lo(v.x); f[1] = bf16hi(v.x); f[2] = bf16lo(v.y); f[3] = bf16hi(v.y);
+    f[4] = bf16lo(v.z); f[5] = bf16hi(v.z); f[6] = bf16lo(v.w); f[7] = bf16hi(v.w);
+  }
+  __device__ static __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+};
+
+template <int N>
+__device__ __forceinline__ void take(const float (&f)[N], int at, Stat& st, TopList& tl, int top, int lane, bool valid) {
+  float vm = f[0];
+#pragma unroll
+  for (int j = 1; j < N; ++j) vm = fmaxf(vm, f[j]);
+  if (valid) {
+    if (vm > st.m) {
+      st.raise(vm);
+      bool skipped = false;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        if (!skipped && f[j] == vm)
+          skipped = true;
+        else
+          st.add(f[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) st.add(f[j]);
+    }
+  }
+  if (top > 0 && __any_sync(kFull, valid && vm >= tl.thr)) {
+#pragma unroll 1
+    for (int j = 0; j < N; ++j) {
+      float x = f[0];
+#pragma unroll
+      for (int k = 1; k < N; ++k) x = j == k ? f[k] : x;
+      tl.offer(x, at + j, valid, top, lane);
+    }
+  }
+}
+
+// Elements [lo, hi) of a row by the `n` threads (whole warps) of a team, thread id `tid`.
+template <typename T>
+__device__ __forceinline__ void scan(const T* x, int lo, int hi, int tid, int n, Stat& st, TopList& tl, int top, int lane) {
+  constexpr int N = Vec<T>::N;
+  constexpr int U = 4;
+  const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(x + lo) & 15u) / sizeof(T));
+  int a0 = lo + (mis == 0 ? 0 : N - mis);  // the first aligned element
+  if (a0 > hi) a0 = hi;
+  const int nv = (hi - a0) / N;
+  const int a1 = a0 + nv * N;
+  // single values before and behind the aligned part: fewer than 2 N, one per lane of the first warps
+  const int head = a0 - lo, singles = head + hi - a1;
+  if (tid - (tid & 31) < singles) {
+    const bool valid = tid < singles;
+    const int at = tid < head ? lo + tid : a1 + tid - head;
+    const float f[1] = {valid ? Vec<T>::one(x + at) : 0.0f};
+    take<1>(f, at, st, tl, top, lane, valid);
+  }
+  int v = tid;
+  for (; v - lane + (U - 1) * n + 31 < nv; v += U * n) {  // warp-uniform: every lane has all U vectors
+    float f[U][N];
+#pragma unroll
+    for (int u = 0; u < U; ++u) Vec<T>::load(x + a0 + (v + u * n) * N, f[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) take<N>(f[u], a0 + (v + u * n) * N, st, tl, top, lane, true);
+  }
+  for (; v - lane < nv; v += n) {
+    const bool valid = v < nv;
+    float f[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] = 0.0f;
+    if (valid) Vec<T>::load(x + a0 + v * N, f);
+    take<N>(f, a0 + v * N, st, tl, top, lane, valid);
+  }
+}
+
+struct LpArgs {
+  const void* logits;
+  long long ld;
+  const long long* ids;
+  float* lp;
+  float* ent;
+  float* top_lp;
+  long long* top_id;
+  int rows, vocab, top;
+};
+
+// The full row once more with every value compared: rows holding NaN, whose vector maxima do not show it.
+template <typename T>
+__device__ __noinline__ void rescan_top(const T* x, int vocab, TopList& tl, int top, int lane) {
+  tl.init();
+  for (int b = 0; b < vocab; b += 32) {
+    const bool valid = b + lane < vocab;
+    tl.offer(valid ? Vec<T>::one(x + b + lane) : 0.0f, b + lane, valid, top, lane);
+  }
+}
+
+// The row's results, by one warp that holds its merged state and list.
+template <typename T>
+__device__ __forceinline__ void finish(const LpArgs& a, int row, const T* x, Stat st, TopList tl, int lane) {
+  const float nan = __int_as_float(0x7fc00000);
+  st.m = __shfl_sync(kFull, st.m, 0);  // one lane's merge order, so that all results of a row agree
+  st.r = __shfl_sync(kFull, st.r, 0);
+  st.t = __shfl_sync(kFull, st.t, 0);
+  const float lr = log1pf(st.r);
+  const bool bad = isnan(st.r) || st.m == INFINITY || st.r < 0.0f;  // NaN or +inf in the row, or nothing above -inf
+  if (lane == 0) {
+    const long long id = a.ids == nullptr ? -1 : a.ids[row];
+    if (a.lp != nullptr)
+      a.lp[row] = bad || id < 0 || id >= a.vocab ? nan : (Vec<T>::one(x + id) - st.m) - lr;
+    a.ent[row] = bad ? nan : lr + st.t / (1.0f + st.r);
+  }
+  if (a.top > 0) {
+    if (bad) rescan_top(x, a.vocab, tl, a.top, lane);
+    if (lane < a.top) {
+      a.top_lp[static_cast<long long>(row) * a.top + lane] = bad ? nan : (tl.v - st.m) - lr;
+      a.top_id[static_cast<long long>(row) * a.top + lane] = tl.i;
+    }
+  }
+}
+
+__device__ __forceinline__ void warp_merge(Stat& st) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m = __shfl_xor_sync(kFull, st.m, o), r = __shfl_xor_sync(kFull, st.r, o), t = __shfl_xor_sync(kFull, st.t, o);
+    st.merge(m, r, t);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kWarpRowThreads) logprobs_warp_kernel(const LpArgs a) {
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+  const int lane = threadIdx.x & 31, row = blockIdx.x * (kWarpRowThreads / 32) + (threadIdx.x >> 5);
+  if (row >= a.rows) return;
+  const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+  Stat st;
+  TopList tl;
+  st.init();
+  tl.init();
+  scan(x, 0, a.vocab, lane, 32, st, tl, a.top, lane);
+  warp_merge(st);
+  finish(a, row, x, st, tl, lane);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads) logprobs_row_kernel(const LpArgs a) {
+  constexpr int kWarps = kRowThreads / 32;
+  __shared__ float sm[kWarps], sr[kWarps], stt[kWarps];
+  __shared__ float lv[kWarps][kMaxTop];
+  __shared__ int li[kWarps][kMaxTop];
+  __shared__ float cm[kMaxCluster], cr[kMaxCluster], ct[kMaxCluster];  // the leader's slots, one per CTA
+  __shared__ float cv[kMaxCluster][kMaxTop];
+  __shared__ int ci[kMaxCluster][kMaxTop];
+  pdl_launch_dependents();
+  if (gridDim.y > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // this CTA has started
+  pdl_wait_prior_grids();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int C = gridDim.y, rank = blockIdx.y, row = blockIdx.x;  // the cluster is gridDim.y CTAs along y
+  const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+  const int part = (a.vocab + C - 1) / C;
+  const int lo = rank * part < a.vocab ? rank * part : a.vocab, hi = lo + part < a.vocab ? lo + part : a.vocab;
+  Stat st;
+  TopList tl;
+  st.init();
+  tl.init();
+  scan(x, lo, hi, tid, kRowThreads, st, tl, a.top, lane);
+  warp_merge(st);
+  if (lane == 0) sm[warp] = st.m, sr[warp] = st.r, stt[warp] = st.t;
+  lv[warp][lane] = tl.v;
+  li[warp][lane] = tl.i;
+  __syncthreads();
+  if (warp == 0) {
+    st.init();
+    if (lane < kWarps) st.m = sm[lane], st.r = sr[lane], st.t = stt[lane];
+    warp_merge(st);
+    if (a.top > 0)
+      for (int w = 1; w < kWarps; ++w) tl.offer(lv[w][lane], li[w][lane], lane < a.top && li[w][lane] != 0x7fffffff, a.top, lane);
+  }
+  if (C > 1) {
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // every CTA has started: its memory can be written
+    if (warp == 0) {
+      if (lane == 0) {
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_addr(&cm[rank]), 0)), "f"(st.m) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_addr(&cr[rank]), 0)), "f"(st.r) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_addr(&ct[rank]), 0)), "f"(st.t) : "memory");
+      }
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_addr(&cv[rank][lane]), 0)), "f"(tl.v) : "memory");
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(smem_addr(&ci[rank][lane]), 0)), "r"(tl.i) : "memory");
+    }
+    cluster_sync_unaligned();  // every CTA's slot written and visible to the leader
+    if (rank != 0) return;
+    if (warp == 0) {
+      st.init();
+      if (lane < C) st.m = cm[lane], st.r = cr[lane], st.t = ct[lane];
+      warp_merge(st);
+      if (a.top > 0)
+        for (int c = 1; c < C; ++c) tl.offer(cv[c][lane], ci[c][lane], lane < a.top && ci[c][lane] != 0x7fffffff, a.top, lane);
+    }
+  }
+  if (warp == 0) finish(a, row, x, st, tl, lane);
+}
+
+template <typename T>
+cudaError_t launch(const LpArgs& a, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.stream = s;
+  if (a.vocab <= 2048) {
+    cfg.gridDim = dim3((a.rows + kWarpRowThreads / 32 - 1) / (kWarpRowThreads / 32));
+    cfg.blockDim = dim3(kWarpRowThreads);
+    set_launch_attrs(cfg, attr);
+    return cudaLaunchKernelEx(&cfg, logprobs_warp_kernel<T>, a);
+  }
+  int C = 1;
+  while (C < kMaxCluster && a.rows * C < tc_sm_count() && a.vocab / (2 * C) >= 4096) C *= 2;
+  cfg.gridDim = dim3(a.rows, C);
+  cfg.blockDim = dim3(kRowThreads);
+  set_launch_attrs(cfg, attr, C);
+  return cudaLaunchKernelEx(&cfg, logprobs_row_kernel<T>, a);
+}
+
+}  // namespace
+}  // namespace bp
+
+extern "C" int bp_token_logprobs(const void* logits, long long ld, int dtype, const int64_t* ids, float* logprob,
+                                 float* entropy, float* top_logprob, int64_t* top_id, int rows, int vocab, int top,
+                                 void* stream) {
+  using namespace bp;
+  clear_error();
+  if (rows < 0 || vocab < 0) return fail(BP_ERR_INVALID_ARGUMENT, "negative size (rows=%d vocab=%d)", rows, vocab);
+  if (dtype != BP_DTYPE_BF16 && dtype != BP_DTYPE_F32)
+    return fail(BP_ERR_INVALID_ARGUMENT, "logits dtype %d is not bf16 or fp32", dtype);
+  if (top < 0 || top > kMaxTop || top > vocab)
+    return fail(BP_ERR_INVALID_ARGUMENT, "top must be 0..%d and at most vocab (got %d of %d)", kMaxTop, top, vocab);
+  if (rows == 0) return BP_OK;
+  if (vocab == 0) return fail(BP_ERR_INVALID_ARGUMENT, "rows of an empty vocabulary have no distribution");
+  if (logits == nullptr || entropy == nullptr || (ids == nullptr) != (logprob == nullptr) ||
+      (top > 0 && (top_logprob == nullptr || top_id == nullptr)))
+    return fail(BP_ERR_INVALID_ARGUMENT, "a pointer is NULL (ids and logprob: both or neither)");
+  if (ld < vocab) return fail(BP_ERR_INVALID_ARGUMENT, "ld must be >= vocab");
+  if (vocab > (1 << 30)) return fail(BP_ERR_UNSUPPORTED, "vocab %d is above 2^30", vocab);
+  const uintptr_t es = dtype == BP_DTYPE_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(logits) % es != 0 || (reinterpret_cast<uintptr_t>(ids) & 7u) != 0 ||
+      (reinterpret_cast<uintptr_t>(top_id) & 7u) != 0)
+    return fail(BP_ERR_MISALIGNED, "logits, ids and top_id need their elements' alignment");
+  int st = require_sm100();
+  if (st != BP_OK) return st;
+  LpArgs a{logits, ld, reinterpret_cast<const long long*>(ids), logprob, entropy, top_logprob,
+           reinterpret_cast<long long*>(top_id), rows, vocab, top};
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = dtype == BP_DTYPE_F32 ? launch<float>(a, s) : launch<__nv_bfloat16>(a, s);
+  if (e != cudaSuccess) return fail(BP_ERR_CUDA, "token_logprobs launch: %s", cudaGetErrorString(e));
+  return check_launch("token_logprobs");
+}

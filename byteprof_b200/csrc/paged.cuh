@@ -1,0 +1,68 @@
+// Shared by the paged-attention kernels: the arguments, the cut of the work into units, and the partial
+// results that the join kernel adds up.
+//
+// Sequence s has rows [q_start[s], q_start[s + 1]) of q and kv_len[s] cached positions, its last row at
+// position kv_len[s] - 1; row t of it sees the positions up to its own. The g = nh / nkv query heads that share a
+// kv head are rows of one matrix: packed row i of (s, kv head h) is token i / g, head h * g + i % g. An item is
+// (s, h, a tile of packed rows); a unit is one block of keys of an item. Units are numbered over all items in the
+// order s, h, tile, key block, and CTA c of G takes the units [c * share, (c + 1) * share): every CTA reads the same
+// number of blocks whatever the lengths are, and the lengths are read on the device, so that a captured graph
+// serves every length. An item that lies in one CTA's share is written out by it; otherwise each CTA leaves its
+// part (running maximum, sum, unnormalised output; fp32) in the workspace, in slot 2 c + 1 if the item starts in
+// its share and 2 c if it started before, and the join kernel merges them in CTA order.
+#pragma once
+
+#include "bp_common.cuh"
+
+namespace bp {
+
+constexpr unsigned kPagedFull = 0xffffffffu;
+
+struct PagedArgs {
+  const __nv_bfloat16* q;
+  long long ldq;
+  const __nv_bfloat16* kp;
+  const __nv_bfloat16* vp;
+  int num_pages, page_log2;
+  const int* pages;
+  long long ld_pages;
+  int max_pages;
+  const int* q_start;
+  const int* kv_len;
+  int seqs, rows, nh, nkv, g, hd;
+  float scale_log2;  // softmax scale * log2(e)
+  __nv_bfloat16* out;
+  long long ldo;
+  float* part_o;     // [2 G, tile rows, hd]
+  float* part_ml;    // [2 G, tile rows, 2]
+  int G;
+  int min_share;
+};
+
+__device__ __forceinline__ float pg_ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// A sequence as the kernels see it: rows clipped to the call's, cached length clipped to the table's.
+struct PagedSeq {
+  int first, n;       // rows [first, first + n) of q
+  int kv;             // cached positions
+  int bad;            // the lowest position beyond the table (INT_MAX: none)
+  long long pos0;     // position of row `first`
+};
+__device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int s) {
+  PagedSeq r;
+  const int b = a.q_start[s], e = a.q_start[s + 1], kv = a.kv_len[s];
+  const int b0 = b > 0 ? b : 0, e0 = e < a.rows ? e : a.rows;
+  r.first = b0;
+  r.n = e0 > b0 ? e0 - b0 : 0;
+  const long long cap = static_cast<long long>(a.max_pages) << a.page_log2;
+  r.kv = kv < 0 ? 0 : (kv < cap ? kv : static_cast<int>(cap));
+  r.bad = kv > cap ? r.kv : 0x7fffffff;
+  r.pos0 = static_cast<long long>(kv) - (static_cast<long long>(e) - b) + (b0 - b);
+  return r;
+}
+
+}  // namespace bp

@@ -10,6 +10,7 @@ GEMMs (byteprof/optim/bolmo.py:32-136, bolmo_loop.py:36-64):
   * gate_softcap(g, b, cap)  cap * tanh((g + b) / cap), in place
   * DecodeAttention          one query position over a static KV cache (q/k RMSNorm, rotary
                              embedding, cache write, split attention)
+  * token_logprobs(logits, ids, top)  log probabilities of given tokens, entropies, top alternatives
   * decode_finish(logits, b, out)  out = [argmax(logits), sigmoid(b) >= 0.5]
   * GlobStep                 the whole global-model step (all OLMo-2 blocks) as one persistent kernel
   * LocStep                  the local encoder or decoder step (one mLSTM layer and its heads) as one
@@ -161,6 +162,33 @@ def decode_finish(logits: torch.Tensor, boundary_logit: torch.Tensor | None, out
         _lib.call("bp_decode_finish", logits.data_ptr(), logits.numel(), _lib.ptr(boundary_logit), out.data_ptr(),
                   _lib.stream_of(logits))
     return out
+
+
+def token_logprobs(logits: torch.Tensor, ids: torch.Tensor | None, top: int = 0):
+    """(logprob [R], entropy [R], top_logprob [R, top], top_id [R, top]) of logits [R, V] (bf16 or fp32, rows may be
+    strided) in one pass: log_softmax at ids (int64 [R]; None: logprob is None; an id outside the vocabulary gives NaN),
+    -sum p log p, and the `top` (at most 32) most probable entries, lower index first among equals (top = 0: both
+    None). fp32 results, int64 ids. A row holding NaN or +inf gives NaN."""
+    rows, ld = _rows(logits)
+    vocab = logits.shape[1]
+    code = _act(logits.dtype)
+    if ids is not None and (ids.dtype != torch.int64 or ids.shape != (rows,) or not ids.is_contiguous()):
+        raise ValueError("ids must be a contiguous int64 [R]")
+    if not 0 <= top <= min(32, vocab):
+        raise ValueError(f"top must be 0..32 and at most the vocabulary, got {top}")
+    if vocab == 0 and rows:
+        raise ValueError("rows of an empty vocabulary have no distribution")
+    _lib.require_cuda(logits, ids)
+    f32 = dict(dtype=torch.float32, device=logits.device)
+    lp = torch.empty(rows, **f32) if ids is not None else None
+    ent = torch.empty(rows, **f32)
+    top_lp = torch.empty(rows, top, **f32) if top else None
+    top_id = torch.empty(rows, top, dtype=torch.int64, device=logits.device) if top else None
+    with _lib.on_device(logits):
+        _lib.call("bp_token_logprobs", logits.data_ptr(), ld if rows > 1 else vocab, code, _lib.ptr(ids),
+                  _lib.ptr(lp), ent.data_ptr(), _lib.ptr(top_lp), _lib.ptr(top_id), rows, vocab, top,
+                  _lib.stream_of(logits))
+    return lp, ent, top_lp, top_id
 
 
 def rope_tables(max_pos: int, head_dim: int, theta: float, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:

@@ -1,8 +1,12 @@
-"""int8 weight-only GEMV (one activation row) and the per-row int8 quantizer.
+"""int8 weight-only GEMV (one activation row), the per-row int8 quantizer, and the int8 x int8 product.
 
 Same API as byteprof/quant/triton_int8.py:33-55: `gemv_int8(x, w, scale, cfg=None, out=None)`
 and `quantize_rowwise_int8(w)`. The GEMV runs the skinny kernel family with M = 1
 (bp_gemv_int8); `cfg` is accepted and ignored.
+
+Beyond byteprof: the product in 8-bit integers for any number of rows (csrc/int8_mm.cu, int8_mm_tc.cu), the
+activations quantized too, one scale per token: `quantize_tokens_int8(x)`, `int8_mm(q, scale, w, w_scale)`, and both in
+one call, `int8_linear(x, w, w_scale)`.
 """
 
 from __future__ import annotations
@@ -54,3 +58,66 @@ def quantize_rowwise_int8(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     scale = (wf.abs().amax(dim=1) / 127.0).clamp_min(1e-12).to(w.dtype)
     q = torch.round(wf / scale.float()[:, None]).clamp_(-127, 127).to(torch.int8)
     return q.contiguous(), scale
+
+
+def _rows_of(name: str, t: torch.Tensor, dtypes) -> int:
+    """The row stride of a 2-D tensor with unit column stride."""
+    if t.dim() != 2 or t.dtype not in dtypes or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be 2-D with unit column stride, of type {' or '.join(map(str, dtypes))}")
+    if t.shape[0] <= 1:
+        return -(-t.shape[1] // 16) * 16  # one row: its stride means nothing
+    if t.stride(0) < t.shape[1]:
+        raise ValueError(f"{name}'s rows overlap")
+    return t.stride(0)
+
+
+def quantize_tokens_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """x bf16 [M, K] (rows may be strided) -> (q int8 [M, K], scale fp32 [M]): scale = max(max|row| / 127, 1e-12) and
+    q = rint(row / scale). A row holding Inf or NaN gets a NaN scale. q's rows start at multiples of 16 bytes."""
+    ldx = _rows_of("x", x, (torch.bfloat16,))
+    m, k = x.shape
+    q = torch.empty(m, -(-k // 16) * 16, dtype=torch.int8, device=x.device)
+    scale = torch.empty(m, dtype=torch.float32, device=x.device)
+    _lib.require_cuda(x)
+    with _lib.on_device(x):
+        _lib.call("bp_quantize_rows_int8", x.data_ptr(), ldx, q.data_ptr(), q.shape[1], scale.data_ptr(), m, k,
+                  _lib.stream_of(x))
+    return q[:, :k], scale
+
+
+def int8_mm(q: torch.Tensor, scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None,
+            out: torch.Tensor | None = None) -> torch.Tensor:
+    """q int8 [M, K] with fp32 scale [M], w int8 [N, K] with bf16 or fp32 w_scale [N], bias bf16 [N] or None ->
+    scale[m] * w_scale[n] * sum_k q w + bias [M, N] (bf16, or the type of `out`: bf16 or fp32). The integer sum is
+    exact; one rounding at the end."""
+    ldq, ldw = _rows_of("q", q, (torch.int8,)), _rows_of("w", w, (torch.int8,))
+    m, k = q.shape
+    n = w.shape[0]
+    if w.shape[1] != k:
+        raise ValueError(f"q [M, K] and w [N, K] must agree on K, got {k} and {w.shape[1]}")
+    if scale.dtype != torch.float32 or scale.shape != (m,) or not scale.is_contiguous():
+        raise ValueError("scale must be a contiguous fp32 [M]")
+    if w_scale.dtype not in (torch.bfloat16, torch.float32) or w_scale.shape != (n,) or not w_scale.is_contiguous():
+        raise ValueError("w_scale must be a contiguous bf16 or fp32 [N]")
+    if bias is not None and (bias.dtype != torch.bfloat16 or bias.shape != (n,) or not bias.is_contiguous()):
+        raise ValueError("bias must be a contiguous bf16 [N]")
+    y = out if out is not None else torch.empty(m, n, dtype=torch.bfloat16, device=q.device)
+    if y.shape != (m, n):
+        raise ValueError(f"out must be [{m}, {n}]")
+    ldy = _rows_of("out", y, (torch.bfloat16, torch.float32))
+    _lib.require_cuda(q, scale, w, w_scale, bias, y)
+    for t in (scale, w, w_scale, bias, y):
+        if t is not None and t.device != q.device:
+            raise ValueError("all tensors of a call must be on one device")
+    with _lib.on_device(q):
+        _lib.call("bp_int8_mm", q.data_ptr(), ldq, scale.data_ptr(), w.data_ptr(), ldw, w_scale.data_ptr(),
+                  _lib.dtype_code(w_scale.dtype), _lib.ptr(bias), y.data_ptr(), ldy, _lib.dtype_code(y.dtype), m, n, k,
+                  _lib.stream_of(q))
+    return y
+
+
+def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """x bf16 [M, K] times int8 weights [N, K] with both operands in 8 bits: `quantize_tokens_int8`, then `int8_mm`."""
+    q, scale = quantize_tokens_int8(x)
+    return int8_mm(q, scale, w, w_scale, bias, out)

@@ -23,6 +23,11 @@
  *                       the per-byte pieces of the minimal Bolmo loop: byteprof/optim/bolmo.py:32-136
  *                       (_layer_step, LocalLoop.enc_step / dec_step, GlobalStep.step) and
  *                       byteprof/optim/bolmo_loop.py:36-64 (MinimalPieces: norm, lm_head, argmax)
+ *   bp_paged_append, bp_paged_attention
+ *                       the same step's attention (byteprof/optim/bolmo.py:100-136) for many positions of many sequences
+ *   bp_quantize_rows_int8, bp_int8_mm
+ *                       byteprof/quant/integrate.py:40-49       Int8Linear at more than one row
+ *   bp_token_logprobs   byteprof/evaluate.py:122-166            the log probabilities behind bits per byte
  */
 #ifndef BP_KERNELS_H
 #define BP_KERNELS_H
@@ -380,6 +385,69 @@ int bp_mlstm_accept(const int64_t* ids, const int64_t* tok, int64_t* out, int S,
 int bp_mlstm_commit_state(const float* c_hist, const float* n_hist, const float* m_hist, float* c_cur, float* n_cur,
                           float* m_cur, long long c_count, long long n_count, long long m_count, const void* slot,
                           int slot_bytes, int slots, void* stream);
+
+/*
+ * ---- a prompt in one pass (added without a change of the ABI version: look the symbols up) -----------------
+ *
+ * Paged KV cache: k_pages / v_pages [num_pages, page_size, nkv, head_dim] bf16, contiguous; page_size a power of
+ * two from 8 to 256, head_dim 64 or 128. The call's rows belong to `seqs` sequences packed one behind the other:
+ * rows q_start[s] .. q_start[s + 1] - 1 are the newest positions of sequence s, the last of them at position
+ * kv_len[s] - 1 (q_start int32 [seqs + 1], nondecreasing; kv_len int32 [seqs] counts the new rows). Position p of
+ * sequence s lies in page pages[s * ld_pages + p / page_size], row p % page_size; entries past a sequence's length
+ * are never read. All of these are read on the device, so a captured graph serves every length. Rows at or behind
+ * q_start[seqs] are left as they were. A static cache [max_pos, nkv, head_dim] is the case of consecutive pages.
+ *
+ * bp_paged_append: row t of qkv = q | k | v ([(nh + 2 nkv) * head_dim] bf16, row stride ldqkv) at its position p:
+ *   q_out[t] = rope(q * inv * q_norm_w), cache k = rope(k * inv * k_norm_w), cache v = v, each rounded once to bf16;
+ *   inv = 1 / sqrt(mean(x^2) + eps) over the whole width; the norm weights may both be NULL (no norm), cos_t / sin_t
+ *   (fp32 [max_pos, head_dim / 2], the halves rotated) both NULL (no rotation). A row whose position is negative,
+ *   outside the tables, or in a page outside [0, num_pages) writes NaN to q_out and touches no cache row.
+ *
+ * bp_paged_attention: out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j over the positions j <= p of the row's
+ *   sequence, kv head h / (nh / nkv); q and out [rows, nh, head_dim] bf16 with row strides ldq, ldo. A row that sees
+ *   nothing (a negative position) gives zeros; a row that should see a page outside [0, num_pages) or past the table
+ *   gives NaN. What lies in the cache past kv_len is never used, whatever its bits are; values at visible positions
+ *   must be finite. fp32 scores, maxima and sums; the weights are rounded to bf16 for the product with v.
+ *   workspace: scratch of the size that the next function returns, 256-byte aligned, any contents; calls that overlap in
+ *   time need different ones. Splits long caches over the GPU and joins the parts in a fixed order (deterministic).
+ */
+int bp_paged_append(const void* qkv, long long ldqkv, const void* q_norm_w, const void* k_norm_w, const float* cos_t,
+                    const float* sin_t, int max_pos, const int32_t* pages, long long ld_pages, int max_pages,
+                    const int32_t* q_start, const int32_t* kv_len, int seqs, int rows, void* k_pages, void* v_pages,
+                    int num_pages, int page_size, int nh, int nkv, int head_dim, float eps, void* q_out, long long ldq,
+                    void* stream);
+size_t bp_paged_attention_workspace_bytes(int rows, int seqs, int nh, int nkv, int head_dim);
+int bp_paged_attention(const void* q, long long ldq, const void* k_pages, const void* v_pages, int num_pages,
+                       int page_size, const int32_t* pages, long long ld_pages, int max_pages, const int32_t* q_start,
+                       const int32_t* kv_len, int seqs, int rows, int nh, int nkv, int head_dim, float scale, void* out,
+                       long long ldo, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Activations in 8 bits, one scale per row: scale[m] = max(max_k |x[m, k]| / 127, 1e-12) (fp32),
+ * q[m, k] = rint(x[m, k] / scale[m]); x bf16 [M, K] with row stride ldx, q int8 with row stride ldq. A row holding
+ * Inf or NaN gets a NaN scale and zeros.
+ *
+ * bp_int8_mm: y[m, n] = x_scale[m] * w_scale[n] * sum_k x[m, k] w[n, k] + bias[n]; x int8 [M, K] (row stride ldx), w
+ * int8 [N, K] (ldw), x_scale fp32 [M], w_scale bf16 or fp32 [N], bias bf16 [N] or NULL, y bf16 or fp32 [M, N] (ldy;
+ * exactly the block is written). The sum is exact (K up to 131071); then fp32, rounded once to y's type. Any M, N,
+ * K, strides and alignment; 16-byte aligned x, w and rows (ldx, ldw multiples of 16) run on the tensor cores, the
+ * rest on the CUDA cores, with the same bits. No workspace.
+ */
+int bp_quantize_rows_int8(const void* x, long long ldx, int8_t* q, long long ldq, float* scale, int M, int K,
+                          void* stream);
+int bp_int8_mm(const int8_t* x, long long ldx, const float* x_scale, const int8_t* w, long long ldw, const void* w_scale,
+               int w_scale_dtype, const void* bias, void* y, long long ldy, int y_dtype, int M, int N, int K, void* stream);
+
+/*
+ * One pass over rows of logits (bf16 or fp32 [rows, vocab], row stride ld, any alignment):
+ *   logprob[r] = logits[r, ids[r]] - lse(r) (ids int64; an id outside [0, vocab) gives NaN; ids and logprob may both
+ *   be NULL), entropy[r] = -sum p log p, and with top > 0 (at most 32 and vocab) the `top` most probable entries, the
+ *   larger first and the lower index among equals: top_logprob fp32 and top_id int64 [rows, top].
+ * Logits of -inf have probability 0. A row holding NaN or +inf, or nothing above -inf, gives NaN log probabilities and
+ * entropy; its top_id still orders the logits, NaN as the largest.
+ */
+int bp_token_logprobs(const void* logits, long long ld, int dtype, const int64_t* ids, float* logprob, float* entropy,
+                      float* top_logprob, int64_t* top_id, int rows, int vocab, int top, void* stream);
 
 /*
  * Device error flags raised by the kernels since the last call, then cleared (synchronises the current
