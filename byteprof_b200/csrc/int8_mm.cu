@@ -205,6 +205,10 @@ extern "C" int bp_int8_mm(const int8_t* x, long long ldx, const float* x_scale, 
   const Int8Args a{x, ldx, x_scale, w, ldw, w_scale, w_scale_dtype == BP_DTYPE_F32, static_cast<const __nv_bfloat16*>(bias),
                    y, ldy, y_dtype == BP_DTYPE_F32, M, N, K};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (int8_mm_tc_supported(a)) {
+    st = launch_int8_mm_tc(a, s);
+    return st != BP_OK ? st : check_launch("int8_mm");
+  }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   const int my = (M + kT - 1) / kT;

@@ -34,4 +34,8 @@ __device__ __forceinline__ float int8_value(const Int8Args& a, int acc, float sx
   return a.bias == nullptr ? v : __fadd_rn(v, bias);
 }
 
+// The tensor-core kernel (int8_mm_tc.cu): 16-byte aligned operands with row strides multiples of 16, K > 0.
+bool int8_mm_tc_supported(const Int8Args& a);
+int launch_int8_mm_tc(const Int8Args& a, cudaStream_t stream);
+
 }  // namespace bp

@@ -68,5 +68,6 @@ unsigned int read_device_errors_i8();
 unsigned int read_device_errors_i4tc();
 unsigned int read_device_errors_glob();
 unsigned int read_device_errors_loc();
+unsigned int read_device_errors_int8mm();
 
 }  // namespace bp
