@@ -88,6 +88,42 @@ __device__ __forceinline__ void store1(const Int8Args& a, long long m, int n, fl
     static_cast<__nv_bfloat16*>(a.y)[m * a.ldy + n] = __float2bfloat16_rn(v);
 }
 
+// A thread's row of a tile: kBN int32 columns of its TMEM lane -> scaled values of row m, columns n0 .. ; `drained` is
+// called once when the accumulator has been read.
+template <int kBN, typename F>
+__device__ __forceinline__ void drain_rows(const Int8Args& a, uint32_t src, long long m, int n0, const float* ws,
+                                           const float* bias, int vec, F drained) {
+  const float sx = m < a.M ? a.x_scale[m] : 0.0f;
+#pragma unroll 1
+  for (int c = 0; c < kBN; c += 32) {
+    uint32_t raw[32];
+    tmem_ld_32x32b_x32(src + c, raw);
+    if (c + 32 == kBN) drained();
+    if (m >= a.M) continue;
+    const int n = n0 + c;
+    if (vec && n + 32 <= a.N) {
+      float v[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = int8_value(a, static_cast<int>(raw[j]), sx, ws[c + j], bias[c + j]);
+      if (a.y_f32) {
+        float4* d = reinterpret_cast<float4*>(static_cast<float*>(a.y) + m * a.ldy + n);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      } else {
+        uint4* d = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.y) + m * a.ldy + n);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          d[j] = make_uint4(pack2(v[8 * j], v[8 * j + 1]), pack2(v[8 * j + 2], v[8 * j + 3]),
+                            pack2(v[8 * j + 4], v[8 * j + 5]), pack2(v[8 * j + 6], v[8 * j + 7]));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (n + j < a.N) store1(a, m, n + j, int8_value(a, static_cast<int>(raw[j]), sx, ws[c + j], bias[c + j]));
+    }
+  }
+}
+
 template <int kBN, bool kSwap, bool kCluster>
 __global__ void __launch_bounds__(kThreads, 1)
     int8_mm_tc_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const Int8Args a,
@@ -221,39 +257,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
         const long long m = static_cast<long long>(ia) * kBM + r;
-        const float sx = m < a.M ? a.x_scale[m] : 0.0f;
-#pragma unroll 1
-        for (int c = 0; c < kBN; c += 32) {
-          uint32_t raw[32];
-          tmem_ld_32x32b_x32(src + c, raw);
-          if (c + 32 == kBN) {
-            tc_fence_before_sync();
-            mbar_arrive(&s.tempty[buf]);
-          }
-          if (m >= a.M) continue;
-          const int n = ib * kBN + c;
-          if (vec && n + 32 <= a.N) {
-            float v[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = int8_value(a, static_cast<int>(raw[j]), sx, s.ws[buf][c + j], s.bias[buf][c + j]);
-            if (a.y_f32) {
-              float4* d = reinterpret_cast<float4*>(static_cast<float*>(a.y) + m * a.ldy + n);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) d[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-            } else {
-              uint4* d = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.y) + m * a.ldy + n);
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                d[j] = make_uint4(pack2(v[8 * j], v[8 * j + 1]), pack2(v[8 * j + 2], v[8 * j + 3]),
-                                  pack2(v[8 * j + 4], v[8 * j + 5]), pack2(v[8 * j + 6], v[8 * j + 7]));
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (n + j < a.N)
-                store1(a, m, n + j, int8_value(a, static_cast<int>(raw[j]), sx, s.ws[buf][c + j], s.bias[buf][c + j]));
-          }
-        }
+        drain_rows<kBN>(a, src, m, ib * kBN, s.ws[buf], s.bias[buf], vec, [&] {
+          tc_fence_before_sync();
+          mbar_arrive(&s.tempty[buf]);
+        });
       }
     }
   }
@@ -393,6 +400,178 @@ int launch_split(const Int8Args& a, cudaStream_t stream) {
   return p.S > 1 ? launch<kBN, kSwap, true>(a, p, stream) : launch<kBN, kSwap, false>(a, p, stream);
 }
 
+// ---- many rows: pairs of CTAs -------------------------------------------------------------------------
+// A 256 x 256 tile per pair (cta_group::2): each CTA loads 128 tokens and 128 channels per K slice for the MMA work
+// for which a CTA by itself loads 128 and 256. The tile sizes are set by that: the operands come from L2, and
+// with 48 KB per CTA and K slice the L2 delivers them at 10 TB/s while the tensor cores wait two thirds of the time
+// (8192 x 2048 -> 16384: 318 us).
+struct PairSmem {
+  static constexpr int kStages = 6;
+  static constexpr int kStageBytes = 2 * kBM * kBK;
+  uint8_t ring[kStages * kStageBytes];  // 128 token rows, then 128 channel rows, per stage
+  float ws[2][256], bias[2][256];
+  uint64_t full[kStages], empty[kStages], tfull[2], tempty[2], mma_done;
+  uint32_t tmem_base;
+  int abort;
+};
+constexpr int kPairN = 256;
+
+__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
+    int8_mm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const Int8Args a,
+                        const Part p, const int vec) {
+  constexpr int kStages = PairSmem::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  PairSmem& s = *reinterpret_cast<PairSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int t0 = blockIdx.x / 2, step = p.grid / 2, tiles = p.ta * p.tb;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&s.tfull[b], 1);
+      mbar_init(&s.tempty[b], 2 * kEpiThreads);
+    }
+    mbar_init(&s.mma_done, 1);
+    s.abort = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&ta);
+    tma_prefetch_desc(&tb);
+  }
+  if (warp == 1) tmem_alloc_pair(&s.tmem_base, 512);
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_unaligned();  // the peer's barriers are initialised before anything arrives on them
+  tc_fence_after_sync();
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+  const uint32_t tmem = s.tmem_base;
+  volatile int* abort = &s.abort;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int i = 0;
+      bool ok = true;
+      for (int t = t0; t < tiles && ok; t += step) {
+        int ia, ib;
+        tile_of(p, t, ia, ib);
+        for (int kb = 0; kb < p.kb; ++kb, ++i) {
+          const int st = i % kStages;
+          if (i >= kStages && !mbar_wait(&s.empty[st], static_cast<uint32_t>((i / kStages) + 1) & 1u, abort)) {
+            ok = false;
+            break;
+          }
+          uint8_t* dst = s.ring + st * PairSmem::kStageBytes;
+          const uint32_t bar = mapa_shared(smem_addr(&s.full[st]), 0);  // the leader's barrier counts both CTAs' bytes
+          if (rank == 0) mbar_arrive_expect_tx(&s.full[st], 2 * PairSmem::kStageBytes);
+          tma_load_2d_pair(dst, &ta, bar, kb * kBK, ia * 2 * kBM + rank * kBM);
+          tma_load_2d_pair(dst + kBM * kBK, &tb, bar, kb * kBK, ib * kPairN + rank * (kPairN / 2));
+        }
+      }
+      if (rank == 0)
+        for (int st = 0; st < kStages && st < i; ++st) wait_drain(&s.full[st], static_cast<uint32_t>((i - 1 - st) / kStages) & 1u);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = umma_idesc_s8(2 * kBM, kPairN);
+      int i = 0, it = 0;
+      bool ok = true;
+      for (int t = t0; t < tiles && ok; t += step, ++it) {
+        const int buf = it & 1;
+        if (it >= 2 && !mbar_wait(&s.tempty[buf], static_cast<uint32_t>((it >> 1) + 1) & 1u, abort)) break;
+        tc_fence_after_sync();
+        const uint32_t dacc = tmem + static_cast<uint32_t>(buf * kPairN);
+        for (int kb = 0; kb < p.kb; ++kb, ++i) {
+          const int st = i % kStages;
+          if (!mbar_wait(&s.full[st], static_cast<uint32_t>(i / kStages) & 1u, abort)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t ab = smem_addr(s.ring + st * PairSmem::kStageBytes), bb = ab + kBM * kBK;
+#pragma unroll
+          for (int kk = 0; kk < kBK / 32; ++kk)
+            umma_i8_pair(dacc, umma_desc_sw128(ab + 32 * kk), umma_desc_sw128(bb + 32 * kk), idesc,
+                         (kb > 0 || kk > 0) ? 1u : 0u);
+          umma_commit_pair(&s.empty[st]);
+        }
+        if (ok) umma_commit_pair(&s.tfull[buf]);
+      }
+      umma_commit_pair(&s.mma_done);
+      wait_drain(&s.mma_done, 0);
+    }
+  } else {
+    const int q = warp & 3, r = 32 * q + lane, et = threadIdx.x - 32 * kEpiWarp0;
+    int it = 0;
+    for (int t = t0; t < tiles; t += step, ++it) {
+      const int buf = it & 1;
+      int ia, ib;
+      tile_of(p, t, ia, ib);
+      for (int j = et; j < kPairN; j += kEpiThreads) {
+        const int n = ib * kPairN + j;
+        s.ws[buf][j] = n < a.N ? int8_w_scale(a, n) : 0.0f;
+        s.bias[buf][j] = n < a.N ? int8_bias(a, n) : 0.0f;
+      }
+      const bool ok = mbar_wait(&s.tfull[buf], static_cast<uint32_t>(it >> 1) & 1u, abort);
+      __syncwarp();
+      if (named_barrier_or(1, kEpiThreads, !ok)) break;
+      tc_fence_after_sync();
+      const uint32_t src = tmem + (static_cast<uint32_t>(32 * q) << 16) + static_cast<uint32_t>(buf * kPairN);
+      const uint32_t done = mapa_shared(smem_addr(&s.tempty[buf]), 0);
+      drain_rows<kPairN>(a, src, (static_cast<long long>(ia) * 2 + rank) * kBM + r, ib * kPairN, s.ws[buf], s.bias[buf], vec, [&] {
+        tc_fence_before_sync();
+        mbar_arrive_cluster(done);
+      });
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_unaligned();  // the leader's MMAs have read the peer's memory, every copy has landed in both
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+int launch_pair(const Int8Args& a, cudaStream_t stream) {
+  static bool ready[64] = {false};
+  constexpr size_t smem = sizeof(PairSmem) + 1024;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !ready[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(int8_mm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return fail(BP_ERR_CUDA, "cudaFuncSetAttribute(smem %zu): %s", smem, cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
+  Part p;
+  p.ta = (a.M + 2 * kBM - 1) / (2 * kBM);
+  p.tb = (a.N + kPairN - 1) / kPairN;
+  p.kb = (a.K + kBK - 1) / kBK;
+  p.S = 1;
+  const int pairs = tc_sm_count() / 2, tiles = p.ta * p.tb;
+  p.grid = 2 * (tiles < pairs ? tiles : pairs);
+  CUtensorMap ta, tb;
+  int st = tc_encode_2d(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.x, a.K, a.M, a.ldx, kBK, kBM, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  if (st != BP_OK) return st;
+  st = tc_encode_2d(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w, a.K, a.N, a.ldw, kBK, kBM, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  if (st != BP_OK) return st;
+  const int es = a.y_f32 ? 4 : 2;
+  const int vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && (a.ldy * es) % 16 == 0;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = dim3(p.grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  set_launch_attrs(cfg, attr);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, int8_mm_pair_kernel, ta, tb, a, p, vec);
+  if (e != cudaSuccess) return fail(BP_ERR_CUDA, "int8_mm launch (pairs, M=%d N=%d K=%d): %s", a.M, a.N, a.K, cudaGetErrorString(e));
+  return BP_OK;
+}
+
 }  // namespace
 
 bool int8_mm_tc_supported(const Int8Args& a) {
@@ -406,7 +585,7 @@ int launch_int8_mm_tc(const Int8Args& a, cudaStream_t stream) {
   if (a.M <= 64) return launch_split<64, true>(a, stream);
   const long long tiles = static_cast<long long>((a.M + kBM - 1) / kBM) * ((a.N + 255) / 256);
   if (tiles > (1 << 29)) return fail(BP_ERR_UNSUPPORTED, "int8_mm: too many tiles (M=%d N=%d)", a.M, a.N);
-  if (tiles >= tc_sm_count()) return launch<256, false, false>(a, partition<256, false>(a), stream);
+  if (tiles >= tc_sm_count()) return launch_pair(a, stream);
   return launch_split<128, false>(a, stream);
 }
 

@@ -39,7 +39,8 @@ def check(y, q, s, w, ws, bias=None):
 
 SHAPES = [(1, 1, 1), (1, 8192, 2048), (3, 37, 100), (16, 2048, 2048), (17, 129, 64), (33, 1000, 272), (64, 64, 8192),
           (100, 300, 17), (127, 256, 48), (128, 128, 128), (129, 257, 144), (250, 2048, 512), (509, 2048, 1040),
-          (1, 100352, 256), (2, 5, 131056), (700, 513, 2048), (1025, 640, 96)]
+          (1, 100352, 256), (2, 5, 131056), (700, 513, 2048), (1025, 640, 96), (2500, 4001, 272),
+          (385, 13000, 1040), (4097, 4608, 16)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
