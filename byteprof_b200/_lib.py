@@ -75,6 +75,9 @@ _SIGNATURES = {
     "bp_quantize_rows_int8": (c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p]),
     "bp_int8_mm": (c_int, [c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_void_p,
                            c_longlong, c_int, c_int, c_int, c_int, c_void_p]),
+    "bp_int8_linear_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "bp_int8_linear": (c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_void_p, c_longlong,
+                               c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "bp_token_logprobs": (c_int, [c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                                   c_int, c_int, c_void_p]),
     "bp_device_errors": (c_int, [ctypes.POINTER(ctypes.c_uint)]),

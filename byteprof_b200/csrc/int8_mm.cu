@@ -31,15 +31,23 @@ __device__ __forceinline__ uint32_t abs_max8(const uint4 v, uint32_t m) {
   return m;
 }
 
-__device__ __forceinline__ uint32_t q4(float a, float b, float c, float d, float s) {
-  const int i0 = __float2int_rn(__fdiv_rn(a, s)), i1 = __float2int_rn(__fdiv_rn(b, s)),
-            i2 = __float2int_rn(__fdiv_rn(c, s)), i3 = __float2int_rn(__fdiv_rn(d, s));
-  return (i0 & 0xff) | ((i1 & 0xff) << 8) | ((i2 & 0xff) << 16) | (static_cast<uint32_t>(i3) << 24);
+// rint(x / s) with the division correctly rounded. The product with 1 / s is within 2^-22 of the quotient (relative;
+// |quotient| < 128: 2^-15 absolute), so only a product that close to a half-integer needs the division itself.
+__device__ __forceinline__ int q1(float x, float s, float inv) {
+  const float y = x * inv;
+  float r = rintf(y);
+  if (fabsf(fabsf(y - r) - 0.5f) < 1e-4f) r = rintf(__fdiv_rn(x, s));
+  return static_cast<int>(r);
 }
 
-__device__ __forceinline__ uint2 q8(const uint4 v, float s) {
-  return make_uint2(q4(bf16lo(v.x), bf16hi(v.x), bf16lo(v.y), bf16hi(v.y), s),
-                    q4(bf16lo(v.z), bf16hi(v.z), bf16lo(v.w), bf16hi(v.w), s));
+__device__ __forceinline__ uint32_t q4(float a, float b, float c, float d, float s, float inv) {
+  return (q1(a, s, inv) & 0xff) | ((q1(b, s, inv) & 0xff) << 8) | ((q1(c, s, inv) & 0xff) << 16) |
+         (static_cast<uint32_t>(q1(d, s, inv)) << 24);
+}
+
+__device__ __forceinline__ uint2 q8(const uint4 v, float s, float inv) {
+  return make_uint2(q4(bf16lo(v.x), bf16hi(v.x), bf16lo(v.y), bf16hi(v.y), s, inv),
+                    q4(bf16lo(v.z), bf16hi(v.z), bf16lo(v.w), bf16hi(v.w), s, inv));
 }
 
 // kVec: rows are 16-byte aligned and K a multiple of 8 (q rows 8-byte aligned).
@@ -74,18 +82,19 @@ __global__ void __launch_bounds__(kQThreads) quantize_rows_kernel(const __nv_bfl
   for (int w = 0; w < kQThreads / 32; ++w) m = max(m, red[w]);
   const bool bad = m >= 0x7f800000u;
   const float s = fmaxf(__fdiv_rn(__uint_as_float(m), 127.0f), 1e-12f);
+  const float inv = 1.0f / s;
   if (tid == 0) scale[blockIdx.x] = bad ? __uint_as_float(0x7fc00000u) : s;
   if (kVec) {
 #pragma unroll
     for (int i = 0; i < kQCache; ++i) {
       const int c = tid + i * kQThreads;
-      if (c < chunks) *reinterpret_cast<uint2*>(qr + c * 8) = bad ? make_uint2(0, 0) : q8(keep[i], s);
+      if (c < chunks) *reinterpret_cast<uint2*>(qr + c * 8) = bad ? make_uint2(0, 0) : q8(keep[i], s, inv);
     }
     for (int c = tid + kQCache * kQThreads; c < chunks; c += kQThreads)
-      *reinterpret_cast<uint2*>(qr + c * 8) = bad ? make_uint2(0, 0) : q8(ldg16(xr + c * 8), s);
+      *reinterpret_cast<uint2*>(qr + c * 8) = bad ? make_uint2(0, 0) : q8(ldg16(xr + c * 8), s, inv);
   } else {
     for (int k = tid; k < K; k += kQThreads)
-      qr[k] = bad ? 0 : static_cast<int8_t>(__float2int_rn(__fdiv_rn(__bfloat162float(xr[k]), s)));
+      qr[k] = bad ? 0 : static_cast<int8_t>(q1(__bfloat162float(xr[k]), s, inv));
   }
 }
 
@@ -180,6 +189,30 @@ extern "C" int bp_quantize_rows_int8(const void* x, long long ldx, int8_t* q, lo
                                            static_cast<const __nv_bfloat16*>(x), ldx, q, ldq, scale, K);
   if (e != cudaSuccess) return fail(BP_ERR_CUDA, "quantize_rows_int8 launch: %s", cudaGetErrorString(e));
   return check_launch("quantize_rows_int8");
+}
+
+extern "C" size_t bp_int8_linear_workspace_bytes(int M, int K) {
+  if (M <= 0 || K < 0) return 0;
+  return (static_cast<size_t>(M) * 4 + 255) / 256 * 256 + static_cast<size_t>(M) * ((static_cast<size_t>(K) + 15) / 16 * 16);
+}
+
+extern "C" int bp_int8_linear(const void* x, long long ldx, const int8_t* w, long long ldw, const void* w_scale,
+                              int w_scale_dtype, const void* bias, void* y, long long ldy, int y_dtype, int M, int N,
+                              int K, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace bp;
+  clear_error();
+  if (M > 0 && K >= 0) {
+    const size_t need = bp_int8_linear_workspace_bytes(M, K);
+    if (workspace == nullptr || workspace_bytes < need)
+      return fail(BP_ERR_INVALID_ARGUMENT, "int8_linear needs a workspace of %zu bytes (got %zu)", need, workspace_bytes);
+    if (!aligned(workspace, 256)) return fail(BP_ERR_MISALIGNED, "workspace must be 256-byte aligned");
+  }
+  const long long ldq = (static_cast<long long>(K) + 15) / 16 * 16;
+  float* scale = static_cast<float*>(workspace);
+  int8_t* q = static_cast<int8_t*>(workspace) + (static_cast<size_t>(M > 0 ? M : 0) * 4 + 255) / 256 * 256;
+  const int st = bp_quantize_rows_int8(x, ldx, q, ldq, scale, M, K, stream);
+  if (st != BP_OK) return st;
+  return bp_int8_mm(q, ldq, scale, w, ldw, w_scale, w_scale_dtype, bias, y, ldy, y_dtype, M, N, K, stream);
 }
 
 extern "C" int bp_int8_mm(const int8_t* x, long long ldx, const float* x_scale, const int8_t* w, long long ldw,

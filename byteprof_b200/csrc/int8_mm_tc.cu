@@ -405,20 +405,27 @@ int launch_split(const Int8Args& a, cudaStream_t stream) {
 // for which a CTA by itself loads 128 and 256. The tile sizes are set by that: the operands come from L2, and
 // with 48 KB per CTA and K slice the L2 delivers them at 10 TB/s while the tensor cores wait two thirds of the time
 // (8192 x 2048 -> 16384: 318 us).
+// Eight warps drain: four take the tile's first 128 channels, four the others, each group in two steps of 64 channels
+// through 16 KB of shared memory and a TMA store (bf16). A warp that stores its lanes' rows straight from registers
+// needs 32 transactions per instruction, and one group of four warps took longer than the tile's MMAs at K = 2048.
 struct PairSmem {
-  static constexpr int kStages = 6;
+  static constexpr int kStages = 5;
   static constexpr int kStageBytes = 2 * kBM * kBK;
   uint8_t ring[kStages * kStageBytes];  // 128 token rows, then 128 channel rows, per stage
+  uint8_t out[2][kBM * 128];            // per group: 128 rows x 64 bf16, 128-byte swizzle
   float ws[2][256], bias[2][256];
   uint64_t full[kStages], empty[kStages], tfull[2], tempty[2], mma_done;
   uint32_t tmem_base;
   int abort;
 };
 constexpr int kPairN = 256;
+constexpr int kPairEpi = 256;
+constexpr int kPairThreads = 32 * kEpiWarp0 + kPairEpi;
 
-__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
-    int8_mm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const Int8Args a,
-                        const Part p, const int vec) {
+// vec: 0: y's rows are not 16-byte aligned; 1: they are (fp32); 2: bf16 through `ty`, a map of y in 64 x 128 boxes
+__global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
+    int8_mm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
+                        const __grid_constant__ CUtensorMap ty, const Int8Args a, const Part p, const int vec) {
   constexpr int kStages = PairSmem::kStages;
   extern __shared__ uint8_t smem_raw[];
   PairSmem& s = *reinterpret_cast<PairSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -433,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&s.tfull[b], 1);
-      mbar_init(&s.tempty[b], 2 * kEpiThreads);
+      mbar_init(&s.tempty[b], 2 * kPairEpi);
     }
     mbar_init(&s.mma_done, 1);
     s.abort = 0;
@@ -504,28 +511,64 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       wait_drain(&s.mma_done, 0);
     }
   } else {
-    const int q = warp & 3, r = 32 * q + lane, et = threadIdx.x - 32 * kEpiWarp0;
+    const int q = warp & 3, r = 32 * q + lane, et = threadIdx.x - 32 * kEpiWarp0, grp = et / 128;
+    uint8_t* stage = s.out[grp];
     int it = 0;
     for (int t = t0; t < tiles; t += step, ++it) {
       const int buf = it & 1;
       int ia, ib;
       tile_of(p, t, ia, ib);
-      for (int j = et; j < kPairN; j += kEpiThreads) {
-        const int n = ib * kPairN + j;
-        s.ws[buf][j] = n < a.N ? int8_w_scale(a, n) : 0.0f;
-        s.bias[buf][j] = n < a.N ? int8_bias(a, n) : 0.0f;
+      {
+        const int n = ib * kPairN + et;
+        s.ws[buf][et] = n < a.N ? int8_w_scale(a, n) : 0.0f;
+        s.bias[buf][et] = n < a.N ? int8_bias(a, n) : 0.0f;
       }
       const bool ok = mbar_wait(&s.tfull[buf], static_cast<uint32_t>(it >> 1) & 1u, abort);
       __syncwarp();
-      if (named_barrier_or(1, kEpiThreads, !ok)) break;
+      if (named_barrier_or(1, kPairEpi, !ok)) break;
       tc_fence_after_sync();
-      const uint32_t src = tmem + (static_cast<uint32_t>(32 * q) << 16) + static_cast<uint32_t>(buf * kPairN);
+      const int c0 = grp * 128;
+      const uint32_t src = tmem + (static_cast<uint32_t>(32 * q) << 16) + static_cast<uint32_t>(buf * kPairN + c0);
       const uint32_t done = mapa_shared(smem_addr(&s.tempty[buf]), 0);
-      drain_rows<kPairN>(a, src, (static_cast<long long>(ia) * 2 + rank) * kBM + r, ib * kPairN, s.ws[buf], s.bias[buf], vec, [&] {
+      const int m0 = (ia * 2 + rank) * kBM;
+      auto drained = [&] {
         tc_fence_before_sync();
         mbar_arrive_cluster(done);
-      });
+      };
+      if (vec != 2) {
+        drain_rows<128>(a, src, static_cast<long long>(m0) + r, ib * kPairN + c0, s.ws[buf] + c0, s.bias[buf] + c0, vec, drained);
+        continue;
+      }
+      const float sx = m0 + r < a.M ? a.x_scale[m0 + r] : 0.0f;
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        if (et % 128 == 0) tma_store_wait<false>();  // the store before has read the buffer
+        named_barrier_sync(2 + grp, 128);
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t raw[32];
+          tmem_ld_32x32b_x32(src + h * 64 + c, raw);
+          if (h == 1 && c == 32) drained();
+          const float* ws = s.ws[buf] + c0 + h * 64 + c;
+          const float* bias = s.bias[buf] + c0 + h * 64 + c;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = int8_value(a, static_cast<int>(raw[8 * j + e]), sx, ws[8 * j + e], bias[8 * j + e]);
+            *reinterpret_cast<uint4*>(stage + r * 128 + (((c / 8 + j) ^ (r & 7)) * 16)) =
+                make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+          }
+        }
+        fence_async_shared();
+        named_barrier_sync(2 + grp, 128);
+        if (et % 128 == 0) {
+          tma_store_2d(&ty, stage, ib * kPairN + c0 + h * 64, m0);
+          tma_store_commit();
+        }
+      }
     }
+    if (et % 128 == 0) tma_store_wait<true>();
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -559,15 +602,21 @@ int launch_pair(const Int8Args& a, cudaStream_t stream) {
   st = tc_encode_2d(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w, a.K, a.N, a.ldw, kBK, kBM, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
   if (st != BP_OK) return st;
   const int es = a.y_f32 ? 4 : 2;
-  const int vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && (a.ldy * es) % 16 == 0;
+  int vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && (a.ldy * es) % 16 == 0;
+  CUtensorMap ty = ta;
+  if (vec && !a.y_f32) {
+    st = tc_encode_2d(&ty, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.y, a.N, a.M, a.ldy * 2, 64, kBM, CU_TENSOR_MAP_L2_PROMOTION_NONE);
+    if (st != BP_OK) return st;
+    vec = 2;
+  }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3(p.grid);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kPairThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   set_launch_attrs(cfg, attr);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, int8_mm_pair_kernel, ta, tb, a, p, vec);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, int8_mm_pair_kernel, ta, tb, ty, a, p, vec);
   if (e != cudaSuccess) return fail(BP_ERR_CUDA, "int8_mm launch (pairs, M=%d N=%d K=%d): %s", a.M, a.N, a.K, cudaGetErrorString(e));
   return BP_OK;
 }

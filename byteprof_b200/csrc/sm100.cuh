@@ -106,6 +106,24 @@ __device__ __forceinline__ void tma_load_4d_hint(void* dst, const CUtensorMap* m
         "l"(policy)
       : "memory");
 }
+// 2D tile store shared -> global memory (parts outside the tensor are dropped), grouped with tma_store_commit.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_addr(src)), "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// The thread's committed stores have read their shared memory (kDone: are complete).
+template <bool kDone>
+__device__ __forceinline__ void tma_store_wait() {
+  if (kDone)
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  else
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+// Shared-memory writes of this thread before asynchronous copies (or MMAs) that read them.
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // Requests a 2D tile of the tensor into L2 (no shared-memory destination, no completion to wait for).
 __device__ __forceinline__ void tma_prefetch_l2_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)),

@@ -60,21 +60,27 @@ def quantize_rowwise_int8(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return q.contiguous(), scale
 
 
-def _rows_of(name: str, t: torch.Tensor, dtypes) -> int:
+def _rows_of(name: str, t: torch.Tensor) -> int:
     """The row stride of a 2-D tensor with unit column stride."""
-    if t.dim() != 2 or t.dtype not in dtypes or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name} must be 2-D with unit column stride, of type {' or '.join(map(str, dtypes))}")
-    if t.shape[0] <= 1:
-        return -(-t.shape[1] // 16) * 16  # one row: its stride means nothing
-    if t.stride(0) < t.shape[1]:
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be 2-D")
+    rows, cols = t.shape
+    if t.stride(1) != 1 and cols > 1:
+        raise ValueError(f"{name} must have unit column stride")
+    if rows <= 1:
+        return (cols + 15) // 16 * 16  # one row: its stride means nothing
+    ld = t.stride(0)
+    if ld < cols:
         raise ValueError(f"{name}'s rows overlap")
-    return t.stride(0)
+    return ld
 
 
 def quantize_tokens_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """x bf16 [M, K] (rows may be strided) -> (q int8 [M, K], scale fp32 [M]): scale = max(max|row| / 127, 1e-12) and
     q = rint(row / scale). A row holding Inf or NaN gets a NaN scale. q's rows start at multiples of 16 bytes."""
-    ldx = _rows_of("x", x, (torch.bfloat16,))
+    if x.dtype != torch.bfloat16:
+        raise ValueError("x must be bf16 [M, K]")
+    ldx = _rows_of("x", x)
     m, k = x.shape
     q = torch.empty(m, -(-k // 16) * 16, dtype=torch.int8, device=x.device)
     scale = torch.empty(m, dtype=torch.float32, device=x.device)
@@ -85,39 +91,64 @@ def quantize_tokens_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return q[:, :k], scale
 
 
+def _operands(w: torch.Tensor, w_scale: torch.Tensor, bias, out, m: int, k: int, dev: torch.device):
+    """Checks the weights' side of a product; returns (ldw, w_scale's code, y, ldy, y's code)."""
+    if w.dtype != torch.int8:
+        raise ValueError("w must be int8 [N, K]")
+    ldw = _rows_of("w", w)
+    n = w.shape[0]
+    if w.shape[1] != k:
+        raise ValueError(f"the operands must agree on K, got {k} and {w.shape[1]}")
+    if w_scale.dtype not in (torch.bfloat16, torch.float32) or w_scale.shape != (n,) or not w_scale.is_contiguous():
+        raise ValueError("w_scale must be a contiguous bf16 or fp32 [N]")
+    if bias is not None and (bias.dtype != torch.bfloat16 or bias.shape != (n,) or not bias.is_contiguous()):
+        raise ValueError("bias must be a contiguous bf16 [N]")
+    if out is None:
+        y, ldy, code = torch.empty(m, n, dtype=torch.bfloat16, device=dev), n, _lib.BP_DTYPE_BF16
+    else:
+        y, ldy, code = out, _rows_of("out", out), _lib.dtype_code(out.dtype)
+        if y.shape != (m, n) or code not in (_lib.BP_DTYPE_BF16, _lib.BP_DTYPE_F32):
+            raise ValueError(f"out must be bf16 or fp32 [{m}, {n}]")
+        if y.device != dev:
+            raise ValueError("all tensors of a call must be on one device")
+    if w.device != dev or w_scale.device != dev or (bias is not None and bias.device != dev):
+        raise ValueError("all tensors of a call must be on one device")
+    return ldw, _lib.dtype_code(w_scale.dtype), y, ldy, code
+
+
 def int8_mm(q: torch.Tensor, scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None,
             out: torch.Tensor | None = None) -> torch.Tensor:
     """q int8 [M, K] with fp32 scale [M], w int8 [N, K] with bf16 or fp32 w_scale [N], bias bf16 [N] or None ->
     scale[m] * w_scale[n] * sum_k q w + bias [M, N] (bf16, or the type of `out`: bf16 or fp32). The integer sum is
     exact; one rounding at the end."""
-    ldq, ldw = _rows_of("q", q, (torch.int8,)), _rows_of("w", w, (torch.int8,))
+    if q.dtype != torch.int8:
+        raise ValueError("q must be int8 [M, K]")
+    ldq = _rows_of("q", q)
     m, k = q.shape
-    n = w.shape[0]
-    if w.shape[1] != k:
-        raise ValueError(f"q [M, K] and w [N, K] must agree on K, got {k} and {w.shape[1]}")
-    if scale.dtype != torch.float32 or scale.shape != (m,) or not scale.is_contiguous():
-        raise ValueError("scale must be a contiguous fp32 [M]")
-    if w_scale.dtype not in (torch.bfloat16, torch.float32) or w_scale.shape != (n,) or not w_scale.is_contiguous():
-        raise ValueError("w_scale must be a contiguous bf16 or fp32 [N]")
-    if bias is not None and (bias.dtype != torch.bfloat16 or bias.shape != (n,) or not bias.is_contiguous()):
-        raise ValueError("bias must be a contiguous bf16 [N]")
-    y = out if out is not None else torch.empty(m, n, dtype=torch.bfloat16, device=q.device)
-    if y.shape != (m, n):
-        raise ValueError(f"out must be [{m}, {n}]")
-    ldy = _rows_of("out", y, (torch.bfloat16, torch.float32))
-    _lib.require_cuda(q, scale, w, w_scale, bias, y)
-    for t in (scale, w, w_scale, bias, y):
-        if t is not None and t.device != q.device:
-            raise ValueError("all tensors of a call must be on one device")
+    if scale.dtype != torch.float32 or scale.shape != (m,) or not scale.is_contiguous() or scale.device != q.device:
+        raise ValueError("scale must be a contiguous fp32 [M] on q's device")
+    ldw, wsd, y, ldy, yd = _operands(w, w_scale, bias, out, m, k, q.device)
+    _lib.require_cuda(q)
     with _lib.on_device(q):
-        _lib.call("bp_int8_mm", q.data_ptr(), ldq, scale.data_ptr(), w.data_ptr(), ldw, w_scale.data_ptr(),
-                  _lib.dtype_code(w_scale.dtype), _lib.ptr(bias), y.data_ptr(), ldy, _lib.dtype_code(y.dtype), m, n, k,
-                  _lib.stream_of(q))
+        _lib.call("bp_int8_mm", q.data_ptr(), ldq, scale.data_ptr(), w.data_ptr(), ldw, w_scale.data_ptr(), wsd,
+                  _lib.ptr(bias), y.data_ptr(), ldy, yd, m, w.shape[0], k, _lib.stream_of(q))
     return y
 
 
 def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None,
                 out: torch.Tensor | None = None) -> torch.Tensor:
-    """x bf16 [M, K] times int8 weights [N, K] with both operands in 8 bits: `quantize_tokens_int8`, then `int8_mm`."""
-    q, scale = quantize_tokens_int8(x)
-    return int8_mm(q, scale, w, w_scale, bias, out)
+    """x bf16 [M, K] times int8 weights [N, K] with both operands in 8 bits: `quantize_tokens_int8`, then `int8_mm`, in
+    one call of the library (the same bits)."""
+    if x.dtype != torch.bfloat16:
+        raise ValueError("x must be bf16 [M, K]")
+    ldx = _rows_of("x", x)
+    m, k = x.shape
+    dev = x.device
+    ldw, wsd, y, ldy, yd = _operands(w, w_scale, bias, out, m, k, dev)
+    _lib.require_cuda(x)
+    with _lib.on_device(x):
+        need = (4 * m + 255) // 256 * 256 + m * ((k + 15) // 16 * 16)  # bp_int8_linear_workspace_bytes
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        _lib.call("bp_int8_linear", x.data_ptr(), ldx, w.data_ptr(), ldw, w_scale.data_ptr(), wsd, _lib.ptr(bias),
+                  y.data_ptr(), ldy, yd, m, w.shape[0], k, ws.data_ptr(), need, _lib.stream_of(x))
+    return y

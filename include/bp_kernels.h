@@ -432,7 +432,14 @@ int bp_paged_attention(const void* q, long long ldq, const void* k_pages, const 
  * exactly the block is written). The sum is exact (K up to 131071); then fp32, rounded once to y's type. Any M, N,
  * K, strides and alignment; 16-byte aligned x, w and rows (ldx, ldw multiples of 16) run on the tensor cores, the
  * rest on the CUDA cores, with the same bits. No workspace.
+ *
+ * bp_int8_linear: both in one call, x bf16; q and scale go to the caller's workspace (the size the next function
+ * returns, 256-byte aligned, any contents; calls that overlap in time need different ones).
  */
+size_t bp_int8_linear_workspace_bytes(int M, int K);
+int bp_int8_linear(const void* x, long long ldx, const int8_t* w, long long ldw, const void* w_scale, int w_scale_dtype,
+                   const void* bias, void* y, long long ldy, int y_dtype, int M, int N, int K, void* workspace,
+                   size_t workspace_bytes, void* stream);
 int bp_quantize_rows_int8(const void* x, long long ldx, int8_t* q, long long ldq, float* scale, int M, int K,
                           void* stream);
 int bp_int8_mm(const int8_t* x, long long ldx, const float* x_scale, const int8_t* w, long long ldw, const void* w_scale,

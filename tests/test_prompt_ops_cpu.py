@@ -8,7 +8,7 @@ import torch
 from byteprof_b200 import _lib
 from byteprof_b200.optim.decode_ops import token_logprobs
 from byteprof_b200.optim.paged import PagedCache
-from byteprof_b200.quant.int8 import int8_mm, quantize_tokens_int8
+from byteprof_b200.quant.int8 import int8_linear, int8_mm, quantize_tokens_int8
 
 P = ctypes.c_void_p(256)
 BF16 = torch.bfloat16
@@ -66,6 +66,12 @@ def test_int8_statuses(kw, status, msg):
 
 def test_quantizer_and_logprobs_statuses():
     L = _lib.lib()
+    need = L.bp_int8_linear_workspace_bytes(3, 50)
+    assert need == 256 + 3 * 64 and L.bp_int8_linear_workspace_bytes(0, 50) == 0
+    lin = (P, 50, P, 50, P, 0, None, P, 8, 0, 3, 8, 50)
+    assert L.bp_int8_linear(*lin, P, need - 1, None) == 1 and b"workspace" in L.bp_last_error()
+    assert L.bp_int8_linear(*lin, ctypes.c_void_p(264), need, None) == 3
+    assert L.bp_int8_linear(*lin[:10], 0, 8, 50, None, 0, None) == 0
     assert L.bp_quantize_rows_int8(P, 63, P, 64, P, 2, 64, None) == 1
     assert L.bp_quantize_rows_int8(None, 64, P, 64, P, 2, 64, None) == 1
     assert L.bp_quantize_rows_int8(None, 0, None, 0, None, 0, 64, None) == 0
@@ -132,8 +138,18 @@ def test_python_refusals():
         int8_mm(i8[:1].expand(3, 64), torch.ones(3), i8, torch.ones(3))
     with pytest.raises(ValueError, match="CUDA"):
         int8_mm(i8, torch.ones(3), i8, torch.ones(3))
-    with pytest.raises(ValueError, match="2-D"):
+    with pytest.raises(ValueError, match="bf16"):
         quantize_tokens_int8(torch.zeros(3, 8))
+    x16, one = torch.zeros(3, 64, dtype=BF16), torch.ones(3)
+    for call in (lambda: quantize_tokens_int8(x16[0]), lambda: int8_linear(x16[0], i8, one)):
+        with pytest.raises(ValueError, match="2-D"):
+            call()
+    with pytest.raises(ValueError, match="unit column"):
+        int8_linear(x16.t().contiguous().t(), i8, one)
+    with pytest.raises(ValueError, match="bf16 or fp32"):
+        int8_linear(x16, i8, one, out=torch.zeros(3, 3, dtype=torch.int8))
+    with pytest.raises(ValueError, match="CUDA"):
+        int8_linear(x16, i8, one)
     x = torch.zeros(2, 9)
     with pytest.raises(ValueError, match="top"):
         token_logprobs(x, None, 10)
