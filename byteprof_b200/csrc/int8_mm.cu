@@ -17,84 +17,66 @@ namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
 
-// ---- quantizer: one CTA per row -----------------------------------------------------------------------
+// ---- quantizer ------------------------------------------------------------------------------------------
+// A team of threads per row: one warp up to 2048 values (8 rows per CTA and no barrier: with a CTA per row the
+// barrier and the single load in flight per thread held 8192 x 2048 at 23 us), else the CTA. Each thread keeps up to 8
+// chunks of 8 values in registers between the maximum and the rounding.
 constexpr int kQThreads = 256;
-constexpr int kQCache = 4;  // 8-value chunks a thread keeps between the maximum and the rounding
+constexpr int kQCache = 8;
 
-__device__ __forceinline__ uint32_t abs_max8(const uint4 v, uint32_t m) {
-  const uint32_t* w = &v.x;
+template <int kTeam>
+__device__ __forceinline__ uint32_t team_max(uint32_t m, uint32_t* red) {
+  m = __reduce_max_sync(kFull, m);
+  if (kTeam > 32) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    m = max(m, (w[i] << 16) & 0x7fffffffu);
-    m = max(m, w[i] & 0x7fff0000u);
+    for (int w = 0; w < kQThreads / 32; ++w) m = max(m, red[w]);
   }
   return m;
 }
 
-// rint(x / s) with the division correctly rounded. The product with 1 / s is within 2^-22 of the quotient (relative;
-// |quotient| < 128: 2^-15 absolute), so only a product that close to a half-integer needs the division itself.
-__device__ __forceinline__ int q1(float x, float s, float inv) {
-  const float y = x * inv;
-  float r = rintf(y);
-  if (fabsf(fabsf(y - r) - 0.5f) < 1e-4f) r = rintf(__fdiv_rn(x, s));
-  return static_cast<int>(r);
-}
-
-__device__ __forceinline__ uint32_t q4(float a, float b, float c, float d, float s, float inv) {
-  return (q1(a, s, inv) & 0xff) | ((q1(b, s, inv) & 0xff) << 8) | ((q1(c, s, inv) & 0xff) << 16) |
-         (static_cast<uint32_t>(q1(d, s, inv)) << 24);
-}
-
-__device__ __forceinline__ uint2 q8(const uint4 v, float s, float inv) {
-  return make_uint2(q4(bf16lo(v.x), bf16hi(v.x), bf16lo(v.y), bf16hi(v.y), s, inv),
-                    q4(bf16lo(v.z), bf16hi(v.z), bf16lo(v.w), bf16hi(v.w), s, inv));
-}
-
 // kVec: rows are 16-byte aligned and K a multiple of 8 (q rows 8-byte aligned).
-template <bool kVec>
+template <bool kVec, int kTeam>
 __global__ void __launch_bounds__(kQThreads) quantize_rows_kernel(const __nv_bfloat16* x, long long ldx, int8_t* q,
-                                                                  long long ldq, float* scale, int K) {
+                                                                  long long ldq, float* scale, int M, int K) {
   __shared__ uint32_t red[kQThreads / 32];
   pdl_launch_dependents();
   pdl_wait_prior_grids();
-  const int tid = threadIdx.x;
-  const __nv_bfloat16* xr = x + blockIdx.x * ldx;
-  int8_t* qr = q + blockIdx.x * ldq;
+  const int tid = threadIdx.x % kTeam, row = blockIdx.x * (kQThreads / kTeam) + threadIdx.x / kTeam;
+  if (row >= M) return;  // whole teams
+  const __nv_bfloat16* xr = x + row * ldx;
+  int8_t* qr = q + row * ldq;
   const int chunks = K / 8;
   uint32_t m = 0;
   uint4 keep[kQCache];
   if (kVec) {
 #pragma unroll
     for (int i = 0; i < kQCache; ++i) {
-      const int c = tid + i * kQThreads;
+      const int c = tid + i * kTeam;
       keep[i] = c < chunks ? ldg16(xr + c * 8) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < kQCache; ++i) m = abs_max8(keep[i], m);
-    for (int c = tid + kQCache * kQThreads; c < chunks; c += kQThreads) m = abs_max8(ldg16(xr + c * 8), m);
+    for (int c = tid + kQCache * kTeam; c < chunks; c += kTeam) m = abs_max8(ldg16(xr + c * 8), m);
   } else {
-    for (int k = tid; k < K; k += kQThreads) m = max(m, __float_as_uint(__bfloat162float(xr[k])) & 0x7fffffffu);
+    for (int k = tid; k < K; k += kTeam) m = max(m, __float_as_uint(__bfloat162float(xr[k])) & 0x7fffffffu);
   }
-  m = __reduce_max_sync(kFull, m);
-  if ((tid & 31) == 0) red[tid >> 5] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kQThreads / 32; ++w) m = max(m, red[w]);
+  m = team_max<kTeam>(m, red);
   const bool bad = m >= 0x7f800000u;
-  const float s = fmaxf(__fdiv_rn(__uint_as_float(m), 127.0f), 1e-12f);
+  const float s = int8_row_scale(m);
   const float inv = 1.0f / s;
-  if (tid == 0) scale[blockIdx.x] = bad ? __uint_as_float(0x7fc00000u) : s;
+  if (tid == 0) scale[row] = bad ? __uint_as_float(0x7fc00000u) : s;
   if (kVec) {
 #pragma unroll
     for (int i = 0; i < kQCache; ++i) {
-      const int c = tid + i * kQThreads;
+      const int c = tid + i * kTeam;
       if (c < chunks) *reinterpret_cast<uint2*>(qr + c * 8) = bad ? make_uint2(0, 0) : q8(keep[i], s, inv);
     }
-    for (int c = tid + kQCache * kQThreads; c < chunks; c += kQThreads)
+    for (int c = tid + kQCache * kTeam; c < chunks; c += kTeam)
       *reinterpret_cast<uint2*>(qr + c * 8) = bad ? make_uint2(0, 0) : q8(ldg16(xr + c * 8), s, inv);
   } else {
-    for (int k = tid; k < K; k += kQThreads)
-      qr[k] = bad ? 0 : static_cast<int8_t>(q1(__bfloat162float(xr[k]), s, inv));
+    for (int k = tid; k < K; k += kTeam) qr[k] = bad ? 0 : static_cast<int8_t>(q1(__bfloat162float(xr[k]), s, inv));
   }
 }
 
@@ -163,6 +145,26 @@ __global__ void __launch_bounds__(256) int8_mm_dp4a_kernel(const Int8Args a) {
 
 bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+// The product's argument checks (before any device work for empty problems); x is int8 or, fused, bf16.
+int check_mm(const void* x, uintptr_t x_align, long long ldx, const void* x_scale, const int8_t* w, long long ldw,
+             const void* w_scale, int w_scale_dtype, const void* bias, const void* y, long long ldy, int y_dtype, int M, int N,
+             int K) {
+  if (M < 0 || N < 0 || K < 0) return fail(BP_ERR_INVALID_ARGUMENT, "negative size (M=%d N=%d K=%d)", M, N, K);
+  if (y_dtype != BP_DTYPE_BF16 && y_dtype != BP_DTYPE_F32)
+    return fail(BP_ERR_INVALID_ARGUMENT, "output dtype %d is not bf16 or fp32", y_dtype);
+  if (w_scale_dtype != BP_DTYPE_BF16 && w_scale_dtype != BP_DTYPE_F32)
+    return fail(BP_ERR_INVALID_ARGUMENT, "weight-scale dtype %d is not bf16 or fp32", w_scale_dtype);
+  if (M == 0 || N == 0) return BP_OK;
+  if (y == nullptr || x_scale == nullptr || w_scale == nullptr || (K > 0 && (x == nullptr || w == nullptr)))
+    return fail(BP_ERR_INVALID_ARGUMENT, "a pointer argument is NULL");
+  if (ldx < K || ldw < K || ldy < N) return fail(BP_ERR_INVALID_ARGUMENT, "row strides must cover a row");
+  if (K > 131071) return fail(BP_ERR_UNSUPPORTED, "K = %d: the int32 sums hold K up to 131071", K);
+  if (!aligned(x, x_align) || !aligned(y, y_dtype == BP_DTYPE_F32 ? 4 : 2) || !aligned(x_scale, 4) ||
+      !aligned(w_scale, w_scale_dtype == BP_DTYPE_F32 ? 4 : 2) || !aligned(bias, 2))
+    return fail(BP_ERR_MISALIGNED, "y, the scales and bias need their elements' alignment");
+  return require_sm100();
+}
+
 }  // namespace
 }  // namespace bp
 
@@ -181,12 +183,15 @@ extern "C" int bp_quantize_rows_int8(const void* x, long long ldx, int8_t* q, lo
   const bool vec = K % 8 == 0 && ldx % 8 == 0 && ldq % 8 == 0 && aligned(x, 16) && aligned(q, 8);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
-  cfg.gridDim = dim3(M);
+  const bool warp_rows = K <= 2048;
+  cfg.gridDim = dim3(warp_rows ? (M + kQThreads / 32 - 1) / (kQThreads / 32) : M);
   cfg.blockDim = dim3(kQThreads);
   cfg.stream = static_cast<cudaStream_t>(stream);
   set_launch_attrs(cfg, attr);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, vec ? quantize_rows_kernel<true> : quantize_rows_kernel<false>,
-                                           static_cast<const __nv_bfloat16*>(x), ldx, q, ldq, scale, K);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg,
+                                           vec ? (warp_rows ? quantize_rows_kernel<true, 32> : quantize_rows_kernel<true, kQThreads>)
+                                               : (warp_rows ? quantize_rows_kernel<false, 32> : quantize_rows_kernel<false, kQThreads>),
+                                           static_cast<const __nv_bfloat16*>(x), ldx, q, ldq, scale, M, K);
   if (e != cudaSuccess) return fail(BP_ERR_CUDA, "quantize_rows_int8 launch: %s", cudaGetErrorString(e));
   return check_launch("quantize_rows_int8");
 }
@@ -207,6 +212,16 @@ extern "C" int bp_int8_linear(const void* x, long long ldx, const int8_t* w, lon
       return fail(BP_ERR_INVALID_ARGUMENT, "int8_linear needs a workspace of %zu bytes (got %zu)", need, workspace_bytes);
     if (!aligned(workspace, 256)) return fail(BP_ERR_MISALIGNED, "workspace must be 256-byte aligned");
   }
+  if (M > 0 && N > 0 && K > 0) {
+    const Int8Args a{nullptr, 0, nullptr, w, ldw, w_scale, w_scale_dtype == BP_DTYPE_F32,
+                     static_cast<const __nv_bfloat16*>(bias), y, ldy, y_dtype == BP_DTYPE_F32, M, N, K};
+    if (int8_fused_supported(a, x, ldx)) {
+      int st = check_mm(x, 16, ldx, workspace, w, ldw, w_scale, w_scale_dtype, bias, y, ldy, y_dtype, M, N, K);
+      if (st != BP_OK) return st;
+      st = launch_int8_fused(a, static_cast<const __nv_bfloat16*>(x), ldx, static_cast<cudaStream_t>(stream));
+      return st != BP_OK ? st : check_launch("int8_linear");
+    }
+  }
   const long long ldq = (static_cast<long long>(K) + 15) / 16 * 16;
   float* scale = static_cast<float*>(workspace);
   int8_t* q = static_cast<int8_t*>(workspace) + (static_cast<size_t>(M > 0 ? M : 0) * 4 + 255) / 256 * 256;
@@ -220,21 +235,9 @@ extern "C" int bp_int8_mm(const int8_t* x, long long ldx, const float* x_scale, 
                           int M, int N, int K, void* stream) {
   using namespace bp;
   clear_error();
-  if (M < 0 || N < 0 || K < 0) return fail(BP_ERR_INVALID_ARGUMENT, "negative size (M=%d N=%d K=%d)", M, N, K);
-  if (y_dtype != BP_DTYPE_BF16 && y_dtype != BP_DTYPE_F32)
-    return fail(BP_ERR_INVALID_ARGUMENT, "output dtype %d is not bf16 or fp32", y_dtype);
-  if (w_scale_dtype != BP_DTYPE_BF16 && w_scale_dtype != BP_DTYPE_F32)
-    return fail(BP_ERR_INVALID_ARGUMENT, "weight-scale dtype %d is not bf16 or fp32", w_scale_dtype);
-  if (M == 0 || N == 0) return BP_OK;
-  if (y == nullptr || x_scale == nullptr || w_scale == nullptr || (K > 0 && (x == nullptr || w == nullptr)))
-    return fail(BP_ERR_INVALID_ARGUMENT, "a pointer argument is NULL");
-  if (ldx < K || ldw < K || ldy < N) return fail(BP_ERR_INVALID_ARGUMENT, "row strides must cover a row");
-  if (K > 131071) return fail(BP_ERR_UNSUPPORTED, "K = %d: the int32 sums hold K up to 131071", K);
-  if (!aligned(y, y_dtype == BP_DTYPE_F32 ? 4 : 2) || !aligned(x_scale, 4) ||
-      !aligned(w_scale, w_scale_dtype == BP_DTYPE_F32 ? 4 : 2) || !aligned(bias, 2))
-    return fail(BP_ERR_MISALIGNED, "y, the scales and bias need their elements' alignment");
-  int st = require_sm100();
+  int st = check_mm(x, 1, ldx, x_scale, w, ldw, w_scale, w_scale_dtype, bias, y, ldy, y_dtype, M, N, K);
   if (st != BP_OK) return st;
+  if (M == 0 || N == 0) return BP_OK;
   const Int8Args a{x, ldx, x_scale, w, ldw, w_scale, w_scale_dtype == BP_DTYPE_F32, static_cast<const __nv_bfloat16*>(bias),
                    y, ldy, y_dtype == BP_DTYPE_F32, M, N, K};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -27,28 +27,36 @@ constexpr int kEpiWarp0 = 2;
 constexpr int kEpiThreads = 128;
 constexpr int kMaxSplit = 8;
 
-template <int kBN>
+// Two CTAs fit an SM (shared memory, TMEM, registers): one's prologue and epilogue run under the other's loads, and under
+// programmatic dependent launch the next kernel's. With one CTA and twice the stages every launch exposed its own:
+// 8.5 us for one row of 2048 -> 8192, whose weights take 2.6 us.
+template <int kBN, bool kFuse>
 struct Cfg {
-  static constexpr int kStageBytes = (kBM + kBN) * kBK;
-  static constexpr int kStages = kBN >= 256 ? 4 : kBN >= 128 ? 6 : 8;
+  static constexpr int kStageBytes = (kBM + (kFuse ? 0 : kBN)) * kBK;
+  static constexpr int kStages = kFuse ? 4 : kBN >= 128 ? 3 : kBN >= 64 ? 4 : 5;
+  static constexpr int kRingBytes = kStages * kStageBytes;
   // in cluster mode the ring's memory holds the partials: S x kBN / 4 x (128 / S + 1) x 16 bytes
-  static constexpr int kRedBytes = kMaxSplit * (kBN / 4) * (kBM / kMaxSplit + 1) * 16;
-  static constexpr int kRingBytes = kStages * kStageBytes > kRedBytes ? kStages * kStageBytes : kRedBytes;
+  static_assert(kRingBytes >= 4 * kBN * (kBM + kMaxSplit), "partials");
   static constexpr uint32_t kTmemCols = 2 * kBN < 32 ? 32 : 2 * kBN;
 };
 
-template <int kBN>
+template <int kBN, bool kFuse>
 struct Smem {
-  uint8_t ring[Cfg<kBN>::kRingBytes];  // 1024-byte aligned stages: A rows, then B rows
-  float ws[2][256];                    // w_scale and bias of the tile's channels (kSwap = false), or x_scale (kSwap)
-  float bias[2][256];
-  uint64_t full[Cfg<kBN>::kStages], empty[Cfg<kBN>::kStages], tfull[2], tempty[2], mma_done;
+  uint8_t ring[Cfg<kBN, kFuse>::kRingBytes];  // 1024-byte aligned stages: A rows, then B rows
+  float ws[2][kBN];                           // w_scale and bias of the tile's channels (kSwap: x_scale of its tokens)
+  float bias[2][kBN];
+  float lane_scale[2][kBM];                   // cluster mode: the scales (kSwap: and biases) of the tile's lanes
+  uint64_t full[Cfg<kBN, kFuse>::kStages], empty[Cfg<kBN, kFuse>::kStages], tfull[2], tempty[2], mma_done, quantized;
   uint32_t tmem_base;
   int abort;
+  float row_scale[16];  // kFuse
+  uint32_t red[16];
 };
 
-template <int kBN>
-constexpr size_t smem_bytes() { return sizeof(Smem<kBN>) + 1024; }
+template <int kBN, bool kFuse>
+constexpr size_t smem_bytes() { return (sizeof(Smem<kBN, kFuse>) + 1023) / 1024 * 1024 + 1024; }
+
+constexpr size_t kFuseBytes = 32 * 1024;  // the quantized tokens of a CTA's K range (kFuse)
 
 struct Part {
   int ta, tb;   // tiles along the MMA's M and N
@@ -56,6 +64,9 @@ struct Part {
   int S;        // CTAs per tile (cluster), 1: persistent
   int grid;
 };
+
+// K blocks of the longest range of the split.
+inline int fuse_blocks(const Part& p) { return (p.kb + p.S - 1) / p.S; }
 
 __device__ __forceinline__ void wait_drain(uint64_t* bar, uint32_t parity) {
   const unsigned long long t0 = globaltimer();
@@ -124,14 +135,95 @@ __device__ __forceinline__ void drain_rows(const Int8Args& a, uint32_t src, long
   }
 }
 
-template <int kBN, bool kSwap, bool kCluster>
-__global__ void __launch_bounds__(kThreads, 1)
+// Adds the S partials of L rows (m0 ..) of a tile and stores them; `red` is [S][kBN / 4][L + 1] groups of 4 columns; sx
+// holds the rows' scales, ws and bias the columns'.
+template <int kBN>
+__device__ __forceinline__ void finish_rows(const Int8Args& a, const int4* red, int S, int L, long long m0, int n0, int vec,
+                                            int threads, const float* sx, const float* ws, const float* bias) {
+#pragma unroll 2
+  for (int i = threadIdx.x; i < L * (kBN / 4); i += threads) {
+    const int c4 = i % (kBN / 4), ll = i / (kBN / 4), n = n0 + 4 * c4;
+    const long long m = m0 + ll;
+    if (m >= a.M || n >= a.N) continue;
+    int4 acc = make_int4(0, 0, 0, 0);
+    for (int src = 0; src < S; ++src) {
+      const int4 v = red[(src * (kBN / 4) + c4) * (L + 1) + ll];
+      acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+    }
+    const int* av = &acc.x;
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = int8_value(a, av[j], sx[ll], ws[4 * c4 + j], bias[4 * c4 + j]);
+    if (vec && n + 4 <= a.N) {
+      if (a.y_f32)
+        *reinterpret_cast<float4*>(static_cast<float*>(a.y) + m * a.ldy + n) = make_float4(v[0], v[1], v[2], v[3]);
+      else
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.y) + m * a.ldy + n) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n + j < a.N) store1(a, m, n + j, v[j]);
+    }
+  }
+}
+
+// The K blocks [k0, k1) of the tokens' rows in 8 bits, as the MMA reads them: [block][kBN rows][128 bytes], 128-byte
+// swizzle, zeros past M and K. Called by `n` threads (whole warps, not all of the CTA).
+template <int kBN>
+__device__ __forceinline__ void quantize_range(const Int8Args& a, const __nv_bfloat16* x, long long ldx, uint8_t* dst, int k0, int k1,
+                                               float* row_scale, uint32_t* red, int tid, int n) {
+  const int chunks = a.K / 8;  // K is a multiple of 8
+  if (tid < 16) red[tid] = 0;
+  named_barrier_sync(1, n);
+  constexpr int kU = 8;  // loads in flight
+  for (int i0 = tid; i0 - (tid & 31) < a.M * chunks; i0 += kU * n) {
+    uint4 v[kU];
+    int row[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int i = i0 + u * n;
+      row[u] = i / chunks;
+      v[u] = row[u] < a.M ? ldg16(x + row[u] * ldx + (i - row[u] * chunks) * 8) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const uint32_t mx = abs_max8(v[u], 0);
+      const int first = __shfl_sync(0xffffffffu, row[u], 0);
+      if (__all_sync(0xffffffffu, row[u] == first)) {
+        const uint32_t all = __reduce_max_sync(0xffffffffu, mx);
+        if ((tid & 31) == 0 && first < a.M) atomicMax(&red[first], all);
+      } else if (row[u] < a.M) {
+        atomicMax(&red[row[u]], mx);
+      }
+    }
+  }
+  named_barrier_sync(1, n);
+  if (tid < a.M) row_scale[tid] = red[tid] >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : int8_row_scale(red[tid]);
+  const int per = kBN * 16, all = (k1 - k0) * per;  // 8-value pieces of a block
+  for (int i = tid; i < all; i += n) {
+    const int b = i / per, r = i % per / 16, c = i % 16, k = (k0 + b) * kBK + c * 8;
+    uint2 v = make_uint2(0, 0);
+    if (r < a.M && k < a.K && red[r] < 0x7f800000u) {
+      const float s = int8_row_scale(red[r]);
+      v = q8(ldg16(x + r * ldx + k), s, 1.0f / s);
+    }
+    *reinterpret_cast<uint2*>(dst + b * kBN * kBK + r * kBK + (((c / 2) ^ (r & 7)) * 16) + (c & 1) * 8) = v;
+  }
+  named_barrier_sync(1, n);  // row_scale is visible to the epilogue
+}
+
+// kFuse (kSwap, up to 16 tokens): x is bf16 and every CTA quantizes its K range of it itself, while the weights stream:
+// one launch instead of two, where launches are most of the time. The rows' maxima need all of K, which is little
+// for few rows (the entry takes M * K up to 8192 values).
+template <int kBN, bool kSwap, bool kCluster, bool kFuse>
+__global__ void __launch_bounds__(kThreads, 2)
     int8_mm_tc_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const Int8Args a,
-                      const Part p, const int vec) {
-  using C = Cfg<kBN>;
+                      const Part p, const int vec, const __nv_bfloat16* xb, const long long ldxb) {
+  using C = Cfg<kBN, kFuse>;
   constexpr int kStages = C::kStages;
   extern __shared__ uint8_t smem_raw[];
-  Smem<kBN>& s = *reinterpret_cast<Smem<kBN>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  Smem<kBN, kFuse>& s = *reinterpret_cast<Smem<kBN, kFuse>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* fused = reinterpret_cast<uint8_t*>(&s) + (sizeof(Smem<kBN, kFuse>) + 1023) / 1024 * 1024;  // kFuse: [K block][kBN][128]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = kCluster ? blockIdx.y : 0;
   const int t0 = blockIdx.x, step = kCluster ? 1 << 30 : p.grid, tiles = p.ta * p.tb;
@@ -151,7 +243,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     s.abort = 0;
     mbar_fence_init();
     tma_prefetch_desc(&ta);
-    tma_prefetch_desc(&tb);
+    if (!kFuse) tma_prefetch_desc(&tb);
+    mbar_init(&s.quantized, kThreads - 32);
+    mbar_fence_init();
   }
   if (warp == 1) {
     tmem_alloc(&s.tmem_base, C::kTmemCols);
@@ -179,16 +273,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           uint8_t* dst = s.ring + st * C::kStageBytes;
-          mbar_arrive_expect_tx(&s.full[st], C::kStageBytes);
+          mbar_arrive_expect_tx(&s.full[st], kFuse ? kBM * kBK : C::kStageBytes);
           tma_load_2d(dst, &ta, &s.full[st], kb * kBK, ia * kBM);
-          tma_load_2d(dst + kBM * kBK, &tb, &s.full[st], kb * kBK, ib * kBN);
+          if (!kFuse) tma_load_2d(dst + kBM * kBK, &tb, &s.full[st], kb * kBK, ib * kBN);
         }
       }
       for (int st = 0; st < kStages && st < i; ++st)  // the last copy issued into each stage has landed
         wait_drain(&s.full[st], static_cast<uint32_t>((i - 1 - st) / kStages) & 1u);
     }
-  } else if (warp == 1) {
+  } else if (kFuse) {
+    quantize_range<kBN>(a, xb, ldxb, fused, k0, k1, s.row_scale, s.red, threadIdx.x - 32, kThreads - 32);
+    fence_async_shared();
+    mbar_arrive(&s.quantized);
+  }
+  if (warp == 1) {
     if (lane == 0) {
+      if (kFuse) mbar_wait(&s.quantized, 0, abort);
       constexpr uint32_t idesc = umma_idesc_s8(kBM, kBN);
       int i = 0, it = 0;
       bool ok = true;
@@ -204,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           tc_fence_after_sync();
-          const uint32_t ab = smem_addr(s.ring + st * C::kStageBytes), bb = ab + kBM * kBK;
+          const uint32_t ab = smem_addr(s.ring + st * C::kStageBytes), bb = kFuse ? smem_addr(fused) + (kb - k0) * kBN * kBK : ab + kBM * kBK;
 #pragma unroll
           for (int kk = 0; kk < kBK / 32; ++kk)
             umma_i8(dacc, umma_desc_sw128(ab + 32 * kk), umma_desc_sw128(bb + 32 * kk), idesc, (kb > k0 || kk > 0) ? 1u : 0u);
@@ -215,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       umma_commit(&s.mma_done);
       wait_drain(&s.mma_done, 0);
     }
-  } else if (!kCluster) {
+  } else if (!kCluster && warp >= kEpiWarp0) {
     const int q = warp & 3, r = 32 * q + lane, et = threadIdx.x - 32 * kEpiWarp0;
     int it = 0;
     for (int t = t0; t < tiles; t += step, ++it) {
@@ -223,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int ia, ib;
       tile_of(p, t, ia, ib);
       if (kSwap) {
-        for (int j = et; j < kBN; j += kEpiThreads) s.ws[buf][j] = ib * kBN + j < a.M ? a.x_scale[ib * kBN + j] : 0.0f;
+        for (int j = et; j < kBN; j += kEpiThreads) s.ws[buf][j] = ib * kBN + j >= a.M ? 0.0f : kFuse ? s.row_scale[j] : a.x_scale[ib * kBN + j];
       } else {
         for (int j = et; j < kBN; j += kEpiThreads) {
           const int n = ib * kBN + j;
@@ -266,7 +366,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   if constexpr (kCluster) {
-    // one tile per cluster. The partials go through the ring's memory: every CTA's MMAs have read it ...
+    // one tile per cluster. The scales are fetched under the MMAs
+    int ia, ib;
+    tile_of(p, t0, ia, ib);
+    if (warp >= kEpiWarp0) {
+      const int et = threadIdx.x - 32 * kEpiWarp0;
+      if (kSwap) {
+        const int n = ia * kBM + et;
+        s.lane_scale[0][et] = n < a.N ? int8_w_scale(a, n) : 0.0f;
+        s.lane_scale[1][et] = n < a.N ? int8_bias(a, n) : 0.0f;
+        if (et < kBN) s.ws[0][et] = ib * kBN + et >= a.M ? 0.0f : kFuse ? s.row_scale[et & 15] : a.x_scale[ib * kBN + et];
+      } else {
+        const long long m = static_cast<long long>(ia) * kBM + et;
+        s.lane_scale[0][et] = m < a.M ? a.x_scale[m] : 0.0f;
+        for (int j = et; j < kBN; j += kEpiThreads) {
+          const int n = ib * kBN + j;
+          s.ws[0][j] = n < a.N ? int8_w_scale(a, n) : 0.0f;
+          s.bias[0][j] = n < a.N ? int8_bias(a, n) : 0.0f;
+        }
+      }
+    }
+    // the partials go through the ring's memory: every CTA's MMAs have read it ...
     if (warp >= kEpiWarp0 && !mbar_wait(&s.tfull[0], 0, abort)) *abort = 1;
     __syncwarp();
     cluster_sync_unaligned();
@@ -291,46 +411,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     cluster_sync_unaligned();  // ... and every partial has landed
     if (!*abort) {
-      int ia, ib;
-      tile_of(p, t0, ia, ib);
       const int4* red = reinterpret_cast<const int4*>(s.ring);
       if (kSwap) {
+#pragma unroll 2
         for (int i = threadIdx.x; i < L * kBN; i += kThreads) {
           const int ll = i % L, j = i / L, n = ia * kBM + rank * L + ll, m = ib * kBN + j;
           if (m >= a.M || n >= a.N) continue;
           int acc = 0;
           for (int src = 0; src < S; ++src)
             acc += reinterpret_cast<const int*>(red + (src * (kBN / 4) + j / 4) * (L + 1) + ll)[j & 3];
-          store1(a, m, n, int8_value(a, acc, a.x_scale[m], int8_w_scale(a, n), int8_bias(a, n)));
+          store1(a, m, n, int8_value(a, acc, s.ws[0][j], s.lane_scale[0][rank * L + ll], s.lane_scale[1][rank * L + ll]));
         }
       } else {
-        for (int i = threadIdx.x; i < L * (kBN / 4); i += kThreads) {
-          const int c4 = i % (kBN / 4), ll = i / (kBN / 4), n = ib * kBN + 4 * c4;
-          const long long m = static_cast<long long>(ia) * kBM + rank * L + ll;
-          if (m >= a.M || n >= a.N) continue;
-          int4 acc = make_int4(0, 0, 0, 0);
-          for (int src = 0; src < S; ++src) {
-            const int4 v = red[(src * (kBN / 4) + c4) * (L + 1) + ll];
-            acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-          }
-          const int* av = &acc.x;
-          const float sx = a.x_scale[m];
-          float v[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            v[j] = n + j < a.N ? int8_value(a, av[j], sx, int8_w_scale(a, n + j), int8_bias(a, n + j)) : 0.0f;
-          if (vec && n + 4 <= a.N) {
-            if (a.y_f32)
-              *reinterpret_cast<float4*>(static_cast<float*>(a.y) + m * a.ldy + n) = make_float4(v[0], v[1], v[2], v[3]);
-            else
-              *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.y) + m * a.ldy + n) =
-                  make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (n + j < a.N) store1(a, m, n + j, v[j]);
-          }
-        }
+        finish_rows<kBN>(a, red, S, L, static_cast<long long>(ia) * kBM + rank * L, ib * kBN, vec, kThreads,
+                         s.lane_scale[0] + rank * L, s.ws[0], s.bias[0]);
       }
     }
   }
@@ -343,16 +437,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int kBN, bool kSwap, bool kCluster>
-int launch(const Int8Args& a, const Part& p, cudaStream_t stream) {
-  auto* kern = int8_mm_tc_kernel<kBN, kSwap, kCluster>;
+template <int kBN, bool kSwap, bool kCluster, bool kFuse>
+int launch(const Int8Args& a, const Part& p, cudaStream_t stream, const __nv_bfloat16* xb = nullptr, long long ldxb = 0) {
+  auto* kern = int8_mm_tc_kernel<kBN, kSwap, kCluster, kFuse>;
+  constexpr size_t smem_max = smem_bytes<kBN, kFuse>() + (kFuse ? kFuseBytes : 0);
+  const size_t smem = smem_bytes<kBN, kFuse>() + (kFuse ? static_cast<size_t>(fuse_blocks(p)) * kBN * kBK : 0);
   static bool ready[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !ready[dev]) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(smem_bytes<kBN>()));
-    if (e != cudaSuccess) return fail(BP_ERR_CUDA, "cudaFuncSetAttribute(smem %zu): %s", smem_bytes<kBN>(), cudaGetErrorString(e));
+                                               static_cast<int>(smem_max));
+    if (e != cudaSuccess) return fail(BP_ERR_CUDA, "cudaFuncSetAttribute(smem %zu): %s", smem_max, cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }
   const int8_t* A = kSwap ? a.w : a.x;
@@ -361,19 +457,23 @@ int launch(const Int8Args& a, const Part& p, cudaStream_t stream) {
   int st = tc_encode_2d(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, a.K, kSwap ? a.N : a.M, kSwap ? a.ldw : a.ldx, kBK, kBM,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
   if (st != BP_OK) return st;
-  st = tc_encode_2d(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, B, a.K, kSwap ? a.M : a.N, kSwap ? a.ldx : a.ldw, kBK, kBN,
-                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
-  if (st != BP_OK) return st;
+  if (kFuse) {
+    tb = ta;
+  } else {
+    st = tc_encode_2d(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, B, a.K, kSwap ? a.M : a.N, kSwap ? a.ldx : a.ldw, kBK, kBN,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+    if (st != BP_OK) return st;
+  }
   const int es = a.y_f32 ? 4 : 2;
   const int vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && (a.ldy * es) % 16 == 0;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = kCluster ? dim3(p.ta * p.tb, p.S) : dim3(p.grid);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem_bytes<kBN>();
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   set_launch_attrs(cfg, attr, kCluster ? p.S : 1);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tb, a, p, vec);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tb, a, p, vec, xb, ldxb);
   if (e != cudaSuccess)
     return fail(BP_ERR_CUDA, "int8_mm launch (M=%d N=%d K=%d BN=%d S=%d): %s", a.M, a.N, a.K, kBN, p.S, cudaGetErrorString(e));
   return BP_OK;
@@ -387,17 +487,23 @@ Part partition(const Int8Args& a) {
   p.kb = (a.K + kBK - 1) / kBK;
   p.S = 1;
   const long long tiles = static_cast<long long>(p.ta) * p.tb;
-  p.grid = static_cast<int>(tiles < tc_sm_count() ? tiles : tc_sm_count());
+  p.grid = static_cast<int>(tiles < 2 * tc_sm_count() ? tiles : 2 * tc_sm_count());
   return p;
 }
 
 // Few tiles for the GPU: the CTAs of a cluster share a tile's K.
 template <int kBN, bool kSwap>
-int launch_split(const Int8Args& a, cudaStream_t stream) {
+Part split_partition(const Int8Args& a) {
   Part p = partition<kBN, kSwap>(a);
-  const int sms = tc_sm_count(), tiles = p.ta * p.tb;
-  while (p.S < kMaxSplit && static_cast<long long>(tiles) * p.S * 2 <= sms && p.S * 2 <= p.kb) p.S *= 2;
-  return p.S > 1 ? launch<kBN, kSwap, true>(a, p, stream) : launch<kBN, kSwap, false>(a, p, stream);
+  const long long ctas = 2 * tc_sm_count(), tiles = static_cast<long long>(p.ta) * p.tb;
+  while (p.S < kMaxSplit && tiles * p.S * 2 <= ctas && p.S * 2 <= p.kb) p.S *= 2;
+  return p;
+}
+
+template <int kBN, bool kFuse>
+int launch_swap(const Int8Args& a, cudaStream_t stream, const __nv_bfloat16* xb = nullptr, long long ldxb = 0) {
+  const Part p = split_partition<kBN, true>(a);
+  return p.S > 1 ? launch<kBN, true, true, kFuse>(a, p, stream, xb, ldxb) : launch<kBN, true, false, kFuse>(a, p, stream, xb, ldxb);
 }
 
 // ---- many rows: pairs of CTAs -------------------------------------------------------------------------
@@ -420,18 +526,24 @@ struct PairSmem {
 };
 constexpr int kPairN = 256;
 constexpr int kPairEpi = 256;
+constexpr int kMaxPairSplit = 4;  // a cluster of 8 CTAs; the partials, 4 (S + 128) KB, fit the ring
 constexpr int kPairThreads = 32 * kEpiWarp0 + kPairEpi;
 
+// kSplit: a cluster of p.S pairs shares one tile's K; the partials meet as in the single-CTA kernel, each CTA finishing
+// 128 / S of its half's lanes.
 // vec: 0: y's rows are not 16-byte aligned; 1: they are (fp32); 2: bf16 through `ty`, a map of y in 64 x 128 boxes
-__global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
+template <bool kSplit>
+__global__ void __launch_bounds__(kPairThreads, 1)
     int8_mm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                         const __grid_constant__ CUtensorMap ty, const Int8Args a, const Part p, const int vec) {
   constexpr int kStages = PairSmem::kStages;
   extern __shared__ uint8_t smem_raw[];
   PairSmem& s = *reinterpret_cast<PairSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = static_cast<int>(cluster_ctarank());
-  const int t0 = blockIdx.x / 2, step = p.grid / 2, tiles = p.ta * p.tb;
+  const int crank = static_cast<int>(cluster_ctarank()), rank = crank & 1, leader = crank & ~1, part = crank >> 1;
+  const int t0 = blockIdx.x / (2 * p.S), step = kSplit ? 1 << 30 : p.grid / 2, tiles = p.ta * p.tb;
+  const int k0 = kSplit ? static_cast<int>(static_cast<long long>(part) * p.kb / p.S) : 0;
+  const int k1 = kSplit ? static_cast<int>(static_cast<long long>(part + 1) * p.kb / p.S) : p.kb;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -465,14 +577,14 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       for (int t = t0; t < tiles && ok; t += step) {
         int ia, ib;
         tile_of(p, t, ia, ib);
-        for (int kb = 0; kb < p.kb; ++kb, ++i) {
+        for (int kb = k0; kb < k1; ++kb, ++i) {
           const int st = i % kStages;
           if (i >= kStages && !mbar_wait(&s.empty[st], static_cast<uint32_t>((i / kStages) + 1) & 1u, abort)) {
             ok = false;
             break;
           }
           uint8_t* dst = s.ring + st * PairSmem::kStageBytes;
-          const uint32_t bar = mapa_shared(smem_addr(&s.full[st]), 0);  // the leader's barrier counts both CTAs' bytes
+          const uint32_t bar = mapa_shared(smem_addr(&s.full[st]), leader);  // the leader's barrier counts both CTAs' bytes
           if (rank == 0) mbar_arrive_expect_tx(&s.full[st], 2 * PairSmem::kStageBytes);
           tma_load_2d_pair(dst, &ta, bar, kb * kBK, ia * 2 * kBM + rank * kBM);
           tma_load_2d_pair(dst + kBM * kBK, &tb, bar, kb * kBK, ib * kPairN + rank * (kPairN / 2));
@@ -491,7 +603,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         if (it >= 2 && !mbar_wait(&s.tempty[buf], static_cast<uint32_t>((it >> 1) + 1) & 1u, abort)) break;
         tc_fence_after_sync();
         const uint32_t dacc = tmem + static_cast<uint32_t>(buf * kPairN);
-        for (int kb = 0; kb < p.kb; ++kb, ++i) {
+        for (int kb = k0; kb < k1; ++kb, ++i) {
           const int st = i % kStages;
           if (!mbar_wait(&s.full[st], static_cast<uint32_t>(i / kStages) & 1u, abort)) {
             ok = false;
@@ -502,15 +614,15 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
 #pragma unroll
           for (int kk = 0; kk < kBK / 32; ++kk)
             umma_i8_pair(dacc, umma_desc_sw128(ab + 32 * kk), umma_desc_sw128(bb + 32 * kk), idesc,
-                         (kb > 0 || kk > 0) ? 1u : 0u);
-          umma_commit_pair(&s.empty[st]);
+                         (kb > k0 || kk > 0) ? 1u : 0u);
+          umma_commit_pair(&s.empty[st], leader);
         }
-        if (ok) umma_commit_pair(&s.tfull[buf]);
+        if (ok) umma_commit_pair(&s.tfull[buf], leader);
       }
-      umma_commit_pair(&s.mma_done);
+      umma_commit_pair(&s.mma_done, leader);
       wait_drain(&s.mma_done, 0);
     }
-  } else {
+  } else if (!kSplit) {
     const int q = warp & 3, r = 32 * q + lane, et = threadIdx.x - 32 * kEpiWarp0, grp = et / 128;
     uint8_t* stage = s.out[grp];
     int it = 0;
@@ -529,7 +641,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       tc_fence_after_sync();
       const int c0 = grp * 128;
       const uint32_t src = tmem + (static_cast<uint32_t>(32 * q) << 16) + static_cast<uint32_t>(buf * kPairN + c0);
-      const uint32_t done = mapa_shared(smem_addr(&s.tempty[buf]), 0);
+      const uint32_t done = mapa_shared(smem_addr(&s.tempty[buf]), leader);
       const int m0 = (ia * 2 + rank) * kBM;
       auto drained = [&] {
         tc_fence_before_sync();
@@ -570,6 +682,43 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     }
     if (et % 128 == 0) tma_store_wait<true>();
   }
+  if constexpr (kSplit) {
+    int ia, ib;
+    tile_of(p, t0, ia, ib);
+    if (warp >= kEpiWarp0) {
+      const int et = threadIdx.x - 32 * kEpiWarp0, n = ib * kPairN + et;
+      const long long m = (static_cast<long long>(ia) * 2 + rank) * kBM + et;
+      s.ws[0][et] = n < a.N ? int8_w_scale(a, n) : 0.0f;
+      s.bias[0][et] = n < a.N ? int8_bias(a, n) : 0.0f;
+      if (et < kBM) s.ws[1][et] = m < a.M ? a.x_scale[m] : 0.0f;
+    }
+    if (warp >= kEpiWarp0 && !mbar_wait(&s.tfull[0], 0, abort)) *abort = 1;
+    __syncwarp();
+    cluster_sync_unaligned();  // every pair's MMAs have read the rings
+    const int S = p.S, L = kBM / S;
+    if (warp >= kEpiWarp0) {
+      tc_fence_after_sync();
+      const int q = warp & 3, r = 32 * q + lane, ll = r % L, c0 = (threadIdx.x - 32 * kEpiWarp0) / 128 * 128;
+      const uint32_t dst = mapa_shared(smem_addr(s.ring), static_cast<uint32_t>(2 * (r / L) + rank));
+      const uint32_t src = tmem + (static_cast<uint32_t>(32 * q) << 16);
+#pragma unroll 1
+      for (int c = c0; c < c0 + 128; c += 16) {
+        float raw[16];
+        tmem_ld_32x32b_x16(src + c, raw);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
+                           dst + static_cast<uint32_t>(((part * (kPairN / 4) + c / 4 + j) * (L + 1) + ll) * 16)),
+                       "f"(raw[4 * j]), "f"(raw[4 * j + 1]), "f"(raw[4 * j + 2]), "f"(raw[4 * j + 3])
+                       : "memory");
+      }
+      tc_fence_before_sync();
+    }
+    cluster_sync_unaligned();
+    if (!*abort)
+      finish_rows<kPairN>(a, reinterpret_cast<const int4*>(s.ring), S, L, (static_cast<long long>(ia) * 2 + rank) * kBM + part * L,
+                          ib * kPairN, vec, kPairThreads, s.ws[1] + part * L, s.ws[0], s.bias[0]);
+  }
   tc_fence_before_sync();
   __syncthreads();
   cluster_sync_unaligned();  // the leader's MMAs have read the peer's memory, every copy has landed in both
@@ -579,23 +728,30 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   }
 }
 
-int launch_pair(const Int8Args& a, cudaStream_t stream) {
-  static bool ready[64] = {false};
-  constexpr size_t smem = sizeof(PairSmem) + 1024;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !ready[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(int8_mm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return fail(BP_ERR_CUDA, "cudaFuncSetAttribute(smem %zu): %s", smem, cudaGetErrorString(e));
-    if (dev >= 0 && dev < 64) ready[dev] = true;
-  }
+Part pair_partition(const Int8Args& a) {
   Part p;
   p.ta = (a.M + 2 * kBM - 1) / (2 * kBM);
   p.tb = (a.N + kPairN - 1) / kPairN;
   p.kb = (a.K + kBK - 1) / kBK;
   p.S = 1;
-  const int pairs = tc_sm_count() / 2, tiles = p.ta * p.tb;
-  p.grid = 2 * (tiles < pairs ? tiles : pairs);
+  const long long pairs = tc_sm_count() / 2, tiles = static_cast<long long>(p.ta) * p.tb;
+  while (p.S < kMaxPairSplit && tiles * p.S * 2 <= pairs && p.S * 2 <= p.kb) p.S *= 2;
+  p.grid = static_cast<int>(2 * (tiles < pairs ? tiles : pairs));
+  return p;
+}
+
+template <bool kSplit>
+int launch_pair(const Int8Args& a, const Part& p, cudaStream_t stream) {
+  auto* kern = int8_mm_pair_kernel<kSplit>;
+  static bool ready[64] = {false};
+  constexpr size_t smem = sizeof(PairSmem) + 1024;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !ready[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return fail(BP_ERR_CUDA, "cudaFuncSetAttribute(smem %zu): %s", smem, cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
   CUtensorMap ta, tb;
   int st = tc_encode_2d(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.x, a.K, a.M, a.ldx, kBK, kBM, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
   if (st != BP_OK) return st;
@@ -604,19 +760,24 @@ int launch_pair(const Int8Args& a, cudaStream_t stream) {
   const int es = a.y_f32 ? 4 : 2;
   int vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && (a.ldy * es) % 16 == 0;
   CUtensorMap ty = ta;
-  if (vec && !a.y_f32) {
+  if (!kSplit && vec && !a.y_f32) {
     st = tc_encode_2d(&ty, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.y, a.N, a.M, a.ldy * 2, 64, kBM, CU_TENSOR_MAP_L2_PROMOTION_NONE);
     if (st != BP_OK) return st;
     vec = 2;
   }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
-  cfg.gridDim = dim3(p.grid);
+  cfg.gridDim = dim3(kSplit ? p.ta * p.tb * p.S * 2 : p.grid);
   cfg.blockDim = dim3(kPairThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   set_launch_attrs(cfg, attr);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, int8_mm_pair_kernel, ta, tb, ty, a, p, vec);
+  attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+  attr[cfg.numAttrs].val.clusterDim.x = 2 * p.S;
+  attr[cfg.numAttrs].val.clusterDim.y = 1;
+  attr[cfg.numAttrs].val.clusterDim.z = 1;
+  ++cfg.numAttrs;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tb, ty, a, p, vec);
   if (e != cudaSuccess) return fail(BP_ERR_CUDA, "int8_mm launch (pairs, M=%d N=%d K=%d): %s", a.M, a.N, a.K, cudaGetErrorString(e));
   return BP_OK;
 }
@@ -629,13 +790,31 @@ bool int8_mm_tc_supported(const Int8Args& a) {
 }
 
 int launch_int8_mm_tc(const Int8Args& a, cudaStream_t stream) {
-  if (a.M <= 16) return launch_split<16, true>(a, stream);
-  if (a.M <= 32) return launch_split<32, true>(a, stream);
-  if (a.M <= 64) return launch_split<64, true>(a, stream);
-  const long long tiles = static_cast<long long>((a.M + kBM - 1) / kBM) * ((a.N + 255) / 256);
-  if (tiles > (1 << 29)) return fail(BP_ERR_UNSUPPORTED, "int8_mm: too many tiles (M=%d N=%d)", a.M, a.N);
-  if (tiles >= tc_sm_count()) return launch_pair(a, stream);
-  return launch_split<128, false>(a, stream);
+  if (a.M <= 16) return launch_swap<16, false>(a, stream);
+  if (a.M <= 32) return launch_swap<32, false>(a, stream);
+  if (a.M <= 64) return launch_swap<64, false>(a, stream);
+  // Both forms stream 256 operand rows per CTA and K slice, at the rate of the L2; what differs is how many slices an SM
+  // has to take (two CTAs of the one kernel share it), waves included.
+  const Part p = pair_partition(a);
+  const long long sms = tc_sm_count(), pt = static_cast<long long>(p.ta) * p.tb;
+  if (pt > (1 << 28)) return fail(BP_ERR_UNSUPPORTED, "int8_mm: too many tiles (M=%d N=%d)", a.M, a.N);
+  const Part o = split_partition<128, false>(a);
+  const long long ot = static_cast<long long>(o.ta) * o.tb;
+  const long long pair_cost = (2 * pt * p.S + sms - 1) / sms * ((p.kb + p.S - 1) / p.S);
+  const long long one_cost = (ot * o.S + sms - 1) / sms * ((o.kb + o.S - 1) / o.S);
+  if (pair_cost < one_cost) return p.S > 1 ? launch_pair<true>(a, p, stream) : launch_pair<false>(a, p, stream);
+  return o.S > 1 ? launch<128, false, true, false>(a, o, stream) : launch<128, false, false, false>(a, o, stream);
+}
+
+bool int8_fused_supported(const Int8Args& a, const void* x, long long ldx) {
+  if (a.M > 16 || a.K % 8 != 0 || static_cast<long long>(a.M) * a.K > 8192 || ldx % 8 != 0 || a.ldw % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(x) % 16 != 0 || reinterpret_cast<uintptr_t>(a.w) % 16 != 0)
+    return false;
+  return static_cast<size_t>(fuse_blocks(split_partition<16, true>(a))) * 16 * kBK <= kFuseBytes;
+}
+
+int launch_int8_fused(const Int8Args& a, const __nv_bfloat16* x, long long ldx, cudaStream_t stream) {
+  return launch_swap<16, true>(a, stream, x, ldx);
 }
 
 BP_DEFINE_DEVICE_ERROR_READER(read_device_errors_int8mm)
