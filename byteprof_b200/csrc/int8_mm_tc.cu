@@ -6,8 +6,8 @@
 //  * Many rows (kSwap = false): 128 tokens are the MMA's M, kBN channels its N. With enough tiles for the GPU the
 //    grid is persistent and two accumulators alternate, so that a tile's epilogue runs under the next tile's
 //    MMAs.
-//  * Few rows (kSwap = true): the weights are the MMA's M (128 channels) and the tokens its N, padded to 16, 32 or
-//    64: the weights stream once, whatever the number of tokens.
+//  * Few rows (kSwap = true): the weights are the MMA's M (128 channels) and the tokens its N, padded to 16 or
+//    32: the weights stream once, whatever the number of tokens.
 //  * Few tiles: the S CTAs of a cluster split a tile's K; their int32 partials meet in distributed shared memory
 //    (the ring's memory, free by then), each CTA finishing 128 / S of the tile's lanes. Integer sums do not depend
 //    on the order, so all forms give the same bits as the CUDA-core kernel.
@@ -33,7 +33,7 @@ constexpr int kMaxSplit = 8;
 template <int kBN, bool kFuse>
 struct Cfg {
   static constexpr int kStageBytes = (kBM + (kFuse ? 0 : kBN)) * kBK;
-  static constexpr int kStages = kFuse ? 4 : kBN >= 128 ? 3 : kBN >= 64 ? 4 : 5;
+  static constexpr int kStages = kFuse ? 4 : kBN >= 128 ? 3 : 5;
   static constexpr int kRingBytes = kStages * kStageBytes;
   // in cluster mode the ring's memory holds the partials: S x kBN / 4 x (128 / S + 1) x 16 bytes
   static_assert(kRingBytes >= 4 * kBN * (kBM + kMaxSplit), "partials");
@@ -168,7 +168,7 @@ __device__ __forceinline__ void finish_rows(const Int8Args& a, const int4* red, 
 }
 
 // The K blocks [k0, k1) of the tokens' rows in 8 bits, as the MMA reads them: [block][kBN rows][128 bytes], 128-byte
-// swizzle, zeros past M and K. Called by `n` threads (whole warps, not all of the CTA).
+// swizzle, zeros past K. Called by `n` threads (whole warps, not all of the CTA).
 template <int kBN>
 __device__ __forceinline__ void quantize_range(const Int8Args& a, const __nv_bfloat16* x, long long ldx, uint8_t* dst, int k0, int k1,
                                                float* row_scale, uint32_t* red, int tid, int n) {
@@ -199,15 +199,16 @@ __device__ __forceinline__ void quantize_range(const Int8Args& a, const __nv_bfl
   }
   named_barrier_sync(1, n);
   if (tid < a.M) row_scale[tid] = red[tid] >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : int8_row_scale(red[tid]);
-  const int per = kBN * 16, all = (k1 - k0) * per;  // 8-value pieces of a block
-  for (int i = tid; i < all; i += n) {
-    const int b = i / per, r = i % per / 16, c = i % 16, k = (k0 + b) * kBK + c * 8;
-    uint2 v = make_uint2(0, 0);
-    if (r < a.M && k < a.K && red[r] < 0x7f800000u) {
-      const float s = int8_row_scale(red[r]);
-      v = q8(ldg16(x + r * ldx + k), s, 1.0f / s);
+  // the MMA's columns past M read what lies here and nobody reads them
+  const int span = (k1 - k0) * 16;  // 8-value pieces of a row
+  for (int r = 0; r < a.M; ++r) {
+    const bool bad = red[r] >= 0x7f800000u;
+    const float s = int8_row_scale(red[r]), inv = 1.0f / s;
+    for (int i = tid; i < span; i += n) {
+      const int b = i / 16, c = i % 16, k = (k0 + b) * kBK + c * 8;
+      const uint2 v = k < a.K && !bad ? q8(ldg16(x + r * ldx + k), s, inv) : make_uint2(0, 0);
+      *reinterpret_cast<uint2*>(dst + b * kBN * kBK + r * kBK + (((c / 2) ^ (r & 7)) * 16) + (c & 1) * 8) = v;
     }
-    *reinterpret_cast<uint2*>(dst + b * kBN * kBK + r * kBK + (((c / 2) ^ (r & 7)) * 16) + (c & 1) * 8) = v;
   }
   named_barrier_sync(1, n);  // row_scale is visible to the epilogue
 }
@@ -491,12 +492,17 @@ Part partition(const Int8Args& a) {
   return p;
 }
 
-// Few tiles for the GPU: the CTAs of a cluster share a tile's K.
+// Few tiles for the GPU: the 8 or 4 CTAs of a cluster share a tile's K. Meeting in distributed shared memory costs 3 to
+// 5 us, so a split has to save more (one row, weights cold: 8192 -> 2048 takes 22.5 us whole, 10.5 in 4, 8.7 in 8;
+// 8192 -> 8192 23 whole, 16.5 in 4; 2048 -> 8192 8.7 whole, 8.9 in 4; two CTAs gained nowhere).
 template <int kBN, bool kSwap>
 Part split_partition(const Int8Args& a) {
   Part p = partition<kBN, kSwap>(a);
   const long long ctas = 2 * tc_sm_count(), tiles = static_cast<long long>(p.ta) * p.tb;
-  while (p.S < kMaxSplit && tiles * p.S * 2 <= ctas && p.S * 2 <= p.kb) p.S *= 2;
+  if (tiles * 8 <= ctas && p.kb >= 8)
+    p.S = 8;
+  else if (tiles * 4 <= ctas && p.kb >= 32)
+    p.S = 4;
   return p;
 }
 
@@ -526,24 +532,18 @@ struct PairSmem {
 };
 constexpr int kPairN = 256;
 constexpr int kPairEpi = 256;
-constexpr int kMaxPairSplit = 4;  // a cluster of 8 CTAs; the partials, 4 (S + 128) KB, fit the ring
 constexpr int kPairThreads = 32 * kEpiWarp0 + kPairEpi;
 
-// kSplit: a cluster of p.S pairs shares one tile's K; the partials meet as in the single-CTA kernel, each CTA finishing
-// 128 / S of its half's lanes.
 // vec: 0: y's rows are not 16-byte aligned; 1: they are (fp32); 2: bf16 through `ty`, a map of y in 64 x 128 boxes
-template <bool kSplit>
-__global__ void __launch_bounds__(kPairThreads, 1)
+__global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     int8_mm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                         const __grid_constant__ CUtensorMap ty, const Int8Args a, const Part p, const int vec) {
   constexpr int kStages = PairSmem::kStages;
   extern __shared__ uint8_t smem_raw[];
   PairSmem& s = *reinterpret_cast<PairSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int crank = static_cast<int>(cluster_ctarank()), rank = crank & 1, leader = crank & ~1, part = crank >> 1;
-  const int t0 = blockIdx.x / (2 * p.S), step = kSplit ? 1 << 30 : p.grid / 2, tiles = p.ta * p.tb;
-  const int k0 = kSplit ? static_cast<int>(static_cast<long long>(part) * p.kb / p.S) : 0;
-  const int k1 = kSplit ? static_cast<int>(static_cast<long long>(part + 1) * p.kb / p.S) : p.kb;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int t0 = blockIdx.x / 2, step = p.grid / 2, tiles = p.ta * p.tb;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -577,14 +577,14 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       for (int t = t0; t < tiles && ok; t += step) {
         int ia, ib;
         tile_of(p, t, ia, ib);
-        for (int kb = k0; kb < k1; ++kb, ++i) {
+        for (int kb = 0; kb < p.kb; ++kb, ++i) {
           const int st = i % kStages;
           if (i >= kStages && !mbar_wait(&s.empty[st], static_cast<uint32_t>((i / kStages) + 1) & 1u, abort)) {
             ok = false;
             break;
           }
           uint8_t* dst = s.ring + st * PairSmem::kStageBytes;
-          const uint32_t bar = mapa_shared(smem_addr(&s.full[st]), leader);  // the leader's barrier counts both CTAs' bytes
+          const uint32_t bar = mapa_shared(smem_addr(&s.full[st]), 0);  // the leader's barrier counts both CTAs' bytes
           if (rank == 0) mbar_arrive_expect_tx(&s.full[st], 2 * PairSmem::kStageBytes);
           tma_load_2d_pair(dst, &ta, bar, kb * kBK, ia * 2 * kBM + rank * kBM);
           tma_load_2d_pair(dst + kBM * kBK, &tb, bar, kb * kBK, ib * kPairN + rank * (kPairN / 2));
@@ -603,7 +603,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         if (it >= 2 && !mbar_wait(&s.tempty[buf], static_cast<uint32_t>((it >> 1) + 1) & 1u, abort)) break;
         tc_fence_after_sync();
         const uint32_t dacc = tmem + static_cast<uint32_t>(buf * kPairN);
-        for (int kb = k0; kb < k1; ++kb, ++i) {
+        for (int kb = 0; kb < p.kb; ++kb, ++i) {
           const int st = i % kStages;
           if (!mbar_wait(&s.full[st], static_cast<uint32_t>(i / kStages) & 1u, abort)) {
             ok = false;
@@ -614,15 +614,15 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
           for (int kk = 0; kk < kBK / 32; ++kk)
             umma_i8_pair(dacc, umma_desc_sw128(ab + 32 * kk), umma_desc_sw128(bb + 32 * kk), idesc,
-                         (kb > k0 || kk > 0) ? 1u : 0u);
-          umma_commit_pair(&s.empty[st], leader);
+                         (kb > 0 || kk > 0) ? 1u : 0u);
+          umma_commit_pair(&s.empty[st]);
         }
-        if (ok) umma_commit_pair(&s.tfull[buf], leader);
+        if (ok) umma_commit_pair(&s.tfull[buf]);
       }
-      umma_commit_pair(&s.mma_done, leader);
+      umma_commit_pair(&s.mma_done);
       wait_drain(&s.mma_done, 0);
     }
-  } else if (!kSplit) {
+  } else {
     const int q = warp & 3, r = 32 * q + lane, et = threadIdx.x - 32 * kEpiWarp0, grp = et / 128;
     uint8_t* stage = s.out[grp];
     int it = 0;
@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       tc_fence_after_sync();
       const int c0 = grp * 128;
       const uint32_t src = tmem + (static_cast<uint32_t>(32 * q) << 16) + static_cast<uint32_t>(buf * kPairN + c0);
-      const uint32_t done = mapa_shared(smem_addr(&s.tempty[buf]), leader);
+      const uint32_t done = mapa_shared(smem_addr(&s.tempty[buf]), 0);
       const int m0 = (ia * 2 + rank) * kBM;
       auto drained = [&] {
         tc_fence_before_sync();
@@ -682,43 +682,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     if (et % 128 == 0) tma_store_wait<true>();
   }
-  if constexpr (kSplit) {
-    int ia, ib;
-    tile_of(p, t0, ia, ib);
-    if (warp >= kEpiWarp0) {
-      const int et = threadIdx.x - 32 * kEpiWarp0, n = ib * kPairN + et;
-      const long long m = (static_cast<long long>(ia) * 2 + rank) * kBM + et;
-      s.ws[0][et] = n < a.N ? int8_w_scale(a, n) : 0.0f;
-      s.bias[0][et] = n < a.N ? int8_bias(a, n) : 0.0f;
-      if (et < kBM) s.ws[1][et] = m < a.M ? a.x_scale[m] : 0.0f;
-    }
-    if (warp >= kEpiWarp0 && !mbar_wait(&s.tfull[0], 0, abort)) *abort = 1;
-    __syncwarp();
-    cluster_sync_unaligned();  // every pair's MMAs have read the rings
-    const int S = p.S, L = kBM / S;
-    if (warp >= kEpiWarp0) {
-      tc_fence_after_sync();
-      const int q = warp & 3, r = 32 * q + lane, ll = r % L, c0 = (threadIdx.x - 32 * kEpiWarp0) / 128 * 128;
-      const uint32_t dst = mapa_shared(smem_addr(s.ring), static_cast<uint32_t>(2 * (r / L) + rank));
-      const uint32_t src = tmem + (static_cast<uint32_t>(32 * q) << 16);
-#pragma unroll 1
-      for (int c = c0; c < c0 + 128; c += 16) {
-        float raw[16];
-        tmem_ld_32x32b_x16(src + c, raw);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
-                           dst + static_cast<uint32_t>(((part * (kPairN / 4) + c / 4 + j) * (L + 1) + ll) * 16)),
-                       "f"(raw[4 * j]), "f"(raw[4 * j + 1]), "f"(raw[4 * j + 2]), "f"(raw[4 * j + 3])
-                       : "memory");
-      }
-      tc_fence_before_sync();
-    }
-    cluster_sync_unaligned();
-    if (!*abort)
-      finish_rows<kPairN>(a, reinterpret_cast<const int4*>(s.ring), S, L, (static_cast<long long>(ia) * 2 + rank) * kBM + part * L,
-                          ib * kPairN, vec, kPairThreads, s.ws[1] + part * L, s.ws[0], s.bias[0]);
-  }
   tc_fence_before_sync();
   __syncthreads();
   cluster_sync_unaligned();  // the leader's MMAs have read the peer's memory, every copy has landed in both
@@ -735,20 +698,17 @@ Part pair_partition(const Int8Args& a) {
   p.kb = (a.K + kBK - 1) / kBK;
   p.S = 1;
   const long long pairs = tc_sm_count() / 2, tiles = static_cast<long long>(p.ta) * p.tb;
-  while (p.S < kMaxPairSplit && tiles * p.S * 2 <= pairs && p.S * 2 <= p.kb) p.S *= 2;
   p.grid = static_cast<int>(2 * (tiles < pairs ? tiles : pairs));
   return p;
 }
 
-template <bool kSplit>
 int launch_pair(const Int8Args& a, const Part& p, cudaStream_t stream) {
-  auto* kern = int8_mm_pair_kernel<kSplit>;
   static bool ready[64] = {false};
   constexpr size_t smem = sizeof(PairSmem) + 1024;
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !ready[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    const cudaError_t e = cudaFuncSetAttribute(int8_mm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return fail(BP_ERR_CUDA, "cudaFuncSetAttribute(smem %zu): %s", smem, cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }
@@ -760,24 +720,19 @@ int launch_pair(const Int8Args& a, const Part& p, cudaStream_t stream) {
   const int es = a.y_f32 ? 4 : 2;
   int vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && (a.ldy * es) % 16 == 0;
   CUtensorMap ty = ta;
-  if (!kSplit && vec && !a.y_f32) {
+  if (vec && !a.y_f32) {
     st = tc_encode_2d(&ty, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.y, a.N, a.M, a.ldy * 2, 64, kBM, CU_TENSOR_MAP_L2_PROMOTION_NONE);
     if (st != BP_OK) return st;
     vec = 2;
   }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
-  cfg.gridDim = dim3(kSplit ? p.ta * p.tb * p.S * 2 : p.grid);
+  cfg.gridDim = dim3(p.grid);
   cfg.blockDim = dim3(kPairThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   set_launch_attrs(cfg, attr);
-  attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-  attr[cfg.numAttrs].val.clusterDim.x = 2 * p.S;
-  attr[cfg.numAttrs].val.clusterDim.y = 1;
-  attr[cfg.numAttrs].val.clusterDim.z = 1;
-  ++cfg.numAttrs;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tb, ty, a, p, vec);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, int8_mm_pair_kernel, ta, tb, ty, a, p, vec);
   if (e != cudaSuccess) return fail(BP_ERR_CUDA, "int8_mm launch (pairs, M=%d N=%d K=%d): %s", a.M, a.N, a.K, cudaGetErrorString(e));
   return BP_OK;
 }
@@ -792,17 +747,17 @@ bool int8_mm_tc_supported(const Int8Args& a) {
 int launch_int8_mm_tc(const Int8Args& a, cudaStream_t stream) {
   if (a.M <= 16) return launch_swap<16, false>(a, stream);
   if (a.M <= 32) return launch_swap<32, false>(a, stream);
-  if (a.M <= 64) return launch_swap<64, false>(a, stream);
-  // Both forms stream 256 operand rows per CTA and K slice, at the rate of the L2; what differs is how many slices an SM
-  // has to take (two CTAs of the one kernel share it), waves included.
+  // Both forms stream 256 operand rows per CTA and K slice at the rate of the L2, about 0.4 us a slice, and what differs is
+  // how many slices an SM has to take, waves included; meeting in a cluster costs a split about ten slices
+  // (2048 x 2048 -> 16384: 53 us in pairs, 72 in single CTAs; 509 x 8192 -> 2048: 26 in pairs, 18 split in 4).
   const Part p = pair_partition(a);
   const long long sms = tc_sm_count(), pt = static_cast<long long>(p.ta) * p.tb;
   if (pt > (1 << 28)) return fail(BP_ERR_UNSUPPORTED, "int8_mm: too many tiles (M=%d N=%d)", a.M, a.N);
   const Part o = split_partition<128, false>(a);
   const long long ot = static_cast<long long>(o.ta) * o.tb;
-  const long long pair_cost = (2 * pt * p.S + sms - 1) / sms * ((p.kb + p.S - 1) / p.S);
-  const long long one_cost = (ot * o.S + sms - 1) / sms * ((o.kb + o.S - 1) / o.S);
-  if (pair_cost < one_cost) return p.S > 1 ? launch_pair<true>(a, p, stream) : launch_pair<false>(a, p, stream);
+  const long long pair_cost = (2 * pt + sms - 1) / sms * p.kb;
+  const long long one_cost = (ot * o.S + sms - 1) / sms * ((o.kb + o.S - 1) / o.S) + (o.S > 1 ? 10 : 0);
+  if (a.M > kBM && pair_cost <= one_cost) return launch_pair(a, p, stream);
   return o.S > 1 ? launch<128, false, true, false>(a, o, stream) : launch<128, false, false, false>(a, o, stream);
 }
 

@@ -278,13 +278,13 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, u
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Arrives once on the barrier at this shared-memory offset in both CTAs of the pair (cluster ranks `leader` and
-// leader + 1) when the pair's operations are complete.
-__device__ __forceinline__ void umma_commit_pair(uint64_t* bar, int leader) {
+// Arrives once on the barrier at this shared-memory offset in both CTAs (cluster ranks 0 and 1) when the pair's
+// operations are complete.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
           smem_addr(bar)),
-      "h"(static_cast<uint16_t>(3 << leader))
+      "h"(static_cast<uint16_t>(3))
       : "memory");
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
