@@ -65,4 +65,8 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int s) {
   return r;
 }
 
+// The kernel for many rows (paged_attn_tc.cu): scratch bytes, and the launch (a's G, min_share and parts are set there).
+size_t paged_tc_workspace_bytes(int hd);
+int launch_paged_tc(PagedArgs a, void* workspace, cudaStream_t stream);
+
 }  // namespace bp

@@ -452,6 +452,10 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 constexpr int kCtasPerSm = 2;
 
+// Up to 32 packed rows per sequence and kv head on average (the lengths themselves are on the device): two tiles of the
+// 16-row kernel, which then reads each key twice; the other kernel pads to 128.
+bool few_rows(int rows, int seqs, int g) { return static_cast<long long>(rows) * g <= 32LL * seqs; }
+
 int few_grid() { return kCtasPerSm * tc_sm_count(); }
 
 template <int HD>
@@ -485,7 +489,8 @@ cudaError_t launch_few(const PagedArgs& a, cudaStream_t s) {
 extern "C" size_t bp_paged_attention_workspace_bytes(int rows, int seqs, int nh, int nkv, int head_dim) {
   using namespace bp;
   if (rows <= 0 || seqs <= 0 || nkv <= 0 || nh < nkv || head_dim <= 0) return 0;
-  return static_cast<size_t>(2 * few_grid()) * kRows * (head_dim + 2) * sizeof(float);
+  return few_rows(rows, seqs, nh / nkv) ? static_cast<size_t>(2 * few_grid()) * kRows * (head_dim + 2) * sizeof(float)
+                                        : paged_tc_workspace_bytes(head_dim);
 }
 
 extern "C" int bp_paged_attention(const void* q, long long ldq, const void* k_pages, const void* v_pages, int num_pages,
@@ -505,7 +510,10 @@ extern "C" int bp_paged_attention(const void* q, long long ldq, const void* k_pa
   if (page_size < 8 || page_size > 256 || (page_size & (page_size - 1)) != 0)
     return fail(BP_ERR_UNSUPPORTED, "page_size must be a power of two from 8 to 256 (got %d)", page_size);
   if (rows > (1 << 20)) return fail(BP_ERR_UNSUPPORTED, "paged attention takes at most 2^20 rows per call (got %d)", rows);
+  if (static_cast<long long>(num_pages) * page_size > 0x7fffffffLL - 256)
+    return fail(BP_ERR_UNSUPPORTED, "the cache holds at most 2^31 positions (got %d pages of %d)", num_pages, page_size);
   if (rows == 0 || seqs == 0) return BP_OK;
+  if (num_pages < 1) return fail(BP_ERR_INVALID_ARGUMENT, "a cache of no pages");
   if (q == nullptr || pages == nullptr || q_start == nullptr || kv_len == nullptr || k_pages == nullptr ||
       v_pages == nullptr || out == nullptr)
     return fail(BP_ERR_INVALID_ARGUMENT, "a pointer argument is NULL");
@@ -544,6 +552,10 @@ extern "C" int bp_paged_attention(const void* q, long long ldq, const void* k_pa
   a.scale_log2 = scale * 1.4426950408889634f;
   a.out = static_cast<__nv_bfloat16*>(out);
   a.ldo = ldo;
+  if (!few_rows(rows, seqs, a.g)) {
+    st = launch_paged_tc(a, workspace, static_cast<cudaStream_t>(stream));
+    return st != BP_OK ? st : check_launch("paged_attention");
+  }
   a.G = few_grid();
   a.min_share = 1;
   a.part_o = static_cast<float*>(workspace);

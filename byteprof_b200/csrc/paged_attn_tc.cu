@@ -1,0 +1,750 @@
+// Attention of many new rows over a paged cache on the 5th-generation tensor cores (bp_paged_attention's kernel for
+// prompts and chunks; few rows: paged_attn.cu).
+//
+//   S = q K^T, p = exp2(scale S - m), O += p V, l += sum p, out = O / l: one pass over the keys per tile of rows.
+//
+//  * An item is 256 packed rows (two tiles of 128) of one sequence and kv head, a unit is 128 keys of it (paged.cuh); CTAs
+//    take equal ranges of units, whatever the lengths.
+//  * Warp 0 finds the pages and loads K and V tiles by TMA, one box per page (page rows are strided by the kv heads):
+//    the 128-byte swizzled tile serves as K (K-major) and as V (keys are the second product's K dimension: MN-major).
+//    A page that is not there is fetched from behind the pool, which TMA fills with zeros.
+//  * Warp 1 issues the MMAs of both tiles in turn: S0, S1, then per key block P0 V, S0', P1 V, S1', so that one
+//    tile's softmax runs under the other's products. S (fp32), P (bf16, over S) and O (fp32) live in TMEM.
+//  * Two warpgroups do the softmax, one thread per row: 128 scores into registers, mask (only where the row's limit lies
+//    in the block), maximum, exp2, P back to TMEM. The running maximum moves only when a score exceeds it by 2^8:
+//    then O is rescaled in TMEM by the same threads, which is rare after the first block.
+//
+// Bound by the tensor cores and the special-function units alike: a block of 128 x 128 scores takes 1024 clocks of MMA
+// (head_dim 128) and 1024 of exp2.
+#include <cudaTypedefs.h>
+
+#include "paged.cuh"
+#include "skinny_internal.h"
+#include "sm100.cuh"
+
+namespace bp {
+namespace {
+
+constexpr int kTile = 128;                // rows per tile, keys per unit
+constexpr int kItemRows = 2 * kTile;
+constexpr int kSlots = 4;                 // K and V tiles in the ring
+constexpr int kThreads = 384;
+constexpr int kWarps = kThreads / 32;
+constexpr int kSmWarp0 = 4;               // softmax warpgroups: warps 4..7 (tile 0) and 8..11 (tile 1)
+constexpr int kBadRing = 16;
+constexpr float kLazy = 8.0f;
+constexpr int kScanSeqs = 512;
+// register split: launched with 168 per thread (64512), 4 warps keep 80, 8 warps take 208: 63488
+constexpr int kRegsLaunch = 168, kRegsLow = 80, kRegsHigh = 208;
+static_assert(128 * kRegsLow + 256 * kRegsHigh <= kThreads * kRegsLaunch, "register split");
+
+// 32 lanes x 128 TMEM columns into registers, complete when it returns.
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+      "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, "
+      "%51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63, %64, %65, %66, %67, %68, %69, "
+      "%70, %71, %72, %73, %74, %75, %76, %77, %78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, "
+      "%89, %90, %91, %92, %93, %94, %95, %96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, "
+      "%107, %108, %109, %110, %111, %112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, "
+      "%123, %124, %125, %126, %127}, [%128];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
+        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
+        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
+        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]), "=r"(r[64]),
+        "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]), "=r"(r[72]),
+        "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]), "=r"(r[80]),
+        "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]),
+        "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]),
+        "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
+        "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]),
+        "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]),
+        "=r"(r[118]), "=r"(r[119]), "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]),
+        "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      : "r"(taddr)
+      : "memory");
+}
+
+// 32 lanes x 32 registers into TMEM columns (complete at tmem_st_wait).
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+               "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+               "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+               "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+               "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D[tmem] (+)= A[tmem] . B[smem], bf16, fp32 accumulator.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// MN-major operand with 128-byte swizzling: 64 values of N per 128-byte row, one row per k, 8-row groups 1024 bytes
+// apart, the next 64 values of N `lbo` bytes away.
+__device__ __forceinline__ uint64_t umma_desc_mn(uint32_t saddr, uint32_t lbo) {
+  return umma_desc_sw128(saddr) - (static_cast<uint64_t>(1) << 16) + (static_cast<uint64_t>(lbo >> 4) << 16);
+}
+
+// ---- the cut of the work ----------------------------------------------------------------------------------
+// Blocks of 128 keys that packed rows up to `last` (exclusive) of a sequence see (at least `floor`).
+__device__ __forceinline__ int blocks_of(const PagedArgs& a, const PagedSeq& q, int last, int floor) {
+  long long vis = q.pos0 + (last - 1) / a.g + 1;
+  if (vis > q.kv) vis = q.kv;
+  const int n = vis <= 0 ? 0 : static_cast<int>((vis + kTile - 1) / kTile);
+  return n > floor ? n : floor;
+}
+__device__ __forceinline__ int item_units(const PagedArgs& a, const PagedSeq& q, int nrows, int tile) {
+  return blocks_of(a, q, min(nrows, (tile + 1) * kItemRows), 1);
+}
+__device__ __forceinline__ int item_tiles(int nrows) { return (nrows + kItemRows - 1) / kItemRows; }
+
+struct Scan {
+  long long units[kScanSeqs];  // of one kv head, per sequence of the block at hand
+  long long warp_sum[kWarps], total, before;
+  int seq;
+};
+
+// units[] of the sequences s0 .. s0 + kScanSeqs; called by all threads, ends with a barrier.
+template <int kN>
+__device__ void scan_units(const PagedArgs& a, Scan& sc, int s0) {
+  const int count = min(kScanSeqs, a.seqs - s0), lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < count; i += kN) {
+    const PagedSeq q = paged_seq(a, s0 + i);
+    const int nrows = q.n * a.g, nt = item_tiles(nrows);
+    long long u = 0;
+    if (nt > 16)
+      u = -1;  // a warp's work
+    else
+      for (int t = 0; t < nt; ++t) u += item_units(a, q, nrows, t);
+    sc.units[i] = u;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x / 32; i < count; i += kN / 32) {
+    if (sc.units[i] >= 0) continue;
+    const PagedSeq q = paged_seq(a, s0 + i);
+    const int nrows = q.n * a.g, nt = item_tiles(nrows);
+    long long u = 0;
+    for (int t = lane; t < nt; t += 32) u += item_units(a, q, nrows, t);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(kPagedFull, u, o);
+    __syncwarp();
+    if (lane == 0) sc.units[i] = u;
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ long long share_of(const PagedArgs& a, long long total) {
+  const long long s = (total + a.G - 1) / a.G;
+  return s > a.min_share ? s : a.min_share;
+}
+
+// The total of all units (sc.total).
+template <int kN>
+__device__ void scan_total(const PagedArgs& a, Scan& sc) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long total = 0;
+  for (int s0 = 0; s0 < a.seqs; s0 += kScanSeqs) {
+    scan_units<kN>(a, sc, s0);
+    const int count = min(kScanSeqs, a.seqs - s0);
+    for (int i = threadIdx.x; i < count; i += kN) total += sc.units[i];
+    if (s0 + kScanSeqs < a.seqs) __syncthreads();
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(kPagedFull, total, o);
+  if (lane == 0) sc.warp_sum[warp] = total;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    total = 0;
+    for (int w = 0; w < kN / 32; ++w) total += sc.warp_sum[w];
+    sc.total = total * a.nkv;
+  }
+  __syncthreads();
+}
+
+// The sequence of unit u (sc.seq) and the units before it (sc.before); after scan_total. All threads.
+template <int kN>
+__device__ void scan_find(const PagedArgs& a, Scan& sc, long long u) {
+  long long base = 0;
+  for (int s0 = 0; s0 < a.seqs; s0 += kScanSeqs) {
+    if (a.seqs > kScanSeqs) scan_units<kN>(a, sc, s0);
+    const int count = min(kScanSeqs, a.seqs - s0);
+    if (threadIdx.x < 32) {
+      const int lane = threadIdx.x;
+      long long run = base;
+      int hit = -1;
+      long long hit_before = 0;
+      for (int i0 = 0; i0 < count; i0 += 32) {
+        const long long mine = i0 + lane < count ? sc.units[i0 + lane] * a.nkv : 0;
+        long long pre = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long v = __shfl_up_sync(kPagedFull, pre, o);
+          if (lane >= o) pre += v;
+        }
+        const long long start = run + pre - mine;
+        const unsigned m = __ballot_sync(kPagedFull, mine > 0 && u >= start && u < start + mine);
+        if (m != 0) {
+          const int src = __ffs(m) - 1;
+          hit = s0 + i0 + src;
+          hit_before = __shfl_sync(kPagedFull, start, src);
+          break;
+        }
+        run += __shfl_sync(kPagedFull, pre, 31);
+      }
+      if (lane == 0) {
+        sc.seq = hit;
+        sc.before = hit >= 0 ? hit_before : run;
+      }
+    }
+    __syncthreads();
+    if (sc.seq >= 0) return;
+    base = sc.before;
+    __syncthreads();
+  }
+}
+
+// A CTA's walk over its units: one segment (a range of key blocks of one item) at a time. Every role walks by itself.
+struct Walk {
+  PagedSeq q;
+  int s, h, tile, nrows, tiles;
+  int off, end, per;        // the segment's blocks, the item's
+  int blocks[2];            // what each 128-row tile sees of the item
+  long long left;           // units of the CTA after this segment
+
+  __device__ __forceinline__ void item(const PagedArgs& a) {
+    per = item_units(a, q, nrows, tile);
+    const int r0 = tile * kItemRows;
+    blocks[0] = blocks_of(a, q, min(nrows, r0 + kTile), 0);
+    blocks[1] = nrows > r0 + kTile ? blocks_of(a, q, min(nrows, r0 + kItemRows), 0) : 0;
+  }
+  __device__ __forceinline__ void enter(const PagedArgs& a) {
+    q = paged_seq(a, s);
+    nrows = q.n * a.g;
+    tiles = item_tiles(nrows);
+  }
+  // `rel`: units behind the start of sequence `seq`, each kv head of which has `head` units
+  __device__ void start(const PagedArgs& a, int seq, long long rel, long long head, long long count) {
+    s = seq;
+    enter(a);
+    h = static_cast<int>(rel / head);
+    long long r = rel % head;
+    for (tile = 0;; ++tile) {
+      const int n = item_units(a, q, nrows, tile);
+      if (r < n) break;
+      r -= n;
+    }
+    item(a);
+    off = static_cast<int>(r);
+    end = static_cast<int>(per - off < count ? per : off + count);
+    left = count - (end - off);
+  }
+  __device__ bool next(const PagedArgs& a) {
+    if (left <= 0) return false;
+    if (++tile == tiles) {
+      tile = 0;
+      if (++h == a.nkv) {
+        h = 0;
+        do {
+          ++s;
+          enter(a);
+        } while (nrows == 0);
+      }
+    }
+    item(a);
+    off = 0;
+    end = static_cast<int>(per < left ? per : left);
+    left -= end;
+    return true;
+  }
+  // blocks [off, until(i)) of the segment are tile i's
+  __device__ __forceinline__ int until(int i) const { return min(end, blocks[i]); }
+};
+
+template <int HD>
+struct Smem {
+  static constexpr int kTileBytes = kTile * HD * 2;
+  uint8_t q[2][kTileBytes];
+  uint8_t kv[kSlots][kTileBytes];
+  uint64_t full[kSlots], empty[kSlots], q_full[2], s_full[2], p_full[2], o_done[2], mma_done;
+  int bad[kBadRing];
+  uint32_t tmem_base;
+  int abort;
+  Scan scan;
+};
+
+__device__ __forceinline__ void wait_drain(uint64_t* bar, uint32_t parity) {
+  const unsigned long long t0 = globaltimer();
+  while (!mbar_try_wait(bar, parity)) {
+    if (globaltimer() - t0 > kWaitLimitNs) {
+      atomicOr(&g_bp_device_errors, BP_DEVERR_TIMEOUT);
+      return;
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const PagedArgs a) {
+  constexpr int kHalf = kTile * 128;  // bytes of 64 head dimensions of a tile
+  constexpr int kTileBytes = Smem<HD>::kTileBytes;
+  extern __shared__ uint8_t smem_raw[];
+  Smem<HD>& s = *reinterpret_cast<Smem<HD>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.q_full[i], kTile);
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.p_full[i], kTile);
+      mbar_init(&s.o_done[i], 1);
+    }
+    mbar_init(&s.mma_done, 1);
+    s.abort = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+  }
+  if (warp == 1) {
+    tmem_alloc(&s.tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+  const uint32_t tmem = s.tmem_base;
+  volatile int* abort = &s.abort;
+
+  scan_total<kThreads>(a, s.scan);
+  const long long share = share_of(a, s.scan.total), u0 = blockIdx.x * share;
+  const long long count = s.scan.total - u0 < share ? s.scan.total - u0 : share;
+  if (count > 0) scan_find<kThreads>(a, s.scan, u0);
+  __syncthreads();
+  const bool work = count > 0;
+  const int seq0 = s.scan.seq;
+  const long long rel0 = u0 - s.scan.before, head0 = work ? s.scan.units[seq0 % kScanSeqs] : 1;
+
+  if (warp < kSmWarp0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
+    if (warp == 0 && work) {
+      // ---- pages and TMA: K(b), V(b) per block, alternating in the ring ----
+      Walk w;
+      w.start(a, seq0, rel0, head0, count);
+      const int rows_per = min(1 << a.page_log2, kTile), np = kTile / rows_per;  // rows and boxes per block
+      const int mask = (1 << a.page_log2) - 1, none = a.num_pages << a.page_log2;
+      int t = 0, issued = 0;  // blocks, slots
+      bool ok = true;
+      do {
+        const int* table = a.pages + static_cast<long long>(w.s) * a.ld_pages;
+        for (int b = w.off; b < w.end && ok; ++b, ++t) {
+          const int key = b * kTile + lane * rows_per;
+          int row = none, bad = w.q.bad;
+          if (lane < np && key < w.q.kv) {
+            const int page = __ldg(table + (key >> a.page_log2));
+            if (page >= 0 && page < a.num_pages)
+              row = (page << a.page_log2) + (key & mask);
+            else
+              bad = min(bad, key);
+          }
+          bad = __reduce_min_sync(kPagedFull, bad);
+          if (lane == 0) s.bad[t % kBadRing] = bad;
+          for (int kv = 0; kv < 2 && ok; ++kv, ++issued) {
+            const int slot = issued % kSlots;
+            int go = 1;
+            if (lane == 0) {
+              if (issued >= kSlots) go = mbar_wait(&s.empty[slot], static_cast<uint32_t>((issued / kSlots) + 1) & 1u, abort);
+              if (go) mbar_arrive_expect_tx(&s.full[slot], kTileBytes);
+            }
+            ok = __shfl_sync(kPagedFull, go, 0) != 0;
+            if (!ok) break;
+            if (lane < np) {
+#pragma unroll
+              for (int c = 0; c < HD / 64; ++c)
+                tma_load_3d(s.kv[slot] + c * kHalf + lane * rows_per * 128, kv == 0 ? &tk : &tv, &s.full[slot], c * 64, row, w.h);
+            }
+            __syncwarp();
+          }
+        }
+      } while (ok && w.next(a));
+      if (lane == 0)
+        for (int i = 0; i < kSlots && i < issued; ++i) wait_drain(&s.full[i], static_cast<uint32_t>((issued - 1 - i) / kSlots) & 1u);
+    } else if (warp == 1 && work) {
+      // ---- MMA ----
+      Walk w;
+      w.start(a, seq0, rel0, head0, count);
+      constexpr uint32_t idesc_s = umma_idesc_bf16(kTile, kTile);
+      constexpr uint32_t idesc_o = umma_idesc_bf16(kTile, HD) | (1u << 16);  // B is MN-major
+      int idx = 0, seg[2] = {0, 0}, np_[2] = {0, 0};  // ring position; segments and blocks of each tile so far
+      bool ok = true;
+      // waits are one lane's, the answer is the warp's
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        int go = 1;
+        if (lane == 0) go = mbar_wait(bar, parity, abort);
+        __syncwarp();
+        return __shfl_sync(kPagedFull, go, 0) != 0;
+      };
+      auto scores = [&](int i, int slot) {
+        if (lane == 0) {
+          const uint32_t qa = smem_addr(s.q[i]), kb = smem_addr(s.kv[slot]);
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k)
+            umma_f16(tmem + i * kTile, umma_desc_sw128(qa + (k / 4) * kHalf + (k % 4) * 32),
+                     umma_desc_sw128(kb + (k / 4) * kHalf + (k % 4) * 32), idesc_s, k > 0 ? 1u : 0u);
+          umma_commit(&s.s_full[i]);
+        }
+      };
+      do {
+        const int un[2] = {w.until(0), w.until(1)};
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (un[i] > w.off && ok) ok = wait(&s.q_full[i], static_cast<uint32_t>(seg[i]++) & 1u);
+        if (ok) ok = wait(&s.full[idx % kSlots], static_cast<uint32_t>(idx / kSlots) & 1u);
+        if (!ok) break;
+        tc_fence_after_sync();
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (un[i] > w.off) scores(i, idx % kSlots);
+        if (lane == 0) umma_commit(&s.empty[idx % kSlots]);
+        for (int b = w.off; b < w.end && ok; ++b) {
+          const int vslot = (idx + 1) % kSlots, kslot = (idx + 2) % kSlots;
+          const bool more = b + 1 < w.end;
+          ok = wait(&s.full[vslot], static_cast<uint32_t>((idx + 1) / kSlots) & 1u);
+          if (!ok) break;
+          const int valid = w.q.kv - b * kTile;
+          if (valid < kTile) {  // values past the sequence's end may be NaN, which p = 0 does not hide
+            const int v0 = valid > 0 ? valid : 0;
+            for (int c = lane; c < (kTile - v0) * 8 * (HD / 64); c += 32) {
+              const int half = c / ((kTile - v0) * 8), r = c % ((kTile - v0) * 8);
+              *reinterpret_cast<uint4*>(s.kv[vslot] + half * kHalf + (v0 * 8 + r) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_async_shared();
+            __syncwarp();
+          }
+          bool have_k = false;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (b < un[i] && ok) {
+              ok = wait(&s.p_full[i], static_cast<uint32_t>(np_[i]++) & 1u);
+              if (!ok) break;
+              tc_fence_after_sync();
+              if (lane == 0) {
+                const uint32_t vb = smem_addr(s.kv[vslot]);
+#pragma unroll
+                for (int k = 0; k < kTile / 16; ++k)
+                  umma_f16_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + k * 8, umma_desc_mn(vb + k * 2048, kHalf), idesc_o,
+                              (b > w.off || k > 0) ? 1u : 0u);
+                umma_commit(&s.o_done[i]);
+              }
+            }
+            if (more && b + 1 < un[i] && ok) {
+              if (!have_k) {
+                ok = wait(&s.full[kslot], static_cast<uint32_t>((idx + 2) / kSlots) & 1u);
+                if (!ok) break;
+                tc_fence_after_sync();
+                have_k = true;
+              }
+              scores(i, kslot);
+            }
+          }
+          if (!ok) break;
+          if (lane == 0) {
+            umma_commit(&s.empty[vslot]);
+            if (more) umma_commit(&s.empty[kslot]);
+          }
+          idx += 2;
+        }
+      } while (ok && w.next(a));
+      if (lane == 0) {
+        umma_commit(&s.mma_done);
+        wait_drain(&s.mma_done, 0);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
+    if (work) {
+      // ---- softmax: one thread per packed row ----
+      const int i = (warp - kSmWarp0) / 4, r = threadIdx.x & (kTile - 1);
+      const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+      const uint32_t ts = tmem + lanes + i * kTile, to = tmem + lanes + 2 * kTile + i * kTile;
+      const float sc = a.scale_log2;
+      Walk w;
+      w.start(a, seq0, rel0, head0, count);
+      int n = 0, t0 = 0;  // blocks of this tile so far; blocks of the CTA before the segment
+      bool ok = true;
+      do {
+        const int until = w.until(i), pr = w.tile * kItemRows + i * kTile + r;  // packed row
+        const bool live = pr < w.nrows;
+        const int tok = live ? pr / a.g : 0, head = w.h * a.g + (live ? pr % a.g : 0);
+        float m = -INFINITY, l = 0.0f;
+        int bad = w.q.bad;
+        const long long pos = live ? w.q.pos0 + tok : -1;
+        const long long vis = pos + 1 < w.q.kv ? pos + 1 : w.q.kv;  // visible keys
+        if (until > w.off) {
+          // q into shared memory, K-major with the 128-byte swizzle
+          const __nv_bfloat16* src = a.q + static_cast<long long>(w.q.first + tok) * a.ldq + head * HD;
+#pragma unroll
+          for (int c = 0; c < HD / 8; ++c)
+            *reinterpret_cast<uint4*>(s.q[i] + (c / 8) * kHalf + r * 128 + (((c % 8) ^ (r & 7)) * 16)) =
+                live ? ldg16(src + c * 8) : make_uint4(0, 0, 0, 0);
+          fence_async_shared();
+          mbar_arrive(&s.q_full[i]);
+          for (int b = w.off; b < until; ++b, ++n) {
+            ok = mbar_wait(&s.s_full[i], static_cast<uint32_t>(n) & 1u, abort);
+            if (!__all_sync(kPagedFull, ok)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after_sync();
+            uint32_t x[kTile];
+            tmem_ld128(ts, x);
+            bad = min(bad, s.bad[(t0 + b - w.off) % kBadRing]);
+            const long long lim = vis - static_cast<long long>(b) * kTile;
+            if (__any_sync(kPagedFull, lim < kTile)) {
+              const int lim32 = lim > kTile ? kTile : (lim < 0 ? 0 : static_cast<int>(lim));
+#pragma unroll
+              for (int c = 0; c < kTile; ++c) x[c] = c < lim32 ? x[c] : 0xff800000u;
+            }
+            float mx[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(x[c]);
+#pragma unroll
+            for (int c = 4; c < kTile; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(x[c]));
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+            if (__any_sync(kPagedFull, top > m + kLazy)) {
+              const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.0f : pg_ex2(m - mn);
+              m = mn;
+              l *= f;
+              if (b > w.off) {  // O holds the blocks before, under the old maximum
+                ok = mbar_wait(&s.o_done[i], static_cast<uint32_t>(n - 1) & 1u, abort);
+                if (!__all_sync(kPagedFull, ok)) {
+                  ok = false;
+                  break;
+                }
+                tc_fence_after_sync();
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 32) {
+                  uint32_t o[32];
+                  tmem_ld_32x32b_x32(to + c, o);
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                  tmem_st32(to + c, o);
+                }
+              }
+            }
+            const float neg = m == -INFINITY ? 0.0f : -m;
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < kTile; c += 64) {
+              uint32_t p[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const float e0 = pg_ex2(fmaf(__uint_as_float(x[c + 2 * j]), sc, neg));
+                const float e1 = pg_ex2(fmaf(__uint_as_float(x[c + 2 * j + 1]), sc, neg));
+                sum[j & 1] += e0;
+                sum[2 + (j & 1)] += e1;
+                p[j] = pack2(e0, e1);
+              }
+              tmem_st32(ts + c / 2, p);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_st_wait();
+            tc_fence_before_sync();
+            mbar_arrive(&s.p_full[i]);
+          }
+          if (!ok) break;
+          ok = mbar_wait(&s.o_done[i], static_cast<uint32_t>(n - 1) & 1u, abort);
+          if (!__all_sync(kPagedFull, ok)) break;
+          tc_fence_after_sync();
+        }
+        if (pos >= bad) l = __int_as_float(0x7fc00000);
+        const bool any = until > w.off, whole = w.off == 0 && w.end == w.per;
+        if (whole) {
+          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+          __nv_bfloat16* dst = a.out + static_cast<long long>(w.q.first + tok) * a.ldo + head * HD;
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 32) {
+            uint32_t o[32];
+            if (any)
+              tmem_ld_32x32b_x32(to + c, o);
+            else
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = 0;
+            if (live) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                uint32_t v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  v[e] = pack2(__uint_as_float(o[8 * j + 2 * e]) * inv, __uint_as_float(o[8 * j + 2 * e + 1]) * inv);
+                *reinterpret_cast<uint4*>(dst + c + 8 * j) = make_uint4(v[0], v[1], v[2], v[3]);
+              }
+            }
+          }
+        } else {
+          const size_t at = static_cast<size_t>(2 * blockIdx.x + (w.off == 0 ? 1 : 0)) * kItemRows + i * kTile + r;
+          float* dst = a.part_o + at * HD;
+          if (any) {
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(to + c, o);
+              if (live) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  *reinterpret_cast<uint4*>(dst + c + 4 * j) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+              }
+            }
+          }
+          if (live) reinterpret_cast<float2*>(a.part_ml)[at] = make_float2(any ? m : -INFINITY, l);
+        }
+        tc_fence_before_sync();
+        t0 += w.end - w.off;
+      } while (w.next(a));
+    }
+  }
+  tc_fence_before_sync();
+  cta_teardown_barrier();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the item that starts in CTA c's share and goes on behind it: block (c, rows / 32), one warp per 4 rows.
+constexpr int kJoinThreads = 256;
+template <int HD>
+__global__ void __launch_bounds__(kJoinThreads) paged_tc_join_kernel(const PagedArgs a) {
+  __shared__ Scan sc;
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x;
+  scan_total<kJoinThreads>(a, sc);
+  const long long share = share_of(a, sc.total), u = (c + 1) * share;  // the first unit behind the share
+  if (u >= sc.total) return;
+  scan_find<kJoinThreads>(a, sc, u - 1);
+  __syncthreads();
+  Walk w;
+  w.start(a, sc.seq, u - 1 - sc.before, sc.units[sc.seq % kScanSeqs], 1);
+  const long long first = u - 1 - w.off, last = first + w.per - 1;  // the item's units
+  if (first < c * share || last < u) return;
+  const int c1 = static_cast<int>(last / share);
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
+  constexpr int kPer = HD / 32;
+  for (int k = 0; k < 4; ++k) {
+    const int row = blockIdx.y * 32 + warp * 4 + k, pr = w.tile * kItemRows + row;
+    if (pr >= w.nrows) return;
+    float m = -INFINITY;
+    for (int d = c + lane; d <= c1; d += 32) m = fmaxf(m, ml[static_cast<size_t>(2 * d + (d == c)) * kItemRows + row].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kPagedFull, m, o));
+    float l = 0.0f, acc[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) acc[j] = 0.0f;
+#pragma unroll 4
+    for (int d = c; d <= c1; ++d) {
+      const size_t at = static_cast<size_t>(2 * d + (d == c)) * kItemRows + row;
+      const float2 p = ml[at];
+      if (p.x == -INFINITY) {  // nothing seen there: no output was left (a NaN sum still counts)
+        if (isnan(p.y)) l = p.y;
+        continue;
+      }
+      const float f = pg_ex2(p.x - m);
+      l = fmaf(f, p.y, l);
+      const float* src = a.part_o + at * HD + lane * kPer;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) acc[j] = fmaf(f, src[j], acc[j]);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    __nv_bfloat16* dst = a.out + static_cast<long long>(w.q.first + pr / a.g) * a.ldo + (w.h * a.g + pr % a.g) * HD + lane * kPer;
+#pragma unroll
+    for (int j = 0; j < kPer; j += 2) *reinterpret_cast<uint32_t*>(dst + j) = pack2(acc[j] * inv, acc[j + 1] * inv);
+  }
+}
+
+template <int HD>
+int launch(PagedArgs a, cudaStream_t stream) {
+  static bool ready[64] = {false};
+  constexpr size_t smem = sizeof(Smem<HD>) + 1024;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !ready[dev]) {
+    cudaFuncAttributes at;
+    cudaError_t e = cudaFuncGetAttributes(&at, paged_tc_kernel<HD>);
+    if (e == cudaSuccess && at.numRegs < kRegsLaunch)  // the register split would wait for registers that are not there
+      return fail(BP_ERR_UNSUPPORTED, "paged attention was built with %d registers per thread, %d expected", at.numRegs, kRegsLaunch);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(paged_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return fail(BP_ERR_CUDA, "cudaFuncSetAttribute(smem %zu): %s", smem, cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
+  const int ps = 1 << a.page_log2;
+  const uint64_t rows = static_cast<uint64_t>(a.num_pages) << a.page_log2;
+  CUtensorMap tk, tv;
+  const uint64_t dims[3] = {HD, rows, static_cast<uint64_t>(a.nkv)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(a.nkv) * HD * 2, HD * 2};
+  const uint32_t box[3] = {64, static_cast<uint32_t>(ps < kTile ? ps : kTile), 1};
+  int st = tc_encode(&tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.kp, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  if (st != BP_OK) return st;
+  st = tc_encode(&tv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.vp, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  if (st != BP_OK) return st;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = dim3(a.G);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  set_launch_attrs(cfg, attr);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, paged_tc_kernel<HD>, tk, tv, a);
+  if (e == cudaSuccess && a.G > 1) {
+    cfg.gridDim = dim3(a.G - 1, kItemRows / 32);
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, paged_tc_join_kernel<HD>, a);
+  }
+  if (e != cudaSuccess) return fail(BP_ERR_CUDA, "paged_attention launch (many rows): %s", cudaGetErrorString(e));
+  return BP_OK;
+}
+
+}  // namespace
+
+size_t paged_tc_workspace_bytes(int hd) {
+  return static_cast<size_t>(2 * tc_sm_count()) * kItemRows * (hd + 2) * sizeof(float);
+}
+
+int launch_paged_tc(PagedArgs a, void* workspace, cudaStream_t stream) {
+  a.G = tc_sm_count();
+  a.min_share = 4;  // a part costs its write and its join: as much as about two blocks
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o + static_cast<size_t>(2 * a.G) * kItemRows * a.hd;
+  return a.hd == 128 ? launch<128>(a, stream) : launch<64>(a, stream);
+}
+
+BP_DEFINE_DEVICE_ERROR_READER(read_device_errors_paged)
+
+}  // namespace bp

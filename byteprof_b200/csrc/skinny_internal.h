@@ -69,5 +69,6 @@ unsigned int read_device_errors_i4tc();
 unsigned int read_device_errors_glob();
 unsigned int read_device_errors_loc();
 unsigned int read_device_errors_int8mm();
+unsigned int read_device_errors_paged();
 
 }  // namespace bp

@@ -689,7 +689,7 @@ BP_DEFINE_DEVICE_ERROR_READER(read_device_errors_tc)
 
 unsigned int read_and_clear_device_errors() {
   return read_device_errors_tc() | read_device_errors_i8() | read_device_errors_i4tc() | read_device_errors_glob() |
-         read_device_errors_loc() | read_device_errors_int8mm();
+         read_device_errors_loc() | read_device_errors_int8mm() | read_device_errors_paged();
 }
 
 }  // namespace bp

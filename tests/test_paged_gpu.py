@@ -80,7 +80,12 @@ MANY = [
     ([130], [0], 4, 2, 128, 16), ([128], [0], 1, 1, 128, 128), ([257], [511], 4, 4, 128, 64), ([300, 1, 77], [0, 900, 5], 8, 2, 64, 32),
     ([1000], [0], 6, 2, 64, 8), ([129, 127, 1], [1, 0, 128], 16, 16, 128, 256), ([700], [1300], 3, 1, 128, 16),
     ([64, 511, 33, 200], [100, 3, 0, 1024], 14, 2, 64, 64), ([333], [77], 5, 5, 128, 8),
+    ([128], [30000], 1, 1, 128, 16), ([130], [20000], 2, 1, 64, 256), ([700], [0], 8, 1, 64, 16), ([2000], [37], 12, 1, 128, 32),
+    ([33] * 600, [i % 50 for i in range(600)], 1, 1, 64, 16), ([0, 500, 0, 1, 0], [0, 3, 9, 2, 0], 4, 4, 128, 16),
 ]
+
+
+FEW.append(([1] * 1100, [(7 * i) % 90 for i in range(1100)], 2, 1, 64, 32))
 
 
 @pytest.mark.parametrize("news,befores,nh,nkv,hd,page", FEW + MANY)

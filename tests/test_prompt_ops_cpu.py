@@ -24,7 +24,8 @@ def attention(**kw):
 @pytest.mark.parametrize("kw,status,msg", [
     (dict(rows=-1), 1, b"negative"), (dict(nh=3), 1, b"multiple"), (dict(nkv=0), 1, b"multiple"), (dict(nh=2048, nkv=1), 1, b"1024"),
     (dict(hd=96), 2, b"head_dim"), (dict(page_size=24), 2, b"page_size"), (dict(page_size=4), 2, b"page_size"),
-    (dict(page_size=512), 2, b"page_size"), (dict(rows=1 << 21), 2, b"2^20"), (dict(q=None), 1, b"NULL"), (dict(pages=None), 1, b"NULL"),
+    (dict(page_size=512), 2, b"page_size"), (dict(rows=1 << 21), 2, b"2^20"), (dict(num_pages=0), 1, b"no pages"),
+    (dict(num_pages=1 << 27), 2, b"2^31"), (dict(q=None), 1, b"NULL"), (dict(pages=None), 1, b"NULL"),
     (dict(ldq=255), 1, b"strides"), (dict(ld_pages=3), 1, b"strides"), (dict(scale=0.0), 1, b"scale"),
     (dict(scale=float("nan")), 1, b"scale"), (dict(q=ctypes.c_void_p(264)), 3, b"aligned"), (dict(ldo=260), 3, b"aligned"),
     (dict(rows=0, q=None), 0, b""), (dict(seqs=0, pages=None), 0, b"")])
