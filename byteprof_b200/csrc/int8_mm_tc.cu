@@ -291,6 +291,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (lane == 0) {
       if (kFuse) mbar_wait(&s.quantized, 0, abort);
       constexpr uint32_t idesc = umma_idesc_s8(kBM, kBN);
+      // descriptors of the first stage; the others are address differences away (in units of 16 bytes)
+      const uint64_t ring = umma_desc_sw128(smem_addr(s.ring)), planes = kFuse ? umma_desc_sw128(smem_addr(fused)) : 0;
       int i = 0, it = 0;
       bool ok = true;
       for (int t = t0; t < tiles && ok; t += step, ++it) {
@@ -305,10 +307,10 @@ __global__ void __launch_bounds__(kThreads, 2)
             break;
           }
           tc_fence_after_sync();
-          const uint32_t ab = smem_addr(s.ring + st * C::kStageBytes), bb = kFuse ? smem_addr(fused) + (kb - k0) * kBN * kBK : ab + kBM * kBK;
+          const uint64_t da = ring + st * (C::kStageBytes >> 4),
+                         db = kFuse ? planes + (kb - k0) * (kBN * kBK >> 4) : da + (kBM * kBK >> 4);
 #pragma unroll
-          for (int kk = 0; kk < kBK / 32; ++kk)
-            umma_i8(dacc, umma_desc_sw128(ab + 32 * kk), umma_desc_sw128(bb + 32 * kk), idesc, (kb > k0 || kk > 0) ? 1u : 0u);
+          for (int kk = 0; kk < kBK / 32; ++kk) umma_i8(dacc, da + 2 * kk, db + 2 * kk, idesc, (kb > k0 || kk > 0) ? 1u : 0u);
           umma_commit(&s.empty[st]);
         }
         if (ok) umma_commit(&s.tfull[buf]);
@@ -596,6 +598,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
       constexpr uint32_t idesc = umma_idesc_s8(2 * kBM, kPairN);
+      const uint64_t ring = umma_desc_sw128(smem_addr(s.ring));
       int i = 0, it = 0;
       bool ok = true;
       for (int t = t0; t < tiles && ok; t += step, ++it) {
@@ -610,11 +613,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             break;
           }
           tc_fence_after_sync();
-          const uint32_t ab = smem_addr(s.ring + st * PairSmem::kStageBytes), bb = ab + kBM * kBK;
+          const uint64_t da = ring + st * (PairSmem::kStageBytes >> 4), db = da + (kBM * kBK >> 4);
 #pragma unroll
-          for (int kk = 0; kk < kBK / 32; ++kk)
-            umma_i8_pair(dacc, umma_desc_sw128(ab + 32 * kk), umma_desc_sw128(bb + 32 * kk), idesc,
-                         (kb > 0 || kk > 0) ? 1u : 0u);
+          for (int kk = 0; kk < kBK / 32; ++kk) umma_i8_pair(dacc, da + 2 * kk, db + 2 * kk, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
           umma_commit_pair(&s.empty[st]);
         }
         if (ok) umma_commit_pair(&s.tfull[buf]);

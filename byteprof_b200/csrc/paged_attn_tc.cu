@@ -398,6 +398,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       w.start(a, seq0, rel0, head0, count);
       constexpr uint32_t idesc_s = umma_idesc_bf16(kTile, kTile);
       constexpr uint32_t idesc_o = umma_idesc_bf16(kTile, HD) | (1u << 16);  // B is MN-major
+      // descriptors of the first tiles; the others are address differences away (in units of 16 bytes)
+      const uint64_t dq = umma_desc_sw128(smem_addr(s.q[0])), dk = umma_desc_sw128(smem_addr(s.kv[0])),
+                     dv = umma_desc_mn(smem_addr(s.kv[0]), kHalf);
       int idx = 0, seg[2] = {0, 0}, np_[2] = {0, 0};  // ring position; segments and blocks of each tile so far
       bool ok = true;
       // waits are one lane's, the answer is the warp's
@@ -409,11 +412,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       auto scores = [&](int i, int slot) {
         if (lane == 0) {
-          const uint32_t qa = smem_addr(s.q[i]), kb = smem_addr(s.kv[slot]);
+          const uint64_t da = dq + i * (kTileBytes >> 4), db = dk + slot * (kTileBytes >> 4);
 #pragma unroll
-          for (int k = 0; k < HD / 16; ++k)
-            umma_f16(tmem + i * kTile, umma_desc_sw128(qa + (k / 4) * kHalf + (k % 4) * 32),
-                     umma_desc_sw128(kb + (k / 4) * kHalf + (k % 4) * 32), idesc_s, k > 0 ? 1u : 0u);
+          for (int k = 0; k < HD / 16; ++k) {
+            constexpr int kStep = 32 >> 4, kNext = kHalf >> 4;
+            umma_f16(tmem + i * kTile, da + (k / 4) * kNext + (k % 4) * kStep, db + (k / 4) * kNext + (k % 4) * kStep, idesc_s,
+                     k > 0 ? 1u : 0u);
+          }
           umma_commit(&s.s_full[i]);
         }
       };
@@ -452,10 +457,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!ok) break;
               tc_fence_after_sync();
               if (lane == 0) {
-                const uint32_t vb = smem_addr(s.kv[vslot]);
+                const uint64_t dvb = dv + vslot * (kTileBytes >> 4);
 #pragma unroll
                 for (int k = 0; k < kTile / 16; ++k)
-                  umma_f16_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + k * 8, umma_desc_mn(vb + k * 2048, kHalf), idesc_o,
+                  umma_f16_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + k * 8, dvb + k * (2048 >> 4), idesc_o,
                               (b > w.off || k > 0) ? 1u : 0u);
                 umma_commit(&s.o_done[i]);
               }
