@@ -27,15 +27,15 @@ namespace {
 
 constexpr int kTile = 128;                // rows per tile, keys per unit
 constexpr int kItemRows = 2 * kTile;
-constexpr int kSlots = 4;                 // K and V tiles in the ring
+constexpr int kSlots = 4;                 // K and V tiles in the ring (two blocks)
 constexpr int kThreads = 384;
 constexpr int kWarps = kThreads / 32;
 constexpr int kSmWarp0 = 4;               // softmax warpgroups: warps 4..7 (tile 0) and 8..11 (tile 1)
 constexpr int kBadRing = 16;
 constexpr float kLazy = 8.0f;
 constexpr int kScanSeqs = 512;
-// register split: launched with 168 per thread (64512), 4 warps keep 80, 8 warps take 208: 63488
-constexpr int kRegsLaunch = 168, kRegsLow = 80, kRegsHigh = 208;
+// register split: launched with 168 per thread (64512), 4 warps keep 120, 8 warps take 192: 64512
+constexpr int kRegsLaunch = 168, kRegsLow = 120, kRegsHigh = 192;
 static_assert(128 * kRegsLow + 256 * kRegsHigh <= kThreads * kRegsLaunch, "register split");
 
 // 32 lanes x 128 TMEM columns into registers, complete when it returns.
@@ -280,7 +280,7 @@ struct Smem {
   static constexpr int kTileBytes = kTile * HD * 2;
   uint8_t q[2][kTileBytes];
   uint8_t kv[kSlots][kTileBytes];
-  uint64_t full[kSlots], empty[kSlots], q_full[2], s_full[2], p_full[2], o_done[2], mma_done;
+  uint64_t full[kSlots], empty[kSlots], q_full[2], s_full[2], p_full[2], o_done[2], tail_go, tail, mma_done;
   int bad[kBadRing];
   uint32_t tmem_base;
   int abort;
@@ -318,9 +318,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.q_full[i], kTile);
       mbar_init(&s.s_full[i], 1);
-      mbar_init(&s.p_full[i], kTile);
+      mbar_init(&s.p_full[i], 4);
       mbar_init(&s.o_done[i], 1);
     }
+    mbar_init(&s.tail_go, 1);
+    mbar_init(&s.tail, 32);
     mbar_init(&s.mma_done, 1);
     s.abort = 0;
     mbar_fence_init();
@@ -336,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after_sync();
   pdl_launch_dependents();
   pdl_wait_prior_grids();
-  const uint32_t tmem = s.tmem_base;
+  constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's
   volatile int* abort = &s.abort;
 
   scan_total<kThreads>(a, s.scan);
@@ -393,100 +395,112 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0)
         for (int i = 0; i < kSlots && i < issued; ++i) wait_drain(&s.full[i], static_cast<uint32_t>((issued - 1 - i) / kSlots) & 1u);
     } else if (warp == 1 && work) {
-      // ---- MMA ----
-      Walk w;
-      w.start(a, seq0, rel0, head0, count);
-      constexpr uint32_t idesc_s = umma_idesc_bf16(kTile, kTile);
-      constexpr uint32_t idesc_o = umma_idesc_bf16(kTile, HD) | (1u << 16);  // B is MN-major
-      // descriptors of the first tiles; the others are address differences away (in units of 16 bytes)
-      const uint64_t dq = umma_desc_sw128(smem_addr(s.q[0])), dk = umma_desc_sw128(smem_addr(s.kv[0])),
-                     dv = umma_desc_mn(smem_addr(s.kv[0]), kHalf);
-      int idx = 0, seg[2] = {0, 0}, np_[2] = {0, 0};  // ring position; segments and blocks of each tile so far
-      bool ok = true;
-      // waits are one lane's, the answer is the warp's
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        int go = 1;
-        if (lane == 0) go = mbar_wait(bar, parity, abort);
-        __syncwarp();
-        return __shfl_sync(kPagedFull, go, 0) != 0;
-      };
-      auto scores = [&](int i, int slot) {
-        if (lane == 0) {
-          const uint64_t da = dq + i * (kTileBytes >> 4), db = dk + slot * (kTileBytes >> 4);
+      // ---- MMA: one thread, from wait to wait as short as it can be written ----
+      if (lane == 0) {
+        constexpr uint32_t idesc_s = umma_idesc_bf16(kTile, kTile);
+        constexpr uint32_t idesc_o = umma_idesc_bf16(kTile, HD) | (1u << 16);  // B is MN-major
+        // Block number `blk` of the CTA has K in slot 0 or 2 and V in slot 1 or 3. The two cases are written out, so that
+        // every descriptor is a constant of the kernel: one that is computed has to be moved to uniform registers for
+        // each MMA.
+        const uint64_t dq = umma_desc_sw128(smem_addr(s.q[0])), dk = umma_desc_sw128(smem_addr(s.kv[0])),
+                       dv = umma_desc_mn(smem_addr(s.kv[0]), kHalf);
+        constexpr int kT = kTileBytes >> 4;
+        auto scores_of = [&](int i, int slot) {
+          const uint64_t da = dq + i * kT, db = dk + slot * kT;
 #pragma unroll
           for (int k = 0; k < HD / 16; ++k) {
-            constexpr int kStep = 32 >> 4, kNext = kHalf >> 4;
-            umma_f16(tmem + i * kTile, da + (k / 4) * kNext + (k % 4) * kStep, db + (k / 4) * kNext + (k % 4) * kStep, idesc_s,
-                     k > 0 ? 1u : 0u);
+            constexpr int kNext = kHalf >> 4;
+            umma_f16(tmem + i * kTile, da + (k / 4) * kNext + (k % 4) * 2, db + (k / 4) * kNext + (k % 4) * 2, idesc_s, k > 0 ? 1u : 0u);
           }
           umma_commit(&s.s_full[i]);
-        }
-      };
-      do {
-        const int un[2] = {w.until(0), w.until(1)};
+        };
+        auto scores = [&](int i, int blk) {
+          if (blk & 1)
+            scores_of(i, 2);
+          else
+            scores_of(i, 0);
+        };
+        auto output_of = [&](int i, int slot, uint32_t more) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (un[i] > w.off && ok) ok = wait(&s.q_full[i], static_cast<uint32_t>(seg[i]++) & 1u);
-        if (ok) ok = wait(&s.full[idx % kSlots], static_cast<uint32_t>(idx / kSlots) & 1u);
-        if (!ok) break;
-        tc_fence_after_sync();
+          for (int k = 0; k < kTile / 16; ++k)
+            umma_f16_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + k * 8, dv + slot * kT + k * (2048 >> 4), idesc_o,
+                        k > 0 ? 1u : more);
+          umma_commit(&s.o_done[i]);
+        };
+        auto output = [&](int i, int blk, uint32_t more) {
+          if (blk & 1)
+            output_of(i, 3, more);
+          else
+            output_of(i, 1, more);
+        };
+        Walk w;
+        w.start(a, seq0, rel0, head0, count);
+        int blk = 0;  // blocks so far: K of block blk is tile 2 blk of the ring, V tile 2 blk + 1
+        uint32_t seg[2] = {0, 0}, pn[2] = {0, 0}, tails = 0;  // phases: q_full and p_full per tile, tail
+        bool ok = true;
+        do {
+          const int un[2] = {w.until(0), w.until(1)};
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (un[i] > w.off) scores(i, idx % kSlots);
-        if (lane == 0) umma_commit(&s.empty[idx % kSlots]);
-        for (int b = w.off; b < w.end && ok; ++b) {
-          const int vslot = (idx + 1) % kSlots, kslot = (idx + 2) % kSlots;
-          const bool more = b + 1 < w.end;
-          ok = wait(&s.full[vslot], static_cast<uint32_t>((idx + 1) / kSlots) & 1u);
+          for (int i = 0; i < 2; ++i)
+            if (un[i] > w.off) ok = ok && mbar_wait(&s.q_full[i], seg[i]++ & 1u, abort);
+          ok = ok && mbar_wait(&s.full[(2 * blk) & 3], (blk >> 1) & 1, abort);
           if (!ok) break;
-          const int valid = w.q.kv - b * kTile;
-          if (valid < kTile) {  // values past the sequence's end may be NaN, which p = 0 does not hide
-            const int v0 = valid > 0 ? valid : 0;
-            for (int c = lane; c < (kTile - v0) * 8 * (HD / 64); c += 32) {
-              const int half = c / ((kTile - v0) * 8), r = c % ((kTile - v0) * 8);
-              *reinterpret_cast<uint4*>(s.kv[vslot] + half * kHalf + (v0 * 8 + r) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_async_shared();
-            __syncwarp();
-          }
-          bool have_k = false;
+          tc_fence_after_sync();
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (b < un[i] && ok) {
-              ok = wait(&s.p_full[i], static_cast<uint32_t>(np_[i]++) & 1u);
-              if (!ok) break;
-              tc_fence_after_sync();
-              if (lane == 0) {
-                const uint64_t dvb = dv + vslot * (kTileBytes >> 4);
-#pragma unroll
-                for (int k = 0; k < kTile / 16; ++k)
-                  umma_f16_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + k * 8, dvb + k * (2048 >> 4), idesc_o,
-                              (b > w.off || k > 0) ? 1u : 0u);
-                umma_commit(&s.o_done[i]);
-              }
+          for (int i = 0; i < 2; ++i)
+            if (un[i] > w.off) scores(i, blk);
+          umma_commit(&s.empty[(2 * blk) & 3]);
+          for (int b = w.off; b < w.end; ++b, ++blk) {
+            const bool more = b + 1 < w.end;
+            ok = mbar_wait(&s.full[(2 * blk + 1) & 3], (blk >> 1) & 1, abort);
+            if (ok && w.q.kv - b * kTile < kTile) {  // warp 2 clears what lies past the end
+              mbar_arrive(&s.tail_go);
+              ok = mbar_wait(&s.tail, tails++ & 1u, abort);
             }
-            if (more && b + 1 < un[i] && ok) {
-              if (!have_k) {
-                ok = wait(&s.full[kslot], static_cast<uint32_t>((idx + 2) / kSlots) & 1u);
+            if (ok && more) ok = mbar_wait(&s.full[(2 * blk + 2) & 3], ((blk + 1) >> 1) & 1, abort);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (b < un[i] && ok) {
+                ok = mbar_wait(&s.p_full[i], pn[i]++ & 1u, abort);
                 if (!ok) break;
                 tc_fence_after_sync();
-                have_k = true;
+                output(i, blk, b > w.off ? 1u : 0u);
+                if (b + 1 < un[i]) scores(i, blk + 1);
               }
-              scores(i, kslot);
             }
+            if (!ok) break;
+            umma_commit(&s.empty[(2 * blk + 1) & 3]);
+            if (more) umma_commit(&s.empty[(2 * blk + 2) & 3]);
           }
-          if (!ok) break;
-          if (lane == 0) {
-            umma_commit(&s.empty[vslot]);
-            if (more) umma_commit(&s.empty[kslot]);
-          }
-          idx += 2;
-        }
-      } while (ok && w.next(a));
-      if (lane == 0) {
+        } while (ok && w.next(a));
         umma_commit(&s.mma_done);
         wait_drain(&s.mma_done, 0);
       }
+    } else if (warp == 2 && work) {
+      // ---- the last block of a sequence: values past its end may be NaN, which p = 0 does not hide ----
+      Walk w;
+      w.start(a, seq0, rel0, head0, count);
+      int blk = 0;
+      uint32_t tails = 0;
+      bool ok = true;
+      do {
+        for (int b = w.off; b < w.end && ok; ++b, ++blk) {
+          const int valid = w.q.kv - b * kTile;
+          if (valid >= kTile) continue;
+          ok = mbar_wait(&s.tail_go, tails++ & 1u, abort);  // the tile has landed
+          if (!__all_sync(kPagedFull, ok)) {
+            ok = false;
+            break;
+          }
+          const int v0 = valid > 0 ? valid : 0;
+          for (int c = lane; c < (kTile - v0) * 8 * (HD / 64); c += 32) {
+            const int half = c / ((kTile - v0) * 8), r = c % ((kTile - v0) * 8);
+            *reinterpret_cast<uint4*>(s.kv[(2 * blk + 1) & 3] + half * kHalf + (v0 * 8 + r) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_async_shared();
+          mbar_arrive(&s.tail);
+        }
+      } while (ok && w.next(a));
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
@@ -578,7 +592,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tmem_st_wait();
             tc_fence_before_sync();
-            mbar_arrive(&s.p_full[i]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.p_full[i]);
           }
           if (!ok) break;
           ok = mbar_wait(&s.o_done[i], static_cast<uint32_t>(n - 1) & 1u, abort);
