@@ -34,6 +34,7 @@ constexpr int kSmWarp0 = 4;               // softmax warpgroups: warps 4..7 (til
 constexpr int kBadRing = 16;
 constexpr float kLazy = 8.0f;
 constexpr int kScanSeqs = 512;
+constexpr uint32_t kBase = 1024;          // shared-memory address of the tiles
 // register split: launched with 168 per thread (64512), 4 warps keep 120, 8 warps take 192: 64512
 constexpr int kRegsLaunch = 168, kRegsLow = 120, kRegsHigh = 192;
 static_assert(128 * kRegsLow + 256 * kRegsHigh <= kThreads * kRegsLaunch, "register split");
@@ -94,10 +95,15 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       : "memory");
 }
 
+// umma_desc_sw128 of a constant address.
+__host__ __device__ constexpr uint64_t umma_desc_at(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) |
+         (2ull << 61);
+}
 // MN-major operand with 128-byte swizzling: 64 values of N per 128-byte row, one row per k, 8-row groups 1024 bytes
 // apart, the next 64 values of N `lbo` bytes away.
-__device__ __forceinline__ uint64_t umma_desc_mn(uint32_t saddr, uint32_t lbo) {
-  return umma_desc_sw128(saddr) - (static_cast<uint64_t>(1) << 16) + (static_cast<uint64_t>(lbo >> 4) << 16);
+__host__ __device__ constexpr uint64_t umma_desc_mn_at(uint32_t saddr, uint32_t lbo) {
+  return umma_desc_at(saddr) - (1ull << 16) + (static_cast<uint64_t>(lbo >> 4) << 16);
 }
 
 // ---- the cut of the work ----------------------------------------------------------------------------------
@@ -280,7 +286,7 @@ struct Smem {
   static constexpr int kTileBytes = kTile * HD * 2;
   uint8_t q[2][kTileBytes];
   uint8_t kv[kSlots][kTileBytes];
-  uint64_t full[kSlots], empty[kSlots], q_full[2], s_full[2], p_full[2], o_done[2], tail_go, tail, mma_done;
+  uint64_t full[kSlots], empty[kSlots], q_full[2], s_full[2], p_full[2][2], o_done[2], tail_go, tail, mma_done;
   int bad[kBadRing];
   uint32_t tmem_base;
   int abort;
@@ -297,6 +303,25 @@ __device__ __forceinline__ void wait_drain(uint64_t* bar, uint32_t parity) {
   }
 }
 
+// Two fp32 values in a register pair, and arithmetic on both at once.
+__device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float f32x2_lo(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float f32x2_hi(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&p);
@@ -308,8 +333,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kHalf = kTile * 128;  // bytes of 64 head dimensions of a tile
   constexpr int kTileBytes = Smem<HD>::kTileBytes;
   extern __shared__ uint8_t smem_raw[];
-  Smem<HD>& s = *reinterpret_cast<Smem<HD>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // The kernel has no static shared memory, so the dynamic part starts in the first 1024 bytes, and its tiles at kBase.
+  if (smem_addr(smem_raw) > kBase) {
+    if (threadIdx.x == 0) atomicOr(&g_bp_device_errors, BP_DEVERR_TIMEOUT);
+    return;
+  }
+  Smem<HD>& s = *reinterpret_cast<Smem<HD>*>(smem_raw + (kBase - smem_addr(smem_raw)));
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&s.full[i], 1);
@@ -318,7 +348,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.q_full[i], kTile);
       mbar_init(&s.s_full[i], 1);
-      mbar_init(&s.p_full[i], 4);
+      mbar_init(&s.p_full[i][0], 4);
+      mbar_init(&s.p_full[i][1], 4);
       mbar_init(&s.o_done[i], 1);
     }
     mbar_init(&s.tail_go, 1);
@@ -399,11 +430,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) {
         constexpr uint32_t idesc_s = umma_idesc_bf16(kTile, kTile);
         constexpr uint32_t idesc_o = umma_idesc_bf16(kTile, HD) | (1u << 16);  // B is MN-major
-        // Block number `blk` of the CTA has K in slot 0 or 2 and V in slot 1 or 3. The two cases are written out, so that
-        // every descriptor is a constant of the kernel: one that is computed has to be moved to uniform registers for
-        // each MMA.
-        const uint64_t dq = umma_desc_sw128(smem_addr(s.q[0])), dk = umma_desc_sw128(smem_addr(s.kv[0])),
-                       dv = umma_desc_mn(smem_addr(s.kv[0]), kHalf);
+        // Block number `blk` of the CTA has K in slot 0 or 2 and V in slot 1 or 3. The two cases are written out and the
+        // shared memory starts at a known address, so that every descriptor and barrier is a constant of the kernel:
+        // one that is computed has to be moved to uniform registers for each MMA.
+        constexpr uint64_t dq = umma_desc_at(kBase), dk = umma_desc_at(kBase + 2 * kTileBytes),
+                           dv = umma_desc_mn_at(kBase + 2 * kTileBytes, kHalf);
         constexpr int kT = kTileBytes >> 4;
         auto scores_of = [&](int i, int slot) {
           const uint64_t da = dq + i * kT, db = dk + slot * kT;
@@ -420,18 +451,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           else
             scores_of(i, 0);
         };
-        auto output_of = [&](int i, int slot, uint32_t more) {
+        // the first or second 64 keys of a block
+        auto output_of = [&](int i, int slot, int half, uint32_t more) {
 #pragma unroll
-          for (int k = 0; k < kTile / 16; ++k)
-            umma_f16_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + k * 8, dv + slot * kT + k * (2048 >> 4), idesc_o,
-                        k > 0 ? 1u : more);
-          umma_commit(&s.o_done[i]);
+          for (int k = 0; k < kTile / 32; ++k)
+            umma_f16_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + half * 32 + k * 8, dv + slot * kT + (half * 4 + k) * (2048 >> 4),
+                        idesc_o, k > 0 ? 1u : more);
         };
-        auto output = [&](int i, int blk, uint32_t more) {
+        auto output = [&](int i, int blk, int half, uint32_t more) {
           if (blk & 1)
-            output_of(i, 3, more);
+            output_of(i, 3, half, more);
           else
-            output_of(i, 1, more);
+            output_of(i, 1, half, more);
         };
         Walk w;
         w.start(a, seq0, rel0, head0, count);
@@ -457,15 +488,26 @@ __global__ void __launch_bounds__(kThreads, 1)
               mbar_arrive(&s.tail_go);
               ok = mbar_wait(&s.tail, tails++ & 1u, abort);
             }
-            if (ok && more) ok = mbar_wait(&s.full[(2 * blk + 2) & 3], ((blk + 1) >> 1) & 1, abort);
+            bool have_k = !more;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               if (b < un[i] && ok) {
-                ok = mbar_wait(&s.p_full[i], pn[i]++ & 1u, abort);
-                if (!ok) break;
+                const uint32_t ph = pn[i]++ & 1u;
+                ok = mbar_wait(&s.p_full[i][0], ph, abort);
                 tc_fence_after_sync();
-                output(i, blk, b > w.off ? 1u : 0u);
-                if (b + 1 < un[i]) scores(i, blk + 1);
+                if (ok) output(i, blk, 0, b > w.off ? 1u : 0u);
+                ok = ok && mbar_wait(&s.p_full[i][1], ph, abort);
+                tc_fence_after_sync();
+                if (!ok) break;
+                output(i, blk, 1, 1u);
+                umma_commit(&s.o_done[i]);
+                if (b + 1 < un[i]) {
+                  if (!have_k) ok = mbar_wait(&s.full[(2 * blk + 2) & 3], ((blk + 1) >> 1) & 1, abort);
+                  if (!ok) break;
+                  have_k = true;
+                  tc_fence_after_sync();
+                  scores(i, blk + 1);
+                }
               }
             }
             if (!ok) break;
@@ -549,9 +591,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             float mx[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(x[c]);
+            for (int c = 0; c < 4; ++c) mx[c] = fmaxf(__uint_as_float(x[c]), __uint_as_float(x[c + 4]));
 #pragma unroll
-            for (int c = 4; c < kTile; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(x[c]));
+            for (int c = 8; c < kTile; c += 8)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                mx[j] = fmaxf(fmaxf(mx[j], __uint_as_float(x[c + j])), __uint_as_float(x[c + 4 + j]));
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
             if (__any_sync(kPagedFull, top > m + kLazy)) {
               const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.0f : pg_ex2(m - mn);
@@ -575,25 +620,25 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
             const float neg = m == -INFINITY ? 0.0f : -m;
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const uint64_t sc2 = f32x2(sc, sc), neg2 = f32x2(neg, neg);
+            uint64_t sum2[2] = {0, 0};
 #pragma unroll
-            for (int c = 0; c < kTile; c += 64) {
+            for (int h = 0; h < 2; ++h) {  // 64 keys at a time: the second product starts on the first half
               uint32_t p[32];
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
-                const float e0 = pg_ex2(fmaf(__uint_as_float(x[c + 2 * j]), sc, neg));
-                const float e1 = pg_ex2(fmaf(__uint_as_float(x[c + 2 * j + 1]), sc, neg));
-                sum[j & 1] += e0;
-                sum[2 + (j & 1)] += e1;
+                const uint64_t y = fma_f32x2(f32x2(__uint_as_float(x[h * 64 + 2 * j]), __uint_as_float(x[h * 64 + 2 * j + 1])), sc2, neg2);
+                const float e0 = pg_ex2(f32x2_lo(y)), e1 = pg_ex2(f32x2_hi(y));
+                sum2[j & 1] = add_f32x2(sum2[j & 1], f32x2(e0, e1));
                 p[j] = pack2(e0, e1);
               }
-              tmem_st32(ts + c / 2, p);
+              tmem_st32(ts + h * 32, p);
+              tmem_st_wait();
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&s.p_full[i][h]);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_st_wait();
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s.p_full[i]);
+            l += (f32x2_lo(sum2[0]) + f32x2_hi(sum2[0])) + (f32x2_lo(sum2[1]) + f32x2_hi(sum2[1]));
           }
           if (!ok) break;
           ok = mbar_wait(&s.o_done[i], static_cast<uint32_t>(n - 1) & 1u, abort);
