@@ -453,8 +453,9 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 constexpr int kCtasPerSm = 2;
 
 // Up to 32 packed rows per sequence and kv head on average (the lengths themselves are on the device): two tiles of the
-// 16-row kernel, which then reads each key twice; the other kernel pads to 128.
-bool few_rows(int rows, int seqs, int g) { return static_cast<long long>(rows) * g <= 32LL * seqs; }
+// 16-row kernel, which then reads each key twice; the other kernel pads to 128
+// and takes groups of up to 128 heads.
+bool few_rows(int rows, int seqs, int g) { return static_cast<long long>(rows) * g <= 32LL * seqs || g > 128; }
 
 int few_grid() { return kCtasPerSm * tc_sm_count(); }
 

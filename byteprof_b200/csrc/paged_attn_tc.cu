@@ -107,17 +107,20 @@ __host__ __device__ constexpr uint64_t umma_desc_mn_at(uint32_t saddr, uint32_t 
 }
 
 // ---- the cut of the work ----------------------------------------------------------------------------------
-// Blocks of 128 keys that packed rows up to `last` (exclusive) of a sequence see (at least `floor`).
-__device__ __forceinline__ int blocks_of(const PagedArgs& a, const PagedSeq& q, int last, int floor) {
-  long long vis = q.pos0 + (last - 1) / a.g + 1;
+// A tile holds the g heads of 128 / g tokens (g <= 128; the few rows left over idle), an item two tiles.
+__device__ __forceinline__ int tile_tokens(const PagedArgs& a) { return kTile / a.g; }
+__device__ __forceinline__ int item_tiles(const PagedArgs& a, int n) { return (n + 2 * tile_tokens(a) - 1) / (2 * tile_tokens(a)); }
+// Blocks of 128 keys that the tokens up to `last` (exclusive) of a sequence see.
+__device__ __forceinline__ int blocks_of(const PagedSeq& q, int last) {
+  long long vis = q.pos0 + last;
   if (vis > q.kv) vis = q.kv;
-  const int n = vis <= 0 ? 0 : static_cast<int>((vis + kTile - 1) / kTile);
-  return n > floor ? n : floor;
+  return vis <= 0 ? 0 : static_cast<int>((static_cast<uint32_t>(vis) + kTile - 1) / kTile);
 }
-__device__ __forceinline__ int item_units(const PagedArgs& a, const PagedSeq& q, int nrows, int tile) {
-  return blocks_of(a, q, min(nrows, (tile + 1) * kItemRows), 1);
+// An item's units: its blocks (at least one) and kSetup more, what loading q, filling the pipeline and storing cost.
+constexpr int kSetup = 1;
+__device__ __forceinline__ int item_units(const PagedArgs& a, const PagedSeq& q, int tile) {
+  return kSetup + max(1, blocks_of(q, min(q.n, (tile + 1) * 2 * tile_tokens(a))));
 }
-__device__ __forceinline__ int item_tiles(int nrows) { return (nrows + kItemRows - 1) / kItemRows; }
 
 struct Scan {
   long long units[kScanSeqs];  // of one kv head, per sequence of the block at hand
@@ -125,31 +128,20 @@ struct Scan {
   int seq;
 };
 
-// units[] of the sequences s0 .. s0 + kScanSeqs; called by all threads, ends with a barrier.
+// units[] of the sequences s0 .. s0 + kScanSeqs: 8 lanes per sequence; called by all threads, ends with a barrier.
 template <int kN>
 __device__ void scan_units(const PagedArgs& a, Scan& sc, int s0) {
-  const int count = min(kScanSeqs, a.seqs - s0), lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < count; i += kN) {
-    const PagedSeq q = paged_seq(a, s0 + i);
-    const int nrows = q.n * a.g, nt = item_tiles(nrows);
+  const int count = min(kScanSeqs, a.seqs - s0), sub = threadIdx.x & 7;
+  for (int i = threadIdx.x / 8; i - (threadIdx.x & 31) / 8 < count; i += kN / 8) {
     long long u = 0;
-    if (nt > 16)
-      u = -1;  // a warp's work
-    else
-      for (int t = 0; t < nt; ++t) u += item_units(a, q, nrows, t);
-    sc.units[i] = u;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x / 32; i < count; i += kN / 32) {
-    if (sc.units[i] >= 0) continue;
-    const PagedSeq q = paged_seq(a, s0 + i);
-    const int nrows = q.n * a.g, nt = item_tiles(nrows);
-    long long u = 0;
-    for (int t = lane; t < nt; t += 32) u += item_units(a, q, nrows, t);
+    if (i < count) {
+      const PagedSeq q = paged_seq(a, s0 + i);
+      const int nt = item_tiles(a, q.n);
+      for (int t = sub; t < nt; t += 8) u += item_units(a, q, t);
+    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(kPagedFull, u, o);
-    __syncwarp();
-    if (lane == 0) sc.units[i] = u;
+    for (int o = 4; o > 0; o >>= 1) u += __shfl_xor_sync(kPagedFull, u, o);
+    if (i < count && sub == 0) sc.units[i] = u;
   }
   __syncthreads();
 }
@@ -227,55 +219,60 @@ __device__ void scan_find(const PagedArgs& a, Scan& sc, long long u) {
 // A CTA's walk over its units: one segment (a range of key blocks of one item) at a time. Every role walks by itself.
 struct Walk {
   PagedSeq q;
-  int s, h, tile, nrows, tiles;
+  int s, h, tile, tiles;
   int off, end, per;        // the segment's blocks, the item's
-  int blocks[2];            // what each 128-row tile sees of the item
+  int blocks[2];            // what each tile sees of the item
   long long left;           // units of the CTA after this segment
 
-  __device__ __forceinline__ void item(const PagedArgs& a) {
-    per = item_units(a, q, nrows, tile);
-    const int r0 = tile * kItemRows;
-    blocks[0] = blocks_of(a, q, min(nrows, r0 + kTile), 0);
-    blocks[1] = nrows > r0 + kTile ? blocks_of(a, q, min(nrows, r0 + kItemRows), 0) : 0;
-  }
   __device__ __forceinline__ void enter(const PagedArgs& a) {
     q = paged_seq(a, s);
-    nrows = q.n * a.g;
-    tiles = item_tiles(nrows);
+    tiles = item_tiles(a, q.n);
   }
-  // `rel`: units behind the start of sequence `seq`, each kv head of which has `head` units
-  __device__ void start(const PagedArgs& a, int seq, long long rel, long long head, long long count) {
+  // the units [v0, v1) of the item are the CTA's
+  __device__ __forceinline__ void segment(const PagedArgs& a, int v0, int v1) {
+    const int t0 = tile * 2 * tile_tokens(a), t1 = t0 + tile_tokens(a);
+    blocks[0] = blocks_of(q, min(q.n, t1));
+    blocks[1] = q.n > t1 ? blocks_of(q, min(q.n, t1 + tile_tokens(a))) : 0;
+    off = max(v0 - kSetup, 0);
+    end = max(v1 - kSetup, 0);
+  }
+  // `rel`: units behind the start of sequence `seq`, each kv head of which has `head` units. False: nothing to do.
+  __device__ bool start(const PagedArgs& a, int seq, long long rel, long long head, long long count) {
     s = seq;
     enter(a);
     h = static_cast<int>(rel / head);
     long long r = rel % head;
+    int n;
     for (tile = 0;; ++tile) {
-      const int n = item_units(a, q, nrows, tile);
+      n = item_units(a, q, tile);
       if (r < n) break;
       r -= n;
     }
-    item(a);
-    off = static_cast<int>(r);
-    end = static_cast<int>(per - off < count ? per : off + count);
-    left = count - (end - off);
+    per = n - kSetup;
+    const int v0 = static_cast<int>(r), v1 = static_cast<int>(n - v0 < count ? n : v0 + count);
+    segment(a, v0, v1);
+    left = count - (v1 - v0);
+    return off < end || next(a);
   }
   __device__ bool next(const PagedArgs& a) {
-    if (left <= 0) return false;
-    if (++tile == tiles) {
-      tile = 0;
-      if (++h == a.nkv) {
-        h = 0;
-        do {
-          ++s;
-          enter(a);
-        } while (nrows == 0);
+    while (left > 0) {
+      if (++tile == tiles) {
+        tile = 0;
+        if (++h == a.nkv) {
+          h = 0;
+          do {
+            ++s;
+            enter(a);
+          } while (q.n == 0);
+        }
       }
+      const int n = item_units(a, q, tile), v1 = static_cast<int>(n < left ? n : left);
+      per = n - kSetup;
+      segment(a, 0, v1);
+      left -= v1;
+      if (off < end) return true;  // (the share may end in an item's setup: nothing of it is done here)
     }
-    item(a);
-    off = 0;
-    end = static_cast<int>(per < left ? per : left);
-    left -= end;
-    return true;
+    return false;
   }
   // blocks [off, until(i)) of the segment are tile i's
   __device__ __forceinline__ int until(int i) const { return min(end, blocks[i]); }
@@ -286,7 +283,7 @@ struct Smem {
   static constexpr int kTileBytes = kTile * HD * 2;
   uint8_t q[2][kTileBytes];
   uint8_t kv[kSlots][kTileBytes];
-  uint64_t full[kSlots], empty[kSlots], q_full[2], s_full[2], p_full[2][2], o_done[2], tail_go, tail, mma_done;
+  uint64_t full[kSlots], empty[kSlots], q_full[2], q_done[2], s_full[2], p_full[2][2], o_done[2], tail_go, tail, mma_done;
   int bad[kBadRing];
   uint32_t tmem_base;
   int abort;
@@ -329,7 +326,8 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1)
-    paged_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const PagedArgs a) {
+    paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                    const __grid_constant__ CUtensorMap tv, const PagedArgs a) {
   constexpr int kHalf = kTile * 128;  // bytes of 64 head dimensions of a tile
   constexpr int kTileBytes = Smem<HD>::kTileBytes;
   extern __shared__ uint8_t smem_raw[];
@@ -346,7 +344,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&s.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s.q_full[i], kTile);
+      mbar_init(&s.q_full[i], 1);
+      mbar_init(&s.q_done[i], 1);
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.p_full[i][0], 4);
       mbar_init(&s.p_full[i][1], 4);
@@ -357,6 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&s.mma_done, 1);
     s.abort = 0;
     mbar_fence_init();
+    tma_prefetch_desc(&tq);
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tv);
   }
@@ -384,14 +384,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < kSmWarp0) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
     if (warp == 0 && work) {
-      // ---- pages and TMA: K(b), V(b) per block, alternating in the ring ----
+      // ---- pages and TMA: K(b), V(b) per block, alternating in the ring; q behind a segment's first K ----
       Walk w;
-      w.start(a, seq0, rel0, head0, count);
       const int rows_per = min(1 << a.page_log2, kTile), np = kTile / rows_per;  // rows and boxes per block
       const int mask = (1 << a.page_log2) - 1, none = a.num_pages << a.page_log2;
-      int t = 0, issued = 0;  // blocks, slots
+      const uint32_t q_bytes = static_cast<uint32_t>(tile_tokens(a) * a.g) * (HD * 2);
+      int t = 0, issued = 0;      // blocks, ring tiles
+      uint32_t qn[2] = {0, 0};    // q tiles loaded
       bool ok = true;
-      do {
+      for (bool more = w.start(a, seq0, rel0, head0, count); more && ok; more = w.next(a)) {
         const int* table = a.pages + static_cast<long long>(w.s) * a.ld_pages;
         for (int b = w.off; b < w.end && ok; ++b, ++t) {
           const int key = b * kTile + lane * rows_per;
@@ -420,11 +421,29 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tma_load_3d(s.kv[slot] + c * kHalf + lane * rows_per * 128, kv == 0 ? &tk : &tv, &s.full[slot], c * 64, row, w.h);
             }
             __syncwarp();
+            if (kv == 0 && b == w.off) {
+              if (lane == 0) {
+                for (int i = 0; i < 2 && go; ++i) {
+                  if (w.until(i) <= w.off) continue;
+                  if (qn[i] > 0) go = mbar_wait(&s.q_done[i], (qn[i] + 1) & 1u, abort);  // its last scores are issued
+                  if (!go) break;
+                  ++qn[i];
+                  mbar_arrive_expect_tx(&s.q_full[i], q_bytes);
+                  for (int c = 0; c < HD / 64; ++c)
+                    tma_load_3d(s.q[i] + c * kHalf, &tq, &s.q_full[i], c * 64, w.h * a.g,
+                                w.q.first + (2 * w.tile + i) * tile_tokens(a));
+                }
+              }
+              ok = __shfl_sync(kPagedFull, go, 0) != 0;
+            }
           }
         }
-      } while (ok && w.next(a));
-      if (lane == 0)
+      }
+      if (lane == 0) {
         for (int i = 0; i < kSlots && i < issued; ++i) wait_drain(&s.full[i], static_cast<uint32_t>((issued - 1 - i) / kSlots) & 1u);
+        for (int i = 0; i < 2; ++i)
+          if (qn[i] > 0) wait_drain(&s.q_full[i], (qn[i] + 1) & 1u);
+      }
     } else if (warp == 1 && work) {
       // ---- MMA: one thread, from wait to wait as short as it can be written ----
       if (lane == 0) {
@@ -465,11 +484,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             output_of(i, 1, half, more);
         };
         Walk w;
-        w.start(a, seq0, rel0, head0, count);
         int blk = 0;  // blocks so far: K of block blk is tile 2 blk of the ring, V tile 2 blk + 1
         uint32_t seg[2] = {0, 0}, pn[2] = {0, 0}, tails = 0;  // phases: q_full and p_full per tile, tail
         bool ok = true;
-        do {
+        for (bool on = w.start(a, seq0, rel0, head0, count); on && ok; on = w.next(a)) {
           const int un[2] = {w.until(0), w.until(1)};
 #pragma unroll
           for (int i = 0; i < 2; ++i)
@@ -479,7 +497,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after_sync();
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            if (un[i] > w.off) scores(i, blk);
+            if (un[i] > w.off) {
+              scores(i, blk);
+              if (w.off + 1 == un[i]) umma_commit(&s.q_done[i]);
+            }
           umma_commit(&s.empty[(2 * blk) & 3]);
           for (int b = w.off; b < w.end; ++b, ++blk) {
             const bool more = b + 1 < w.end;
@@ -507,6 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   have_k = true;
                   tc_fence_after_sync();
                   scores(i, blk + 1);
+                  if (b + 2 == un[i]) umma_commit(&s.q_done[i]);
                 }
               }
             }
@@ -514,18 +536,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             umma_commit(&s.empty[(2 * blk + 1) & 3]);
             if (more) umma_commit(&s.empty[(2 * blk + 2) & 3]);
           }
-        } while (ok && w.next(a));
+        }
         umma_commit(&s.mma_done);
         wait_drain(&s.mma_done, 0);
       }
     } else if (warp == 2 && work) {
       // ---- the last block of a sequence: values past its end may be NaN, which p = 0 does not hide ----
       Walk w;
-      w.start(a, seq0, rel0, head0, count);
       int blk = 0;
       uint32_t tails = 0;
       bool ok = true;
-      do {
+      for (bool on = w.start(a, seq0, rel0, head0, count); on && ok; on = w.next(a)) {
         for (int b = w.off; b < w.end && ok; ++b, ++blk) {
           const int valid = w.q.kv - b * kTile;
           if (valid >= kTile) continue;
@@ -542,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           fence_async_shared();
           mbar_arrive(&s.tail);
         }
-      } while (ok && w.next(a));
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
@@ -553,26 +574,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t ts = tmem + lanes + i * kTile, to = tmem + lanes + 2 * kTile + i * kTile;
       const float sc = a.scale_log2;
       Walk w;
-      w.start(a, seq0, rel0, head0, count);
       int n = 0, t0 = 0;  // blocks of this tile so far; blocks of the CTA before the segment
       bool ok = true;
-      do {
-        const int until = w.until(i), pr = w.tile * kItemRows + i * kTile + r;  // packed row
-        const bool live = pr < w.nrows;
-        const int tok = live ? pr / a.g : 0, head = w.h * a.g + (live ? pr % a.g : 0);
+      const int rt = r / a.g, rh = r % a.g;
+      for (bool on = w.start(a, seq0, rel0, head0, count); on && ok; on = w.next(a)) {
+        const int until = w.until(i), token = (2 * w.tile + i) * tile_tokens(a) + rt;
+        const bool live = rt < tile_tokens(a) && token < w.q.n;
+        const int tok = live ? token : 0, head = w.h * a.g + rh;
         float m = -INFINITY, l = 0.0f;
         int bad = w.q.bad;
         const long long pos = live ? w.q.pos0 + tok : -1;
         const long long vis = pos + 1 < w.q.kv ? pos + 1 : w.q.kv;  // visible keys
         if (until > w.off) {
-          // q into shared memory, K-major with the 128-byte swizzle
-          const __nv_bfloat16* src = a.q + static_cast<long long>(w.q.first + tok) * a.ldq + head * HD;
-#pragma unroll
-          for (int c = 0; c < HD / 8; ++c)
-            *reinterpret_cast<uint4*>(s.q[i] + (c / 8) * kHalf + r * 128 + (((c % 8) ^ (r & 7)) * 16)) =
-                live ? ldg16(src + c * 8) : make_uint4(0, 0, 0, 0);
-          fence_async_shared();
-          mbar_arrive(&s.q_full[i]);
           for (int b = w.off; b < until; ++b, ++n) {
             ok = mbar_wait(&s.s_full[i], static_cast<uint32_t>(n) & 1u, abort);
             if (!__all_sync(kPagedFull, ok)) {
@@ -688,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_before_sync();
         t0 += w.end - w.off;
-      } while (w.next(a));
+      }
     }
   }
   tc_fence_before_sync();
@@ -712,16 +725,26 @@ __global__ void __launch_bounds__(kJoinThreads) paged_tc_join_kernel(const Paged
   if (u >= sc.total) return;
   scan_find<kJoinThreads>(a, sc, u - 1);
   __syncthreads();
-  Walk w;
-  w.start(a, sc.seq, u - 1 - sc.before, sc.units[sc.seq % kScanSeqs], 1);
-  const long long first = u - 1 - w.off, last = first + w.per - 1;  // the item's units
-  if (first < c * share || last < u) return;
+  // the item of the share's last unit, if its block 0 is in this share and its last block is not
+  const PagedSeq q = paged_seq(a, sc.seq);
+  const long long head = sc.units[sc.seq % kScanSeqs], rel = u - 1 - sc.before;
+  const int h = static_cast<int>(rel / head);
+  long long r = rel % head;
+  int tile = 0, n;
+  for (;; ++tile) {
+    n = item_units(a, q, tile);
+    if (r < n) break;
+    r -= n;
+  }
+  const long long first = u - 1 - r + kSetup, last = first + n - kSetup - 1;  // the item's blocks as units
+  if (first < c * share || first >= u || last < u) return;
   const int c1 = static_cast<int>(last / share);
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
   constexpr int kPer = HD / 32;
   for (int k = 0; k < 4; ++k) {
-    const int row = blockIdx.y * 32 + warp * 4 + k, pr = w.tile * kItemRows + row;
-    if (pr >= w.nrows) return;
+    const int row = blockIdx.y * 32 + warp * 4 + k;
+    const int rt = (row % kTile) / a.g, token = (2 * tile + row / kTile) * tile_tokens(a) + rt;
+    if (rt >= tile_tokens(a) || token >= q.n) continue;
     float m = -INFINITY;
     for (int d = c + lane; d <= c1; d += 32) m = fmaxf(m, ml[static_cast<size_t>(2 * d + (d == c)) * kItemRows + row].x);
 #pragma unroll
@@ -744,7 +767,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_tc_join_kernel(const Paged
       for (int j = 0; j < kPer; ++j) acc[j] = fmaf(f, src[j], acc[j]);
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    __nv_bfloat16* dst = a.out + static_cast<long long>(w.q.first + pr / a.g) * a.ldo + (w.h * a.g + pr % a.g) * HD + lane * kPer;
+    __nv_bfloat16* dst = a.out + static_cast<long long>(q.first + token) * a.ldo + (h * a.g + (row % kTile) % a.g) * HD + lane * kPer;
 #pragma unroll
     for (int j = 0; j < kPer; j += 2) *reinterpret_cast<uint32_t*>(dst + j) = pack2(acc[j] * inv, acc[j + 1] * inv);
   }
@@ -768,11 +791,17 @@ int launch(PagedArgs a, cudaStream_t stream) {
   }
   const int ps = 1 << a.page_log2;
   const uint64_t rows = static_cast<uint64_t>(a.num_pages) << a.page_log2;
-  CUtensorMap tk, tv;
+  CUtensorMap tq, tk, tv;
+  const uint64_t qdims[3] = {HD, static_cast<uint64_t>(a.nh), static_cast<uint64_t>(a.rows)};
+  const uint64_t qstrides[2] = {HD * 2, static_cast<uint64_t>(a.ldq) * 2};
+  const uint32_t qbox[3] = {64, static_cast<uint32_t>(a.g), static_cast<uint32_t>(kTile / a.g)};
+  int st = tc_encode(&tq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.q, qdims, qstrides, qbox, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
+  if (st != BP_OK) return st;
   const uint64_t dims[3] = {HD, rows, static_cast<uint64_t>(a.nkv)};
   const uint64_t strides[2] = {static_cast<uint64_t>(a.nkv) * HD * 2, HD * 2};
   const uint32_t box[3] = {64, static_cast<uint32_t>(ps < kTile ? ps : kTile), 1};
-  int st = tc_encode(&tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.kp, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+  st = tc_encode(&tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.kp, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
   if (st != BP_OK) return st;
   st = tc_encode(&tv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.vp, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -785,7 +814,7 @@ int launch(PagedArgs a, cudaStream_t stream) {
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   set_launch_attrs(cfg, attr);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, paged_tc_kernel<HD>, tk, tv, a);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, paged_tc_kernel<HD>, tq, tk, tv, a);
   if (e == cudaSuccess && a.G > 1) {
     cfg.gridDim = dim3(a.G - 1, kItemRows / 32);
     cfg.blockDim = dim3(kJoinThreads);
@@ -804,7 +833,7 @@ size_t paged_tc_workspace_bytes(int hd) {
 
 int launch_paged_tc(PagedArgs a, void* workspace, cudaStream_t stream) {
   a.G = tc_sm_count();
-  a.min_share = 4;  // a part costs its write and its join: as much as about two blocks
+  a.min_share = 4;  // a part costs its write and its join
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + static_cast<size_t>(2 * a.G) * kItemRows * a.hd;
   return a.hd == 128 ? launch<128>(a, stream) : launch<64>(a, stream);
