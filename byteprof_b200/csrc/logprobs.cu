@@ -7,16 +7,20 @@
 //   m = max x, R = sum over all but one instance of the maximum of exp(x - m), T = sum exp(x - m) (m - x):
 //   lse = m + log1p(R), logprob = x_id - lse, entropy = log1p(R) + T / (1 + R).
 // R leaves the maximum's own term (1) out, so a row whose probability is all on one token keeps the small
-// rest that 1 + R would round away. Two parts merge as (m1 >= m2, f = exp(m2 - m1)):
+// rest that 1 + R would round away. A thread sets its largest value so far aside without a branch: of (largest,
+// new value) the smaller one goes into the sums, taken relative to a reference that moves only when the largest
+// exceeds it by kLazy. (Moving it with every new maximum costs a rescale whenever any of 32 lanes has one, which is
+// at nearly every vector of a row.) Two parts merge as (m1 >= m2, f = exp(m2 - m1)):
 //   R = R1 + f (1 + R2), T = T1 + f (T2 + (m1 - m2)(1 + R2)).
-// An empty part is m = -FLT_MAX, R = -1 (a total of 0). All of it in fp32, over short chains (a thread's share).
+// All of it in fp32, over short chains (a thread's share).
 //
-// Top alternatives: each warp keeps its best `top` (value, index) sorted across its lanes; a vector of logits
-// is looked at only when its maximum reaches the warp's last entry, so after the first few hundred values
-// almost none are. Order: larger value first, NaN as the largest, the lower index among equals.
+// Top alternatives: values are looked at in the order of 64-bit keys (value, then lower index), each warp keeps its
+// best 32 sorted across its lanes, and vectors whose maximum reaches the last wanted entry put their candidates
+// into a buffer of the warp; 32 of them are sorted and merged at once (20 steps of a bitonic network, where
+// inserting them one by one took 150 clocks each: 50 us for one row of 100352 with 20 alternatives).
 //
 // Memory bound: rows * vocab values read once. One warp per row for short rows, one CTA or a cluster of up
-// to 8 CTAs for long ones, merged in rank order (deterministic).
+// to 8 CTAs for long ones, merged in a fixed order (deterministic).
 #include <float.h>
 
 #include "bp_common.cuh"
@@ -38,28 +42,52 @@ __device__ __forceinline__ float ex2(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
-struct Stat {
-  float m, r, t;
-  __device__ __forceinline__ void init() { m = -FLT_MAX, r = -1.0f, t = 0.0f; }
-  // adds one value that is not the implicit maximum (x <= m, or NaN)
+constexpr float kLazy = 4.0f;
+
+// A thread's running sums: mx, the largest value, is in neither of s = sum exp(x - ref), t = sum exp(x - ref)(ref - x).
+struct Run {
+  float mx, ref, s, t;
+  __device__ __forceinline__ void init() { mx = -INFINITY, ref = -FLT_MAX, s = 0.0f, t = 0.0f; }
   __device__ __forceinline__ void add(float x) {
-    const float d = m - x;
-    const float e = ex2(d * -kLog2e);
-    r += e;
+    const float lo = min_nan(mx, x);
+    mx = max_nan(mx, x);
+    const float d = ref - lo, e = ex2(d * -kLog2e);
+    s += e;
     t = fmaf(e, fminf(d, 1e30f), t);  // -inf: e = 0, and 0 * inf would be NaN
   }
-  // raises the maximum to vm > m: the old part joins the rest
-  __device__ __forceinline__ void raise(float vm) {
-    const float n = r + 1.0f, f = ex2((m - vm) * kLog2e);
-    if (n == 0.0f || f == 0.0f) {
-      r = isnan(n) ? n : 0.0f;
-      t = 0.0f;
-    } else {
-      r = n * f;
-      t = (t + n * (vm - m)) * f;
+  // before values up to vm are added
+  __device__ __forceinline__ void make_room(float vm) {
+    if (vm > ref + kLazy) move(vm);
+  }
+  __device__ __forceinline__ void move(float to) {
+    const float f = ex2((ref - to) * kLog2e);
+    t = f == 0.0f ? 0.0f : (t + s * (to - ref)) * f;
+    s *= f;
+    ref = to;
+  }
+};
+
+// A finished part: R and T as above, relative to m; m = -inf: nothing, NaN: a NaN was seen.
+struct Stat {
+  float m, r, t;
+  __device__ __forceinline__ void from(Run a) {
+    m = a.mx;
+    r = t = 0.0f;
+    if (a.mx > -INFINITY) {
+      a.move(a.mx);
+      r = a.s, t = a.t;
     }
-    m = vm;
   }
   __device__ __forceinline__ void merge(float m2, float r2, float t2) {
     if (m2 > m) {
@@ -67,50 +95,82 @@ struct Stat {
       m = m2, r = r2, t = t2;
       m2 = a, r2 = b, t2 = c;
     }
-    const float n = r2 + 1.0f, f = m2 == m ? 1.0f : ex2((m2 - m) * kLog2e);
-    if (n == 0.0f) return;
-    if (f == 0.0f) {
-      if (isnan(n)) r = n;
-      return;
+    const float f = m2 == m ? (m2 > -INFINITY ? 1.0f : 0.0f) : ex2((m2 - m) * kLog2e);
+    if (f > 0.0f) {
+      r += f * (1.0f + r2);
+      t += f * (t2 + (m - m2) * (1.0f + r2));
     }
-    r += f * n;
-    t += f * (t2 + (m - m2) * n);
+    m = max_nan(m, m2);
   }
 };
 
-// torch order: NaN is the largest value; the lower index wins among equals.
-__device__ __forceinline__ bool better(float a, int ia, float b, int ib) {
-  const bool na = isnan(a), nb = isnan(b);
-  if (na || nb) return na && (!nb || ia < ib);
-  return a > b || (a == b && ia < ib);
+// ---- top alternatives -------------------------------------------------------------------------------------
+// Keys in torch's order: NaN is the largest value, the lower index wins among equals (and -0 equals 0). 0: none.
+__device__ __forceinline__ unsigned long long key_of(float x, int i) {
+  x += 0.0f;
+  const uint32_t u = __float_as_uint(x);
+  const uint32_t o = isnan(x) ? 0xffffffffu : u ^ (static_cast<int>(u) < 0 ? 0xffffffffu : 0x80000000u);
+  return static_cast<unsigned long long>(o) << 32 | ~static_cast<uint32_t>(i);
+}
+__device__ __forceinline__ float key_value(unsigned long long k) {
+  const uint32_t o = static_cast<uint32_t>(k >> 32);
+  return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+__device__ __forceinline__ int key_index(unsigned long long k) { return static_cast<int>(~static_cast<uint32_t>(k)); }
+
+__device__ __forceinline__ unsigned long long exchange(unsigned long long k, int lane, int stride, bool down) {
+  const unsigned long long o = __shfl_xor_sync(kFull, k, stride);
+  return ((lane & stride) == 0) == down ? (k > o ? k : o) : (k < o ? k : o);
+}
+// The larger 32 of two lists sorted downwards across the lanes, sorted.
+__device__ __forceinline__ unsigned long long merge_sorted(unsigned long long a, unsigned long long b, int lane) {
+  const unsigned long long r = __shfl_sync(kFull, b, 31 - lane);
+  unsigned long long k = a > r ? a : r;
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) k = exchange(k, lane, s, true);
+  return k;
+}
+__device__ __forceinline__ unsigned long long sort_down(unsigned long long k, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int s = size >> 1; s > 0; s >>= 1) k = exchange(k, lane, s, (lane & size) == 0 || size == 32);
+  return k;
 }
 
-// A warp's sorted list: lane l holds the l-th best so far (index INT_MAX: none).
+constexpr int kBuf = 64;  // a warp's candidates: up to 31 waiting and 32 more
 struct TopList {
-  float v;
-  int i;
-  float thr;  // the last wanted entry
-  int thr_i;
-  __device__ __forceinline__ void init() { v = -INFINITY, i = 0x7fffffff, thr = -INFINITY, thr_i = 0x7fffffff; }
-  __device__ __forceinline__ void insert(float x, int ix, int top, int lane) {
-    const int pos = __popc(__ballot_sync(kFull, lane < top && better(v, i, x, ix)));
-    const float pv = __shfl_up_sync(kFull, v, 1);
-    const int pi = __shfl_up_sync(kFull, i, 1);
-    if (lane > pos) v = pv, i = pi;
-    if (lane == pos) v = x, i = ix;
-    thr = __shfl_sync(kFull, v, top - 1);
-    thr_i = __shfl_sync(kFull, i, top - 1);
+  unsigned long long list;       // lane l: the l-th best so far
+  unsigned long long thr;        // the last wanted entry
+  float thr_v;
+  int waiting;
+  unsigned long long* buf;
+  __device__ __forceinline__ void init(unsigned long long* b) { list = 0, thr = 0, thr_v = -INFINITY, waiting = 0, buf = b; }
+  __device__ __forceinline__ void join(unsigned long long sorted, int top, int lane) {
+    list = merge_sorted(list, sorted, lane);
+    thr = __shfl_sync(kFull, list, top - 1);
+    thr_v = thr == 0 ? -INFINITY : key_value(thr);
   }
   // every lane offers one value (or none)
   __device__ __forceinline__ void offer(float x, int ix, bool valid, int top, int lane) {
-    unsigned mask = __ballot_sync(kFull, valid && better(x, ix, thr, thr_i));
-    while (mask != 0) {
-      const int src = __ffs(mask) - 1;
-      mask &= mask - 1;
-      const float bx = __shfl_sync(kFull, x, src);
-      const int bi = __shfl_sync(kFull, ix, src);
-      if (better(bx, bi, thr, thr_i)) insert(bx, bi, top, lane);
-    }
+    const unsigned long long k = valid ? key_of(x, ix) : 0;
+    const unsigned mask = __ballot_sync(kFull, k > thr);
+    if (mask == 0) return;
+    if (k > thr) buf[waiting + __popc(mask & ((1u << lane) - 1))] = k;
+    waiting += __popc(mask);
+    if (waiting >= 32) flush(top, lane);
+  }
+  __device__ __forceinline__ void flush(int top, int lane) {
+    __syncwarp();
+    const unsigned long long k = lane < waiting ? buf[lane] : 0, rest = 32 + lane < waiting ? buf[32 + lane] : 0;
+    __syncwarp();
+    join(sort_down(k, lane), top, lane);
+    buf[lane] = rest;
+    waiting = waiting > 32 ? waiting - 32 : 0;
+    __syncwarp();
+  }
+  __device__ __forceinline__ void finish(int top, int lane) {
+    if (waiting > 0) flush(top, lane);
   }
 };
 
@@ -137,40 +197,33 @@ struct Vec<__nv_bfloat16> {
 };
 
 template <int N>
-__device__ __forceinline__ void take(const float (&f)[N], int at, Stat& st, TopList& tl, int top, int lane, bool valid) {
+__device__ __forceinline__ void take(const float (&f)[N], int at, Run& st, TopList& tl, int top, int lane, bool valid) {
   float vm = f[0];
 #pragma unroll
   for (int j = 1; j < N; ++j) vm = fmaxf(vm, f[j]);
   if (valid) {
-    if (vm > st.m) {
-      st.raise(vm);
-      bool skipped = false;
+    st.make_room(vm);
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        if (!skipped && f[j] == vm)
-          skipped = true;
-        else
-          st.add(f[j]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < N; ++j) st.add(f[j]);
-    }
+    for (int j = 0; j < N; ++j) st.add(f[j]);
   }
-  if (top > 0 && __any_sync(kFull, valid && vm >= tl.thr)) {
-#pragma unroll 1
-    for (int j = 0; j < N; ++j) {
+  if (top > 0 && __any_sync(kFull, valid && vm >= tl.thr_v)) {
+    unsigned hits = 0;  // this lane's candidates
+#pragma unroll
+    for (int j = 0; j < N; ++j) hits |= (valid && f[j] >= tl.thr_v ? 1u : 0u) << j;
+    while (__any_sync(kFull, hits != 0)) {
+      const int j = __ffs(hits) - 1;
       float x = f[0];
 #pragma unroll
       for (int k = 1; k < N; ++k) x = j == k ? f[k] : x;
-      tl.offer(x, at + j, valid, top, lane);
+      tl.offer(x, at + j, hits != 0, top, lane);
+      hits &= hits - 1;
     }
   }
 }
 
 // Elements [lo, hi) of a row by the `n` threads (whole warps) of a team, thread id `tid`.
 template <typename T>
-__device__ __forceinline__ void scan(const T* x, int lo, int hi, int tid, int n, Stat& st, TopList& tl, int top, int lane) {
+__device__ __forceinline__ void scan(const T* x, int lo, int hi, int tid, int n, Run& st, TopList& tl, int top, int lane) {
   constexpr int N = Vec<T>::N;
   constexpr int U = 4;
   const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(x + lo) & 15u) / sizeof(T));
@@ -218,11 +271,12 @@ struct LpArgs {
 // The full row once more with every value compared: rows holding NaN, whose vector maxima do not show it.
 template <typename T>
 __device__ __noinline__ void rescan_top(const T* x, int vocab, TopList& tl, int top, int lane) {
-  tl.init();
+  tl.init(tl.buf);
   for (int b = 0; b < vocab; b += 32) {
     const bool valid = b + lane < vocab;
     tl.offer(valid ? Vec<T>::one(x + b + lane) : 0.0f, b + lane, valid, top, lane);
   }
+  tl.finish(top, lane);
 }
 
 // The row's results, by one warp that holds its merged state and list.
@@ -233,7 +287,7 @@ __device__ __forceinline__ void finish(const LpArgs& a, int row, const T* x, Sta
   st.r = __shfl_sync(kFull, st.r, 0);
   st.t = __shfl_sync(kFull, st.t, 0);
   const float lr = log1pf(st.r);
-  const bool bad = isnan(st.r) || st.m == INFINITY || st.r < 0.0f;  // NaN or +inf in the row, or nothing above -inf
+  const bool bad = !(fabsf(st.m) < INFINITY);  // NaN or +inf in the row, or nothing above -inf
   if (lane == 0) {
     const long long id = a.ids == nullptr ? -1 : a.ids[row];
     if (a.lp != nullptr)
@@ -243,8 +297,8 @@ __device__ __forceinline__ void finish(const LpArgs& a, int row, const T* x, Sta
   if (a.top > 0) {
     if (bad) rescan_top(x, a.vocab, tl, a.top, lane);
     if (lane < a.top) {
-      a.top_lp[static_cast<long long>(row) * a.top + lane] = bad ? nan : (tl.v - st.m) - lr;
-      a.top_id[static_cast<long long>(row) * a.top + lane] = tl.i;
+      a.top_lp[static_cast<long long>(row) * a.top + lane] = bad ? nan : (key_value(tl.list) - st.m) - lr;
+      a.top_id[static_cast<long long>(row) * a.top + lane] = key_index(tl.list);
     }
   }
 }
@@ -259,16 +313,20 @@ __device__ __forceinline__ void warp_merge(Stat& st) {
 
 template <typename T>
 __global__ void __launch_bounds__(kWarpRowThreads) logprobs_warp_kernel(const LpArgs a) {
+  __shared__ unsigned long long buf[kWarpRowThreads / 32][kBuf];
   pdl_launch_dependents();
   pdl_wait_prior_grids();
   const int lane = threadIdx.x & 31, row = blockIdx.x * (kWarpRowThreads / 32) + (threadIdx.x >> 5);
   if (row >= a.rows) return;
   const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+  Run run;
   Stat st;
   TopList tl;
-  st.init();
-  tl.init();
-  scan(x, 0, a.vocab, lane, 32, st, tl, a.top, lane);
+  run.init();
+  tl.init(buf[threadIdx.x >> 5]);
+  scan(x, 0, a.vocab, lane, 32, run, tl, a.top, lane);
+  tl.finish(a.top, lane);
+  st.from(run);
   warp_merge(st);
   finish(a, row, x, st, tl, lane);
 }
@@ -277,11 +335,10 @@ template <typename T>
 __global__ void __launch_bounds__(kRowThreads) logprobs_row_kernel(const LpArgs a) {
   constexpr int kWarps = kRowThreads / 32;
   __shared__ float sm[kWarps], sr[kWarps], stt[kWarps];
-  __shared__ float lv[kWarps][kMaxTop];
-  __shared__ int li[kWarps][kMaxTop];
+  __shared__ unsigned long long buf[kWarps][kBuf];
+  __shared__ unsigned long long lists[kWarps][32];
   __shared__ float cm[kMaxCluster], cr[kMaxCluster], ct[kMaxCluster];  // the leader's slots, one per CTA
-  __shared__ float cv[kMaxCluster][kMaxTop];
-  __shared__ int ci[kMaxCluster][kMaxTop];
+  __shared__ unsigned long long cl[kMaxCluster][32];
   pdl_launch_dependents();
   if (gridDim.y > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // this CTA has started
   pdl_wait_prior_grids();
@@ -290,22 +347,32 @@ __global__ void __launch_bounds__(kRowThreads) logprobs_row_kernel(const LpArgs 
   const T* x = static_cast<const T*>(a.logits) + row * a.ld;
   const int part = (a.vocab + C - 1) / C;
   const int lo = rank * part < a.vocab ? rank * part : a.vocab, hi = lo + part < a.vocab ? lo + part : a.vocab;
+  Run run;
   Stat st;
   TopList tl;
-  st.init();
-  tl.init();
-  scan(x, lo, hi, tid, kRowThreads, st, tl, a.top, lane);
+  run.init();
+  tl.init(buf[warp]);
+  scan(x, lo, hi, tid, kRowThreads, run, tl, a.top, lane);
+  st.from(run);
   warp_merge(st);
   if (lane == 0) sm[warp] = st.m, sr[warp] = st.r, stt[warp] = st.t;
-  lv[warp][lane] = tl.v;
-  li[warp][lane] = tl.i;
-  __syncthreads();
+  if (a.top > 0) {
+    tl.finish(a.top, lane);
+    lists[warp][lane] = tl.list;
+    __syncthreads();
+#pragma unroll
+    for (int w = kWarps / 2; w > 0; w >>= 1) {  // pairs of warps' lists
+      if (warp < w) lists[warp][lane] = merge_sorted(lists[warp][lane], lists[warp + w][lane], lane);
+      __syncthreads();
+    }
+  } else {
+    __syncthreads();
+  }
   if (warp == 0) {
-    st.init();
+    st.m = -INFINITY, st.r = st.t = 0.0f;
     if (lane < kWarps) st.m = sm[lane], st.r = sr[lane], st.t = stt[lane];
     warp_merge(st);
-    if (a.top > 0)
-      for (int w = 1; w < kWarps; ++w) tl.offer(lv[w][lane], li[w][lane], lane < a.top && li[w][lane] != 0x7fffffff, a.top, lane);
+    tl.list = lists[0][lane];
   }
   if (C > 1) {
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // every CTA has started: its memory can be written
@@ -315,17 +382,16 @@ __global__ void __launch_bounds__(kRowThreads) logprobs_row_kernel(const LpArgs 
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_addr(&cr[rank]), 0)), "f"(st.r) : "memory");
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_addr(&ct[rank]), 0)), "f"(st.t) : "memory");
       }
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_addr(&cv[rank][lane]), 0)), "f"(tl.v) : "memory");
-      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(smem_addr(&ci[rank][lane]), 0)), "r"(tl.i) : "memory");
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapa_shared(smem_addr(&cl[rank][lane]), 0)), "l"(tl.list) : "memory");
     }
     cluster_sync_unaligned();  // every CTA's slot written and visible to the leader
     if (rank != 0) return;
     if (warp == 0) {
-      st.init();
+      st.m = -INFINITY, st.r = st.t = 0.0f;
       if (lane < C) st.m = cm[lane], st.r = cr[lane], st.t = ct[lane];
       warp_merge(st);
       if (a.top > 0)
-        for (int c = 1; c < C; ++c) tl.offer(cv[c][lane], ci[c][lane], lane < a.top && ci[c][lane] != 0x7fffffff, a.top, lane);
+        for (int c = 1; c < C; ++c) tl.list = merge_sorted(tl.list, cl[c][lane], lane);
     }
   }
   if (warp == 0) finish(a, row, x, st, tl, lane);
