@@ -53,18 +53,81 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return r;
 }
 
+__device__ __forceinline__ uint32_t max_nan2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t min_nan2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Two fp32 values in a register pair, and arithmetic on both at once.
+__device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float x2_lo(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float x2_hi(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 constexpr float kLazy = 4.0f;
 
-// A thread's running sums: mx, the largest value, is in neither of s = sum exp(x - ref), t = sum exp(x - ref)(ref - x).
+// The largest values so far of a thread's even and odd elements, set aside; `swap` returns what goes into the sums.
+template <typename T>
+struct Aside;
+template <>
+struct Aside<float> {
+  float a = -INFINITY, b = -INFINITY;
+  __device__ __forceinline__ uint64_t swap(float x, float y) {
+    const uint64_t lo = f32x2(min_nan(a, x), min_nan(b, y));
+    a = max_nan(a, x);
+    b = max_nan(b, y);
+    return lo;
+  }
+  __device__ __forceinline__ float even() const { return a; }
+  __device__ __forceinline__ float odd() const { return b; }
+};
+template <>
+struct Aside<__nv_bfloat16> {
+  uint32_t p = 0xff80ff80u;
+  __device__ __forceinline__ uint64_t swap(uint32_t w) {
+    const uint32_t lo = min_nan2(p, w);
+    p = max_nan2(p, w);
+    return f32x2(bf16lo(lo), bf16hi(lo));
+  }
+  __device__ __forceinline__ float even() const { return bf16lo(p); }
+  __device__ __forceinline__ float odd() const { return bf16hi(p); }
+};
+
+// A thread's running sums over what is not set aside, even and odd elements apart: s = sum exp(x - ref),
+// t = sum exp(x - ref)(ref - x).
+template <typename T>
 struct Run {
-  float mx, ref, s, t;
-  __device__ __forceinline__ void init() { mx = -INFINITY, ref = -FLT_MAX, s = 0.0f, t = 0.0f; }
-  __device__ __forceinline__ void add(float x) {
-    const float lo = min_nan(mx, x);
-    mx = max_nan(mx, x);
-    const float d = ref - lo, e = ex2(d * -kLog2e);
-    s += e;
-    t = fmaf(e, fminf(d, 1e30f), t);  // -inf: e = 0, and 0 * inf would be NaN
+  Aside<T> top;
+  float ref = -FLT_MAX;
+  uint64_t s = 0, t = 0;
+  __device__ __forceinline__ void add(uint64_t lo) {
+    const uint64_t d = fma2(lo, f32x2(-1.0f, -1.0f), f32x2(ref, ref)), y = mul2(d, f32x2(-kLog2e, -kLog2e));
+    const uint64_t e = f32x2(ex2(x2_lo(y)), ex2(x2_hi(y)));
+    s = add2(s, e);
+    t = fma2(e, f32x2(fminf(x2_lo(d), 1e30f), fminf(x2_hi(d), 1e30f)), t);  // -inf: e = 0, and 0 * inf would be NaN
   }
   // before values up to vm are added
   __device__ __forceinline__ void make_room(float vm) {
@@ -72,8 +135,9 @@ struct Run {
   }
   __device__ __forceinline__ void move(float to) {
     const float f = ex2((ref - to) * kLog2e);
-    t = f == 0.0f ? 0.0f : (t + s * (to - ref)) * f;
-    s *= f;
+    const uint64_t f2 = f32x2(f, f);
+    t = f == 0.0f ? 0 : mul2(fma2(s, f32x2(to - ref, to - ref), t), f2);
+    s = mul2(s, f2);
     ref = to;
   }
 };
@@ -81,12 +145,17 @@ struct Run {
 // A finished part: R and T as above, relative to m; m = -inf: nothing, NaN: a NaN was seen.
 struct Stat {
   float m, r, t;
-  __device__ __forceinline__ void from(Run a) {
-    m = a.mx;
+  template <typename T>
+  __device__ __forceinline__ void from(Run<T> a) {
+    const float e = a.top.even(), o = a.top.odd();
+    const float mx = fmaxf(e, o);
     r = t = 0.0f;
-    if (a.mx > -INFINITY) {
-      a.move(a.mx);
-      r = a.s, t = a.t;
+    if (mx > -INFINITY) a.move(mx);  // both sums relative to the larger of the two set aside
+    const float lo = fminf(e, o), f = mx > -INFINITY && lo > -INFINITY ? ex2((lo - mx) * kLog2e) : 0.0f;
+    m = max_nan(e, o);
+    if (mx > -INFINITY) {
+      r = x2_lo(a.s) + x2_hi(a.s) + f;  // the smaller one joins the rest
+      t = x2_lo(a.t) + x2_hi(a.t) + (f > 0.0f ? f * (mx - lo) : 0.0f);
     }
   }
   __device__ __forceinline__ void merge(float m2, float r2, float t2) {
@@ -149,7 +218,7 @@ struct TopList {
   __device__ __forceinline__ void join(unsigned long long sorted, int top, int lane) {
     list = merge_sorted(list, sorted, lane);
     thr = __shfl_sync(kFull, list, top - 1);
-    thr_v = thr == 0 ? -INFINITY : key_value(thr);
+    if (thr != 0) thr_v = fmaxf(thr_v, key_value(thr));  // (a first bound stays until the list reaches it)
   }
   // every lane offers one value (or none)
   __device__ __forceinline__ void offer(float x, int ix, bool valid, int top, int lane) {
@@ -179,81 +248,124 @@ struct Vec;
 template <>
 struct Vec<float> {
   static constexpr int N = 4;
-  __device__ static __forceinline__ void load(const float* p, float (&f)[4]) {
-    const float4 v = __ldcs(reinterpret_cast<const float4*>(p));
-    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
-  }
+  using Raw = float4;
+  __device__ static __forceinline__ Raw load(const float* p) { return __ldcs(reinterpret_cast<const float4*>(p)); }
+  __device__ static __forceinline__ Raw fill(float x) { return make_float4(x, -INFINITY, -INFINITY, -INFINITY); }
   __device__ static __forceinline__ float one(const float* p) { return *p; }
+  __device__ static __forceinline__ float at(const Raw& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
+  __device__ static __forceinline__ float largest(const Raw& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+  __device__ static __forceinline__ void add(const Raw& v, Run<float>& r) {
+    r.add(r.top.swap(v.x, v.y));
+    r.add(r.top.swap(v.z, v.w));
+  }
 };
 template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
-  __device__ static __forceinline__ void load(const __nv_bfloat16* p, float (&f)[8]) {
-    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
-    f[0] = bf16lo(v.x); f[1] = bf16hi(v.x); f[2] = bf16lo(v.y); f[3] = bf16hi(v.y);
-    f[4] = bf16lo(v.z); f[5] = bf16hi(v.z); f[6] = bf16lo(v.w); f[7] = bf16hi(v.w);
+  using Raw = uint4;
+  __device__ static __forceinline__ Raw load(const __nv_bfloat16* p) { return __ldcs(reinterpret_cast<const uint4*>(p)); }
+  __device__ static __forceinline__ Raw fill(float x) {
+    return make_uint4(0xff800000u | __float_as_uint(x) >> 16, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
   }
   __device__ static __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  __device__ static __forceinline__ float at(const Raw& v, int j) {
+    const uint32_t w = j < 4 ? (j < 2 ? v.x : v.y) : (j < 6 ? v.z : v.w);
+    return j & 1 ? bf16hi(w) : bf16lo(w);
+  }
+  __device__ static __forceinline__ float largest(const Raw& v) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  __device__ static __forceinline__ void add(const Raw& v, Run<__nv_bfloat16>& r) {
+    r.add(r.top.swap(v.x));
+    r.add(r.top.swap(v.y));
+    r.add(r.top.swap(v.z));
+    r.add(r.top.swap(v.w));
+  }
 };
 
-template <int N>
-__device__ __forceinline__ void take(const float (&f)[N], int at, Run& st, TopList& tl, int top, int lane, bool valid) {
-  float vm = f[0];
-#pragma unroll
-  for (int j = 1; j < N; ++j) vm = fmaxf(vm, f[j]);
-  if (valid) {
-    st.make_room(vm);
-#pragma unroll
-    for (int j = 0; j < N; ++j) st.add(f[j]);
-  }
-  if (top > 0 && __any_sync(kFull, valid && vm >= tl.thr_v)) {
+// One vector of each lane (elements at, at + 1, ..), -inf in the lanes that have none.
+template <typename T>
+__device__ __forceinline__ void take(const typename Vec<T>::Raw& v, int at, Run<T>& run, TopList& tl, int top, int lane, int valid) {
+  const float vm = Vec<T>::largest(v);
+  run.make_room(vm);
+  Vec<T>::add(v, run);
+  if (top > 0 && __any_sync(kFull, valid > 0 && vm >= tl.thr_v)) {
     unsigned hits = 0;  // this lane's candidates
 #pragma unroll
-    for (int j = 0; j < N; ++j) hits |= (valid && f[j] >= tl.thr_v ? 1u : 0u) << j;
+    for (int j = 0; j < Vec<T>::N; ++j) hits |= (j < valid && Vec<T>::at(v, j) >= tl.thr_v ? 1u : 0u) << j;
     while (__any_sync(kFull, hits != 0)) {
       const int j = __ffs(hits) - 1;
-      float x = f[0];
-#pragma unroll
-      for (int k = 1; k < N; ++k) x = j == k ? f[k] : x;
-      tl.offer(x, at + j, hits != 0, top, lane);
+      tl.offer(Vec<T>::at(v, j), at + j, hits != 0, top, lane);
       hits &= hits - 1;
     }
   }
 }
 
-// Elements [lo, hi) of a row by the `n` threads (whole warps) of a team, thread id `tid`.
-template <typename T>
-__device__ __forceinline__ void scan(const T* x, int lo, int hi, int tid, int n, Run& st, TopList& tl, int top, int lane) {
-  constexpr int N = Vec<T>::N;
+// A lower bound of the `top`-th largest value of what n threads (a warp, or the CTA with `share`) hold, one vector
+// maximum each: at least `top` of them reach it. It keeps the first vectors from being candidates altogether.
+template <typename T, int kTeamWarps>
+__device__ __forceinline__ float first_bound(float vm, int top, int lane, int warp, float* share) {
+  // (a NaN maximum counts as nothing: a bound may only be too low)
+  unsigned long long k = sort_down(vm == vm ? key_of(vm, 0) : 0, lane);
+  if (kTeamWarps > 1) {
+    unsigned long long* lists = reinterpret_cast<unsigned long long*>(share);
+    lists[warp * 32 + lane] = k;
+    __syncthreads();
+#pragma unroll
+    for (int w = kTeamWarps / 2; w > 0; w >>= 1) {
+      if (warp < w) lists[warp * 32 + lane] = merge_sorted(lists[warp * 32 + lane], lists[(warp + w) * 32 + lane], lane);
+      __syncthreads();
+    }
+    k = lists[lane];
+    __syncthreads();  // the lists are used again
+  }
+  const unsigned long long b = __shfl_sync(kFull, k, top - 1);
+  return b == 0 ? -INFINITY : key_value(b);
+}
+
+// Elements [lo, hi) of a row by kTeamWarps warps, thread `tid` of them.
+template <typename T, int kTeamWarps>
+__device__ __forceinline__ void scan(const T* x, int lo, int hi, int tid, Run<T>& run, TopList& tl, int top, float* share) {
+  constexpr int N = Vec<T>::N, n = kTeamWarps * 32;
   constexpr int U = 4;
+  using Raw = typename Vec<T>::Raw;
+  const int lane = tid & 31, warp = tid >> 5;
   const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(x + lo) & 15u) / sizeof(T));
   int a0 = lo + (mis == 0 ? 0 : N - mis);  // the first aligned element
   if (a0 > hi) a0 = hi;
   const int nv = (hi - a0) / N;
   const int a1 = a0 + nv * N;
-  // single values before and behind the aligned part: fewer than 2 N, one per lane of the first warps
-  const int head = a0 - lo, singles = head + hi - a1;
-  if (tid - (tid & 31) < singles) {
-    const bool valid = tid < singles;
-    const int at = tid < head ? lo + tid : a1 + tid - head;
-    const float f[1] = {valid ? Vec<T>::one(x + at) : 0.0f};
-    take<1>(f, at, st, tl, top, lane, valid);
+  const Raw none = Vec<T>::fill(-INFINITY);
+  // the first U vectors of each thread (or none), all in flight, and the bound they give
+  Raw f[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) f[u] = tid + u * n < nv ? Vec<T>::load(x + a0 + (tid + u * n) * N) : none;
+  if (top > 0) {
+    float vm = Vec<T>::largest(f[0]);
+#pragma unroll
+    for (int u = 1; u < U; ++u) vm = fmaxf(vm, Vec<T>::largest(f[u]));
+    tl.thr_v = first_bound<T, kTeamWarps>(vm, top, lane, warp, share);
   }
-  int v = tid;
+#pragma unroll
+  for (int u = 0; u < U; ++u) take<T>(f[u], a0 + (tid + u * n) * N, run, tl, top, lane, tid + u * n < nv ? N : 0);
+  // single values before and behind the aligned part: fewer than 2 N, one per lane of the first warp
+  const int head = a0 - lo, singles = head + hi - a1;
+  if (warp == 0 && singles > 0) {
+    const int at = tid < head ? lo + tid : a1 + tid - head;
+    take<T>(tid < singles ? Vec<T>::fill(Vec<T>::one(x + at)) : none, at, run, tl, top, lane, tid < singles ? 1 : 0);
+  }
+  int v = tid + U * n;
   for (; v - lane + (U - 1) * n + 31 < nv; v += U * n) {  // warp-uniform: every lane has all U vectors
-    float f[U][N];
 #pragma unroll
-    for (int u = 0; u < U; ++u) Vec<T>::load(x + a0 + (v + u * n) * N, f[u]);
+    for (int u = 0; u < U; ++u) f[u] = Vec<T>::load(x + a0 + (v + u * n) * N);
 #pragma unroll
-    for (int u = 0; u < U; ++u) take<N>(f[u], a0 + (v + u * n) * N, st, tl, top, lane, true);
+    for (int u = 0; u < U; ++u) take<T>(f[u], a0 + (v + u * n) * N, run, tl, top, lane, N);
   }
   for (; v - lane < nv; v += n) {
-    const bool valid = v < nv;
-    float f[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = 0.0f;
-    if (valid) Vec<T>::load(x + a0 + v * N, f);
-    take<N>(f, a0 + v * N, st, tl, top, lane, valid);
+    f[0] = v < nv ? Vec<T>::load(x + a0 + v * N) : none;
+    take<T>(f[0], a0 + v * N, run, tl, top, lane, v < nv ? N : 0);
   }
 }
 
@@ -319,12 +431,11 @@ __global__ void __launch_bounds__(kWarpRowThreads) logprobs_warp_kernel(const Lp
   const int lane = threadIdx.x & 31, row = blockIdx.x * (kWarpRowThreads / 32) + (threadIdx.x >> 5);
   if (row >= a.rows) return;
   const T* x = static_cast<const T*>(a.logits) + row * a.ld;
-  Run run;
+  Run<T> run;
   Stat st;
   TopList tl;
-  run.init();
   tl.init(buf[threadIdx.x >> 5]);
-  scan(x, 0, a.vocab, lane, 32, run, tl, a.top, lane);
+  scan<T, 1>(x, 0, a.vocab, lane, run, tl, a.top, nullptr);
   tl.finish(a.top, lane);
   st.from(run);
   warp_merge(st);
@@ -347,12 +458,11 @@ __global__ void __launch_bounds__(kRowThreads) logprobs_row_kernel(const LpArgs 
   const T* x = static_cast<const T*>(a.logits) + row * a.ld;
   const int part = (a.vocab + C - 1) / C;
   const int lo = rank * part < a.vocab ? rank * part : a.vocab, hi = lo + part < a.vocab ? lo + part : a.vocab;
-  Run run;
+  Run<T> run;
   Stat st;
   TopList tl;
-  run.init();
   tl.init(buf[warp]);
-  scan(x, lo, hi, tid, kRowThreads, run, tl, a.top, lane);
+  scan<T, kWarps>(x, lo, hi, tid, run, tl, a.top, reinterpret_cast<float*>(lists));
   st.from(run);
   warp_merge(st);
   if (lane == 0) sm[warp] = st.m, sr[warp] = st.r, stt[warp] = st.t;
