@@ -34,7 +34,6 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxTop = 32;
 constexpr int kWarpRowThreads = 256;  // 8 rows per CTA
-constexpr int kRowThreads = 512;
 constexpr int kMaxCluster = 8;
 
 __device__ __forceinline__ float ex2(float v) {
@@ -175,31 +174,35 @@ struct Stat {
 
 // ---- top alternatives -------------------------------------------------------------------------------------
 // Keys in torch's order: NaN is the largest value, the lower index wins among equals (and -0 equals 0). 0: none.
-__device__ __forceinline__ unsigned long long key_of(float x, int i) {
+__device__ __forceinline__ uint32_t ordered(float x) {
   x += 0.0f;
   const uint32_t u = __float_as_uint(x);
-  const uint32_t o = isnan(x) ? 0xffffffffu : u ^ (static_cast<int>(u) < 0 ? 0xffffffffu : 0x80000000u);
-  return static_cast<unsigned long long>(o) << 32 | ~static_cast<uint32_t>(i);
+  return isnan(x) ? 0xffffffffu : u ^ (static_cast<int>(u) < 0 ? 0xffffffffu : 0x80000000u);
 }
-__device__ __forceinline__ float key_value(unsigned long long k) {
-  const uint32_t o = static_cast<uint32_t>(k >> 32);
-  return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+__device__ __forceinline__ float from_ordered(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
+__device__ __forceinline__ unsigned long long key_of(float x, int i) {
+  return static_cast<unsigned long long>(ordered(x)) << 32 | ~static_cast<uint32_t>(i);
 }
+__device__ __forceinline__ float key_value(unsigned long long k) { return from_ordered(static_cast<uint32_t>(k >> 32)); }
 __device__ __forceinline__ int key_index(unsigned long long k) { return static_cast<int>(~static_cast<uint32_t>(k)); }
 
-__device__ __forceinline__ unsigned long long exchange(unsigned long long k, int lane, int stride, bool down) {
-  const unsigned long long o = __shfl_xor_sync(kFull, k, stride);
+// (K: 64-bit keys, or the ordered values alone)
+template <typename K>
+__device__ __forceinline__ K exchange(K k, int lane, int stride, bool down) {
+  const K o = __shfl_xor_sync(kFull, k, stride);
   return ((lane & stride) == 0) == down ? (k > o ? k : o) : (k < o ? k : o);
 }
 // The larger 32 of two lists sorted downwards across the lanes, sorted.
-__device__ __forceinline__ unsigned long long merge_sorted(unsigned long long a, unsigned long long b, int lane) {
-  const unsigned long long r = __shfl_sync(kFull, b, 31 - lane);
-  unsigned long long k = a > r ? a : r;
+template <typename K>
+__device__ __forceinline__ K merge_sorted(K a, K b, int lane) {
+  const K r = __shfl_sync(kFull, b, 31 - lane);
+  K k = a > r ? a : r;
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) k = exchange(k, lane, s, true);
   return k;
 }
-__device__ __forceinline__ unsigned long long sort_down(unsigned long long k, int lane) {
+template <typename K>
+__device__ __forceinline__ K sort_down(K k, int lane) {
 #pragma unroll
   for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
@@ -306,11 +309,10 @@ __device__ __forceinline__ void take(const typename Vec<T>::Raw& v, int at, Run<
 // A lower bound of the `top`-th largest value of what n threads (a warp, or the CTA with `share`) hold, one vector
 // maximum each: at least `top` of them reach it. It keeps the first vectors from being candidates altogether.
 template <typename T, int kTeamWarps>
-__device__ __forceinline__ float first_bound(float vm, int top, int lane, int warp, float* share) {
+__device__ __forceinline__ float first_bound(float vm, int top, int lane, int warp, uint32_t* lists) {
   // (a NaN maximum counts as nothing: a bound may only be too low)
-  unsigned long long k = sort_down(vm == vm ? key_of(vm, 0) : 0, lane);
+  uint32_t k = sort_down(vm == vm ? ordered(vm) : 0u, lane);
   if (kTeamWarps > 1) {
-    unsigned long long* lists = reinterpret_cast<unsigned long long*>(share);
     lists[warp * 32 + lane] = k;
     __syncthreads();
 #pragma unroll
@@ -321,13 +323,13 @@ __device__ __forceinline__ float first_bound(float vm, int top, int lane, int wa
     k = lists[lane];
     __syncthreads();  // the lists are used again
   }
-  const unsigned long long b = __shfl_sync(kFull, k, top - 1);
-  return b == 0 ? -INFINITY : key_value(b);
+  const uint32_t b = __shfl_sync(kFull, k, top - 1);
+  return b == 0 ? -INFINITY : from_ordered(b);
 }
 
 // Elements [lo, hi) of a row by kTeamWarps warps, thread `tid` of them.
 template <typename T, int kTeamWarps>
-__device__ __forceinline__ void scan(const T* x, int lo, int hi, int tid, Run<T>& run, TopList& tl, int top, float* share) {
+__device__ __forceinline__ void scan(const T* x, int lo, int hi, int tid, Run<T>& run, TopList& tl, int top, uint32_t* share) {
   constexpr int N = Vec<T>::N, n = kTeamWarps * 32;
   constexpr int U = 4;
   using Raw = typename Vec<T>::Raw;
@@ -442,7 +444,7 @@ __global__ void __launch_bounds__(kWarpRowThreads) logprobs_warp_kernel(const Lp
   finish(a, row, x, st, tl, lane);
 }
 
-template <typename T>
+template <typename T, int kRowThreads>
 __global__ void __launch_bounds__(kRowThreads) logprobs_row_kernel(const LpArgs a) {
   constexpr int kWarps = kRowThreads / 32;
   __shared__ float sm[kWarps], sr[kWarps], stt[kWarps];
@@ -462,7 +464,7 @@ __global__ void __launch_bounds__(kRowThreads) logprobs_row_kernel(const LpArgs 
   Stat st;
   TopList tl;
   tl.init(buf[warp]);
-  scan<T, kWarps>(x, lo, hi, tid, run, tl, a.top, reinterpret_cast<float*>(lists));
+  scan<T, kWarps>(x, lo, hi, tid, run, tl, a.top, reinterpret_cast<uint32_t*>(lists));
   st.from(run);
   warp_merge(st);
   if (lane == 0) sm[warp] = st.m, sr[warp] = st.r, stt[warp] = st.t;
@@ -520,10 +522,13 @@ cudaError_t launch(const LpArgs& a, cudaStream_t s) {
   }
   int C = 1;
   while (C < kMaxCluster && a.rows * C < tc_sm_count() && a.vocab / (2 * C) >= 4096) C *= 2;
+  // Enough rows to fill the GPU run on 8 warps each (what a warp does once per row, its sorts above all, is a third of the
+  // work at 100352 values on 16); few rows on 16 warps in each of the cluster's CTAs
+  const bool many = C == 1;
   cfg.gridDim = dim3(a.rows, C);
-  cfg.blockDim = dim3(kRowThreads);
+  cfg.blockDim = dim3(many ? 256 : 512);
   set_launch_attrs(cfg, attr, C);
-  return cudaLaunchKernelEx(&cfg, logprobs_row_kernel<T>, a);
+  return many ? cudaLaunchKernelEx(&cfg, logprobs_row_kernel<T, 256>, a) : cudaLaunchKernelEx(&cfg, logprobs_row_kernel<T, 512>, a);
 }
 
 }  // namespace
