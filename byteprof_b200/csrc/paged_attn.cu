@@ -8,7 +8,7 @@
 //
 // Few rows (single tokens, drafts, grouped heads of one token): memory bound, the keys and values are read once.
 // A unit is 64 keys x one tile of 16 packed rows; each of the 4 warps takes 16 of the 64 keys, straight from
-// global memory into mma.sync operand registers: the head dimension is summed in an order that lets a thread
+// global memory into the pieces that its threads hand to mma.sync: the head dimension is summed in an order that lets a thread
 // read 16 consecutive bytes of a key (the same order for q), and the output's columns are numbered so that a
 // thread reads 16 consecutive bytes of a value row. No shared memory, no barrier in the loop. The tensor core
 // does 16 rows for the price of one here; 16 rows at HBM speed need a tenth of what mma.sync can do, so tcgen05 has
@@ -24,6 +24,7 @@ namespace {
 constexpr int kRows = 16;   // packed rows per tile
 constexpr int kKeys = 64;   // keys per unit
 constexpr int kWarps = 4;
+constexpr int kSlotRows = kWarps * kRows;  // rows of a part: up to 4 heads of a tile
 constexpr int kThreads = 32 * kWarps;
 constexpr float kLazy = 8.0f;  // the running maximum moves when a score exceeds it by this much (log2 units)
 
@@ -46,12 +47,22 @@ struct FewUnits {
   int tiles, per;  // row tiles per kv head, units per item
   long long all;
 };
-__device__ __forceinline__ FewUnits few_units(const PagedArgs& a, const PagedSeq& q) {
+// `hp`: kv heads per CTA (below).
+__device__ __forceinline__ FewUnits few_units(const PagedArgs& a, const PagedSeq& q, int hp) {
   FewUnits u;
   u.tiles = static_cast<int>((static_cast<long long>(q.n) * a.g + kRows - 1) / kRows);
   u.per = q.kv > kKeys ? (q.kv + kKeys - 1) / kKeys : 1;
-  u.all = static_cast<long long>(a.nkv) * u.tiles * u.per;
+  u.all = static_cast<long long>(a.nkv / hp) * u.tiles * u.per;
   return u;
+}
+
+// How many kv heads the warps of a CTA take side by side over the same keys (the other warps take other keys). A key's
+// heads lie next to each other, so 4 at a time read 1 KB of DRAM in one go instead of 256 bytes here and the rest some
+// other time (head_dim 128); with too few units for that, the heads go to CTAs of their own. `one`: units at one head per CTA.
+__device__ __forceinline__ int heads_per_cta(const PagedArgs& a, long long one) {
+  if (a.nkv % 4 == 0 && one >= 16LL * a.G) return 4;
+  if (a.nkv % 2 == 0 && one >= 8LL * a.G) return 2;
+  return 1;
 }
 
 __device__ __forceinline__ long long share_of(const PagedArgs& a, long long total) {
@@ -68,7 +79,7 @@ struct Located {
 __device__ long long total_units(const PagedArgs& a, long long* sm) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long t = 0;
-  for (int s = threadIdx.x; s < a.seqs; s += kThreads) t += few_units(a, paged_seq(a, s)).all;
+  for (int s = threadIdx.x; s < a.seqs; s += kThreads) t += few_units(a, paged_seq(a, s), 1).all;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(kPagedFull, t, o);
   if (lane == 0) sm[warp] = t;
@@ -79,12 +90,12 @@ __device__ long long total_units(const PagedArgs& a, long long* sm) {
   __syncthreads();
   return t;
 }
-__device__ Located locate(const PagedArgs& a, long long u, long long* sm) {
+__device__ Located locate(const PagedArgs& a, long long u, int hp, long long* sm) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long base = 0;
   for (int s0 = 0; s0 < a.seqs; s0 += kThreads) {
     const int s = s0 + threadIdx.x;
-    const long long mine = s < a.seqs ? few_units(a, paged_seq(a, s)).all : 0;
+    const long long mine = s < a.seqs ? few_units(a, paged_seq(a, s), hp).all : 0;
     long long pre = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -114,56 +125,68 @@ __device__ Located locate(const PagedArgs& a, long long u, long long* sm) {
   return {-1, 0};
 }
 
+// Each warp has a ring of kStages units of its 16 keys and values; a thread copies exactly the 16-byte pieces that it
+// will read itself, piece i of lane l at [i][l], so that its own wait_group is all the synchronisation there is.
+constexpr int kStages = 3;
 template <int HD>
 struct FewSmem {
-  float o[kWarps][kRows][HD + 4];
-  float m[kWarps][kRows], l[kWarps][kRows];
+  static constexpr int kPieces = 2 * (HD / 32) + 4 * (HD / 64);  // of the keys, then of the values
+  union {
+    uint4 ring[kWarps][kStages][kPieces][32];
+    struct {
+      float o[kWarps][kRows][HD + 4];
+      float m[kWarps][kRows], l[kWarps][kRows];
+    };
+  };
   long long scan[kWarps + 2];
 };
 
-// One warp's 16 keys of a unit: the cache rows of keys base.. and base + 8.. (a page holds at least 8 positions and
-// base is a multiple of 16), -1 where there is none. `bad`: the lowest position whose page is not in the pool.
-__device__ __forceinline__ void find_rows(const PagedArgs& a, const int* table, int base, int kv, long long (&row)[2],
-                                          int& bad) {
+// 16 bytes global -> shared, zeros when !ok (nothing is read then).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+
+// Pages of a warp's 16 keys of a unit: of keys base.. and base + 8.. (a page holds at least 8 positions and base is a
+// multiple of 16).
+__device__ __forceinline__ void find_pages(const PagedArgs& a, const int* table, int base, int kv, int (&page)[2]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) page[i] = base + 8 * i < kv ? __ldg(table + ((base + 8 * i) >> a.page_log2)) : 0;
+}
+
+// Requests the keys base + 8 i + lane / 4, dims 32 c + 8 (lane % 4) .., and the values base + 2 (lane % 4) + {0, 1, 8, 9},
+// dims 64 h + 8 (lane / 4) .. Past the end they are zero (what lies there may be NaN, and p = 0 would not hide it). `bad`:
+// the lowest position whose page is not in the pool.
+template <int HD>
+__device__ __forceinline__ void request(const PagedArgs& a, const int (&page)[2], int base, int kv, int h, int lane, uint32_t dst,
+                                        int& bad) {
+  const long long ld = static_cast<long long>(a.nkv) * HD;
+  const int in_page = base & ((1 << a.page_log2) - 1);
+  long long row[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int key = base + 8 * i;
-    int page = -1;
-    if (key < kv) {
-      page = __ldg(table + (key >> a.page_log2));
-      if (page < 0 || page >= a.num_pages) {
-        page = -1;
-        bad = key < bad ? key : bad;
-      }
-    }
-    row[i] = page < 0 ? -1 : (static_cast<long long>(page) << a.page_log2) + (key & ((1 << a.page_log2) - 1));
+    const bool have = page[i] >= 0 && page[i] < a.num_pages;
+    if (!have && key < kv) bad = key < bad ? key : bad;
+    row[i] = !have || key >= kv ? -1
+                                : (static_cast<long long>(page[i]) << a.page_log2) + (a.page_log2 == 3 ? 0 : in_page + 8 * i);
   }
-}
-// k[i][c]: key base + 8 i + lane / 4, dims 32 c + 8 (lane % 4) ..
-template <int HD>
-__device__ __forceinline__ void load_k(const PagedArgs& a, const long long (&row)[2], int base, int kv, int h, int lane,
-                                       uint4 (&k)[2][HD / 32]) {
+  dst += lane * 16;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int j = lane >> 2;
     const bool ok = row[i] >= 0 && base + 8 * i + j < kv;
-    const __nv_bfloat16* p = a.kp + ((ok ? row[i] + j : 0) * (a.nkv * HD) + h * HD + (lane & 3) * 8);
+    const __nv_bfloat16* p = a.kp + ((ok ? row[i] + j : 0) * ld + h * HD + (lane & 3) * 8);
 #pragma unroll
-    for (int c = 0; c < HD / 32; ++c) k[i][c] = ok ? ldg16(p + 32 * c) : make_uint4(0, 0, 0, 0);
+    for (int c = 0; c < HD / 32; ++c) copy16(dst + (i * (HD / 32) + c) * 512, p + 32 * c, ok);
   }
-}
-// v[i][hh]: keys base + 2 (lane % 4) + {0, 1, 8, 9}, dims 64 hh + 8 (lane / 4) ..; zero past the end (what lies there
-// may be NaN, and p = 0 would not hide it)
-template <int HD>
-__device__ __forceinline__ void load_v(const PagedArgs& a, const long long (&row)[2], int base, int kv, int h, int lane,
-                                       uint4 (&v)[4][HD / 64]) {
+  dst += 2 * (HD / 32) * 512;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int j = 2 * (lane & 3) + (i & 1);
     const bool ok = row[i >> 1] >= 0 && base + 8 * (i >> 1) + j < kv;
-    const __nv_bfloat16* p = a.vp + ((ok ? row[i >> 1] + j : 0) * (a.nkv * HD) + h * HD + (lane >> 2) * 8);
+    const __nv_bfloat16* p = a.vp + ((ok ? row[i >> 1] + j : 0) * ld + h * HD + (lane >> 2) * 8);
 #pragma unroll
-    for (int hh = 0; hh < HD / 64; ++hh) v[i][hh] = ok ? ldg16(p + 64 * hh) : make_uint4(0, 0, 0, 0);
+    for (int hh = 0; hh < HD / 64; ++hh) copy16(dst + (i * (HD / 64) + hh) * 512, p + 64 * hh, ok);
   }
 }
 
@@ -174,21 +197,23 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const PagedArgs 
   pdl_launch_dependents();
   pdl_wait_prior_grids();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long total = total_units(a, sm.scan);
+  const long long one = total_units(a, sm.scan);
+  const int hp = heads_per_cta(a, one), hl = warp % hp, part = warp / hp, step = kKeys / hp;
+  const long long total = one / hp;
   const long long share = share_of(a, total);
   long long u = blockIdx.x * share;
   const long long u1 = u + share < total ? u + share : total;
   if (u >= u1) return;
-  const Located at = locate(a, u, sm.scan);
+  const Located at = locate(a, u, hp, sm.scan);
   int s = at.s;
   long long before = at.before;
   PagedSeq seq = paged_seq(a, s);
-  FewUnits fu = few_units(a, seq);
+  FewUnits fu = few_units(a, seq, hp);
   while (true) {
     // the segment of this item in the CTA's share
     const long long rel = u - before;
     const int item = static_cast<int>(rel / fu.per), off = static_cast<int>(rel % fu.per);
-    const int h = item / fu.tiles, tile = item % fu.tiles;
+    const int h = item / fu.tiles * hp + hl, tile = item % fu.tiles;
     const int end = static_cast<int>(fu.per - off < u1 - u ? fu.per : off + (u1 - u));
     const int* table = a.pages + static_cast<long long>(s) * a.ld_pages;
 
@@ -215,27 +240,36 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const PagedArgs 
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
     int bad = seq.bad;
 
-    // keys and values of the next unit are requested as soon as this unit's product has read the registers
-    uint4 kr[2][HD / 32], vr[4][HD / 64];
-    long long row[2];
-    find_rows(a, table, off * kKeys + warp * 16, seq.kv, row, bad);
-    load_k<HD>(a, row, off * kKeys + warp * 16, seq.kv, h, lane, kr);
-    load_v<HD>(a, row, off * kKeys + warp * 16, seq.kv, h, lane, vr);
-    for (int b = off; b < end; ++b) {
-      const int base = b * kKeys + warp * 16;
+    // the ring is kStages units ahead, the pages one more
+    uint4(*ring)[FewSmem<HD>::kPieces][32] = sm.ring[warp];
+    int page[2];
+    const int s0 = off * hp, s1 = end * hp;  // steps of `step` keys of the segment, 16 of them this warp's
+#pragma unroll
+    for (int st = 0; st < kStages; ++st) {
+      const int base = (s0 + st) * step + part * 16;
+      if (s0 + st < s1) {
+        find_pages(a, table, base, seq.kv, page);
+        request<HD>(a, page, base, seq.kv, h, lane, smem_addr(ring[st]), bad);
+      }
+      cp_async_commit();
+    }
+    find_pages(a, table, (s0 + kStages) * step + part * 16, s0 + kStages < s1 ? seq.kv : 0, page);
+    int st = 0;
+    for (int b = s0; b < s1; ++b) {
+      const int base = b * step + part * 16;
+      cp_async_wait<kStages - 1>();
+      const uint4* kr = &ring[st][0][lane];
+      const uint4* vr = &ring[st][2 * (HD / 32)][lane];
       float sc[2][4];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.0f;
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c) {
-          mma16816(sc[i], qa[c].x, qb[c].x, qa[c].y, qb[c].y, kr[i][c].x, kr[i][c].y);
-          mma16816(sc[i], qa[c].z, qb[c].z, qa[c].w, qb[c].w, kr[i][c].z, kr[i][c].w);
+          const uint4 k = kr[(i * (HD / 32) + c) * 32];
+          mma16816(sc[i], qa[c].x, qb[c].x, qa[c].y, qb[c].y, k.x, k.y);
+          mma16816(sc[i], qa[c].z, qb[c].z, qa[c].w, qb[c].w, k.z, k.w);
         }
-      }
-      if (b + 1 < end) {
-        find_rows(a, table, base + kKeys, seq.kv, row, bad);
-        load_k<HD>(a, row, base + kKeys, seq.kv, h, lane, kr);
       }
       // scores in log2 units, hidden keys -inf; sc[i][2 r + e] is row r (of the thread's two), key base + 8 i + 2 (lane % 4) + e
       float mx[2] = {-INFINITY, -INFINITY};
@@ -280,10 +314,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const PagedArgs 
                      a3 = pack2(p[1][2], p[1][3]);
 #pragma unroll
       for (int hh = 0; hh < HD / 64; ++hh) {
-        const uint32_t* w0 = &vr[0][hh].x;
-        const uint32_t* w1 = &vr[1][hh].x;
-        const uint32_t* w2 = &vr[2][hh].x;
-        const uint32_t* w3 = &vr[3][hh].x;
+        const uint4 v0 = vr[(0 * (HD / 64) + hh) * 32], v1 = vr[(1 * (HD / 64) + hh) * 32], v2 = vr[(2 * (HD / 64) + hh) * 32],
+                    v3 = vr[(3 * (HD / 64) + hh) * 32];
+        const uint32_t* w0 = &v0.x;
+        const uint32_t* w1 = &v1.x;
+        const uint32_t* w2 = &v2.x;
+        const uint32_t* w3 = &v3.x;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           mma16816(o[8 * hh + 2 * w], a0, a1, a2, a3, __byte_perm(w0[w], w1[w], 0x5410), __byte_perm(w2[w], w3[w], 0x5410));
@@ -291,9 +327,14 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const PagedArgs 
                    __byte_perm(w2[w], w3[w], 0x7632));
         }
       }
-      if (b + 1 < end) load_v<HD>(a, row, base + kKeys, seq.kv, h, lane, vr);
+      if (b + kStages < s1) request<HD>(a, page, base + kStages * step, seq.kv, h, lane, smem_addr(ring[st]), bad);
+      cp_async_commit();
+      find_pages(a, table, base + (kStages + 1) * step, b + kStages + 1 < s1 ? seq.kv : 0, page);
+      st = st + 1 == kStages ? 0 : st + 1;
     }
-    // the 4 warps' parts meet in shared memory
+    // the 4 warps' parts meet in shared memory (the rings' memory: every warp is through with its own)
+    cp_async_wait<0>();
+    __syncthreads();
     bad = __reduce_min_sync(kPagedFull, bad);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -319,40 +360,36 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const PagedArgs 
     const bool whole = off == 0 && end == fu.per;
     const int slot = 2 * blockIdx.x + (off == 0 ? 1 : 0);
     constexpr int kPer = HD / 8;  // dims per thread: 8 threads per row
-    {
-      const int row = tid / 8, d0 = (tid % 8) * kPer;
+    for (int j = 0; j < hp; ++j) {  // warps j, j + hp, .. hold parts of head j
+      const int row = tid / 8, d0 = (tid % 8) * kPer, hj = item / fu.tiles * hp + j;
       const int r = tile * kRows + row;
       if (r < nrows) {
         float mm = -INFINITY, ll = 0.0f, acc[kPer];
+        for (int w = j; w < kWarps; w += hp) mm = fmaxf(mm, sm.m[w][row]);
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sm.m[w][row]);
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) acc[j] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int d = 0; d < kPer; ++d) acc[d] = 0.0f;
+        for (int w = j; w < kWarps; w += hp) {
           const float f = sm.m[w][row] == -INFINITY ? 0.0f : pg_ex2(sm.m[w][row] - mm);
           ll += f == 0.0f && !isnan(sm.l[w][row]) ? 0.0f : f * sm.l[w][row];
 #pragma unroll
-          for (int j = 0; j < kPer; ++j) acc[j] = fmaf(f, sm.o[w][row][d0 + j], acc[j]);
+          for (int d = 0; d < kPer; ++d) acc[d] = fmaf(f, sm.o[w][row][d0 + d], acc[d]);
         }
         if (whole) {
           const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
           uint32_t w[kPer / 2];
 #pragma unroll
-          for (int j = 0; j < kPer / 2; ++j) w[j] = pack2(acc[2 * j] * inv, acc[2 * j + 1] * inv);
-          __nv_bfloat16* dst = a.out + (seq.first + r / a.g) * a.ldo + (h * a.g + r % a.g) * HD + d0;
+          for (int d = 0; d < kPer / 2; ++d) w[d] = pack2(acc[2 * d] * inv, acc[2 * d + 1] * inv);
+          __nv_bfloat16* dst = a.out + (seq.first + r / a.g) * a.ldo + (hj * a.g + r % a.g) * HD + d0;
 #pragma unroll
-          for (int j = 0; j < kPer / 8; ++j)
-            reinterpret_cast<uint4*>(dst)[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+          for (int d = 0; d < kPer / 8; ++d)
+            reinterpret_cast<uint4*>(dst)[d] = make_uint4(w[4 * d], w[4 * d + 1], w[4 * d + 2], w[4 * d + 3]);
         } else {
-          float* dst = a.part_o + (static_cast<size_t>(slot) * kRows + row) * HD + d0;
+          const size_t at = static_cast<size_t>(slot) * kSlotRows + j * kRows + row;
+          float* dst = a.part_o + at * HD + d0;
 #pragma unroll
-          for (int j = 0; j < kPer / 4; ++j)
-            reinterpret_cast<float4*>(dst)[j] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
-          if (d0 == 0) {
-            float2* ml = reinterpret_cast<float2*>(a.part_ml) + static_cast<size_t>(slot) * kRows + row;
-            *ml = make_float2(mm, ll);
-          }
+          for (int d = 0; d < kPer / 4; ++d)
+            reinterpret_cast<float4*>(dst)[d] = make_float4(acc[4 * d], acc[4 * d + 1], acc[4 * d + 2], acc[4 * d + 3]);
+          if (d0 == 0) reinterpret_cast<float2*>(a.part_ml)[at] = make_float2(mm, ll);
         }
       }
     }
@@ -365,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const PagedArgs 
         ++s;
         seq = paged_seq(a, s);
       } while (seq.n == 0);
-      fu = few_units(a, seq);
+      fu = few_units(a, seq, hp);
     }
   }
 }
@@ -386,7 +423,7 @@ __global__ void __launch_bounds__(kThreads) paged_few_join_kernel(const PagedArg
   __syncthreads();
   for (int s = tid; s < a.seqs; s += kThreads) {
     const PagedSeq q = paged_seq(a, s);
-    const long long n = few_units(a, q).all;
+    const long long n = few_units(a, q, 1).all;
     total += n;
     if (q.first + q.n <= t) before += n;
     if (q.n > 0 && t >= q.first && t < q.first + q.n) found[0] = s;
@@ -406,17 +443,18 @@ __global__ void __launch_bounds__(kThreads) paged_few_join_kernel(const PagedArg
   const int s = found[0];
   if (s < 0) return;
   const PagedSeq q = paged_seq(a, s);
-  const FewUnits fu = few_units(a, q);
-  const long long share = share_of(a, total);
+  const int hp = heads_per_cta(a, total), h = head / a.g;
+  const FewUnits fu = few_units(a, q, hp);
+  const long long share = share_of(a, total / hp);
   const int pr = (t - q.first) * a.g + head % a.g;
-  const long long a0 = before + (static_cast<long long>(head / a.g) * fu.tiles + pr / kRows) * fu.per;
+  const long long a0 = before / hp + (static_cast<long long>(h / hp) * fu.tiles + pr / kRows) * fu.per;
   const int c0 = static_cast<int>(a0 / share), c1 = static_cast<int>((a0 + fu.per - 1) / share);
   if (c0 == c1) return;
-  const int row = pr % kRows;
+  const int row = h % hp * kRows + pr % kRows;
   constexpr int kPer = HD / 32;
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
   float m = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, ml[static_cast<size_t>(2 * c + (c == c0)) * kRows + row].x);
+  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, ml[static_cast<size_t>(2 * c + (c == c0)) * kSlotRows + row].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kPagedFull, m, o));
   float l = 0.0f, acc[kPer];
@@ -424,7 +462,7 @@ __global__ void __launch_bounds__(kThreads) paged_few_join_kernel(const PagedArg
   for (int j = 0; j < kPer; ++j) acc[j] = 0.0f;
 #pragma unroll 4
   for (int c = c0 + warp; c <= c1; c += kWarps) {
-    const size_t at = static_cast<size_t>(2 * c + (c == c0)) * kRows + row;
+    const size_t at = static_cast<size_t>(2 * c + (c == c0)) * kSlotRows + row;
     const float2 p = ml[at];
     const float f = p.x == -INFINITY ? 0.0f : pg_ex2(p.x - m);
     l += f == 0.0f && !isnan(p.y) ? 0.0f : f * p.y;
@@ -490,7 +528,7 @@ cudaError_t launch_few(const PagedArgs& a, cudaStream_t s) {
 extern "C" size_t bp_paged_attention_workspace_bytes(int rows, int seqs, int nh, int nkv, int head_dim) {
   using namespace bp;
   if (rows <= 0 || seqs <= 0 || nkv <= 0 || nh < nkv || head_dim <= 0) return 0;
-  return few_rows(rows, seqs, nh / nkv) ? static_cast<size_t>(2 * few_grid()) * kRows * (head_dim + 2) * sizeof(float)
+  return few_rows(rows, seqs, nh / nkv) ? static_cast<size_t>(2 * few_grid()) * kSlotRows * (head_dim + 2) * sizeof(float)
                                         : paged_tc_workspace_bytes(head_dim);
 }
 
@@ -560,7 +598,7 @@ extern "C" int bp_paged_attention(const void* q, long long ldq, const void* k_pa
   a.G = few_grid();
   a.min_share = 1;
   a.part_o = static_cast<float*>(workspace);
-  a.part_ml = a.part_o + static_cast<size_t>(2 * a.G) * kRows * head_dim;
+  a.part_ml = a.part_o + static_cast<size_t>(2 * a.G) * kSlotRows * head_dim;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = head_dim == 128 ? launch_few<128>(a, s) : launch_few<64>(a, s);
   if (e != cudaSuccess) return fail(BP_ERR_CUDA, "paged_attention launch: %s", cudaGetErrorString(e));
