@@ -162,6 +162,29 @@ def on_device(t: torch.Tensor):
     return torch.cuda.device(t.device)
 
 
+def device_of(t: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """The CUDA device index that all given tensors share; raises for CPU tensors and mixed devices."""
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError("the byteprof B200 kernels take CUDA tensors only (there is no CPU path)")
+    for o in others:
+        if o is not None and o.get_device() != dev:
+            raise ValueError("all tensors of a call must be on one CUDA device")
+    return dev
+
+
+_get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def launch(dev: int, name: str, *args) -> None:
+    """`call` on torch's current stream of device `dev` (the entry point's last argument), with that device current."""
+    if _get_device() == dev:
+        call(name, *args, _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+
+
 def require_cuda(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:

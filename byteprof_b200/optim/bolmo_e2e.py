@@ -32,13 +32,16 @@ import ctypes
 
 import numpy as np
 import torch
+import torch.nn.functional as F
 
 from .. import _lib
 
+from ..quant.int8 import int8_linear, quantize_rowwise_int8
 from .bolmo_local import LocalLayer, rmsnorm
 from .decode_ops import (DecodeAttention, GlobStep, LocStep, add_norm, decode_finish, embed_rmsnorm, norm_add,
-                         rope_tables, swiglu)
-from .skinny import skinny_mm
+                         rope_tables, swiglu, token_logprobs)
+from .paged import PagedCache
+from .skinny import MAX_M, skinny_mm
 
 EPS = 1e-6
 
@@ -66,6 +69,7 @@ class GlobalBlock:
         self.w_down = _rnd(gen, device, d, ffn)
         self.mlp_norm = _norm_w(gen, device, d)
         self.attn = DecodeAttention(nh, d // nh, max_pos, device, dtype=act_dtype)
+        self.w8: dict[str, tuple[torch.Tensor, torch.Tensor]] | None = None  # see quantize_prompt
 
     def step(self, x: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
         """x [1, d] (the activation dtype) at patch position `pos` (device int64) -> the block's output [1, d]."""
@@ -73,6 +77,26 @@ class GlobalBlock:
         h = add_norm(skinny_mm(att, self.w_o), x, self.attn_norm, EPS)
         dn = skinny_mm(swiglu(skinny_mm(h, self.w_gu)), self.w_down)
         return add_norm(dn, h, self.mlp_norm, EPS)
+
+
+    def quantize_prompt(self) -> None:
+        """int8 copies of the projections, which `chunk` then uses (int8 activations too: quant.int8.int8_linear)."""
+        self.w8 = {name: quantize_rowwise_int8(getattr(self, name)) for name in ("w_qkv", "w_o", "w_gu", "w_down")}
+
+    def _linear(self, x: torch.Tensor, name: str) -> torch.Tensor:
+        if self.w8 is not None:
+            return int8_linear(x, *self.w8[name])
+        w = getattr(self, name)  # few rows: the skinny kernel; more: a plain library product, as in SkinnyLinear
+        return skinny_mm(x, w) if x.shape[0] <= MAX_M else F.linear(x, w)
+
+    def chunk(self, x: torch.Tensor, cache: PagedCache, pages: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
+              cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+        """x [T, d] bf16, the newest positions of one or more sequences whose keys and values lie in `cache` (tables as in
+        `PagedCache`) -> the block's output [T, d]; appends them to the cache."""
+        q = cache.append(self._linear(x, "w_qkv"), self.nh, pages, q_start, kv_len, self.q_norm, self.k_norm, cos, sin, EPS)
+        att = cache.attend(q, pages, q_start, kv_len).view(x.shape[0], self.d)
+        h = add_norm(self._linear(att, "w_o"), x, self.attn_norm, EPS)
+        return add_norm(self._linear(swiglu(self._linear(h, "w_gu")), "w_down"), h, self.mlp_norm, EPS)
 
 
 class BolmoDecoder:
@@ -297,6 +321,73 @@ class BolmoDecoder:
         self.patches += sum(opened)
         self.parity ^= n & 1
         return tokens.tolist(), [bool(f) for f in flags], opened, wall
+
+    # ---- a prompt in one pass ----
+    def quantize_prompt(self) -> None:
+        """The prompt pass's global projections in 8 bits (the byte loop keeps its bf16 weights)."""
+        for blk in self.blocks:
+            blk.quantize_prompt()
+
+    @torch.no_grad()
+    def prefill(self, prompt: list[int], first_patch: bool = True) -> tuple[torch.Tensor, list[bool], list[bool]]:
+        """All bytes of `prompt` at once from the current state: the local layers scan over the bytes, the global model
+        takes the patches they open as one chunk over its caches (`GlobalBlock.chunk`). Returns (logits [N, vocab] fp32,
+        the boundary flag behind each byte, whether each byte opened a patch); `feed`, `steps` and `generate` go on from
+        there. A byte opens a patch when the byte before it was flagged (the first: when first_patch). bf16 only."""
+        if self.act != torch.bfloat16:
+            raise ValueError("prefill runs bf16 activations only (precision='bf16')")
+        n = len(prompt)
+        if n == 0:
+            return torch.empty(0, self.vocab, dtype=torch.float32, device=self.device), [], []
+        if min(prompt) < 0 or max(prompt) >= self.vocab:
+            raise ValueError(f"byte ids must lie in [0, {self.vocab})")
+        if not first_patch and self.patches == 0:
+            raise ValueError("the first byte of a decoder without patches has to open one")
+        p, dev = self.parity, self.device
+        ids = torch.tensor(prompt, dtype=torch.long).to(dev)
+        # the encoder's state is committed only when the patches are known to fit
+        saved = self.enc.state[0].clone() if self.patches + n > self.max_patches else None
+        h, x = embed_rmsnorm(self.embed, ids, self.enc.norm1, EPS)
+        _, e = self.enc.chunk(h, x, p, out_norm=self.enc_norm, want_sum=False)
+        logit = skinny_mm(e, self.w_boundary, out=torch.empty(n, 1, dtype=torch.float32, device=dev))
+        flags = (torch.sigmoid(logit[:, 0].double()).float() >= 0.5).tolist()  # the host needs them: one synchronisation
+        opened = [bool(first_patch)] + flags[:-1]
+        t = sum(opened)
+        if self.patches + t > self.max_patches:
+            self.enc.state[0].copy_(saved)
+            raise RuntimeError(f"{self.patches + t} patches: more than the static KV cache's {self.max_patches}")
+        values = self.value
+        if t:
+            at = torch.tensor([i for i, o in enumerate(opened) if o], dtype=torch.long).to(dev)
+            g = skinny_mm(e, self.w_patch).index_select(0, at)
+            cache = self.blocks[0].attn.paged()
+            pages = torch.arange(cache.num_pages, dtype=torch.int32, device=dev)[None]
+            q_start = torch.tensor([0, t], dtype=torch.int32).to(dev)
+            kv_len = torch.tensor([self.patches + t], dtype=torch.int32).to(dev)
+            for blk in self.blocks:
+                g = blk.chunk(g, blk.attn.paged(), pages, q_start, kv_len, self.cos, self.sin)
+            values = torch.cat([self.value, rmsnorm(g, self.dec_in_norm, EPS)])
+            self.pos.add_(t)
+            self.patches += t
+        where = torch.tensor(opened, dtype=torch.long).cumsum(0).to(dev)  # 0: the value before the prompt
+        values = values.index_select(0, where)
+        h, x = norm_add(skinny_mm(e, self.w_in), values, self.dec.norm1, EPS)
+        _, xf = self.dec.chunk(h, x, p, out_norm=self.final_norm, want_sum=False)
+        logits = skinny_mm(xf, self.lm_head, out=torch.empty(n, self.vocab, dtype=torch.float32, device=dev))
+        self.value.copy_(values[-1:])
+        self.parity = 1 - p
+        return logits, flags, opened
+
+    @torch.no_grad()
+    def score(self, text: list[int], top: int = 0, first_patch: bool = True):
+        """Log probability of each byte of `text` behind its first, from the current state: one `prefill` and one
+        `token_logprobs` over its rows. Returns (logprob [N - 1], entropy [N - 1], top_logprob, top_id) as
+        `token_logprobs`; bits per byte are -logprob.mean() / ln 2."""
+        if len(text) < 2:
+            raise ValueError("a text of at least two bytes is needed")
+        logits, _, _ = self.prefill(text, first_patch)
+        ids = torch.tensor(text[1:], dtype=torch.long).to(self.device)
+        return token_logprobs(logits[:-1], ids, top)
 
     @torch.no_grad()
     def generate(self, prompt: list[int], n_new: int) -> tuple[list[int], list[bool]]:

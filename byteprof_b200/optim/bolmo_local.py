@@ -102,9 +102,9 @@ class LocalLayer:
         return y, q, k, v, g[:, :nh].reshape(s, nh, 1), g[:, nh:].reshape(s, nh, 1)
 
     def _tail(self, h: torch.Tensor, y: torch.Tensor, s: int, out_norm: torch.Tensor | None, want_sum: bool,
-              out: torch.Tensor | None = None):
+              out: torch.Tensor | None = None, hbuf: torch.Tensor | None = None):
         d, eps = self.d, self.norm_eps
-        z = norm_gate(self.hbuf[:s], y[:, 3 * d:], self.mh_norm, eps,
+        z = norm_gate((self.hbuf if hbuf is None else hbuf)[:s], y[:, 3 * d:], self.mh_norm, eps,
                       out=torch.empty(s, d, dtype=self.act, device=h.device))
         h2, x2 = norm_add(skinny_mm(z, self.w_out), h, self.norm2, eps)
         dn = skinny_mm(swiglu(skinny_mm(x2, self.w_gu)), self.w_down)
@@ -139,6 +139,16 @@ class LocalLayer:
         mlstm_scan(self.current_state(parity), q, k, v, i_pre, f_pre, self.hbuf, self.current_state(1 - parity),
                    self.mlstm_eps)
         return self._tail(h, y, 1, out_norm, want_sum, out)
+
+    def chunk(self, h: torch.Tensor, x: torch.Tensor, parity: int, out_norm: torch.Tensor | None = None,
+              want_sum: bool = True):
+        """Any number of positions [N, d] at once; the state advances by all of them (n, m from buffer `parity` to
+        buffer 1 - parity). Returns as `forward`."""
+        y, q, k, v, i_pre, f_pre = self._project(x)
+        hbuf = torch.empty(h.shape[0], self.nh, self.dh, dtype=self.act, device=h.device)
+        mlstm_scan(self.current_state(parity), q, k, v, i_pre, f_pre, hbuf, self.current_state(1 - parity),
+                   self.mlstm_eps)
+        return self._tail(h, y, h.shape[0], out_norm, want_sum, hbuf=hbuf)
 
 
 class BolmoLocal:

@@ -27,6 +27,7 @@ import ctypes
 import torch
 
 from .. import _lib
+from .paged import PagedCache
 
 NORM_PLAIN, NORM_ADD_FIRST, NORM_ADD_AFTER, NORM_GATE = 0, 1, 2, 3
 
@@ -172,22 +173,19 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor | None, top: int = 0)
     rows, ld = _rows(logits)
     vocab = logits.shape[1]
     code = _act(logits.dtype)
-    if ids is not None and (ids.dtype != torch.int64 or ids.shape != (rows,) or not ids.is_contiguous()):
+    if ids is not None and (ids.dtype is not torch.int64 or ids.shape != (rows,) or not ids.is_contiguous()):
         raise ValueError("ids must be a contiguous int64 [R]")
     if not 0 <= top <= min(32, vocab):
         raise ValueError(f"top must be 0..32 and at most the vocabulary, got {top}")
     if vocab == 0 and rows:
         raise ValueError("rows of an empty vocabulary have no distribution")
-    _lib.require_cuda(logits, ids)
-    f32 = dict(dtype=torch.float32, device=logits.device)
-    lp = torch.empty(rows, **f32) if ids is not None else None
-    ent = torch.empty(rows, **f32)
-    top_lp = torch.empty(rows, top, **f32) if top else None
-    top_id = torch.empty(rows, top, dtype=torch.int64, device=logits.device) if top else None
-    with _lib.on_device(logits):
-        _lib.call("bp_token_logprobs", logits.data_ptr(), ld if rows > 1 else vocab, code, _lib.ptr(ids),
-                  _lib.ptr(lp), ent.data_ptr(), _lib.ptr(top_lp), _lib.ptr(top_id), rows, vocab, top,
-                  _lib.stream_of(logits))
+    dev = _lib.device_of(logits, ids)
+    lp = logits.new_empty(rows, dtype=torch.float32) if ids is not None else None
+    ent = logits.new_empty(rows, dtype=torch.float32)
+    top_lp = logits.new_empty((rows, top), dtype=torch.float32) if top else None
+    top_id = logits.new_empty((rows, top), dtype=torch.int64) if top else None
+    _lib.launch(dev, "bp_token_logprobs", logits.data_ptr(), ld if rows > 1 else vocab, code, _lib.ptr(ids),
+                _lib.ptr(lp), ent.data_ptr(), _lib.ptr(top_lp), _lib.ptr(top_id), rows, vocab, top)
     return lp, ent, top_lp, top_id
 
 
@@ -212,6 +210,14 @@ class DecodeAttention:
     def reset(self) -> None:
         self.k_cache.zero_()
         self.v_cache.zero_()
+
+    def paged(self) -> PagedCache:
+        """The same caches as pages (bf16, max_pos a multiple of 8): `PagedCache.append` and `attend` take many positions
+        in one call, and this object's single positions go on behind them."""
+        size = next((s for s in (64, 32, 16, 8) if self.max_pos % s == 0), None)
+        if size is None:
+            raise ValueError(f"max_pos must be a multiple of 8 to be read as pages, got {self.max_pos}")
+        return PagedCache.over(self.k_cache, self.v_cache, size)
 
     def __call__(self, qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, cos: torch.Tensor,
                  sin: torch.Tensor, pos: torch.Tensor, eps: float, out: torch.Tensor | None = None) -> torch.Tensor:

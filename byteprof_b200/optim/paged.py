@@ -16,9 +16,7 @@ import torch
 from .. import _lib
 
 
-def _i32(name: str, t: torch.Tensor, dim: int) -> None:
-    if t.dtype != torch.int32 or t.dim() != dim or t.stride(-1) != 1:
-        raise ValueError(f"{name} must be a {dim}-D int32 tensor with unit column stride")
+_BF16, _I32, _F32 = torch.bfloat16, torch.int32, torch.float32
 
 
 class PagedCache:
@@ -38,7 +36,7 @@ class PagedCache:
         if self.hd not in (64, 128):
             raise ValueError(f"head_dim must be 64 or 128, got {self.hd}")
         self.k_pages, self.v_pages = k_pages, v_pages
-        self._ws_bytes: dict[tuple[int, int, int], int] = {}
+        self._ws_bytes: dict[tuple[int, int, int, int], int] = {}
 
     @classmethod
     def zeros(cls, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, device: torch.device) -> "PagedCache":
@@ -53,17 +51,18 @@ class PagedCache:
             raise ValueError(f"a [max_pos, n_kv_heads, head_dim] cache with max_pos a multiple of {page_size} expected")
         return cls(*(t.view(-1, page_size, *t.shape[1:]) for t in (k_cache, v_cache)))
 
-    def _where(self, rows: int, pages: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor) -> int:
-        _i32("pages", pages, 2)
-        _i32("q_start", q_start, 1)
-        _i32("kv_len", kv_len, 1)
-        seqs = pages.shape[0]
+    def _where(self, pages: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor) -> tuple[int, int, int]:
+        """(S, max_pages, row stride of pages) of a call's tables."""
+        if pages.dtype is not _I32 or pages.dim() != 2 or q_start.dtype is not _I32 or q_start.dim() != 1 or \
+                kv_len.dtype is not _I32 or kv_len.dim() != 1:
+            raise ValueError("pages [S, max_pages], q_start [S + 1] and kv_len [S] must be int32")
+        seqs, width = pages.shape
+        ld, one = pages.stride()
+        if (one != 1 and width > 1) or q_start.stride(0) != 1 or (kv_len.stride(0) != 1 and seqs > 1):
+            raise ValueError("pages, q_start and kv_len need unit stride along their last dimension")
         if q_start.shape[0] != seqs + 1 or kv_len.shape[0] != seqs:
             raise ValueError("pages [S, max_pages], q_start [S + 1] and kv_len [S] must agree on S")
-        for t in (pages, q_start, kv_len):
-            if t.device != self.k_pages.device:
-                raise ValueError("all tensors of a call must be on the cache's device")
-        return seqs
+        return seqs, width, ld if seqs > 1 else width
 
     def append(self, qkv: torch.Tensor, nh: int, pages: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
                q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, cos: torch.Tensor | None = None,
@@ -74,29 +73,37 @@ class PagedCache:
         `decode_ops.rope_tables` makes them; None: not). A row whose position is outside the tables or the cache gives
         a NaN q and writes nothing; rows behind q_start[S] are left alone."""
         hd, nkv = self.hd, self.nkv
-        if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] != (nh + 2 * nkv) * hd:
-            raise ValueError(f"qkv must be bf16 [T, {(nh + 2 * nkv) * hd}] with unit column stride")
-        rows = qkv.shape[0]
-        seqs = self._where(rows, pages, q_start, kv_len)
+        if qkv.dtype is not _BF16 or qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * hd:
+            raise ValueError(f"qkv must be bf16 [T, {(nh + 2 * nkv) * hd}]")
+        rows, width = qkv.shape
+        ldx, one = qkv.stride()
+        if one != 1:
+            raise ValueError("qkv must have unit column stride")
+        seqs, max_pages, ldp = self._where(pages, q_start, kv_len)
         if (q_norm is None) != (k_norm is None) or (cos is None) != (sin is None):
             raise ValueError("q_norm and k_norm, and cos and sin, come together")
-        for w, n in ((q_norm, nh * hd), (k_norm, nkv * hd)):
-            if w is not None and (w.dtype != torch.bfloat16 or w.numel() != n or not w.is_contiguous()):
-                raise ValueError(f"norm weights must be contiguous bf16 of {n} values")
+        qn = kn = cp = sp = None
+        if q_norm is not None:
+            if q_norm.dtype is not _BF16 or q_norm.numel() != nh * hd or not q_norm.is_contiguous() or \
+                    k_norm.dtype is not _BF16 or k_norm.numel() != nkv * hd or not k_norm.is_contiguous():
+                raise ValueError(f"norm weights must be contiguous bf16 of {nh * hd} and {nkv * hd} values")
+            qn, kn = q_norm.data_ptr(), k_norm.data_ptr()
         max_pos = 0
         if cos is not None:
             max_pos = cos.shape[0]
-            for t in (cos, sin):
-                if t.dtype != torch.float32 or tuple(t.shape) != (max_pos, hd // 2) or not t.is_contiguous():
-                    raise ValueError("cos and sin must be contiguous fp32 [max_pos, head_dim / 2]")
-        q = out if out is not None else torch.empty(rows, nh, hd, dtype=torch.bfloat16, device=qkv.device)
-        ldq = _head_rows("out", q, rows, nh, hd)
-        _lib.require_cuda(qkv, self.k_pages, pages, q_start, kv_len, q_norm, k_norm, cos, sin, q)
-        with _lib.on_device(qkv):
-            _lib.call("bp_paged_append", qkv.data_ptr(), qkv.stride(0) if rows > 1 else qkv.shape[1], _lib.ptr(q_norm), _lib.ptr(k_norm), _lib.ptr(cos),
-                      _lib.ptr(sin), max_pos, pages.data_ptr(), pages.stride(0) if seqs > 1 else pages.shape[1], pages.shape[1], q_start.data_ptr(),
-                      kv_len.data_ptr(), seqs, rows, self.k_pages.data_ptr(), self.v_pages.data_ptr(), self.num_pages,
-                      self.page_size, nh, nkv, hd, eps, q.data_ptr(), ldq, _lib.stream_of(qkv))
+            if cos.dtype is not _F32 or sin.dtype is not _F32 or cos.shape != (max_pos, hd // 2) or sin.shape != cos.shape or \
+                    not cos.is_contiguous() or not sin.is_contiguous():
+                raise ValueError("cos and sin must be contiguous fp32 [max_pos, head_dim / 2]")
+            cp, sp = cos.data_ptr(), sin.data_ptr()
+        dev = _lib.device_of(qkv, self.k_pages, pages, q_start, kv_len, q_norm, k_norm, cos, sin, out)
+        if out is None:
+            q, ldq = qkv.new_empty((rows, nh, hd)), nh * hd
+        else:
+            q, ldq = out, _head_rows("out", out, rows, nh, hd)
+        _lib.launch(dev, "bp_paged_append", qkv.data_ptr(), ldx if rows > 1 else width, qn, kn, cp, sp, max_pos,
+                    pages.data_ptr(), ldp, max_pages, q_start.data_ptr(), kv_len.data_ptr(), seqs, rows,
+                    self.k_pages.data_ptr(), self.v_pages.data_ptr(), self.num_pages, self.page_size, nh, nkv, hd, eps,
+                    q.data_ptr(), ldq)
         return q
 
     def attend(self, q: torch.Tensor, pages: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
@@ -106,30 +113,35 @@ class PagedCache:
         row that should see a page outside the cache gives NaN; rows behind q_start[S] are left alone."""
         if q.dim() != 3 or q.shape[2] != self.hd:
             raise ValueError(f"q must be [T, nh, {self.hd}]")
-        rows, nh = q.shape[0], q.shape[1]
+        rows, nh, hd = q.shape
         if nh % self.nkv or nh == 0:
             raise ValueError(f"nh = {nh} must be a multiple of n_kv_heads = {self.nkv}")
-        seqs = self._where(rows, pages, q_start, kv_len)
-        ldq = _head_rows("q", q, rows, nh, self.hd)
-        y = out if out is not None else torch.empty(rows, nh, self.hd, dtype=torch.bfloat16, device=q.device)
-        ldo = _head_rows("out", y, rows, nh, self.hd)
-        _lib.require_cuda(q, self.k_pages, pages, q_start, kv_len, y)
-        with _lib.on_device(q):
-            need = self._ws_bytes.get((rows, seqs, nh))
-            if need is None:
-                need = int(_lib.lib().bp_paged_attention_workspace_bytes(rows, seqs, nh, self.nkv, self.hd))
-                self._ws_bytes[(rows, seqs, nh)] = need
-            # scratch of this call alone, from torch's allocator: calls on several streams and captured graphs share none
-            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-            _lib.call("bp_paged_attention", q.data_ptr(), ldq, self.k_pages.data_ptr(), self.v_pages.data_ptr(),
-                      self.num_pages, self.page_size, pages.data_ptr(), pages.stride(0) if seqs > 1 else pages.shape[1], pages.shape[1], q_start.data_ptr(),
-                      kv_len.data_ptr(), seqs, rows, nh, self.nkv, self.hd, self.hd ** -0.5 if scale is None else scale,
-                      y.data_ptr(), ldo, ws.data_ptr(), need, _lib.stream_of(q))
+        seqs, max_pages, ldp = self._where(pages, q_start, kv_len)
+        ldq = _head_rows("q", q, rows, nh, hd)
+        dev = _lib.device_of(q, self.k_pages, pages, q_start, kv_len, out)
+        if out is None:
+            y, ldo = q.new_empty((rows, nh, hd)), nh * hd
+        else:
+            y, ldo = out, _head_rows("out", out, rows, nh, hd)
+        need = self._ws_bytes.get((rows, seqs, nh, dev))
+        if need is None:
+            with torch.cuda.device(dev):
+                need = int(_lib.lib().bp_paged_attention_workspace_bytes(rows, seqs, nh, self.nkv, hd))
+            self._ws_bytes[(rows, seqs, nh, dev)] = need
+        # scratch of this call alone, from torch's allocator: calls on several streams and captured graphs share none
+        ws = q.new_empty(need // 2)
+        _lib.launch(dev, "bp_paged_attention", q.data_ptr(), ldq, self.k_pages.data_ptr(), self.v_pages.data_ptr(),
+                    self.num_pages, self.page_size, pages.data_ptr(), ldp, max_pages, q_start.data_ptr(), kv_len.data_ptr(),
+                    seqs, rows, nh, self.nkv, hd, hd ** -0.5 if scale is None else scale, y.data_ptr(), ldo, ws.data_ptr(),
+                    need)
         return y
 
 
 def _head_rows(name: str, t: torch.Tensor, rows: int, nh: int, hd: int) -> int:
     """The row stride of a bf16 [rows, nh, hd] tensor whose rows are contiguous."""
-    if t.dtype != torch.bfloat16 or t.shape != (rows, nh, hd) or t.stride(2) != 1 or (nh > 1 and t.stride(1) != hd):
-        raise ValueError(f"{name} must be bf16 [{rows}, {nh}, {hd}] with contiguous (heads, head_dim) rows")
-    return t.stride(0) if rows > 1 else nh * hd
+    if t.dtype is not _BF16 or t.shape != (rows, nh, hd):
+        raise ValueError(f"{name} must be bf16 [{rows}, {nh}, {hd}]")
+    ld, lh, one = t.stride()
+    if one != 1 or (nh > 1 and lh != hd):
+        raise ValueError(f"{name} must have contiguous (heads, head_dim) rows")
+    return ld if rows > 1 else nh * hd

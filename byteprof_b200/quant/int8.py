@@ -65,11 +65,11 @@ def _rows_of(name: str, t: torch.Tensor) -> int:
     if t.dim() != 2:
         raise ValueError(f"{name} must be 2-D")
     rows, cols = t.shape
-    if t.stride(1) != 1 and cols > 1:
+    ld, one = t.stride()
+    if one != 1 and cols > 1:
         raise ValueError(f"{name} must have unit column stride")
     if rows <= 1:
         return (cols + 15) // 16 * 16  # one row: its stride means nothing
-    ld = t.stride(0)
     if ld < cols:
         raise ValueError(f"{name}'s rows overlap")
     return ld
@@ -84,36 +84,32 @@ def quantize_tokens_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     m, k = x.shape
     q = torch.empty(m, -(-k // 16) * 16, dtype=torch.int8, device=x.device)
     scale = torch.empty(m, dtype=torch.float32, device=x.device)
-    _lib.require_cuda(x)
-    with _lib.on_device(x):
-        _lib.call("bp_quantize_rows_int8", x.data_ptr(), ldx, q.data_ptr(), q.shape[1], scale.data_ptr(), m, k,
-                  _lib.stream_of(x))
+    _lib.launch(_lib.device_of(x), "bp_quantize_rows_int8", x.data_ptr(), ldx, q.data_ptr(), q.shape[1], scale.data_ptr(), m, k)
     return q[:, :k], scale
 
 
-def _operands(w: torch.Tensor, w_scale: torch.Tensor, bias, out, m: int, k: int, dev: torch.device):
-    """Checks the weights' side of a product; returns (ldw, w_scale's code, y, ldy, y's code)."""
-    if w.dtype != torch.int8:
+def _operands(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias, out, m: int, k: int):
+    """Checks the weights' side of a product with x; returns (device, ldw, w_scale's code, y, ldy, y's code)."""
+    if w.dtype is not torch.int8:
         raise ValueError("w must be int8 [N, K]")
     ldw = _rows_of("w", w)
-    n = w.shape[0]
-    if w.shape[1] != k:
-        raise ValueError(f"the operands must agree on K, got {k} and {w.shape[1]}")
-    if w_scale.dtype not in (torch.bfloat16, torch.float32) or w_scale.shape != (n,) or not w_scale.is_contiguous():
+    n, kw = w.shape
+    if kw != k:
+        raise ValueError(f"the operands must agree on K, got {k} and {kw}")
+    wsd = _SCALE_CODE.get(w_scale.dtype)
+    if wsd is None or w_scale.shape != (n,) or not w_scale.is_contiguous():
         raise ValueError("w_scale must be a contiguous bf16 or fp32 [N]")
-    if bias is not None and (bias.dtype != torch.bfloat16 or bias.shape != (n,) or not bias.is_contiguous()):
+    if bias is not None and (bias.dtype is not torch.bfloat16 or bias.shape != (n,) or not bias.is_contiguous()):
         raise ValueError("bias must be a contiguous bf16 [N]")
+    if out is not None and (out.dtype not in _SCALE_CODE or out.shape != (m, n)):
+        raise ValueError(f"out must be bf16 or fp32 [{m}, {n}]")
+    dev = _lib.device_of(x, w, w_scale, bias, out)
     if out is None:
-        y, ldy, code = torch.empty(m, n, dtype=torch.bfloat16, device=dev), n, _lib.BP_DTYPE_BF16
-    else:
-        y, ldy, code = out, _rows_of("out", out), _lib.dtype_code(out.dtype)
-        if y.shape != (m, n) or code not in (_lib.BP_DTYPE_BF16, _lib.BP_DTYPE_F32):
-            raise ValueError(f"out must be bf16 or fp32 [{m}, {n}]")
-        if y.device != dev:
-            raise ValueError("all tensors of a call must be on one device")
-    if w.device != dev or w_scale.device != dev or (bias is not None and bias.device != dev):
-        raise ValueError("all tensors of a call must be on one device")
-    return ldw, _lib.dtype_code(w_scale.dtype), y, ldy, code
+        return dev, ldw, wsd, x.new_empty((m, n), dtype=torch.bfloat16), n, _lib.BP_DTYPE_BF16
+    return dev, ldw, wsd, out, _rows_of("out", out), _SCALE_CODE[out.dtype]
+
+
+_SCALE_CODE = {torch.bfloat16: _lib.BP_DTYPE_BF16, torch.float32: _lib.BP_DTYPE_F32}
 
 
 def int8_mm(q: torch.Tensor, scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None,
@@ -127,11 +123,9 @@ def int8_mm(q: torch.Tensor, scale: torch.Tensor, w: torch.Tensor, w_scale: torc
     m, k = q.shape
     if scale.dtype != torch.float32 or scale.shape != (m,) or not scale.is_contiguous() or scale.device != q.device:
         raise ValueError("scale must be a contiguous fp32 [M] on q's device")
-    ldw, wsd, y, ldy, yd = _operands(w, w_scale, bias, out, m, k, q.device)
-    _lib.require_cuda(q)
-    with _lib.on_device(q):
-        _lib.call("bp_int8_mm", q.data_ptr(), ldq, scale.data_ptr(), w.data_ptr(), ldw, w_scale.data_ptr(), wsd,
-                  _lib.ptr(bias), y.data_ptr(), ldy, yd, m, w.shape[0], k, _lib.stream_of(q))
+    dev, ldw, wsd, y, ldy, yd = _operands(q, w, w_scale, bias, out, m, k)
+    _lib.launch(dev, "bp_int8_mm", q.data_ptr(), ldq, scale.data_ptr(), w.data_ptr(), ldw, w_scale.data_ptr(), wsd,
+                _lib.ptr(bias), y.data_ptr(), ldy, yd, m, w.shape[0], k)
     return y
 
 
@@ -143,12 +137,9 @@ def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: t
         raise ValueError("x must be bf16 [M, K]")
     ldx = _rows_of("x", x)
     m, k = x.shape
-    dev = x.device
-    ldw, wsd, y, ldy, yd = _operands(w, w_scale, bias, out, m, k, dev)
-    _lib.require_cuda(x)
-    with _lib.on_device(x):
-        need = (4 * m + 255) // 256 * 256 + m * ((k + 15) // 16 * 16)  # bp_int8_linear_workspace_bytes
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _lib.call("bp_int8_linear", x.data_ptr(), ldx, w.data_ptr(), ldw, w_scale.data_ptr(), wsd, _lib.ptr(bias),
-                  y.data_ptr(), ldy, yd, m, w.shape[0], k, ws.data_ptr(), need, _lib.stream_of(x))
+    dev, ldw, wsd, y, ldy, yd = _operands(x, w, w_scale, bias, out, m, k)
+    need = (4 * m + 255) // 256 * 256 + m * ((k + 15) // 16 * 16)  # bp_int8_linear_workspace_bytes
+    ws = x.new_empty((need + 1) // 2)
+    _lib.launch(dev, "bp_int8_linear", x.data_ptr(), ldx, w.data_ptr(), ldw, w_scale.data_ptr(), wsd, _lib.ptr(bias),
+                y.data_ptr(), ldy, yd, m, w.shape[0], k, ws.data_ptr(), need)
     return y

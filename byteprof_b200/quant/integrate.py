@@ -4,6 +4,9 @@ Same API as byteprof/quant/integrate.py:22-122:
   * `Int8Linear(lin)`: per-row int8 weights; one-row CUDA inputs run the int8 GEMV kernel
     (bp_gemv_int8), other row counts use the weights dequantized to the activation dtype with
     F.linear on the GPU (the reference's prefill path). Bias added as a separate op.
+    `Int8Linear(lin, act="int8")` quantizes bf16 activations too, one scale per row, and runs the 8-bit
+    integer product for every row count (bp_int8_linear; no counterpart in the reference); scheme
+    "int8_w8a8" of `apply_quantization` swaps it in.
   * `apply_quantization(model, target, scheme, group_size, local_scheme, global_scheme, kernel)`:
     the reference's selection rule (byteprof_b200.quant.select); kernel="skinny" swaps in
     `SkinnyLinear`, the default kernel swaps int8_wo linears for `Int8Linear`. The default int4_wo
@@ -18,13 +21,16 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .int8 import gemv_int8, quantize_rowwise_int8
+from .int8 import gemv_int8, int8_linear, quantize_rowwise_int8
 from .select import group_of, olmo_should_quantize, should_quantize
 
 
 class Int8Linear(nn.Module):
-    def __init__(self, lin: nn.Linear):
+    def __init__(self, lin: nn.Linear, act: str = "bf16"):
         super().__init__()
+        if act not in ("bf16", "int8"):
+            raise ValueError(f"act must be 'bf16' or 'int8', got {act!r}")
+        self.act = act
         self.in_features, self.out_features = lin.in_features, lin.out_features
         q, scale = quantize_rowwise_int8(lin.weight.data)
         self.register_buffer("q", q)
@@ -44,7 +50,12 @@ class Int8Linear(nn.Module):
             return x.new_empty(*x.shape[:-1], self.out_features)
         if not x2.is_cuda:
             raise ValueError("Int8Linear runs on CUDA tensors only (there is no CPU path)")
-        if x2.shape[0] == 1 and x2.dtype == torch.bfloat16:
+        if self.act == "int8" and x2.dtype == torch.bfloat16:
+            fused = self.bias if self.bias is not None and self.bias.dtype == torch.bfloat16 else None
+            y = int8_linear(x2.detach(), self.q, self.scale, None if fused is None else fused.detach())
+            if self.bias is not None and fused is None:
+                y = y + self.bias
+        elif x2.shape[0] == 1 and x2.dtype == torch.bfloat16:
             y = gemv_int8(x2, self.q, self.scale)
             if self.bias is not None:
                 y = y + self.bias
@@ -53,7 +64,8 @@ class Int8Linear(nn.Module):
         return y.reshape(*x.shape[:-1], self.out_features)
 
     def extra_repr(self) -> str:
-        return f"in_features={self.in_features}, out_features={self.out_features}, int8 rowwise (sm_100a GEMV)"
+        how = "int8 rowwise (sm_100a GEMV)" if self.act == "bf16" else "int8 x int8 (sm_100a tensor cores)"
+        return f"in_features={self.in_features}, out_features={self.out_features}, {how}"
 
 
 def _swap(model: nn.Module, name: str, make) -> None:
@@ -80,7 +92,10 @@ def apply_quantization(model: nn.Module, target: str, scheme: str, group_size: i
     for n in names:
         by_scheme.setdefault(scheme_of(n), []).append(n)
     for sch, group_names in by_scheme.items():
-        if kernel == "skinny":
+        if sch == "int8_w8a8":
+            for n in group_names:
+                _swap(model, n, lambda lin: Int8Linear(lin, act="int8"))
+        elif kernel == "skinny":
             from ..optim.skinny_linear import SkinnyLinear
 
             for n in group_names:
