@@ -12,6 +12,8 @@
 // its share and 2 c if it started before, and the join kernel merges them in CTA order.
 #pragma once
 
+#include <cuda.h>
+
 #include "bp_common.cuh"
 
 namespace bp {
@@ -64,6 +66,9 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int s) {
   r.pos0 = static_cast<long long>(kv) - (static_cast<long long>(e) - b) + (b0 - b);
   return r;
 }
+
+// Tensor maps of the cache (paged_attn.cu).
+int paged_maps(const PagedArgs& a, int box_rows, CUtensorMap* tk, CUtensorMap* tv);
 
 // The kernel for many rows (paged_attn_tc.cu): scratch bytes, and the launch (a's G, min_share and parts are set there).
 size_t paged_tc_workspace_bytes(int hd);

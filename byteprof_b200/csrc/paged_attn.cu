@@ -7,13 +7,17 @@
 //   over the keys with the running maximum m and sum; rows that see nothing give zeros.
 //
 // Few rows (single tokens, drafts, grouped heads of one token): memory bound, the keys and values are read once.
-// A unit is 64 keys x one tile of 16 packed rows; each of the 4 warps takes 16 of the 64 keys, straight from
-// global memory into the pieces that its threads hand to mma.sync: the head dimension is summed in an order that lets a thread
-// read 16 consecutive bytes of a key (the same order for q), and the output's columns are numbered so that a
-// thread reads 16 consecutive bytes of a value row. No shared memory, no barrier in the loop. The tensor core
+// A unit is 64 keys x one tile of 16 packed rows. One warp finds the pages and loads the keys and values by TMA (16 rows
+// of 64 dims a box, 128-byte swizzle) into a ring of 3 steps of 32 KB, two CTAs per SM; four warps take 16 keys each
+// of a step. The 16-byte pieces that a thread reads from the swizzled tiles are its mma.sync operands as they are: the
+// head dimension is summed in an order that lets a thread use 8 consecutive values of a key (the same order for q),
+// keys and output columns are numbered so that the 8 lanes of a shared-memory phase touch all banks. The tensor core
 // does 16 rows for the price of one here; 16 rows at HBM speed need a tenth of what mma.sync can do, so tcgen05 has
 // nothing to add. P is rounded to bf16 for the second product (its relative error, 2^-9 at most, averages out over
 // the keys; the sum l adds the unrounded fp32 values).
+// Against registers filled straight from global memory, one unit ahead: 64 streams of up to 8192 keys @@A
+#include <cudaTypedefs.h>
+
 #include "paged.cuh"
 #include "skinny_internal.h"
 #include "sm100.cuh"
@@ -23,9 +27,11 @@ namespace {
 
 constexpr int kRows = 16;   // packed rows per tile
 constexpr int kKeys = 64;   // keys per unit
-constexpr int kWarps = 4;
+constexpr int kWarps = 4;   // that compute; one more loads
 constexpr int kSlotRows = kWarps * kRows;  // rows of a part: up to 4 heads of a tile
-constexpr int kThreads = 32 * kWarps;
+constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kMathThreads = 32 * kWarps;
+constexpr int kStages = 3;
 constexpr float kLazy = 8.0f;  // the running maximum moves when a score exceeds it by this much (log2 units)
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t a0, const uint32_t a1, const uint32_t a2,
@@ -70,6 +76,7 @@ __device__ __forceinline__ long long share_of(const PagedArgs& a, long long tota
   return s > a.min_share ? s : a.min_share;
 }
 
+constexpr int kScan = kThreads / 32;
 // Sum of the units of all sequences, and (for the sequence holding unit `u`) that sequence and the units before it.
 // Every thread of the CTA calls it; `sm` is scratch.
 struct Located {
@@ -86,7 +93,7 @@ __device__ long long total_units(const PagedArgs& a, long long* sm) {
   __syncthreads();
   t = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) t += sm[w];
+  for (int w = 0; w < kThreads / 32; ++w) t += sm[w];
   __syncthreads();
   return t;
 }
@@ -103,21 +110,21 @@ __device__ Located locate(const PagedArgs& a, long long u, int hp, long long* sm
       if (lane >= o) pre += v;
     }
     if (lane == 31) sm[warp] = pre;
-    if (threadIdx.x == 0) sm[kWarps] = -1;
+    if (threadIdx.x == 0) sm[kScan] = -1;
     __syncthreads();
     long long off = base, sum = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kScan; ++w) {
       if (w < warp) off += sm[w];
       sum += sm[w];
     }
     pre += off - mine;  // units before s
     if (mine > 0 && u >= pre && u < pre + mine) {
-      sm[kWarps] = s;
-      sm[kWarps + 1] = pre;
+      sm[kScan] = s;
+      sm[kScan + 1] = pre;
     }
     __syncthreads();
-    const long long hit = sm[kWarps], before = sm[kWarps + 1];
+    const long long hit = sm[kScan], before = sm[kScan + 1];
     __syncthreads();
     if (hit >= 0) return {static_cast<int>(hit), before};
     base += sum;
@@ -125,109 +132,165 @@ __device__ Located locate(const PagedArgs& a, long long u, int hp, long long* sm
   return {-1, 0};
 }
 
-// Each warp has a ring of kStages units of its 16 keys and values; a thread copies exactly the 16-byte pieces that it
-// will read itself, piece i of lane l at [i][l], so that its own wait_group is all the synchronisation there is.
-constexpr int kStages = 3;
 template <int HD>
 struct FewSmem {
-  static constexpr int kPieces = 2 * (HD / 32) + 4 * (HD / 64);  // of the keys, then of the values
-  union {
-    uint4 ring[kWarps][kStages][kPieces][32];
-    struct {
-      float o[kWarps][kRows][HD + 4];
-      float m[kWarps][kRows], l[kWarps][kRows];
-    };
-  };
-  long long scan[kWarps + 2];
+  static constexpr int kWarpTile = kRows * HD * 2;             // 16 keys (or values) of a warp
+  static constexpr int kStageBytes = 2 * kWarps * kWarpTile;   // [warp][K, V][64 dims][16 rows][128 bytes]
+  uint8_t ring[kStages][kStageBytes];
+  float o[kWarps][kRows][64];
+  float m[kWarps][kRows], l[kWarps][kRows];
+  uint64_t full[kStages], empty[kStages];
+  int bad[kStages];
+  int abort;
+  long long scan[kScan + 2];
 };
 
-// 16 bytes global -> shared, zeros when !ok (nothing is read then).
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
-
-// Pages of a warp's 16 keys of a unit: of keys base.. and base + 8.. (a page holds at least 8 positions and base is a
-// multiple of 16).
-__device__ __forceinline__ void find_pages(const PagedArgs& a, const int* table, int base, int kv, int (&page)[2]) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) page[i] = base + 8 * i < kv ? __ldg(table + ((base + 8 * i) >> a.page_log2)) : 0;
-}
-
-// Requests the keys base + 8 i + lane / 4, dims 32 c + 8 (lane % 4) .., and the values base + 2 (lane % 4) + {0, 1, 8, 9},
-// dims 64 h + 8 (lane / 4) .. Past the end they are zero (what lies there may be NaN, and p = 0 would not hide it). `bad`:
-// the lowest position whose page is not in the pool.
-template <int HD>
-__device__ __forceinline__ void request(const PagedArgs& a, const int (&page)[2], int base, int kv, int h, int lane, uint32_t dst,
-                                        int& bad) {
-  const long long ld = static_cast<long long>(a.nkv) * HD;
-  const int in_page = base & ((1 << a.page_log2) - 1);
-  long long row[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int key = base + 8 * i;
-    const bool have = page[i] >= 0 && page[i] < a.num_pages;
-    if (!have && key < kv) bad = key < bad ? key : bad;
-    row[i] = !have || key >= kv ? -1
-                                : (static_cast<long long>(page[i]) << a.page_log2) + (a.page_log2 == 3 ? 0 : in_page + 8 * i);
+// A CTA's walk over its units: one segment (a range of units of one item) at a time.
+struct FewWalk {
+  PagedSeq q;
+  FewUnits fu;
+  int s, item, off, end;
+  long long before, u, u1;
+  __device__ __forceinline__ void segment() {
+    const long long rel = u - before;
+    item = static_cast<int>(rel / fu.per);
+    off = static_cast<int>(rel % fu.per);
+    end = static_cast<int>(fu.per - off < u1 - u ? fu.per : off + (u1 - u));
   }
-  dst += lane * 16;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int j = lane >> 2;
-    const bool ok = row[i] >= 0 && base + 8 * i + j < kv;
-    const __nv_bfloat16* p = a.kp + ((ok ? row[i] + j : 0) * ld + h * HD + (lane & 3) * 8);
-#pragma unroll
-    for (int c = 0; c < HD / 32; ++c) copy16(dst + (i * (HD / 32) + c) * 512, p + 32 * c, ok);
+  __device__ __forceinline__ void start(const PagedArgs& a, const Located& at, int hp, long long first, long long last) {
+    s = at.s;
+    before = at.before;
+    u = first;
+    u1 = last;
+    q = paged_seq(a, s);
+    fu = few_units(a, q, hp);
+    segment();
   }
-  dst += 2 * (HD / 32) * 512;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int j = 2 * (lane & 3) + (i & 1);
-    const bool ok = row[i >> 1] >= 0 && base + 8 * (i >> 1) + j < kv;
-    const __nv_bfloat16* p = a.vp + ((ok ? row[i >> 1] + j : 0) * ld + h * HD + (lane >> 2) * 8);
-#pragma unroll
-    for (int hh = 0; hh < HD / 64; ++hh) copy16(dst + (i * (HD / 64) + hh) * 512, p + 64 * hh, ok);
+  __device__ __forceinline__ bool next(const PagedArgs& a, int hp) {
+    u += end - off;
+    if (u >= u1) return false;
+    if (u - before >= fu.all) {  // on to the next sequence that has rows
+      before += fu.all;
+      do {
+        ++s;
+        q = paged_seq(a, s);
+      } while (q.n == 0);
+      fu = few_units(a, q, hp);
+    }
+    segment();
+    return true;
   }
-}
+};
 
 template <int HD>
-__global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const PagedArgs a) {
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  FewSmem<HD>& sm = *reinterpret_cast<FewSmem<HD>*>(smem_raw);
+__global__ void __launch_bounds__(kThreads, 2)
+    paged_few_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const PagedArgs a) {
+  using S = FewSmem<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  // The kernel has no static shared memory, so the dynamic part starts behind the first 1024 bytes, aligned for the
+  // swizzle; room to align it would cost the second CTA on the SM.
+  if ((smem_addr(smem_raw) & 1023u) != 0) {
+    if (threadIdx.x == 0) atomicOr(&g_bp_device_errors, BP_DEVERR_TIMEOUT);
+    return;
+  }
+  S& sm = *reinterpret_cast<S*>(smem_raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], kWarps);
+    }
+    sm.abort = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+  }
   pdl_launch_dependents();
   pdl_wait_prior_grids();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long one = total_units(a, sm.scan);
-  const int hp = heads_per_cta(a, one), hl = warp % hp, part = warp / hp, step = kKeys / hp;
+  volatile int* abort = &sm.abort;
+  const long long one = total_units(a, sm.scan);  // (its barriers also publish the initialised ones)
+  const int hp = heads_per_cta(a, one), step = kKeys / hp;
   const long long total = one / hp;
-  const long long share = share_of(a, total);
-  long long u = blockIdx.x * share;
-  const long long u1 = u + share < total ? u + share : total;
-  if (u >= u1) return;
-  const Located at = locate(a, u, hp, sm.scan);
-  int s = at.s;
-  long long before = at.before;
-  PagedSeq seq = paged_seq(a, s);
-  FewUnits fu = few_units(a, seq, hp);
-  while (true) {
-    // the segment of this item in the CTA's share
-    const long long rel = u - before;
-    const int item = static_cast<int>(rel / fu.per), off = static_cast<int>(rel % fu.per);
-    const int h = item / fu.tiles * hp + hl, tile = item % fu.tiles;
-    const int end = static_cast<int>(fu.per - off < u1 - u ? fu.per : off + (u1 - u));
-    const int* table = a.pages + static_cast<long long>(s) * a.ld_pages;
+  const long long share = share_of(a, total), u0 = blockIdx.x * share;
+  const long long u1 = u0 + share < total ? u0 + share : total;
+  if (u0 >= u1) return;
+  const Located at = locate(a, u0, hp, sm.scan);
+  FewWalk w;
+  w.start(a, at, hp, u0, u1);
 
+  if (warp == kWarps) {
+    // ---- pages and TMA: one box per lane ----
+    const int box = min(1 << a.page_log2, kRows), per = kRows / box;  // rows of a box, boxes per 16 keys
+    const int boxes = 2 * kWarps * (HD / 64) * per, none = a.num_pages << a.page_log2;
+    // lane: (key or value, 64 dims, warp, rows of its 16)
+    const int sub = lane % per, wi = lane / per % kWarps, half = lane / (per * kWarps) % (HD / 64), kv = lane / (per * kWarps * (HD / 64));
+    const int hl = wi % hp, part = wi / hp;
+    const uint32_t at_off = static_cast<uint32_t>(((wi * 2 + kv) * (HD / 64) + half) * kRows * 128 + sub * box * 128);
+    int n = 0;  // steps issued
+    bool ok = true;
+    do {
+      const int* table = a.pages + static_cast<long long>(w.s) * a.ld_pages;
+      const int h = w.item / w.fu.tiles * hp + hl;
+      const int s1 = w.end * hp;
+      // pages one step ahead of their use
+      int key = w.off * hp * step + part * kRows + sub * box;
+      int page = lane < boxes && key < w.q.kv ? __ldg(table + (key >> a.page_log2)) : -1;
+      for (int b = w.off * hp; b < s1; ++b, ++n) {
+        int row = none, bad = w.q.bad;
+        if (key < w.q.kv && lane < boxes) {
+          if (page >= 0 && page < a.num_pages)
+            row = (page << a.page_log2) + (key & ((1 << a.page_log2) - 1));
+          else
+            bad = min(bad, key);
+        }
+        bad = __reduce_min_sync(kPagedFull, bad);
+        key += step;
+        page = b + 1 < s1 && lane < boxes && key < w.q.kv ? __ldg(table + (key >> a.page_log2)) : -1;
+        const int st = n % kStages;
+        int go = 1;
+        if (lane == 0) {
+          if (n >= kStages) go = mbar_wait(&sm.empty[st], static_cast<uint32_t>((n / kStages) + 1) & 1u, abort);
+          if (go) {
+            sm.bad[st] = bad;
+            mbar_arrive_expect_tx(&sm.full[st], S::kStageBytes);
+          }
+        }
+        ok = __shfl_sync(kPagedFull, go, 0) != 0;
+        if (!ok) break;
+        if (lane < boxes) tma_load_3d(sm.ring[st] + at_off, kv == 0 ? &tk : &tv, &sm.full[st], half * 64, row, h);
+        __syncwarp();
+      }
+    } while (ok && w.next(a, hp));
+    if (lane == 0)  // no copy is in flight when the CTA ends
+      for (int st = 0; st < kStages && st < n; ++st) {
+        const unsigned long long t0 = globaltimer();
+        while (!mbar_try_wait(&sm.full[st], static_cast<uint32_t>((n - 1 - st) / kStages) & 1u)) {
+          if (globaltimer() - t0 > kWaitLimitNs) {
+            atomicOr(&g_bp_device_errors, BP_DEVERR_TIMEOUT);
+            break;
+          }
+        }
+      }
+    __syncwarp();
+    return;
+  }
+
+  const int hl = warp % hp, part = warp / hp, c4 = lane & 3, l4 = lane >> 2;
+  const int kperm = (l4 >> 1) + 4 * (l4 & 1);  // the key (of 8) behind MMA column l4, and the dims' chunk behind output column l4
+  int n = 0;
+  do {
+    const int h = w.item / w.fu.tiles * hp + hl, tile = w.item % w.fu.tiles;
     // q as the A operand: rows lane / 4 and lane / 4 + 8 of the tile, dims 32 c + 8 (lane % 4) ..
-    const int nrows = seq.n * a.g;  // packed rows of the sequence
+    const int nrows = w.q.n * a.g;  // packed rows of the sequence
     uint4 qa[HD / 32], qb[HD / 32];
     long long pos[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = tile * kRows + (lane >> 2) + 8 * i;
+      const int r = tile * kRows + l4 + 8 * i;
       const bool ok = r < nrows;
       const int tok = ok ? r / a.g : 0;
-      const __nv_bfloat16* p = a.q + (seq.first + tok) * a.ldq + (h * a.g + (ok ? r % a.g : 0)) * HD + (lane & 3) * 8;
-      pos[i] = ok ? seq.pos0 + tok : -1;
+      const __nv_bfloat16* p = a.q + (w.q.first + tok) * a.ldq + (h * a.g + (ok ? r % a.g : 0)) * HD + c4 * 8;
+      pos[i] = ok ? w.q.pos0 + tok : -1;
 #pragma unroll
       for (int c = 0; c < HD / 32; ++c) {
         const uint4 v = ok ? ldg16(p + 32 * c) : make_uint4(0, 0, 0, 0);
@@ -238,47 +301,39 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const PagedArgs 
 #pragma unroll
     for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    int bad = seq.bad;
-
-    // the ring is kStages units ahead, the pages one more
-    uint4(*ring)[FewSmem<HD>::kPieces][32] = sm.ring[warp];
-    int page[2];
-    const int s0 = off * hp, s1 = end * hp;  // steps of `step` keys of the segment, 16 of them this warp's
-#pragma unroll
-    for (int st = 0; st < kStages; ++st) {
-      const int base = (s0 + st) * step + part * 16;
-      if (s0 + st < s1) {
-        find_pages(a, table, base, seq.kv, page);
-        request<HD>(a, page, base, seq.kv, h, lane, smem_addr(ring[st]), bad);
+    int bad = w.q.bad;
+    bool dead = false;
+    for (int b = w.off * hp; b < w.end * hp; ++b, ++n) {
+      const int base = b * step + part * kRows, st = n % kStages;
+      const bool ok = mbar_wait(&sm.full[st], static_cast<uint32_t>(n / kStages) & 1u, abort);
+      if (!__all_sync(kPagedFull, ok)) {
+        dead = true;
+        break;
       }
-      cp_async_commit();
-    }
-    find_pages(a, table, (s0 + kStages) * step + part * 16, s0 + kStages < s1 ? seq.kv : 0, page);
-    int st = 0;
-    for (int b = s0; b < s1; ++b) {
-      const int base = b * step + part * 16;
-      cp_async_wait<kStages - 1>();
-      const uint4* kr = &ring[st][0][lane];
-      const uint4* vr = &ring[st][2 * (HD / 32)][lane];
+      bad = min(bad, sm.bad[st]);
+      // piece (row, chunk) of a tile is at row * 128 + (chunk ^ (row & 7)) * 16
+      const uint8_t* kt = sm.ring[st] + warp * 2 * S::kWarpTile;
+      const uint8_t* vt = kt + S::kWarpTile;
       float sc[2][4];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.0f;
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c) {
-          const uint4 k = kr[(i * (HD / 32) + c) * 32];
+          const int chunk = (c & 1) * 4 + c4;
+          const uint4 k = *reinterpret_cast<const uint4*>(kt + (c >> 1) * (kRows * 128) + (8 * i + kperm) * 128 + ((chunk ^ kperm) * 16));
           mma16816(sc[i], qa[c].x, qb[c].x, qa[c].y, qb[c].y, k.x, k.y);
           mma16816(sc[i], qa[c].z, qb[c].z, qa[c].w, qb[c].w, k.z, k.w);
         }
       }
-      // scores in log2 units, hidden keys -inf; sc[i][2 r + e] is row r (of the thread's two), key base + 8 i + 2 (lane % 4) + e
+      // scores in log2 units, hidden keys -inf; sc[i][2 r + e] is row r (of the thread's two), key base + 8 i + lane % 4 + 4 e
       float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int key = base + 8 * i + 2 * (lane & 3) + (e & 1);
-          sc[i][e] = key <= pos[e >> 1] && key < seq.kv ? sc[i][e] * a.scale_log2 : -INFINITY;
+          const int key = base + 8 * i + c4 + 4 * (e & 1);
+          sc[i][e] = key <= pos[e >> 1] && key < w.q.kv ? sc[i][e] * a.scale_log2 : -INFINITY;
           mx[e >> 1] = fmaxf(mx[e >> 1], sc[i][e]);
         }
 #pragma unroll
@@ -312,107 +367,93 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const PagedArgs 
         }
       const uint32_t a0 = pack2(p[0][0], p[0][1]), a1 = pack2(p[0][2], p[0][3]), a2 = pack2(p[1][0], p[1][1]),
                      a3 = pack2(p[1][2], p[1][3]);
+      // values of the keys lane % 4 + {0, 4, 8, 12}, dims 64 hh + 8 perm(lane / 4) ..
+      const bool tail = base + kRows > w.q.kv;  // what lies past the end may be NaN, and p = 0 would not hide it
 #pragma unroll
       for (int hh = 0; hh < HD / 64; ++hh) {
-        const uint4 v0 = vr[(0 * (HD / 64) + hh) * 32], v1 = vr[(1 * (HD / 64) + hh) * 32], v2 = vr[(2 * (HD / 64) + hh) * 32],
-                    v3 = vr[(3 * (HD / 64) + hh) * 32];
-        const uint32_t* w0 = &v0.x;
-        const uint32_t* w1 = &v1.x;
-        const uint32_t* w2 = &v2.x;
-        const uint32_t* w3 = &v3.x;
+        uint4 v[4];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          mma16816(o[8 * hh + 2 * w], a0, a1, a2, a3, __byte_perm(w0[w], w1[w], 0x5410), __byte_perm(w2[w], w3[w], 0x5410));
-          mma16816(o[8 * hh + 2 * w + 1], a0, a1, a2, a3, __byte_perm(w0[w], w1[w], 0x7632),
-                   __byte_perm(w2[w], w3[w], 0x7632));
+        for (int i = 0; i < 4; ++i) {
+          const int row = c4 + 4 * i;
+          v[i] = *reinterpret_cast<const uint4*>(vt + hh * (kRows * 128) + row * 128 + ((kperm ^ (row & 7)) * 16));
+          if (tail && base + row >= w.q.kv) v[i] = make_uint4(0, 0, 0, 0);
+        }
+        const uint32_t* w0 = &v[0].x;
+        const uint32_t* w1 = &v[1].x;
+        const uint32_t* w2 = &v[2].x;
+        const uint32_t* w3 = &v[3].x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          mma16816(o[8 * hh + 2 * j], a0, a1, a2, a3, __byte_perm(w0[j], w1[j], 0x5410), __byte_perm(w2[j], w3[j], 0x5410));
+          mma16816(o[8 * hh + 2 * j + 1], a0, a1, a2, a3, __byte_perm(w0[j], w1[j], 0x7632), __byte_perm(w2[j], w3[j], 0x7632));
         }
       }
-      if (b + kStages < s1) request<HD>(a, page, base + kStages * step, seq.kv, h, lane, smem_addr(ring[st]), bad);
-      cp_async_commit();
-      find_pages(a, table, base + (kStages + 1) * step, b + kStages + 1 < s1 ? seq.kv : 0, page);
-      st = st + 1 == kStages ? 0 : st + 1;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.empty[st]);
     }
-    // the 4 warps' parts meet in shared memory (the rings' memory: every warp is through with its own)
-    cp_async_wait<0>();
-    __syncthreads();
-    bad = __reduce_min_sync(kPagedFull, bad);
+    if (named_barrier_or(1, kMathThreads, dead)) return;  // (all four warps are in the same segment)
+    // the warps' parts meet in shared memory, 64 dims at a time
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       l[r] += __shfl_xor_sync(kPagedFull, l[r], 1);
       l[r] += __shfl_xor_sync(kPagedFull, l[r], 2);
-      const int row = (lane >> 2) + 8 * r;
-      if ((lane & 3) == 0) {
-        sm.m[warp][row] = m[r];
-        sm.l[warp][row] = pos[r] >= bad ? __int_as_float(0x7fc00000) : l[r];
+      if (c4 == 0) {
+        sm.m[warp][l4 + 8 * r] = m[r];
+        sm.l[warp][l4 + 8 * r] = pos[r] >= bad ? __int_as_float(0x7fc00000) : l[r];
       }
+    }
+    const bool whole = w.off == 0 && w.end == w.fu.per;
+    const int slot = 2 * blockIdx.x + (w.off == 0 ? 1 : 0);
 #pragma unroll
-      for (int hh = 0; hh < HD / 64; ++hh)
+    for (int hh = 0; hh < HD / 64; ++hh) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {  // column 2 (lane % 4) + e of tile j is dim 64 hh + 8 column + j
-          float* d = &sm.o[warp][row][64 * hh + (2 * (lane & 3) + e) * 8];
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {  // column 2 (lane % 4) + e of tile j is dim 64 hh + 8 (lane % 4 + 4 e) + j
+          float* d = &sm.o[warp][l4 + 8 * r][(c4 + 4 * e) * 8];
           *reinterpret_cast<float4*>(d) = make_float4(o[8 * hh][2 * r + e], o[8 * hh + 1][2 * r + e], o[8 * hh + 2][2 * r + e],
                                                       o[8 * hh + 3][2 * r + e]);
           *reinterpret_cast<float4*>(d + 4) = make_float4(o[8 * hh + 4][2 * r + e], o[8 * hh + 5][2 * r + e],
                                                           o[8 * hh + 6][2 * r + e], o[8 * hh + 7][2 * r + e]);
         }
-    }
-    __syncthreads();
-    const bool whole = off == 0 && end == fu.per;
-    const int slot = 2 * blockIdx.x + (off == 0 ? 1 : 0);
-    constexpr int kPer = HD / 8;  // dims per thread: 8 threads per row
-    for (int j = 0; j < hp; ++j) {  // warps j, j + hp, .. hold parts of head j
-      const int row = tid / 8, d0 = (tid % 8) * kPer, hj = item / fu.tiles * hp + j;
-      const int r = tile * kRows + row;
-      if (r < nrows) {
-        float mm = -INFINITY, ll = 0.0f, acc[kPer];
-        for (int w = j; w < kWarps; w += hp) mm = fmaxf(mm, sm.m[w][row]);
+      named_barrier_sync(1, kMathThreads);
+      const int row = tid / 8, d0 = (tid % 8) * 8, r = tile * kRows + row;  // 8 threads per row, 8 dims each
+      for (int j = 0; j < hp && r < nrows; ++j) {  // warps j, j + hp, .. hold parts of head j
+        const int hj = w.item / w.fu.tiles * hp + j;
+        float mm = -INFINITY, ll = 0.0f, acc[8];
+        for (int wi = j; wi < kWarps; wi += hp) mm = fmaxf(mm, sm.m[wi][row]);
 #pragma unroll
-        for (int d = 0; d < kPer; ++d) acc[d] = 0.0f;
-        for (int w = j; w < kWarps; w += hp) {
-          const float f = sm.m[w][row] == -INFINITY ? 0.0f : pg_ex2(sm.m[w][row] - mm);
-          ll += f == 0.0f && !isnan(sm.l[w][row]) ? 0.0f : f * sm.l[w][row];
+        for (int d = 0; d < 8; ++d) acc[d] = 0.0f;
+        for (int wi = j; wi < kWarps; wi += hp) {
+          const float f = sm.m[wi][row] == -INFINITY ? 0.0f : pg_ex2(sm.m[wi][row] - mm);
+          ll += f == 0.0f && !isnan(sm.l[wi][row]) ? 0.0f : f * sm.l[wi][row];
 #pragma unroll
-          for (int d = 0; d < kPer; ++d) acc[d] = fmaf(f, sm.o[w][row][d0 + d], acc[d]);
+          for (int d = 0; d < 8; ++d) acc[d] = fmaf(f, sm.o[wi][row][d0 + d], acc[d]);
         }
         if (whole) {
           const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-          uint32_t w[kPer / 2];
-#pragma unroll
-          for (int d = 0; d < kPer / 2; ++d) w[d] = pack2(acc[2 * d] * inv, acc[2 * d + 1] * inv);
-          __nv_bfloat16* dst = a.out + (seq.first + r / a.g) * a.ldo + (hj * a.g + r % a.g) * HD + d0;
-#pragma unroll
-          for (int d = 0; d < kPer / 8; ++d)
-            reinterpret_cast<uint4*>(dst)[d] = make_uint4(w[4 * d], w[4 * d + 1], w[4 * d + 2], w[4 * d + 3]);
+          __nv_bfloat16* dst = a.out + (w.q.first + r / a.g) * a.ldo + (hj * a.g + r % a.g) * HD + hh * 64 + d0;
+          *reinterpret_cast<uint4*>(dst) = make_uint4(pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv),
+                                                      pack2(acc[4] * inv, acc[5] * inv), pack2(acc[6] * inv, acc[7] * inv));
         } else {
-          const size_t at = static_cast<size_t>(slot) * kSlotRows + j * kRows + row;
-          float* dst = a.part_o + at * HD + d0;
-#pragma unroll
-          for (int d = 0; d < kPer / 4; ++d)
-            reinterpret_cast<float4*>(dst)[d] = make_float4(acc[4 * d], acc[4 * d + 1], acc[4 * d + 2], acc[4 * d + 3]);
-          if (d0 == 0) reinterpret_cast<float2*>(a.part_ml)[at] = make_float2(mm, ll);
+          const size_t at_row = static_cast<size_t>(slot) * kSlotRows + j * kRows + row;
+          float* dst = a.part_o + at_row * HD + hh * 64 + d0;
+          reinterpret_cast<float4*>(dst)[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+          reinterpret_cast<float4*>(dst)[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+          if (hh == 0 && d0 == 0) reinterpret_cast<float2*>(a.part_ml)[at_row] = make_float2(mm, ll);
         }
       }
+      named_barrier_sync(1, kMathThreads);  // sm.o is written again
     }
-    u += end - off;
-    if (u >= u1) break;
-    __syncthreads();  // sm.o is written again
-    if (u - before >= fu.all) {  // on to the next sequence that has rows
-      before += fu.all;
-      do {
-        ++s;
-        seq = paged_seq(a, s);
-      } while (seq.n == 0);
-      fu = few_units(a, seq, hp);
-    }
-  }
+  } while (w.next(a, hp));
 }
 
 // Joins the parts of the split items: one CTA per (row, head).
 template <int HD>
-__global__ void __launch_bounds__(kThreads) paged_few_join_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(kMathThreads) paged_few_join_kernel(const PagedArgs a) {
   __shared__ float sm_l[kWarps];
   __shared__ float sm_o[kWarps][HD];
-  __shared__ long long scan[kWarps + 2];
+  __shared__ long long scan[kWarps];
   __shared__ int found[1];
   pdl_launch_dependents();
   pdl_wait_prior_grids();
@@ -421,7 +462,7 @@ __global__ void __launch_bounds__(kThreads) paged_few_join_kernel(const PagedArg
   long long before = 0, total = 0;
   if (tid == 0) found[0] = -1;
   __syncthreads();
-  for (int s = tid; s < a.seqs; s += kThreads) {
+  for (int s = tid; s < a.seqs; s += kMathThreads) {
     const PagedSeq q = paged_seq(a, s);
     const long long n = few_units(a, q, 1).all;
     total += n;
@@ -498,28 +539,37 @@ bool few_rows(int rows, int seqs, int g) { return static_cast<long long>(rows) *
 int few_grid() { return kCtasPerSm * tc_sm_count(); }
 
 template <int HD>
-cudaError_t launch_few(const PagedArgs& a, cudaStream_t s) {
+int launch_few(const PagedArgs& a, cudaStream_t s) {
   static bool ready[64] = {false};
+  constexpr size_t smem = sizeof(FewSmem<HD>);
+  static_assert(2 * (smem + 1024) <= 228 * 1024, "two CTAs per SM");
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !ready[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(paged_few_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(sizeof(FewSmem<HD>)));
-    if (e != cudaSuccess) return e;
+    const cudaError_t e = cudaFuncSetAttribute(paged_few_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return fail(BP_ERR_CUDA, "cudaFuncSetAttribute(smem %zu): %s", smem, cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }
+  CUtensorMap tk, tv;
+  const int ps = 1 << a.page_log2;
+  int st = paged_maps(a, ps < kRows ? ps : kRows, &tk, &tv);
+  if (st != BP_OK) return st;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3(a.G);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(FewSmem<HD>);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   set_launch_attrs(cfg, attr);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, paged_few_kernel<HD>, a);
-  if (e != cudaSuccess) return e;
-  cfg.gridDim = dim3(a.rows, a.nh);
-  cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, paged_few_join_kernel<HD>, a);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, paged_few_kernel<HD>, tk, tv, a);
+  if (e == cudaSuccess) {
+    cfg.gridDim = dim3(a.rows, a.nh);
+    cfg.blockDim = dim3(kMathThreads);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, paged_few_join_kernel<HD>, a);
+  }
+  if (e != cudaSuccess) return fail(BP_ERR_CUDA, "paged_attention launch (few rows): %s", cudaGetErrorString(e));
+  return BP_OK;
 }
 
 }  // namespace
@@ -600,7 +650,22 @@ extern "C" int bp_paged_attention(const void* q, long long ldq, const void* k_pa
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + static_cast<size_t>(2 * a.G) * kSlotRows * head_dim;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = head_dim == 128 ? launch_few<128>(a, s) : launch_few<64>(a, s);
-  if (e != cudaSuccess) return fail(BP_ERR_CUDA, "paged_attention launch: %s", cudaGetErrorString(e));
-  return check_launch("paged_attention");
+  st = head_dim == 128 ? launch_few<128>(a, s) : launch_few<64>(a, s);
+  return st != BP_OK ? st : check_launch("paged_attention");
 }
+
+namespace bp {
+BP_DEFINE_DEVICE_ERROR_READER(read_device_errors_paged_few)
+
+// Maps of the cache's keys and values: [64 dims, box_rows positions, one kv head] at (dim, page * page_size + row, head).
+int paged_maps(const PagedArgs& a, int box_rows, CUtensorMap* tk, CUtensorMap* tv) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(a.hd), static_cast<uint64_t>(a.num_pages) << a.page_log2, static_cast<uint64_t>(a.nkv)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(a.nkv) * a.hd * 2, static_cast<uint64_t>(a.hd) * 2};
+  const uint32_t box[3] = {64, static_cast<uint32_t>(box_rows), 1};
+  const int st = tc_encode(tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.kp, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  if (st != BP_OK) return st;
+  return tc_encode(tv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.vp, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
+}  // namespace bp

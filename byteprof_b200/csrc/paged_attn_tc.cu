@@ -790,7 +790,6 @@ int launch(PagedArgs a, cudaStream_t stream) {
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }
   const int ps = 1 << a.page_log2;
-  const uint64_t rows = static_cast<uint64_t>(a.num_pages) << a.page_log2;
   CUtensorMap tq, tk, tv;
   const uint64_t qdims[3] = {HD, static_cast<uint64_t>(a.nh), static_cast<uint64_t>(a.rows)};
   const uint64_t qstrides[2] = {HD * 2, static_cast<uint64_t>(a.ldq) * 2};
@@ -798,14 +797,7 @@ int launch(PagedArgs a, cudaStream_t stream) {
   int st = tc_encode(&tq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.q, qdims, qstrides, qbox, CU_TENSOR_MAP_SWIZZLE_128B,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
   if (st != BP_OK) return st;
-  const uint64_t dims[3] = {HD, rows, static_cast<uint64_t>(a.nkv)};
-  const uint64_t strides[2] = {static_cast<uint64_t>(a.nkv) * HD * 2, HD * 2};
-  const uint32_t box[3] = {64, static_cast<uint32_t>(ps < kTile ? ps : kTile), 1};
-  st = tc_encode(&tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.kp, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
-                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
-  if (st != BP_OK) return st;
-  st = tc_encode(&tv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.vp, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
-                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  st = paged_maps(a, ps < kTile ? ps : kTile, &tk, &tv);
   if (st != BP_OK) return st;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];

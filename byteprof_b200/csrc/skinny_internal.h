@@ -70,5 +70,6 @@ unsigned int read_device_errors_glob();
 unsigned int read_device_errors_loc();
 unsigned int read_device_errors_int8mm();
 unsigned int read_device_errors_paged();
+unsigned int read_device_errors_paged_few();
 
 }  // namespace bp

@@ -689,7 +689,8 @@ BP_DEFINE_DEVICE_ERROR_READER(read_device_errors_tc)
 
 unsigned int read_and_clear_device_errors() {
   return read_device_errors_tc() | read_device_errors_i8() | read_device_errors_i4tc() | read_device_errors_glob() |
-         read_device_errors_loc() | read_device_errors_int8mm() | read_device_errors_paged();
+         read_device_errors_loc() | read_device_errors_int8mm() | read_device_errors_paged() |
+         read_device_errors_paged_few();
 }
 
 }  // namespace bp
