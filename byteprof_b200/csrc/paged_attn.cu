@@ -66,8 +66,8 @@ __device__ __forceinline__ FewUnits few_units(const PagedArgs& a, const PagedSeq
 // heads lie next to each other, so 4 at a time read 1 KB of DRAM in one go instead of 256 bytes here and the rest some
 // other time (head_dim 128); with too few units for that, the heads go to CTAs of their own. `one`: units at one head per CTA.
 __device__ __forceinline__ int heads_per_cta(const PagedArgs& a, long long one) {
-  if (a.nkv % 4 == 0 && one >= 16LL * a.G) return 4;
-  if (a.nkv % 2 == 0 && one >= 8LL * a.G) return 2;
+  if (a.nkv % 4 == 0 && one >= 64LL * a.G) return 4;
+  if (a.nkv % 2 == 0 && one >= 32LL * a.G) return 2;
   return 1;
 }
 
@@ -84,6 +84,7 @@ struct Located {
   long long before;
 };
 __device__ long long total_units(const PagedArgs& a, long long* sm) {
+  if (a.seqs == 1) return few_units(a, paged_seq(a, 0), 1).all;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long t = 0;
   for (int s = threadIdx.x; s < a.seqs; s += kThreads) t += few_units(a, paged_seq(a, s), 1).all;
@@ -98,6 +99,7 @@ __device__ long long total_units(const PagedArgs& a, long long* sm) {
   return t;
 }
 __device__ Located locate(const PagedArgs& a, long long u, int hp, long long* sm) {
+  if (a.seqs == 1) return {0, 0};
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long base = 0;
   for (int s0 = 0; s0 < a.seqs; s0 += kThreads) {
@@ -208,7 +210,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   pdl_launch_dependents();
   pdl_wait_prior_grids();
   volatile int* abort = &sm.abort;
-  const long long one = total_units(a, sm.scan);  // (its barriers also publish the initialised ones)
+  __syncthreads();  // the barriers are initialised
+  const long long one = total_units(a, sm.scan);
   const int hp = heads_per_cta(a, one), step = kKeys / hp;
   const long long total = one / hp;
   const long long share = share_of(a, total), u0 = blockIdx.x * share;
@@ -460,29 +463,36 @@ __global__ void __launch_bounds__(kMathThreads) paged_few_join_kernel(const Page
   const int t = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // the row's sequence, the units before it, and the total
   long long before = 0, total = 0;
-  if (tid == 0) found[0] = -1;
-  __syncthreads();
-  for (int s = tid; s < a.seqs; s += kMathThreads) {
-    const PagedSeq q = paged_seq(a, s);
-    const long long n = few_units(a, q, 1).all;
-    total += n;
-    if (q.first + q.n <= t) before += n;
-    if (q.n > 0 && t >= q.first && t < q.first + q.n) found[0] = s;
-  }
+  int s = 0;
+  if (a.seqs > 1) {
+    if (tid == 0) found[0] = -1;
+    __syncthreads();
+    for (int i = tid; i < a.seqs; i += kMathThreads) {
+      const PagedSeq q = paged_seq(a, i);
+      const long long n = few_units(a, q, 1).all;
+      total += n;
+      if (q.first + q.n <= t) before += n;
+      if (q.n > 0 && t >= q.first && t < q.first + q.n) found[0] = i;
+    }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(kPagedFull, before, o);
-    total += __shfl_xor_sync(kPagedFull, total, o);
+    for (int o = 16; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(kPagedFull, before, o);
+      total += __shfl_xor_sync(kPagedFull, total, o);
+    }
+    if (lane == 0) scan[warp] = before;
+    __syncthreads();
+    before = scan[0] + scan[1] + scan[2] + scan[3];
+    __syncthreads();
+    if (lane == 0) scan[warp] = total;
+    __syncthreads();
+    total = scan[0] + scan[1] + scan[2] + scan[3];
+    s = found[0];
+    if (s < 0) return;
+  } else {
+    const PagedSeq q = paged_seq(a, 0);
+    if (t < q.first || t >= q.first + q.n) return;
+    total = few_units(a, q, 1).all;
   }
-  if (lane == 0) scan[warp] = before;
-  __syncthreads();
-  before = scan[0] + scan[1] + scan[2] + scan[3];
-  __syncthreads();
-  if (lane == 0) scan[warp] = total;
-  __syncthreads();
-  total = scan[0] + scan[1] + scan[2] + scan[3];
-  const int s = found[0];
-  if (s < 0) return;
   const PagedSeq q = paged_seq(a, s);
   const int hp = heads_per_cta(a, total), h = head / a.g;
   const FewUnits fu = few_units(a, q, hp);
