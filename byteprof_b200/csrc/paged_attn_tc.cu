@@ -39,47 +39,11 @@ constexpr uint32_t kBase = 1024;          // shared-memory address of the tiles
 constexpr int kRegsLaunch = 168, kRegsLow = 120, kRegsHigh = 192;
 static_assert(128 * kRegsLow + 256 * kRegsHigh <= kThreads * kRegsLaunch, "register split");
 
-// 32 lanes x 128 TMEM columns into registers, complete when it returns.
-__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
-      "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
-      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, "
-      "%51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63, %64, %65, %66, %67, %68, %69, "
-      "%70, %71, %72, %73, %74, %75, %76, %77, %78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, "
-      "%89, %90, %91, %92, %93, %94, %95, %96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, "
-      "%107, %108, %109, %110, %111, %112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, "
-      "%123, %124, %125, %126, %127}, [%128];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
-        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
-        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
-        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
-        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]), "=r"(r[64]),
-        "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]), "=r"(r[72]),
-        "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]), "=r"(r[80]),
-        "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]),
-        "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]),
-        "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
-        "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]),
-        "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]),
-        "=r"(r[118]), "=r"(r[119]), "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]),
-        "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
-      : "r"(taddr)
-      : "memory");
-}
-
-// 32 lanes x 32 registers into TMEM columns (complete at tmem_st_wait).
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
-               "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-               "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-               "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-               "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+// 32 lanes x 16 registers into TMEM columns (complete at tmem_st_wait).
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+               "%15, %16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
+               "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -283,7 +247,7 @@ struct Smem {
   static constexpr int kTileBytes = kTile * HD * 2;
   uint8_t q[2][kTileBytes];
   uint8_t kv[kSlots][kTileBytes];
-  uint64_t full[kSlots], empty[kSlots], q_full[2], q_done[2], s_full[2], p_full[2][2], o_done[2], tail_go, tail, mma_done;
+  uint64_t full[kSlots], empty[kSlots], q_full[2], q_done[2], s_full[2], p_full[2], o_done[2], mma_done;
   int bad[kBadRing];
   uint32_t tmem_base;
   int abort;
@@ -324,6 +288,18 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&p);
 }
 
+// kChunk scores of a row; the columns from `lim` on are hidden when `masked`.
+constexpr int kChunk = 32;
+__device__ __forceinline__ void load_scores(uint32_t taddr, uint32_t (&x)[kChunk], bool masked, int lim) {
+  tmem_ld_32x32b_x32(taddr, x);
+#pragma unroll
+  for (int c = 0; c < kChunk; ++c) asm volatile("" : "+r"(x[c]));  // no use moves above the wait
+  if (masked) {
+#pragma unroll
+    for (int c = 0; c < kChunk; ++c) x[c] = c < lim ? x[c] : 0xff800000u;
+  }
+}
+
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -347,12 +323,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&s.q_full[i], 1);
       mbar_init(&s.q_done[i], 1);
       mbar_init(&s.s_full[i], 1);
-      mbar_init(&s.p_full[i][0], 4);
-      mbar_init(&s.p_full[i][1], 4);
+      mbar_init(&s.p_full[i], 5);  // 4 softmax warps and warp 2
       mbar_init(&s.o_done[i], 1);
     }
-    mbar_init(&s.tail_go, 1);
-    mbar_init(&s.tail, 32);
     mbar_init(&s.mma_done, 1);
     s.abort = 0;
     mbar_fence_init();
@@ -470,22 +443,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           else
             scores_of(i, 0);
         };
-        // the first or second 64 keys of a block
-        auto output_of = [&](int i, int slot, int half, uint32_t more) {
+        auto output_of = [&](int i, int slot, uint32_t more) {
 #pragma unroll
-          for (int k = 0; k < kTile / 32; ++k)
-            umma_f16_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + half * 32 + k * 8, dv + slot * kT + (half * 4 + k) * (2048 >> 4),
-                        idesc_o, k > 0 ? 1u : more);
+          for (int k = 0; k < kTile / 16; ++k)
+            umma_f16_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + k * 8, dv + slot * kT + k * (2048 >> 4), idesc_o,
+                        k > 0 ? 1u : more);
+          umma_commit(&s.o_done[i]);
         };
-        auto output = [&](int i, int blk, int half, uint32_t more) {
+        auto output = [&](int i, int blk, uint32_t more) {
           if (blk & 1)
-            output_of(i, 3, half, more);
+            output_of(i, 3, more);
           else
-            output_of(i, 1, half, more);
+            output_of(i, 1, more);
         };
         Walk w;
         int blk = 0;  // blocks so far: K of block blk is tile 2 blk of the ring, V tile 2 blk + 1
-        uint32_t seg[2] = {0, 0}, pn[2] = {0, 0}, tails = 0;  // phases: q_full and p_full per tile, tail
+        uint32_t seg[2] = {0, 0}, pn[2] = {0, 0};  // phases: q_full and p_full per tile
         bool ok = true;
         for (bool on = w.start(a, seq0, rel0, head0, count); on && ok; on = w.next(a)) {
           const int un[2] = {w.until(0), w.until(1)};
@@ -504,29 +477,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           umma_commit(&s.empty[(2 * blk) & 3]);
           for (int b = w.off; b < w.end; ++b, ++blk) {
             const bool more = b + 1 < w.end;
-            ok = mbar_wait(&s.full[(2 * blk + 1) & 3], (blk >> 1) & 1, abort);
-            if (ok && w.q.kv - b * kTile < kTile) {  // warp 2 clears what lies past the end
-              mbar_arrive(&s.tail_go);
-              ok = mbar_wait(&s.tail, tails++ & 1u, abort);
-            }
-            bool have_k = !more;
+            if (b >= un[0] && b >= un[1]) ok = mbar_wait(&s.full[(2 * blk + 1) & 3], (blk >> 1) & 1, abort);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               if (b < un[i] && ok) {
-                const uint32_t ph = pn[i]++ & 1u;
-                ok = mbar_wait(&s.p_full[i][0], ph, abort);
-                tc_fence_after_sync();
-                if (ok) output(i, blk, 0, b > w.off ? 1u : 0u);
-                ok = ok && mbar_wait(&s.p_full[i][1], ph, abort);
-                tc_fence_after_sync();
+                ok = mbar_wait(&s.p_full[i], pn[i]++ & 1u, abort);  // P, and (through warp 2) this block's V and the next K
                 if (!ok) break;
-                output(i, blk, 1, 1u);
-                umma_commit(&s.o_done[i]);
+                tc_fence_after_sync();
+                output(i, blk, b > w.off ? 1u : 0u);
                 if (b + 1 < un[i]) {
-                  if (!have_k) ok = mbar_wait(&s.full[(2 * blk + 2) & 3], ((blk + 1) >> 1) & 1, abort);
-                  if (!ok) break;
-                  have_k = true;
-                  tc_fence_after_sync();
                   scores(i, blk + 1);
                   if (b + 2 == un[i]) umma_commit(&s.q_done[i]);
                 }
@@ -541,27 +500,41 @@ __global__ void __launch_bounds__(kThreads, 1)
         wait_drain(&s.mma_done, 0);
       }
     } else if (warp == 2 && work) {
-      // ---- the last block of a sequence: values past its end may be NaN, which p = 0 does not hide ----
+      // ---- the fifth arrival at p_full: V of the block and K of the next have landed. A wait costs the issuing thread
+      // some 100 clocks in which the tensor cores run dry, so it has one per product. The values past a sequence's end
+      // may be NaN, which p = 0 does not hide: they are cleared here.
       Walk w;
       int blk = 0;
-      uint32_t tails = 0;
+      uint32_t pn[2] = {0, 0};
       bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        int go = 1;
+        if (lane == 0) go = mbar_wait(bar, parity, abort);
+        __syncwarp();
+        return __all_sync(kPagedFull, go != 0) != 0;
+      };
       for (bool on = w.start(a, seq0, rel0, head0, count); on && ok; on = w.next(a)) {
+        const int un[2] = {w.until(0), w.until(1)};
         for (int b = w.off; b < w.end && ok; ++b, ++blk) {
+          ok = wait(&s.full[(2 * blk + 1) & 3], (blk >> 1) & 1);
           const int valid = w.q.kv - b * kTile;
-          if (valid >= kTile) continue;
-          ok = mbar_wait(&s.tail_go, tails++ & 1u, abort);  // the tile has landed
-          if (!__all_sync(kPagedFull, ok)) {
-            ok = false;
-            break;
+          if (ok && valid < kTile) {
+            const int v0 = valid > 0 ? valid : 0;
+            for (int c = lane; c < (kTile - v0) * 8 * (HD / 64); c += 32) {
+              const int half = c / ((kTile - v0) * 8), r = c % ((kTile - v0) * 8);
+              *reinterpret_cast<uint4*>(s.kv[(2 * blk + 1) & 3] + half * kHalf + (v0 * 8 + r) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_async_shared();
+            __syncwarp();
           }
-          const int v0 = valid > 0 ? valid : 0;
-          for (int c = lane; c < (kTile - v0) * 8 * (HD / 64); c += 32) {
-            const int half = c / ((kTile - v0) * 8), r = c % ((kTile - v0) * 8);
-            *reinterpret_cast<uint4*>(s.kv[(2 * blk + 1) & 3] + half * kHalf + (v0 * 8 + r) * 16) = make_uint4(0, 0, 0, 0);
+          if (ok && b + 1 < w.end) ok = wait(&s.full[(2 * blk + 2) & 3], ((blk + 1) >> 1) & 1);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (b >= un[i] || !ok) continue;
+            if (pn[i] > 0) ok = wait(&s.p_full[i], (pn[i] + 1) & 1u);  // the phase before is complete
+            ++pn[i];
+            if (ok && lane == 0) mbar_arrive(&s.p_full[i]);
           }
-          fence_async_shared();
-          mbar_arrive(&s.tail);
         }
       }
     }
@@ -593,23 +566,22 @@ __global__ void __launch_bounds__(kThreads, 1)
               break;
             }
             tc_fence_after_sync();
-            uint32_t x[kTile];
-            tmem_ld128(ts, x);
             bad = min(bad, s.bad[(t0 + b - w.off) % kBadRing]);
             const long long lim = vis - static_cast<long long>(b) * kTile;
-            if (__any_sync(kPagedFull, lim < kTile)) {
-              const int lim32 = lim > kTile ? kTile : (lim < 0 ? 0 : static_cast<int>(lim));
+            const bool masked = __any_sync(kPagedFull, lim < kTile);
+            const int lim32 = lim > kTile ? kTile : (lim < 0 ? 0 : static_cast<int>(lim));
+            // Twice through the scores, kChunk columns at a time in rolled loops: they come from TMEM again faster than the
+            // code of 128 unrolled columns comes from the instruction cache (a second copy of it cost 110 us of 870).
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+            for (int c = 0; c < kTile; c += kChunk) {
+              uint32_t x[kChunk];
+              load_scores(ts + c, x, masked, lim32 - c);
 #pragma unroll
-              for (int c = 0; c < kTile; ++c) x[c] = c < lim32 ? x[c] : 0xff800000u;
+              for (int j = 0; j < kChunk; j += 8)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mx[k] = fmaxf(fmaxf(mx[k], __uint_as_float(x[j + k])), __uint_as_float(x[j + 4 + k]));
             }
-            float mx[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) mx[c] = fmaxf(__uint_as_float(x[c]), __uint_as_float(x[c + 4]));
-#pragma unroll
-            for (int c = 8; c < kTile; c += 8)
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                mx[j] = fmaxf(fmaxf(mx[j], __uint_as_float(x[c + j])), __uint_as_float(x[c + 4 + j]));
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
             if (__any_sync(kPagedFull, top > m + kLazy)) {
               const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.0f : pg_ex2(m - mn);
@@ -623,34 +595,36 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 tc_fence_after_sync();
 #pragma unroll 1
-                for (int c = 0; c < HD; c += 32) {
-                  uint32_t o[32];
-                  tmem_ld_32x32b_x32(to + c, o);
+                for (int c = 0; c < HD; c += 16) {
+                  float o[16];
+                  uint32_t v[16];
+                  tmem_ld_32x32b_x16(to + c, o);
 #pragma unroll
-                  for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                  tmem_st32(to + c, o);
+                  for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(o[j] * f);
+                  tmem_st16(to + c, v);
                 }
               }
             }
             const float neg = m == -INFINITY ? 0.0f : -m;
             const uint64_t sc2 = f32x2(sc, sc), neg2 = f32x2(neg, neg);
             uint64_t sum2[2] = {0, 0};
+#pragma unroll 1
+            for (int c = 0; c < kTile; c += kChunk) {  // P goes over scores that have been read
+              uint32_t x[kChunk], p[kChunk / 2];
+              load_scores(ts + c, x, masked, lim32 - c);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {  // 64 keys at a time: the second product starts on the first half
-              uint32_t p[32];
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const uint64_t y = fma_f32x2(f32x2(__uint_as_float(x[h * 64 + 2 * j]), __uint_as_float(x[h * 64 + 2 * j + 1])), sc2, neg2);
-                const float e0 = pg_ex2(f32x2_lo(y)), e1 = pg_ex2(f32x2_hi(y));
-                sum2[j & 1] = add_f32x2(sum2[j & 1], f32x2(e0, e1));
-                p[j] = pack2(e0, e1);
+              for (int j = 0; j < kChunk / 2; ++j) {
+                const uint64_t y = fma_f32x2(f32x2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), sc2, neg2);
+                const uint64_t e = f32x2(pg_ex2(f32x2_lo(y)), pg_ex2(f32x2_hi(y)));
+                sum2[j & 1] = add_f32x2(sum2[j & 1], e);
+                p[j] = pack2(f32x2_lo(e), f32x2_hi(e));
               }
-              tmem_st32(ts + h * 32, p);
-              tmem_st_wait();
-              tc_fence_before_sync();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&s.p_full[i][h]);
+              tmem_st16(ts + c / 2, p);
             }
+            tmem_st_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.p_full[i]);
             l += (f32x2_lo(sum2[0]) + f32x2_hi(sum2[0])) + (f32x2_lo(sum2[1]) + f32x2_hi(sum2[1]));
           }
           if (!ok) break;
