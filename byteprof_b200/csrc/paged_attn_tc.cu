@@ -39,11 +39,33 @@ constexpr uint32_t kBase = 1024;          // shared-memory address of the tiles
 constexpr int kRegsLaunch = 168, kRegsLow = 120, kRegsHigh = 192;
 static_assert(128 * kRegsLow + 256 * kRegsHigh <= kThreads * kRegsLaunch, "register split");
 
+// 32 lanes x 32 TMEM columns into registers, not waited for.
+__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
 // 32 lanes x 16 registers into TMEM columns (complete at tmem_st_wait).
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
                "%15, %16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
                "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+// 32 lanes x 32 registers into TMEM columns (complete at tmem_st_wait).
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+               "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+               "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+               "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+               "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
                : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -247,7 +269,7 @@ struct Smem {
   static constexpr int kTileBytes = kTile * HD * 2;
   uint8_t q[2][kTileBytes];
   uint8_t kv[kSlots][kTileBytes];
-  uint64_t full[kSlots], empty[kSlots], q_full[2], q_done[2], s_full[2], p_full[2], o_done[2], mma_done;
+  uint64_t full[kSlots], empty[2], q_full[2], q_done[2], s_full[2], p_full[2], o_done[2], mma_done;
   int bad[kBadRing];
   uint32_t tmem_base;
   int abort;
@@ -288,15 +310,18 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&p);
 }
 
-// kChunk scores of a row; the columns from `lim` on are hidden when `masked`.
 constexpr int kChunk = 32;
-__device__ __forceinline__ void load_scores(uint32_t taddr, uint32_t (&x)[kChunk], bool masked, int lim) {
-  tmem_ld_32x32b_x32(taddr, x);
+// N scores of a row; the columns from `lim` on are hidden when `masked`.
+template <int N>
+__device__ __forceinline__ void load_scores(uint32_t taddr, uint32_t (&x)[N], bool masked, int lim) {
 #pragma unroll
-  for (int c = 0; c < kChunk; ++c) asm volatile("" : "+r"(x[c]));  // no use moves above the wait
+  for (int c = 0; c < N; c += 32) tmem_ld32_nowait(taddr + c, x + c);
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int c = 0; c < N; ++c) asm volatile("" : "+r"(x[c]));  // no use moves above the wait
   if (masked) {
 #pragma unroll
-    for (int c = 0; c < kChunk; ++c) x[c] = c < lim ? x[c] : 0xff800000u;
+    for (int c = 0; c < N; ++c) x[c] = c < lim ? x[c] : 0xff800000u;
   }
 }
 
@@ -315,11 +340,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   Smem<HD>& s = *reinterpret_cast<Smem<HD>*>(smem_raw + (kBase - smem_addr(smem_raw)));
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kSlots; ++i) {
-      mbar_init(&s.full[i], 1);
-      mbar_init(&s.empty[i], 1);
-    }
+    for (int i = 0; i < kSlots; ++i) mbar_init(&s.full[i], 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.empty[i], 1);
       mbar_init(&s.q_full[i], 1);
       mbar_init(&s.q_done[i], 1);
       mbar_init(&s.s_full[i], 1);
@@ -383,7 +406,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int slot = issued % kSlots;
             int go = 1;
             if (lane == 0) {
-              if (issued >= kSlots) go = mbar_wait(&s.empty[slot], static_cast<uint32_t>((issued / kSlots) + 1) & 1u, abort);
+              // the slot's last tile, K(t - 2) or V(t - 2), was freed with pair t - 2 or t - 1 (pair p: V(p - 1) and K(p))
+              if (t >= 2) {
+                const int pair = t - 2 + kv;
+                go = mbar_wait(&s.empty[pair & 1], static_cast<uint32_t>(pair >> 1) & 1u, abort);
+              }
               if (go) mbar_arrive_expect_tx(&s.full[slot], kTileBytes);
             }
             ok = __shfl_sync(kPagedFull, go, 0) != 0;
@@ -448,7 +475,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < kTile / 16; ++k)
             umma_f16_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + k * 8, dv + slot * kT + k * (2048 >> 4), idesc_o,
                         k > 0 ? 1u : more);
-          umma_commit(&s.o_done[i]);
         };
         auto output = [&](int i, int blk, uint32_t more) {
           if (blk & 1)
@@ -474,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               scores(i, blk);
               if (w.off + 1 == un[i]) umma_commit(&s.q_done[i]);
             }
-          umma_commit(&s.empty[(2 * blk) & 3]);
+          umma_commit(&s.empty[blk & 1]);  // pair blk: the V before and this K
           for (int b = w.off; b < w.end; ++b, ++blk) {
             const bool more = b + 1 < w.end;
             if (b >= un[0] && b >= un[1]) ok = mbar_wait(&s.full[(2 * blk + 1) & 3], (blk >> 1) & 1, abort);
@@ -486,14 +512,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc_fence_after_sync();
                 output(i, blk, b > w.off ? 1u : 0u);
                 if (b + 1 < un[i]) {
-                  scores(i, blk + 1);
+                  scores(i, blk + 1);  // (its completion is also that of the product before)
                   if (b + 2 == un[i]) umma_commit(&s.q_done[i]);
+                } else {
+                  umma_commit(&s.o_done[i]);
                 }
               }
             }
             if (!ok) break;
-            umma_commit(&s.empty[(2 * blk + 1) & 3]);
-            if (more) umma_commit(&s.empty[(2 * blk + 2) & 3]);
+            if (more) umma_commit(&s.empty[(blk + 1) & 1]);
           }
         }
         umma_commit(&s.mma_done);
@@ -548,6 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float sc = a.scale_log2;
       Walk w;
       int n = 0, t0 = 0;  // blocks of this tile so far; blocks of the CTA before the segment
+      uint32_t segs = 0;  // segments of this tile so far
       bool ok = true;
       const int rt = r / a.g, rh = r % a.g;
       for (bool on = w.start(a, seq0, rel0, head0, count); on && ok; on = w.next(a)) {
@@ -576,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
             for (int c = 0; c < kTile; c += kChunk) {
               uint32_t x[kChunk];
-              load_scores(ts + c, x, masked, lim32 - c);
+              load_scores<kChunk>(ts + c, x, masked, lim32 - c);
 #pragma unroll
               for (int j = 0; j < kChunk; j += 8)
 #pragma unroll
@@ -587,13 +615,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.0f : pg_ex2(m - mn);
               m = mn;
               l *= f;
-              if (b > w.off) {  // O holds the blocks before, under the old maximum
-                ok = mbar_wait(&s.o_done[i], static_cast<uint32_t>(n - 1) & 1u, abort);
-                if (!__all_sync(kPagedFull, ok)) {
-                  ok = false;
-                  break;
-                }
-                tc_fence_after_sync();
+              if (b > w.off) {  // O holds the blocks before (s_full came after their last product), under the old maximum
 #pragma unroll 1
                 for (int c = 0; c < HD; c += 16) {
                   float o[16];
@@ -611,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
             for (int c = 0; c < kTile; c += kChunk) {  // P goes over scores that have been read
               uint32_t x[kChunk], p[kChunk / 2];
-              load_scores(ts + c, x, masked, lim32 - c);
+              load_scores<kChunk>(ts + c, x, masked, lim32 - c);
 #pragma unroll
               for (int j = 0; j < kChunk / 2; ++j) {
                 const uint64_t y = fma_f32x2(f32x2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), sc2, neg2);
@@ -621,14 +643,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               tmem_st16(ts + c / 2, p);
             }
+            l += (f32x2_lo(sum2[0]) + f32x2_hi(sum2[0])) + (f32x2_lo(sum2[1]) + f32x2_hi(sum2[1]));
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.p_full[i]);
-            l += (f32x2_lo(sum2[0]) + f32x2_hi(sum2[0])) + (f32x2_lo(sum2[1]) + f32x2_hi(sum2[1]));
           }
           if (!ok) break;
-          ok = mbar_wait(&s.o_done[i], static_cast<uint32_t>(n - 1) & 1u, abort);
+          ok = mbar_wait(&s.o_done[i], segs++ & 1u, abort);
           if (!__all_sync(kPagedFull, ok)) break;
           tc_fence_after_sync();
         }
