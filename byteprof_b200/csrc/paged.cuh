@@ -9,7 +9,8 @@
 // number of blocks whatever the lengths are, and the lengths are read on the device, so that a captured graph
 // serves every length. An item that lies in one CTA's share is written out by it; otherwise each CTA leaves its
 // part (running maximum, sum, unnormalised output; fp32) in the workspace, in slot 2 c + 1 if the item starts in
-// its share and 2 c if it started before, and the join kernel merges them in CTA order.
+// its share and 2 c if it started before, and names the item that it leaves unfinished; the join kernel merges the
+// parts in CTA order.
 #pragma once
 
 #include <cuda.h>
@@ -37,14 +38,22 @@ struct PagedArgs {
   long long ldo;
   float* part_o;     // [2 G, tile rows, hd]
   float* part_ml;    // [2 G, tile rows, 2]
+  int4* split;       // [G]: the item that starts in a CTA's share and goes on behind it
   int G;
   int min_share;
+  int tile_tokens;   // many rows: tokens per tile
 };
 
 __device__ __forceinline__ float pg_ex2(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
+}
+
+// What CTA c leaves for the join kernel: the item that starts in its share and whose parts end in CTA `last` (> c), as
+// (sequence, kv head or group of heads, tile, last); last = c: none.
+__device__ __forceinline__ void leave_split(const PagedArgs& a, int seq, int head, int tile, int last) {
+  a.split[blockIdx.x] = make_int4(seq, head, tile, last);
 }
 
 // A sequence as the kernels see it: rows clipped to the call's, cached length clipped to the table's.

@@ -216,7 +216,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   const long long total = one / hp;
   const long long share = share_of(a, total), u0 = blockIdx.x * share;
   const long long u1 = u0 + share < total ? u0 + share : total;
-  if (u0 >= u1) return;
+  if (u0 >= u1) {
+    if (tid == 0) leave_split(a, 0, 0, 0, blockIdx.x);
+    return;
+  }
   const Located at = locate(a, u0, hp, sm.scan);
   FewWalk w;
   w.start(a, at, hp, u0, u1);
@@ -231,7 +234,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     const uint32_t at_off = static_cast<uint32_t>(((wi * 2 + kv) * (HD / 64) + half) * kRows * 128 + sub * box * 128);
     int n = 0;  // steps issued
     bool ok = true;
+    int4 open = make_int4(0, 0, 0, blockIdx.x);
     do {
+      if (w.off == 0 && w.end < w.fu.per)
+        open = make_int4(w.s, w.item / w.fu.tiles, w.item % w.fu.tiles,
+                         blockIdx.x + static_cast<int>((w.fu.per - w.end + share - 1) / share));
       const int* table = a.pages + static_cast<long long>(w.s) * a.ld_pages;
       const int h = w.item / w.fu.tiles * hp + hl;
       const int s1 = w.end * hp;
@@ -264,6 +271,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         __syncwarp();
       }
     } while (ok && w.next(a, hp));
+    if (lane == 0) leave_split(a, open.x, open.y | hp << 24, open.z, open.w);
     if (lane == 0)  // no copy is in flight when the CTA ends
       for (int st = 0; st < kStages && st < n; ++st) {
         const unsigned long long t0 = globaltimer();
@@ -451,89 +459,59 @@ __global__ void __launch_bounds__(kThreads, 2)
   } while (w.next(a, hp));
 }
 
-// Joins the parts of the split items: one CTA per (row, head).
+// Joins the item that CTA c left unfinished: block (c, y) takes its rows y, y + kJoinY, .. (a row of 64: 4 heads of 16),
+// the parts of a row dealt to its 4 warps.
+constexpr int kJoinY = 8;
 template <int HD>
 __global__ void __launch_bounds__(kMathThreads) paged_few_join_kernel(const PagedArgs a) {
   __shared__ float sm_l[kWarps];
   __shared__ float sm_o[kWarps][HD];
-  __shared__ long long scan[kWarps];
-  __shared__ int found[1];
   pdl_launch_dependents();
   pdl_wait_prior_grids();
-  const int t = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // the row's sequence, the units before it, and the total
-  long long before = 0, total = 0;
-  int s = 0;
-  if (a.seqs > 1) {
-    if (tid == 0) found[0] = -1;
-    __syncthreads();
-    for (int i = tid; i < a.seqs; i += kMathThreads) {
-      const PagedSeq q = paged_seq(a, i);
-      const long long n = few_units(a, q, 1).all;
-      total += n;
-      if (q.first + q.n <= t) before += n;
-      if (q.n > 0 && t >= q.first && t < q.first + q.n) found[0] = i;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      before += __shfl_xor_sync(kPagedFull, before, o);
-      total += __shfl_xor_sync(kPagedFull, total, o);
-    }
-    if (lane == 0) scan[warp] = before;
-    __syncthreads();
-    before = scan[0] + scan[1] + scan[2] + scan[3];
-    __syncthreads();
-    if (lane == 0) scan[warp] = total;
-    __syncthreads();
-    total = scan[0] + scan[1] + scan[2] + scan[3];
-    s = found[0];
-    if (s < 0) return;
-  } else {
-    const PagedSeq q = paged_seq(a, 0);
-    if (t < q.first || t >= q.first + q.n) return;
-    total = few_units(a, q, 1).all;
-  }
-  const PagedSeq q = paged_seq(a, s);
-  const int hp = heads_per_cta(a, total), h = head / a.g;
-  const FewUnits fu = few_units(a, q, hp);
-  const long long share = share_of(a, total / hp);
-  const int pr = (t - q.first) * a.g + head % a.g;
-  const long long a0 = before / hp + (static_cast<long long>(h / hp) * fu.tiles + pr / kRows) * fu.per;
-  const int c0 = static_cast<int>(a0 / share), c1 = static_cast<int>((a0 + fu.per - 1) / share);
-  if (c0 == c1) return;
-  const int row = h % hp * kRows + pr % kRows;
+  const int c0 = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int4 open = a.split[c0];
+  const int c1 = open.w;
+  if (c1 <= c0) return;
+  const PagedSeq q = paged_seq(a, open.x);
+  const int hp = open.y >> 24, h0 = (open.y & 0xffffff) * hp, nrows = q.n * a.g - open.z * kRows;  // packed rows of the tile
+  const int live = min(nrows, kRows);
   constexpr int kPer = HD / 32;
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
-  float m = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, ml[static_cast<size_t>(2 * c + (c == c0)) * kSlotRows + row].x);
+  for (int k = blockIdx.y; k < hp * live; k += kJoinY) {
+    const int j = k / live, pr = open.z * kRows + k % live, row = j * kRows + k % live;
+    float m = -INFINITY;
+    for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, ml[static_cast<size_t>(2 * c + (c == c0)) * kSlotRows + row].x);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kPagedFull, m, o));
-  float l = 0.0f, acc[kPer];
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kPagedFull, m, o));
+    float l = 0.0f, acc[kPer];
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) acc[j] = 0.0f;
+    for (int d = 0; d < kPer; ++d) acc[d] = 0.0f;
 #pragma unroll 4
-  for (int c = c0 + warp; c <= c1; c += kWarps) {
-    const size_t at = static_cast<size_t>(2 * c + (c == c0)) * kSlotRows + row;
-    const float2 p = ml[at];
-    const float f = p.x == -INFINITY ? 0.0f : pg_ex2(p.x - m);
-    l += f == 0.0f && !isnan(p.y) ? 0.0f : f * p.y;
-    const float* src = a.part_o + at * HD + lane * kPer;
+    for (int c = c0 + warp; c <= c1; c += kWarps) {
+      const size_t at = static_cast<size_t>(2 * c + (c == c0)) * kSlotRows + row;
+      const float2 p = ml[at];
+      const float f = p.x == -INFINITY ? 0.0f : pg_ex2(p.x - m);
+      l += f == 0.0f && !isnan(p.y) ? 0.0f : f * p.y;
+      const float* src = a.part_o + at * HD + lane * kPer;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) acc[j] = fmaf(f, src[j], acc[j]);
-  }
-  if (lane == 0) sm_l[warp] = l;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) sm_o[warp][lane * kPer + j] = acc[j];
-  __syncthreads();
-  if (tid < HD) {
-    float v = 0.0f;
-    l = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      l += sm_l[w];
-      v += sm_o[w][tid];
+      for (int d = 0; d < kPer; ++d) acc[d] = fmaf(f, src[d], acc[d]);
     }
-    a.out[t * a.ldo + head * HD + tid] = __float2bfloat16_rn(l == 0.0f ? 0.0f : v / l);
+    if (lane == 0) sm_l[warp] = l;
+#pragma unroll
+    for (int d = 0; d < kPer; ++d) sm_o[warp][lane * kPer + d] = acc[d];
+    __syncthreads();
+    if (tid < HD) {
+      float v = 0.0f;
+      l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        l += sm_l[w];
+        v += sm_o[w][tid];
+      }
+      a.out[static_cast<long long>(q.first + pr / a.g) * a.ldo + ((h0 + j) * a.g + pr % a.g) * HD + tid] =
+          __float2bfloat16_rn(l == 0.0f ? 0.0f : v / l);
+    }
+    __syncthreads();
   }
 }
 
@@ -573,7 +551,7 @@ int launch_few(const PagedArgs& a, cudaStream_t s) {
   set_launch_attrs(cfg, attr);
   cudaError_t e = cudaLaunchKernelEx(&cfg, paged_few_kernel<HD>, tk, tv, a);
   if (e == cudaSuccess) {
-    cfg.gridDim = dim3(a.rows, a.nh);
+    cfg.gridDim = dim3(a.G, kJoinY);
     cfg.blockDim = dim3(kMathThreads);
     cfg.dynamicSmemBytes = 0;
     e = cudaLaunchKernelEx(&cfg, paged_few_join_kernel<HD>, a);
@@ -588,7 +566,8 @@ int launch_few(const PagedArgs& a, cudaStream_t s) {
 extern "C" size_t bp_paged_attention_workspace_bytes(int rows, int seqs, int nh, int nkv, int head_dim) {
   using namespace bp;
   if (rows <= 0 || seqs <= 0 || nkv <= 0 || nh < nkv || head_dim <= 0) return 0;
-  return few_rows(rows, seqs, nh / nkv) ? static_cast<size_t>(2 * few_grid()) * kSlotRows * (head_dim + 2) * sizeof(float)
+  return few_rows(rows, seqs, nh / nkv) ? static_cast<size_t>(2 * few_grid()) * kSlotRows * (head_dim + 2) * sizeof(float) +
+                                              few_grid() * sizeof(int4)
                                         : paged_tc_workspace_bytes(head_dim);
 }
 
@@ -659,6 +638,7 @@ extern "C" int bp_paged_attention(const void* q, long long ldq, const void* k_pa
   a.min_share = 1;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + static_cast<size_t>(2 * a.G) * kSlotRows * head_dim;
+  a.split = reinterpret_cast<int4*>(a.part_ml + static_cast<size_t>(2 * a.G) * kSlotRows * 2);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   st = head_dim == 128 ? launch_few<128>(a, s) : launch_few<64>(a, s);
   return st != BP_OK ? st : check_launch("paged_attention");

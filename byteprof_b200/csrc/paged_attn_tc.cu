@@ -94,7 +94,7 @@ __host__ __device__ constexpr uint64_t umma_desc_mn_at(uint32_t saddr, uint32_t 
 
 // ---- the cut of the work ----------------------------------------------------------------------------------
 // A tile holds the g heads of 128 / g tokens (g <= 128; the few rows left over idle), an item two tiles.
-__device__ __forceinline__ int tile_tokens(const PagedArgs& a) { return kTile / a.g; }
+__device__ __forceinline__ int tile_tokens(const PagedArgs& a) { return a.tile_tokens; }  // kTile / g
 __device__ __forceinline__ int item_tiles(const PagedArgs& a, int n) { return (n + 2 * tile_tokens(a) - 1) / (2 * tile_tokens(a)); }
 // Blocks of 128 keys that the tokens up to `last` (exclusive) of a sequence see.
 __device__ __forceinline__ int blocks_of(const PagedSeq& q, int last) {
@@ -114,11 +114,56 @@ struct Scan {
   int seq;
 };
 
+__device__ __forceinline__ long long share_of(const PagedArgs& a, long long total) {
+  const long long s = (total + a.G - 1) / a.G;
+  return s > a.min_share ? s : a.min_share;
+}
+
+// A CTA's start: the sequence of its first unit, that unit's place behind the sequence's first, the units of one of its
+// kv heads, and how many units are the CTA's (0: none).
+struct Start {
+  long long share, rel, head, count;
+  int seq;
+};
+
+// Up to 32 sequences: every warp finds it by itself, 32 / seqs lanes per sequence (a cut with barriers between all the
+// warps took 10 us in front of the first load).
+__device__ __forceinline__ Start find_start_few(const PagedArgs& a) {
+  const int lane = threadIdx.x & 31;
+  int lanes = 32;
+  while (lanes * a.seqs > 32) lanes >>= 1;
+  const int seq = lane / lanes, sub = lane % lanes;
+  long long u = 0;
+  if (seq < a.seqs) {
+    const PagedSeq q = paged_seq(a, seq);
+    const int nt = item_tiles(a, q.n);
+    for (int t = sub; t < nt; t += lanes) u += item_units(a, q, t);
+  }
+  for (int o = lanes / 2; o > 0; o >>= 1) u += __shfl_xor_sync(kPagedFull, u, o);
+  const long long mine = sub == 0 ? u * a.nkv : 0;
+  long long pre = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(kPagedFull, pre, o);
+    if (lane >= o) pre += v;
+  }
+  const long long total = __shfl_sync(kPagedFull, pre, 31);
+  Start st;
+  st.share = share_of(a, total);
+  const long long u0 = blockIdx.x * st.share;
+  st.count = total - u0 < st.share ? total - u0 : st.share;
+  const unsigned hit = __ballot_sync(kPagedFull, mine > 0 && u0 >= pre - mine && u0 < pre);
+  const int src = hit != 0 ? __ffs(hit) - 1 : 0;
+  st.seq = src / lanes;
+  st.rel = u0 - __shfl_sync(kPagedFull, pre - mine, src);
+  st.head = __shfl_sync(kPagedFull, u, src);
+  return st;
+}
+
 // units[] of the sequences s0 .. s0 + kScanSeqs: 8 lanes per sequence; called by all threads, ends with a barrier.
-template <int kN>
-__device__ void scan_units(const PagedArgs& a, Scan& sc, int s0) {
+__device__ __noinline__ void scan_units(const PagedArgs& a, Scan& sc, int s0) {
   const int count = min(kScanSeqs, a.seqs - s0), sub = threadIdx.x & 7;
-  for (int i = threadIdx.x / 8; i - (threadIdx.x & 31) / 8 < count; i += kN / 8) {
+  for (int i = threadIdx.x / 8; i - (threadIdx.x & 31) / 8 < count; i += kThreads / 8) {
     long long u = 0;
     if (i < count) {
       const PagedSeq q = paged_seq(a, s0 + i);
@@ -132,43 +177,36 @@ __device__ void scan_units(const PagedArgs& a, Scan& sc, int s0) {
   __syncthreads();
 }
 
-__device__ __forceinline__ long long share_of(const PagedArgs& a, long long total) {
-  const long long s = (total + a.G - 1) / a.G;
-  return s > a.min_share ? s : a.min_share;
-}
-
-// The total of all units (sc.total).
-template <int kN>
-__device__ void scan_total(const PagedArgs& a, Scan& sc) {
+// Any number of sequences; all threads.
+__device__ __noinline__ Start find_start_many(const PagedArgs& a, Scan& sc) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long total = 0;
   for (int s0 = 0; s0 < a.seqs; s0 += kScanSeqs) {
-    scan_units<kN>(a, sc, s0);
+    scan_units(a, sc, s0);
     const int count = min(kScanSeqs, a.seqs - s0);
-    for (int i = threadIdx.x; i < count; i += kN) total += sc.units[i];
+    for (int i = threadIdx.x; i < count; i += kThreads) total += sc.units[i];
     if (s0 + kScanSeqs < a.seqs) __syncthreads();
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(kPagedFull, total, o);
   if (lane == 0) sc.warp_sum[warp] = total;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    total = 0;
-    for (int w = 0; w < kN / 32; ++w) total += sc.warp_sum[w];
-    sc.total = total * a.nkv;
-  }
-  __syncthreads();
-}
-
-// The sequence of unit u (sc.seq) and the units before it (sc.before); after scan_total. All threads.
-template <int kN>
-__device__ void scan_find(const PagedArgs& a, Scan& sc, long long u) {
+  total = 0;
+  for (int w = 0; w < kWarps; ++w) total += sc.warp_sum[w];
+  total *= a.nkv;
+  Start st;
+  st.share = share_of(a, total);
+  const long long u = blockIdx.x * st.share;
+  st.count = total - u < st.share ? total - u : st.share;
+  st.seq = 0;
+  st.rel = 0;
+  st.head = 1;
+  if (st.count <= 0) return st;  // (the same for the whole CTA)
   long long base = 0;
   for (int s0 = 0; s0 < a.seqs; s0 += kScanSeqs) {
-    if (a.seqs > kScanSeqs) scan_units<kN>(a, sc, s0);
+    if (a.seqs > kScanSeqs) scan_units(a, sc, s0);
     const int count = min(kScanSeqs, a.seqs - s0);
     if (threadIdx.x < 32) {
-      const int lane = threadIdx.x;
       long long run = base;
       int hit = -1;
       long long hit_before = 0;
@@ -184,7 +222,7 @@ __device__ void scan_find(const PagedArgs& a, Scan& sc, long long u) {
         const unsigned m = __ballot_sync(kPagedFull, mine > 0 && u >= start && u < start + mine);
         if (m != 0) {
           const int src = __ffs(m) - 1;
-          hit = s0 + i0 + src;
+          hit = i0 + src;
           hit_before = __shfl_sync(kPagedFull, start, src);
           break;
         }
@@ -196,10 +234,16 @@ __device__ void scan_find(const PagedArgs& a, Scan& sc, long long u) {
       }
     }
     __syncthreads();
-    if (sc.seq >= 0) return;
+    if (sc.seq >= 0) {
+      st.seq = s0 + sc.seq;
+      st.rel = u - sc.before;
+      st.head = sc.units[sc.seq];
+      return st;
+    }
     base = sc.before;
     __syncthreads();
   }
+  return st;
 }
 
 // A CTA's walk over its units: one segment (a range of key blocks of one item) at a time. Every role walks by itself.
@@ -208,6 +252,7 @@ struct Walk {
   int s, h, tile, tiles;
   int off, end, per;        // the segment's blocks, the item's
   int blocks[2];            // what each tile sees of the item
+  int rest;                 // the item's units behind the segment
   long long left;           // units of the CTA after this segment
 
   __device__ __forceinline__ void enter(const PagedArgs& a) {
@@ -222,12 +267,17 @@ struct Walk {
     off = max(v0 - kSetup, 0);
     end = max(v1 - kSetup, 0);
   }
-  // `rel`: units behind the start of sequence `seq`, each kv head of which has `head` units. False: nothing to do.
-  __device__ bool start(const PagedArgs& a, int seq, long long rel, long long head, long long count) {
-    s = seq;
+  // False: nothing to do.
+  __device__ bool start(const PagedArgs& a, const Start& st) {
+    const long long rel = st.rel, head = st.head, count = st.count;
+    s = st.seq;
     enter(a);
-    h = static_cast<int>(rel / head);
-    long long r = rel % head;
+    if ((rel | head) >> 32 == 0) {
+      h = static_cast<uint32_t>(rel) / static_cast<uint32_t>(head);
+    } else {
+      h = static_cast<int>(rel / head);
+    }
+    long long r = rel - h * head;
     int n;
     for (tile = 0;; ++tile) {
       n = item_units(a, q, tile);
@@ -237,6 +287,7 @@ struct Walk {
     per = n - kSetup;
     const int v0 = static_cast<int>(r), v1 = static_cast<int>(n - v0 < count ? n : v0 + count);
     segment(a, v0, v1);
+    rest = n - v1;
     left = count - (v1 - v0);
     return off < end || next(a);
   }
@@ -255,6 +306,7 @@ struct Walk {
       const int n = item_units(a, q, tile), v1 = static_cast<int>(n < left ? n : left);
       per = n - kSetup;
       segment(a, 0, v1);
+      rest = n - v1;
       left -= v1;
       if (off < end) return true;  // (the share may end in an item's setup: nothing of it is done here)
     }
@@ -368,14 +420,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's
   volatile int* abort = &s.abort;
 
-  scan_total<kThreads>(a, s.scan);
-  const long long share = share_of(a, s.scan.total), u0 = blockIdx.x * share;
-  const long long count = s.scan.total - u0 < share ? s.scan.total - u0 : share;
-  if (count > 0) scan_find<kThreads>(a, s.scan, u0);
-  __syncthreads();
-  const bool work = count > 0;
-  const int seq0 = s.scan.seq;
-  const long long rel0 = u0 - s.scan.before, head0 = work ? s.scan.units[seq0 % kScanSeqs] : 1;
+  const Start st = a.seqs <= 32 ? find_start_few(a) : find_start_many(a, s.scan);
+  const bool work = st.count > 0;
+  if (!work && threadIdx.x == 0) leave_split(a, 0, 0, 0, blockIdx.x);
 
   if (warp < kSmWarp0) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
@@ -388,7 +435,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       int t = 0, issued = 0;      // blocks, ring tiles
       uint32_t qn[2] = {0, 0};    // q tiles loaded
       bool ok = true;
-      for (bool more = w.start(a, seq0, rel0, head0, count); more && ok; more = w.next(a)) {
+      int4 open = make_int4(0, 0, 0, blockIdx.x);
+      for (bool more = w.start(a, st); more && ok; more = w.next(a)) {
+        if (w.off == 0 && w.rest > 0)
+          open = make_int4(w.s, w.h, w.tile, blockIdx.x + static_cast<int>((w.rest + st.share - 1) / st.share));
         const int* table = a.pages + static_cast<long long>(w.s) * a.ld_pages;
         for (int b = w.off; b < w.end && ok; ++b, ++t) {
           const int key = b * kTile + lane * rows_per;
@@ -440,6 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (lane == 0) {
+        leave_split(a, open.x, open.y, open.z, open.w);
         for (int i = 0; i < kSlots && i < issued; ++i) wait_drain(&s.full[i], static_cast<uint32_t>((issued - 1 - i) / kSlots) & 1u);
         for (int i = 0; i < 2; ++i)
           if (qn[i] > 0) wait_drain(&s.q_full[i], (qn[i] + 1) & 1u);
@@ -486,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int blk = 0;  // blocks so far: K of block blk is tile 2 blk of the ring, V tile 2 blk + 1
         uint32_t seg[2] = {0, 0}, pn[2] = {0, 0};  // phases: q_full and p_full per tile
         bool ok = true;
-        for (bool on = w.start(a, seq0, rel0, head0, count); on && ok; on = w.next(a)) {
+        for (bool on = w.start(a, st); on && ok; on = w.next(a)) {
           const int un[2] = {w.until(0), w.until(1)};
 #pragma unroll
           for (int i = 0; i < 2; ++i)
@@ -540,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         return __all_sync(kPagedFull, go != 0) != 0;
       };
-      for (bool on = w.start(a, seq0, rel0, head0, count); on && ok; on = w.next(a)) {
+      for (bool on = w.start(a, st); on && ok; on = w.next(a)) {
         const int un[2] = {w.until(0), w.until(1)};
         for (int b = w.off; b < w.end && ok; ++b, ++blk) {
           ok = wait(&s.full[(2 * blk + 1) & 3], (blk >> 1) & 1);
@@ -578,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t segs = 0;  // segments of this tile so far
       bool ok = true;
       const int rt = r / a.g, rh = r % a.g;
-      for (bool on = w.start(a, seq0, rel0, head0, count); on && ok; on = w.next(a)) {
+      for (bool on = w.start(a, st); on && ok; on = w.next(a)) {
         const int until = w.until(i), token = (2 * w.tile + i) * tile_tokens(a) + rt;
         const bool live = rt < tile_tokens(a) && token < w.q.n;
         const int tok = live ? token : 0, head = w.h * a.g + rh;
@@ -708,33 +759,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the item that starts in CTA c's share and goes on behind it: block (c, rows / 32), one warp per 4 rows.
+// Joins the item that CTA c left unfinished: block (c, rows / 32), one warp per 4 rows.
 constexpr int kJoinThreads = 256;
 template <int HD>
 __global__ void __launch_bounds__(kJoinThreads) paged_tc_join_kernel(const PagedArgs a) {
-  __shared__ Scan sc;
   pdl_launch_dependents();
   pdl_wait_prior_grids();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x;
-  scan_total<kJoinThreads>(a, sc);
-  const long long share = share_of(a, sc.total), u = (c + 1) * share;  // the first unit behind the share
-  if (u >= sc.total) return;
-  scan_find<kJoinThreads>(a, sc, u - 1);
-  __syncthreads();
-  // the item of the share's last unit, if its block 0 is in this share and its last block is not
-  const PagedSeq q = paged_seq(a, sc.seq);
-  const long long head = sc.units[sc.seq % kScanSeqs], rel = u - 1 - sc.before;
-  const int h = static_cast<int>(rel / head);
-  long long r = rel % head;
-  int tile = 0, n;
-  for (;; ++tile) {
-    n = item_units(a, q, tile);
-    if (r < n) break;
-    r -= n;
-  }
-  const long long first = u - 1 - r + kSetup, last = first + n - kSetup - 1;  // the item's blocks as units
-  if (first < c * share || first >= u || last < u) return;
-  const int c1 = static_cast<int>(last / share);
+  const int4 open = a.split[c];
+  const int c1 = open.w, h = open.y, tile = open.z;
+  if (c1 <= c) return;
+  const PagedSeq q = paged_seq(a, open.x);
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
   constexpr int kPer = HD / 32;
   for (int k = 0; k < 4; ++k) {
@@ -816,7 +851,7 @@ int launch(PagedArgs a, cudaStream_t stream) {
 }  // namespace
 
 size_t paged_tc_workspace_bytes(int hd) {
-  return static_cast<size_t>(2 * tc_sm_count()) * kItemRows * (hd + 2) * sizeof(float);
+  return static_cast<size_t>(2 * tc_sm_count()) * kItemRows * (hd + 2) * sizeof(float) + tc_sm_count() * sizeof(int4);
 }
 
 int launch_paged_tc(PagedArgs a, void* workspace, cudaStream_t stream) {
@@ -824,6 +859,8 @@ int launch_paged_tc(PagedArgs a, void* workspace, cudaStream_t stream) {
   a.min_share = 4;  // a part costs its write and its join
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + static_cast<size_t>(2 * a.G) * kItemRows * a.hd;
+  a.split = reinterpret_cast<int4*>(a.part_ml + static_cast<size_t>(2 * a.G) * kItemRows * 2);
+  a.tile_tokens = kTile / a.g;
   return a.hd == 128 ? launch<128>(a, stream) : launch<64>(a, stream);
 }
 
