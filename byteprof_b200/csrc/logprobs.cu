@@ -14,13 +14,17 @@
 //   R = R1 + f (1 + R2), T = T1 + f (T2 + (m1 - m2)(1 + R2)).
 // All of it in fp32, over short chains (a thread's share).
 //
-// Top alternatives: values are looked at in the order of 64-bit keys (value, then lower index), each warp keeps its
-// best 32 sorted across its lanes, and vectors whose maximum reaches the last wanted entry put their candidates
-// into a buffer of the warp; 32 of them are sorted and merged at once (20 steps of a bitonic network, where
-// inserting them one by one took 150 clocks each: 50 us for one row of 100352 with 20 alternatives).
+// Top alternatives: of 32 groups of threads the largest value that each saw is sorted; the `top`-th of them is a lower
+// bound of the row's `top`-th value. The few threads that saw anything of that size (about `top`) have their share read
+// once more, by a whole warp each; what reaches the bound goes into the warp's buffer as 64-bit keys (value, then lower
+// index), and 32 keys are sorted and merged at once (20 steps of a bitonic network). So the pass over the logits carries
+// nothing for them but the maximum that it has anyway. (Comparing every vector with a bound taken from the first 8192
+// values cost 27 us of 94 for 1500 rows of 100352 with 5 alternatives, since some 60 values of a row reach it.)
 //
-// Memory bound: rows * vocab values read once. One warp per row for short rows, one CTA or a cluster of up
-// to 8 CTAs for long ones, merged in a fixed order (deterministic).
+// Bound by the instructions of the pass (about 14 per pair of values, two of them exp2, which alone take 35 us) and by
+// memory: 1500 rows of 100352 in bf16 take 60 us (5.1 TB/s), 70 us with 5 alternatives; one row on a cluster of 8 CTAs 5.5
+// and 8.7 us. One warp per row for short rows, one CTA or a cluster of up to 8 CTAs for long ones, merged in a fixed order
+// (deterministic).
 #include <float.h>
 
 #include "bp_common.cuh"
@@ -102,6 +106,7 @@ struct Aside<float> {
   }
   __device__ __forceinline__ float even() const { return a; }
   __device__ __forceinline__ float odd() const { return b; }
+  __device__ __forceinline__ float largest() const { return fmaxf(a, b); }
 };
 template <>
 struct Aside<__nv_bfloat16> {
@@ -113,6 +118,7 @@ struct Aside<__nv_bfloat16> {
   }
   __device__ __forceinline__ float even() const { return bf16lo(p); }
   __device__ __forceinline__ float odd() const { return bf16hi(p); }
+  __device__ __forceinline__ float largest() const { return fmaxf(bf16lo(p), bf16hi(p)); }
 };
 
 // A thread's running sums over what is not set aside, even and odd elements apart: s = sum exp(x - ref),
@@ -211,38 +217,39 @@ __device__ __forceinline__ K sort_down(K k, int lane) {
 }
 
 constexpr int kBuf = 64;  // a warp's candidates: up to 31 waiting and 32 more
+// A warp's alternatives, in shared memory (they are touched a few times per row).
 struct TopList {
-  unsigned long long list;       // lane l: the l-th best so far
-  unsigned long long thr;        // the last wanted entry
-  float thr_v;
-  int waiting;
-  unsigned long long* buf;
-  __device__ __forceinline__ void init(unsigned long long* b) { list = 0, thr = 0, thr_v = -INFINITY, waiting = 0, buf = b; }
-  __device__ __forceinline__ void join(unsigned long long sorted, int top, int lane) {
-    list = merge_sorted(list, sorted, lane);
-    thr = __shfl_sync(kFull, list, top - 1);
-    if (thr != 0) thr_v = fmaxf(thr_v, key_value(thr));  // (a first bound stays until the list reaches it)
+  unsigned long long list[32];  // the best so far, sorted; used when `sorted`
+  unsigned long long buf[kBuf];
+  unsigned long long thr;       // the last wanted entry
+  int waiting, sorted;
+  __device__ __forceinline__ void init(int lane) {
+    list[lane] = 0;
+    if (lane == 0) thr = 0, waiting = sorted = 0;
+    __syncwarp();
   }
   // every lane offers one value (or none)
   __device__ __forceinline__ void offer(float x, int ix, bool valid, int top, int lane) {
     const unsigned long long k = valid ? key_of(x, ix) : 0;
-    const unsigned mask = __ballot_sync(kFull, k > thr);
+    const bool in = k > thr;
+    const int have = waiting;
+    __syncwarp();
+    const unsigned mask = __ballot_sync(kFull, in);
     if (mask == 0) return;
-    if (k > thr) buf[waiting + __popc(mask & ((1u << lane) - 1))] = k;
-    waiting += __popc(mask);
-    if (waiting >= 32) flush(top, lane);
+    if (in) buf[have + __popc(mask & ((1u << lane) - 1))] = k;
+    if (lane == 0) waiting = have + __popc(mask);
+    __syncwarp();
+    if (have + __popc(mask) >= 32) flush(have + __popc(mask), top, lane);
   }
-  __device__ __forceinline__ void flush(int top, int lane) {
+  __device__ __noinline__ void flush(int have, int top, int lane) {
+    const unsigned long long k = lane < have ? buf[lane] : 0, rest = 32 + lane < have ? buf[32 + lane] : 0;
+    const unsigned long long best = merge_sorted(list[lane], sort_down(k, lane), lane);
     __syncwarp();
-    const unsigned long long k = lane < waiting ? buf[lane] : 0, rest = 32 + lane < waiting ? buf[32 + lane] : 0;
-    __syncwarp();
-    join(sort_down(k, lane), top, lane);
+    list[lane] = best;
     buf[lane] = rest;
-    waiting = waiting > 32 ? waiting - 32 : 0;
+    if (lane == top - 1) thr = best;
+    if (lane == 0) waiting = have > 32 ? have - 32 : 0, sorted = 1;
     __syncwarp();
-  }
-  __device__ __forceinline__ void finish(int top, int lane) {
-    if (waiting > 0) flush(top, lane);
   }
 };
 
@@ -256,7 +263,10 @@ struct Vec<float> {
   __device__ static __forceinline__ Raw fill(float x) { return make_float4(x, -INFINITY, -INFINITY, -INFINITY); }
   __device__ static __forceinline__ float one(const float* p) { return *p; }
   __device__ static __forceinline__ float at(const Raw& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
-  __device__ static __forceinline__ float largest(const Raw& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+  using Max = float;
+  __device__ static __forceinline__ Max largest(const Raw& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+  __device__ static __forceinline__ Max larger(Max a, Max b) { return fmaxf(a, b); }
+  __device__ static __forceinline__ float value(Max m) { return m; }
   __device__ static __forceinline__ void add(const Raw& v, Run<float>& r) {
     r.add(r.top.swap(v.x, v.y));
     r.add(r.top.swap(v.z, v.w));
@@ -275,11 +285,13 @@ struct Vec<__nv_bfloat16> {
     const uint32_t w = j < 4 ? (j < 2 ? v.x : v.y) : (j < 6 ? v.z : v.w);
     return j & 1 ? bf16hi(w) : bf16lo(w);
   }
-  __device__ static __forceinline__ float largest(const Raw& v) {
+  using Max = __nv_bfloat162;
+  __device__ static __forceinline__ Max largest(const Raw& v) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    return fmaxf(__low2float(m), __high2float(m));
+    return __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
   }
+  __device__ static __forceinline__ Max larger(Max a, Max b) { return __hmax2(a, b); }
+  __device__ static __forceinline__ float value(Max m) { return fmaxf(__low2float(m), __high2float(m)); }
   __device__ static __forceinline__ void add(const Raw& v, Run<__nv_bfloat16>& r) {
     r.add(r.top.swap(v.x));
     r.add(r.top.swap(v.y));
@@ -288,48 +300,55 @@ struct Vec<__nv_bfloat16> {
   }
 };
 
-// One vector of each lane (elements at, at + 1, ..), -inf in the lanes that have none.
-template <typename T>
-__device__ __forceinline__ void take(const typename Vec<T>::Raw& v, int at, Run<T>& run, TopList& tl, int top, int lane, int valid) {
-  const float vm = Vec<T>::largest(v);
-  run.make_room(vm);
-  Vec<T>::add(v, run);
-  if (top > 0 && __any_sync(kFull, valid > 0 && vm >= tl.thr_v)) {
-    unsigned hits = 0;  // this lane's candidates
+// U vectors of a thread, -inf where it has none.
+template <typename T, int U>
+__device__ __forceinline__ void take(const typename Vec<T>::Raw (&v)[U], Run<T>& run) {
+  typename Vec<T>::Max mx = Vec<T>::largest(v[0]);
 #pragma unroll
-    for (int j = 0; j < Vec<T>::N; ++j) hits |= (j < valid && Vec<T>::at(v, j) >= tl.thr_v ? 1u : 0u) << j;
-    while (__any_sync(kFull, hits != 0)) {
-      const int j = __ffs(hits) - 1;
-      tl.offer(Vec<T>::at(v, j), at + j, hits != 0, top, lane);
-      hits &= hits - 1;
-    }
-  }
+  for (int u = 1; u < U; ++u) mx = Vec<T>::larger(mx, Vec<T>::largest(v[u]));
+  run.make_room(Vec<T>::value(mx));
+#pragma unroll
+  for (int u = 0; u < U; ++u) Vec<T>::add(v[u], run);
 }
 
-// A lower bound of the `top`-th largest value of what n threads (a warp, or the CTA with `share`) hold, one vector
-// maximum each: at least `top` of them reach it. It keeps the first vectors from being candidates altogether.
-template <typename T, int kTeamWarps>
-__device__ __forceinline__ float first_bound(float vm, int top, int lane, int warp, uint32_t* lists) {
-  // (a NaN maximum counts as nothing: a bound may only be too low)
-  uint32_t k = sort_down(vm == vm ? ordered(vm) : 0u, lane);
-  if (kTeamWarps > 1) {
-    lists[warp * 32 + lane] = k;
-    __syncthreads();
+// Offers what of the lanes' vectors (elements at, at + 1, ..; `valid` of them) reaches thr_v; the new thr_v.
+template <typename T>
+__device__ __forceinline__ float candidates(const typename Vec<T>::Raw& v, int at, int valid, float thr_v, int top, int lane, TopList* tl) {
+  unsigned hits = 0;
 #pragma unroll
-    for (int w = kTeamWarps / 2; w > 0; w >>= 1) {
-      if (warp < w) lists[warp * 32 + lane] = merge_sorted(lists[warp * 32 + lane], lists[(warp + w) * 32 + lane], lane);
-      __syncthreads();
-    }
-    k = lists[lane];
-    __syncthreads();  // the lists are used again
+  for (int j = 0; j < Vec<T>::N; ++j) hits |= (j < valid && Vec<T>::at(v, j) >= thr_v ? 1u : 0u) << j;
+  if (!__any_sync(kFull, hits != 0)) return thr_v;
+  while (__any_sync(kFull, hits != 0)) {
+    const int j = __ffs(hits) - 1;
+    float x = 0.0f;
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i) x = i == j ? Vec<T>::at(v, i) : x;
+    tl->offer(x, at + j, hits != 0, top, lane);
+    hits &= hits - 1;
   }
-  const uint32_t b = __shfl_sync(kFull, k, top - 1);
+  const unsigned long long thr = tl->thr;
+  return thr != 0 ? fmaxf(thr_v, key_value(thr)) : thr_v;  // (the bound stays until the list reaches it)
+}
+
+// A lower bound of the `top`-th largest value of a row part from its threads' largest values (vm): the largest of each of
+// 32 groups of threads, sorted; `top` of them reach its entry top - 1.
+template <int kTeamWarps>
+__device__ __forceinline__ float bound_of(float vm, int top, int lane, int warp, uint32_t* groups) {
+  uint32_t k = vm == vm ? ordered(vm) : 0u;  // (a NaN maximum counts as nothing: a bound may only be too low)
+  if (kTeamWarps > 1) {
+#pragma unroll
+    for (int o = kTeamWarps / 2; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(kFull, k, o));
+    if (lane % kTeamWarps == 0) groups[warp * (32 / kTeamWarps) + lane / kTeamWarps] = k;
+    __syncthreads();
+    k = groups[lane];
+  }
+  const uint32_t b = __shfl_sync(kFull, sort_down(k, lane), top - 1);
   return b == 0 ? -INFINITY : from_ordered(b);
 }
 
 // Elements [lo, hi) of a row by kTeamWarps warps, thread `tid` of them.
 template <typename T, int kTeamWarps>
-__device__ __forceinline__ void scan(const T* x, int lo, int hi, int tid, Run<T>& run, TopList& tl, int top, uint32_t* share) {
+__device__ __forceinline__ void scan(const T* x, int lo, int hi, int tid, Run<T>& run, TopList* tl, int top, uint32_t* groups) {
   constexpr int N = Vec<T>::N, n = kTeamWarps * 32;
   constexpr int U = 4;
   using Raw = typename Vec<T>::Raw;
@@ -340,34 +359,46 @@ __device__ __forceinline__ void scan(const T* x, int lo, int hi, int tid, Run<T>
   const int nv = (hi - a0) / N;
   const int a1 = a0 + nv * N;
   const Raw none = Vec<T>::fill(-INFINITY);
-  // the first U vectors of each thread (or none), all in flight, and the bound they give
   Raw f[U];
+  int v = tid;
 #pragma unroll
-  for (int u = 0; u < U; ++u) f[u] = tid + u * n < nv ? Vec<T>::load(x + a0 + (tid + u * n) * N) : none;
-  if (top > 0) {
-    float vm = Vec<T>::largest(f[0]);
+  for (int u = 0; u < U; ++u) f[u] = v + u * n < nv ? Vec<T>::load(x + a0 + (v + u * n) * N) : none;
+  for (; v + (2 * U - 1) * n < nv; v += U * n) {
+    Raw g[U];  // the next ones
 #pragma unroll
-    for (int u = 1; u < U; ++u) vm = fmaxf(vm, Vec<T>::largest(f[u]));
-    tl.thr_v = first_bound<T, kTeamWarps>(vm, top, lane, warp, share);
+    for (int u = 0; u < U; ++u) g[u] = Vec<T>::load(x + a0 + (v + (U + u) * n) * N);
+    take<T, U>(f, run);
+#pragma unroll
+    for (int u = 0; u < U; ++u) f[u] = g[u];
   }
+  for (; v < nv; v += U * n) {
+    take<T, U>(f, run);
 #pragma unroll
-  for (int u = 0; u < U; ++u) take<T>(f[u], a0 + (tid + u * n) * N, run, tl, top, lane, tid + u * n < nv ? N : 0);
+    for (int u = 0; u < U; ++u) f[u] = v + (U + u) * n < nv ? Vec<T>::load(x + a0 + (v + (U + u) * n) * N) : none;
+  }
   // single values before and behind the aligned part: fewer than 2 N, one per lane of the first warp
   const int head = a0 - lo, singles = head + hi - a1;
-  if (warp == 0 && singles > 0) {
-    const int at = tid < head ? lo + tid : a1 + tid - head;
-    take<T>(tid < singles ? Vec<T>::fill(Vec<T>::one(x + at)) : none, at, run, tl, top, lane, tid < singles ? 1 : 0);
+  const int single_at = tid < head ? lo + tid : a1 + tid - head;
+  if (tid < singles) {
+    const Raw one[1] = {Vec<T>::fill(Vec<T>::one(x + single_at))};
+    take<T, 1>(one, run);
   }
-  int v = tid + U * n;
-  for (; v - lane + (U - 1) * n + 31 < nv; v += U * n) {  // warp-uniform: every lane has all U vectors
-#pragma unroll
-    for (int u = 0; u < U; ++u) f[u] = Vec<T>::load(x + a0 + (v + u * n) * N);
-#pragma unroll
-    for (int u = 0; u < U; ++u) take<T>(f[u], a0 + (v + u * n) * N, run, tl, top, lane, N);
-  }
-  for (; v - lane < nv; v += n) {
-    f[0] = v < nv ? Vec<T>::load(x + a0 + v * N) : none;
-    take<T>(f[0], a0 + v * N, run, tl, top, lane, v < nv ? N : 0);
+  if (top > 0) {
+    tl->init(lane);
+    const float vm = run.top.largest();
+    float thr_v = bound_of<kTeamWarps>(vm, top, lane, warp, groups);
+    for (unsigned lanes = __ballot_sync(kFull, vm >= thr_v); lanes != 0; lanes &= lanes - 1) {
+      const int src = __ffs(lanes) - 1;  // this lane's share once more, by the whole warp
+      if (warp == 0 && src < singles) {
+        const int at = src < head ? lo + src : a1 + src - head;
+        thr_v = candidates<T>(Vec<T>::fill(Vec<T>::one(x + at)), at, lane == 0 ? 1 : 0, thr_v, top, lane, tl);
+      }
+      for (int w = warp * 32 + src; w < nv; w += 32 * n) {
+        const int mine = w + lane * n;
+        const Raw r = mine < nv ? Vec<T>::load(x + a0 + mine * N) : none;
+        thr_v = candidates<T>(r, a0 + mine * N, mine < nv ? N : 0, thr_v, top, lane, tl);
+      }
+    }
   }
 }
 
@@ -384,18 +415,18 @@ struct LpArgs {
 
 // The full row once more with every value compared: rows holding NaN, whose vector maxima do not show it.
 template <typename T>
-__device__ __noinline__ void rescan_top(const T* x, int vocab, TopList& tl, int top, int lane) {
-  tl.init(tl.buf);
+__device__ __noinline__ void rescan_top(const T* x, int vocab, TopList* tl, int top, int lane) {
+  tl->init(lane);
   for (int b = 0; b < vocab; b += 32) {
     const bool valid = b + lane < vocab;
-    tl.offer(valid ? Vec<T>::one(x + b + lane) : 0.0f, b + lane, valid, top, lane);
+    tl->offer(valid ? Vec<T>::one(x + b + lane) : 0.0f, b + lane, valid, top, lane);
   }
-  tl.finish(top, lane);
+  tl->flush(tl->waiting, top, lane);
 }
 
-// The row's results, by one warp that holds its merged state and list.
+// The row's results, by one warp that holds its merged state and best alternatives (sorted across the lanes).
 template <typename T>
-__device__ __forceinline__ void finish(const LpArgs& a, int row, const T* x, Stat st, TopList tl, int lane) {
+__device__ __forceinline__ void finish(const LpArgs& a, int row, const T* x, Stat st, unsigned long long best, TopList* tl, int lane) {
   const float nan = __int_as_float(0x7fc00000);
   st.m = __shfl_sync(kFull, st.m, 0);  // one lane's merge order, so that all results of a row agree
   st.r = __shfl_sync(kFull, st.r, 0);
@@ -409,10 +440,13 @@ __device__ __forceinline__ void finish(const LpArgs& a, int row, const T* x, Sta
     a.ent[row] = bad ? nan : lr + st.t / (1.0f + st.r);
   }
   if (a.top > 0) {
-    if (bad) rescan_top(x, a.vocab, tl, a.top, lane);
+    if (bad) {
+      rescan_top(x, a.vocab, tl, a.top, lane);
+      best = tl->list[lane];
+    }
     if (lane < a.top) {
-      a.top_lp[static_cast<long long>(row) * a.top + lane] = bad ? nan : (key_value(tl.list) - st.m) - lr;
-      a.top_id[static_cast<long long>(row) * a.top + lane] = key_index(tl.list);
+      a.top_lp[static_cast<long long>(row) * a.top + lane] = bad ? nan : (key_value(best) - st.m) - lr;
+      a.top_id[static_cast<long long>(row) * a.top + lane] = key_index(best);
     }
   }
 }
@@ -425,31 +459,56 @@ __device__ __forceinline__ void warp_merge(Stat& st) {
   }
 }
 
+// The best of the lists and waiting candidates of kWarps warps, sorted across the lanes: by one warp.
+template <int kWarps>
+__device__ __forceinline__ unsigned long long gather(const TopList* tl, int lane) {
+  unsigned long long best = 0;
+  int total = 0, mine = lane < kWarps ? tl[lane].waiting : 0;
+  unsigned lists = __ballot_sync(kFull, lane < kWarps && tl[lane].sorted);
+  for (; lists != 0; lists &= lists - 1) best = merge_sorted(best, tl[__ffs(lists) - 1].list[lane], lane);
+  int before = mine;  // candidates of the warps before
+#pragma unroll
+  for (int o = 1; o < kWarps; o <<= 1) {
+    const int w = __shfl_up_sync(kFull, before, o);
+    if (lane >= o) before += w;
+  }
+  total = __shfl_sync(kFull, before, kWarps - 1);
+  before -= mine;
+  for (int c = 0; c < total; c += 32) {
+    int w = 0, at = c + lane;
+#pragma unroll
+    for (int i = 1; i < kWarps; ++i)
+      if (c + lane >= __shfl_sync(kFull, before, i)) w = i;
+    at -= __shfl_sync(kFull, before, w);
+    best = merge_sorted(best, sort_down(c + lane < total ? tl[w].buf[at] : 0ull, lane), lane);
+  }
+  return best;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kWarpRowThreads) logprobs_warp_kernel(const LpArgs a) {
-  __shared__ unsigned long long buf[kWarpRowThreads / 32][kBuf];
+  __shared__ TopList lists[kWarpRowThreads / 32];
   pdl_launch_dependents();
   pdl_wait_prior_grids();
   const int lane = threadIdx.x & 31, row = blockIdx.x * (kWarpRowThreads / 32) + (threadIdx.x >> 5);
   if (row >= a.rows) return;
   const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+  TopList* tl = &lists[threadIdx.x >> 5];
   Run<T> run;
   Stat st;
-  TopList tl;
-  tl.init(buf[threadIdx.x >> 5]);
   scan<T, 1>(x, 0, a.vocab, lane, run, tl, a.top, nullptr);
-  tl.finish(a.top, lane);
   st.from(run);
   warp_merge(st);
-  finish(a, row, x, st, tl, lane);
+  __syncwarp();
+  finish(a, row, x, st, a.top > 0 ? gather<1>(tl, lane) : 0ull, tl, lane);
 }
 
 template <typename T, int kRowThreads>
-__global__ void __launch_bounds__(kRowThreads) logprobs_row_kernel(const LpArgs a) {
+__global__ void __launch_bounds__(kRowThreads, kRowThreads == 256 ? 4 : 1) logprobs_row_kernel(const LpArgs a) {
   constexpr int kWarps = kRowThreads / 32;
   __shared__ float sm[kWarps], sr[kWarps], stt[kWarps];
-  __shared__ unsigned long long buf[kWarps][kBuf];
-  __shared__ unsigned long long lists[kWarps][32];
+  __shared__ uint32_t groups[32];
+  __shared__ TopList lists[kWarps];
   __shared__ float cm[kMaxCluster], cr[kMaxCluster], ct[kMaxCluster];  // the leader's slots, one per CTA
   __shared__ unsigned long long cl[kMaxCluster][32];
   pdl_launch_dependents();
@@ -462,29 +521,17 @@ __global__ void __launch_bounds__(kRowThreads) logprobs_row_kernel(const LpArgs 
   const int lo = rank * part < a.vocab ? rank * part : a.vocab, hi = lo + part < a.vocab ? lo + part : a.vocab;
   Run<T> run;
   Stat st;
-  TopList tl;
-  tl.init(buf[warp]);
-  scan<T, kWarps>(x, lo, hi, tid, run, tl, a.top, reinterpret_cast<uint32_t*>(lists));
+  scan<T, kWarps>(x, lo, hi, tid, run, &lists[warp], a.top, groups);
   st.from(run);
   warp_merge(st);
   if (lane == 0) sm[warp] = st.m, sr[warp] = st.r, stt[warp] = st.t;
-  if (a.top > 0) {
-    tl.finish(a.top, lane);
-    lists[warp][lane] = tl.list;
-    __syncthreads();
-#pragma unroll
-    for (int w = kWarps / 2; w > 0; w >>= 1) {  // pairs of warps' lists
-      if (warp < w) lists[warp][lane] = merge_sorted(lists[warp][lane], lists[warp + w][lane], lane);
-      __syncthreads();
-    }
-  } else {
-    __syncthreads();
-  }
+  __syncthreads();
+  unsigned long long best = 0;
   if (warp == 0) {
     st.m = -INFINITY, st.r = st.t = 0.0f;
     if (lane < kWarps) st.m = sm[lane], st.r = sr[lane], st.t = stt[lane];
     warp_merge(st);
-    tl.list = lists[0][lane];
+    if (a.top > 0) best = gather<kWarps>(lists, lane);
   }
   if (C > 1) {
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // every CTA has started: its memory can be written
@@ -494,7 +541,7 @@ __global__ void __launch_bounds__(kRowThreads) logprobs_row_kernel(const LpArgs 
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_addr(&cr[rank]), 0)), "f"(st.r) : "memory");
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_addr(&ct[rank]), 0)), "f"(st.t) : "memory");
       }
-      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapa_shared(smem_addr(&cl[rank][lane]), 0)), "l"(tl.list) : "memory");
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapa_shared(smem_addr(&cl[rank][lane]), 0)), "l"(best) : "memory");
     }
     cluster_sync_unaligned();  // every CTA's slot written and visible to the leader
     if (rank != 0) return;
@@ -503,10 +550,10 @@ __global__ void __launch_bounds__(kRowThreads) logprobs_row_kernel(const LpArgs 
       if (lane < C) st.m = cm[lane], st.r = cr[lane], st.t = ct[lane];
       warp_merge(st);
       if (a.top > 0)
-        for (int c = 1; c < C; ++c) tl.list = merge_sorted(tl.list, cl[c][lane], lane);
+        for (int c = 1; c < C; ++c) best = merge_sorted(best, cl[c][lane], lane);
     }
   }
-  if (warp == 0) finish(a, row, x, st, tl, lane);
+  if (warp == 0) finish(a, row, x, st, best, lists, lane);
 }
 
 template <typename T>
