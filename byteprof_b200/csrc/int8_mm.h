@@ -73,7 +73,7 @@ __device__ __forceinline__ float int8_row_scale(uint32_t max_bits) {
 bool int8_mm_tc_supported(const Int8Args& a);
 int launch_int8_mm_tc(const Int8Args& a, cudaStream_t stream);
 
-// The same with the quantizer inside, for up to 16 rows of 16-byte aligned bf16 x (a.x and a.x_scale unused).
+// The same with the quantizer inside, for one or two rows of 16-byte aligned bf16 x (a.x and a.x_scale unused).
 bool int8_fused_supported(const Int8Args& a, const void* x, long long ldx);
 int launch_int8_fused(const Int8Args& a, const __nv_bfloat16* x, long long ldx, cudaStream_t stream);
 

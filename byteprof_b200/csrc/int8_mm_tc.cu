@@ -6,8 +6,7 @@
 //  * Many rows (kSwap = false): 128 tokens are the MMA's M, kBN channels its N. With enough tiles for the GPU the
 //    grid is persistent and two accumulators alternate, so that a tile's epilogue runs under the next tile's
 //    MMAs.
-//  * Few rows (kSwap = true): the weights are the MMA's M (128 channels) and the tokens its N, padded to 16 or
-//    32: the weights stream once, whatever the number of tokens.
+//  * Few rows (kSwap = true): the weights are the MMA's M (128 channels) and the tokens its N, in tiles of 16 or 32.
 //  * Few tiles: the S CTAs of a cluster split a tile's K; their int32 partials meet in distributed shared memory
 //    (the ring's memory, free by then), each CTA finishing 128 / S of the tile's lanes. Integer sums do not depend
 //    on the order, so all forms give the same bits as the CUDA-core kernel.
@@ -746,8 +745,10 @@ bool int8_mm_tc_supported(const Int8Args& a) {
 }
 
 int launch_int8_mm_tc(const Int8Args& a, cudaStream_t stream) {
+  // Up to 64 tokens: the weights as the MMA's rows (8 tokens of 2048 -> 2048 take 10.0 us, 14.6 with the tokens as rows; 64 of
+  // 8192 -> 2048 15.8 and 18.4, of 2048 -> 8192 16.5 and 16.8).
   if (a.M <= 16) return launch_swap<16, false>(a, stream);
-  if (a.M <= 32) return launch_swap<32, false>(a, stream);
+  if (a.M <= 64) return launch_swap<32, false>(a, stream);
   // Both forms stream 256 operand rows per CTA and K slice at the rate of the L2, about 0.4 us a slice, and what differs is
   // how many slices an SM has to take, waves included; meeting in a cluster costs a split about ten slices
   // (2048 x 2048 -> 16384: 53 us in pairs, 72 in single CTAs; 509 x 8192 -> 2048: 26 in pairs, 18 split in 4).
@@ -762,8 +763,11 @@ int launch_int8_mm_tc(const Int8Args& a, cudaStream_t stream) {
   return o.S > 1 ? launch<128, false, true, false>(a, o, stream) : launch<128, false, false, false>(a, o, stream);
 }
 
+// Each CTA quantizes the tokens of its whole K range, so this pays for a row or two: one row of 2048 -> 8192 takes 10.8 us
+// (13.1 in two kernels), of 8192 -> 2048 10.7 (11.7); 2 rows of 2048 -> 8192 12.0 (13.2), of 4096 -> 4096 11.2 (11.1), 3 of
+// 2048 -> 8192 13.2 (13.3), 4 14.2 (13.4).
 bool int8_fused_supported(const Int8Args& a, const void* x, long long ldx) {
-  if (a.M > 16 || a.K % 8 != 0 || static_cast<long long>(a.M) * a.K > 8192 || ldx % 8 != 0 || a.ldw % 16 != 0 ||
+  if (a.M > 2 || a.K % 8 != 0 || static_cast<long long>(a.M) * a.K > 8192 || ldx % 8 != 0 || a.ldw % 16 != 0 ||
       reinterpret_cast<uintptr_t>(x) % 16 != 0 || reinterpret_cast<uintptr_t>(a.w) % 16 != 0)
     return false;
   return static_cast<size_t>(fuse_blocks(split_partition<16, true>(a))) * 16 * kBK <= kFuseBytes;

@@ -23,8 +23,7 @@
 //
 // Bound by the instructions of the pass (about 14 per pair of values, two of them exp2, which alone take 35 us) and by
 // memory: 1500 rows of 100352 in bf16 take 60 us (5.1 TB/s), 70 us with 5 alternatives; one row on a cluster of 8 CTAs 5.5
-// and 8.7 us. One warp per row for short rows, one CTA or a cluster of up to 8 CTAs for long ones, merged in a fixed order
-// (deterministic).
+// and 8.7 us. A row goes to a warp, a CTA or a cluster of up to 8 CTAs (launch), merged in a fixed order (deterministic).
 #include <float.h>
 
 #include "bp_common.cuh"
@@ -504,7 +503,7 @@ __global__ void __launch_bounds__(kWarpRowThreads) logprobs_warp_kernel(const Lp
 }
 
 template <typename T, int kRowThreads>
-__global__ void __launch_bounds__(kRowThreads, kRowThreads == 256 ? 4 : 1) logprobs_row_kernel(const LpArgs a) {
+__global__ void __launch_bounds__(kRowThreads, kRowThreads == 512 ? 1 : 1024 / kRowThreads) logprobs_row_kernel(const LpArgs a) {
   constexpr int kWarps = kRowThreads / 32;
   __shared__ float sm[kWarps], sr[kWarps], stt[kWarps];
   __shared__ uint32_t groups[32];
@@ -561,7 +560,13 @@ cudaError_t launch(const LpArgs& a, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.stream = s;
-  if (a.vocab <= 2048) {
+  // Many rows (4 per SM): short ones a warp each (what a row costs beside its values, sorting and merging above all, is
+  // paid by one warp, and rows do not wait for one another: 4096 rows of 4096 take 19 us, 28 on 4 warps each, 47 on 8),
+  // long ones by as many warps as keep the SMs full (4096 rows of 16384: 44 us on 4 warps, 59 on 8; 1500 of 100352: 75 on
+  // 4, 70 on 8, 122 on 16; a warp each 178). Few rows: 16 warps in each of up to 8 CTAs, a warp only where there is
+  // nothing to split.
+  const bool many = a.rows >= 4 * tc_sm_count();
+  if (a.vocab <= (many ? 8192 : 1024)) {
     cfg.gridDim = dim3((a.rows + kWarpRowThreads / 32 - 1) / (kWarpRowThreads / 32));
     cfg.blockDim = dim3(kWarpRowThreads);
     set_launch_attrs(cfg, attr);
@@ -569,13 +574,13 @@ cudaError_t launch(const LpArgs& a, cudaStream_t s) {
   }
   int C = 1;
   while (C < kMaxCluster && a.rows * C < tc_sm_count() && a.vocab / (2 * C) >= 4096) C *= 2;
-  // Enough rows to fill the GPU run on 8 warps each (what a warp does once per row, its sorts above all, is a third of the
-  // work at 100352 values on 16); few rows on 16 warps in each of the cluster's CTAs
-  const bool many = C == 1;
+  const int threads = many && a.vocab <= 32768 ? 128 : C == 1 ? 256 : 512;
   cfg.gridDim = dim3(a.rows, C);
-  cfg.blockDim = dim3(many ? 256 : 512);
+  cfg.blockDim = dim3(threads);
   set_launch_attrs(cfg, attr, C);
-  return many ? cudaLaunchKernelEx(&cfg, logprobs_row_kernel<T, 256>, a) : cudaLaunchKernelEx(&cfg, logprobs_row_kernel<T, 512>, a);
+  if (threads == 128) return cudaLaunchKernelEx(&cfg, logprobs_row_kernel<T, 128>, a);
+  return threads == 256 ? cudaLaunchKernelEx(&cfg, logprobs_row_kernel<T, 256>, a)
+                        : cudaLaunchKernelEx(&cfg, logprobs_row_kernel<T, 512>, a);
 }
 
 }  // namespace

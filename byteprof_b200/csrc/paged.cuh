@@ -4,9 +4,10 @@
 // Sequence s has rows [q_start[s], q_start[s + 1]) of q and kv_len[s] cached positions, its last row at
 // position kv_len[s] - 1; row t of it sees the positions up to its own. The g = nh / nkv query heads that share a
 // kv head are rows of one matrix: packed row i of (s, kv head h) is token i / g, head h * g + i % g. An item is
-// (s, h, a tile of packed rows); a unit is one block of keys of an item. Units are numbered over all items in the
-// order s, h, tile, key block, and CTA c of G takes the units [c * share, (c + 1) * share): every CTA reads the same
-// number of blocks whatever the lengths are, and the lengths are read on the device, so that a captured graph
+// (s, h, one tile of 16 packed rows) with few rows, (s, h, two tiles of 128 / g whole tokens) with many; a unit is one
+// block of keys of an item (many rows: an item has kSetup units more). Units are numbered over all items in the
+// order s, h, tile, key block, and CTA c of G takes the units [c * share, (c + 1) * share): every CTA has the same
+// number of units whatever the lengths are, and the lengths are read on the device, so that a captured graph
 // serves every length. An item that lies in one CTA's share is written out by it; otherwise each CTA leaves its
 // part (running maximum, sum, unnormalised output; fp32) in the workspace, in slot 2 c + 1 if the item starts in
 // its share and 2 c if it started before, and names the item that it leaves unfinished; the join kernel merges the

@@ -10,7 +10,8 @@
 // Memory bound: (nh + 2 nkv) head_dim values read and written once per row. One CTA per row: both halves of a
 // rotated pair sit in one thread (8 + 8 values). A thread requests its first kKeep pairs before it looks up where the
 // row belongs and keeps them in registers until the two sums are known (6144 values a row; what is beyond is read a
-// second time). Reading everything twice, behind the lookup, took 32 us for 4099 rows of 32 + 2 x 8 heads @@B
+// second time). 4099 rows of 32 + 2 x 8 heads of 64: 21.5 us (2.3 times 50 MB: 4.7 TB/s); reading everything twice,
+// behind the lookup, took 32. One row: 3.1 us, the lookup's and the row's latency.
 #include "bp_common.cuh"
 
 namespace bp {

@@ -13,9 +13,11 @@
 // head dimension is summed in an order that lets a thread use 8 consecutive values of a key (the same order for q),
 // keys and output columns are numbered so that the 8 lanes of a shared-memory phase touch all banks. The tensor core
 // does 16 rows for the price of one here; 16 rows at HBM speed need a tenth of what mma.sync can do, so tcgen05 has
-// nothing to add. P is rounded to bf16 for the second product (its relative error, 2^-9 at most, averages out over
+// nothing to add. P is rounded to bf16 for the second product (its relative error, 2^-8 at most, averages out over
 // the keys; the sum l adds the unrounded fp32 values).
-// Against registers filled straight from global memory, one unit ahead: 64 streams of up to 8192 keys @@A
+// 64 streams of up to 8192 keys, 16 heads of 128: 186 us for 1.13 GB, 6.1 TB/s, where registers filled straight from global
+// memory, one unit ahead, took 225; 5 drafted tokens over 30001 keys 51 us (4.9 TB/s), one token over 4096 10.4 (latency:
+// the cut, one trip through the ring, the join).
 #include <cudaTypedefs.h>
 
 #include "paged.cuh"
@@ -520,8 +522,9 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 constexpr int kCtasPerSm = 2;
 
 // Up to 32 packed rows per sequence and kv head on average (the lengths themselves are on the device): two tiles of the
-// 16-row kernel, which then reads each key twice; the other kernel pads to 128
-// and takes groups of up to 128 heads.
+// 16-row kernel, which then reads each key twice; the other kernel pads to 128 and takes groups of up to 128 heads.
+// 64 sequences over 2048 keys, 8 kv heads of 128: 16 packed rows take 108 us here and 223 there, 32 take 197 and 220, 40
+// take 278 and 220.
 bool few_rows(int rows, int seqs, int g) { return static_cast<long long>(rows) * g <= 32LL * seqs || g > 128; }
 
 int few_grid() { return kCtasPerSm * tc_sm_count(); }

@@ -3,19 +3,28 @@
 //
 //   S = q K^T, p = exp2(scale S - m), O += p V, l += sum p, out = O / l: one pass over the keys per tile of rows.
 //
-//  * An item is 256 packed rows (two tiles of 128) of one sequence and kv head, a unit is 128 keys of it (paged.cuh); CTAs
-//    take equal ranges of units, whatever the lengths.
+//  * An item is two tiles of 128 rows (128 / g tokens with their g heads each) of one sequence and kv head, a unit is 128
+//    keys of it (paged.cuh); CTAs take equal ranges of units, whatever the lengths.
 //  * Warp 0 finds the pages and loads K and V tiles by TMA, one box per page (page rows are strided by the kv heads):
 //    the 128-byte swizzled tile serves as K (K-major) and as V (keys are the second product's K dimension: MN-major).
 //    A page that is not there is fetched from behind the pool, which TMA fills with zeros.
 //  * Warp 1 issues the MMAs of both tiles in turn: S0, S1, then per key block P0 V, S0', P1 V, S1', so that one
 //    tile's softmax runs under the other's products. S (fp32), P (bf16, over S) and O (fp32) live in TMEM.
-//  * Two warpgroups do the softmax, one thread per row: 128 scores into registers, mask (only where the row's limit lies
-//    in the block), maximum, exp2, P back to TMEM. The running maximum moves only when a score exceeds it by 2^8:
-//    then O is rescaled in TMEM by the same threads, which is rare after the first block.
+//  * Warp 2 waits for the V tile of the block and the K tile of the next one in the issuing thread's place, and clears V's
+//    rows behind the sequence's end.
+//  * Two warpgroups do the softmax, one thread per row: twice through its 128 scores in TMEM, for the maximum and for exp2
+//    and P, masked only where a row's limit lies in the block. The running maximum moves only when a score exceeds it by
+//    2^8: then O is rescaled in TMEM by the same threads, which is rare after the first block. P is rounded to bf16
+//    (2^-8 of each p at most), the sum adds the unrounded fp32 values.
 //
-// Bound by the tensor cores and the special-function units alike: a block of 128 x 128 scores takes 1024 clocks of MMA
-// (head_dim 128) and 1024 of exp2.
+// A block of two tiles takes 2048 clocks of MMA (head_dim 128) and 2048 of exp2, each behind the other within a tile; it
+// takes 3300 (a chunk of 4096 rows over 20480 keys, 16 heads of 128: 865 us, 874 TFLOP/s of visible keys at the power cap's
+// 1.73 GHz) to 3800 clocks (9 prompts of 6151 tokens, 32 heads of 64: 94 us), and an item about 5000 more: bound by the
+// hand-overs between the softmax warps and the issuing thread (about 1300 clocks a block and tile), not by either unit.
+// Measured and not kept: exp2 partly as a polynomial on the FMA pipes (910 us and more), one pass over the scores with the
+// block before's maximum (907), an issuing thread per tile (1069 against 890 then), a block's columns in one unrolled
+// piece (instruction fetch: 110 us of 870), per-chunk masks (900), the next item's first scores behind this item's last
+// product (876, and 100 for the prompts).
 #include <cudaTypedefs.h>
 
 #include "paged.cuh"
@@ -117,8 +126,8 @@ struct Start {
   int seq;
 };
 
-// Up to 32 sequences: every warp finds it by itself, 32 / seqs lanes per sequence (a cut with barriers between all the
-// warps took 10 us in front of the first load).
+// Up to 32 sequences: every warp finds it by itself, 32 / seqs lanes per sequence (with the barriers of the cut for
+// more, and the join kernel searching for its items, 9 prompts took 110 us instead of 96).
 __device__ __forceinline__ Start find_start_few(const PagedArgs& a) {
   const int lane = threadIdx.x & 31;
   int lanes = 32;

@@ -48,6 +48,27 @@ def test_against_float64(dtype, rows, vocab, top):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,top", [(600, 1025, 3), (601, 8192, 32), (600, 8193, 32), (593, 20001, 6), (600, 33000, 5),
+                                            (3, 1024, 9), (3, 1025, 9), (2, 1500, 0)])
+def test_many_rows_and_the_lengths_where_the_split_changes(dtype, rows, vocab, top):
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = (2 * torch.randn(rows, vocab, generator=g, device="cuda")).to(dtype)
+    x[0] = 1.5  # ties alone
+    x[1, : vocab - 2] = float("-inf")
+    ids = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    ids[1] = vocab - 1
+    lp, ent, tl, ti = token_logprobs(x, ids, top)
+    wl, we, wt, wi = want(x, ids, top)
+    close(lp, wl)
+    close(ent, we)
+    if top:
+        assert torch.equal(ti, wi)
+        seen = wt > float("-inf")  # row 1 has two values
+        close(tl[seen], wt[seen])
+        assert torch.equal(tl > float("-inf"), seen)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("vocab", [300, 6001, 40000])
 def test_unaligned_strided_rows_and_ties(dtype, vocab):
     g = torch.Generator(device="cuda").manual_seed(vocab)
