@@ -212,9 +212,9 @@ __device__ __forceinline__ void quantize_range(const Int8Args& a, const __nv_bfl
   named_barrier_sync(1, n);  // row_scale is visible to the epilogue
 }
 
-// kFuse (kSwap, up to 16 tokens): x is bf16 and every CTA quantizes its K range of it itself, while the weights stream:
+// kFuse (kSwap, one or two tokens): x is bf16 and every CTA quantizes its K range of it itself, while the weights stream:
 // one launch instead of two, where launches are most of the time. The rows' maxima need all of K, which is little
-// for few rows (the entry takes M * K up to 8192 values).
+// then (int8_fused_supported).
 template <int kBN, bool kSwap, bool kCluster, bool kFuse>
 __global__ void __launch_bounds__(kThreads, 2)
     int8_mm_tc_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const Int8Args a,

@@ -10,7 +10,7 @@
 // Memory bound: (nh + 2 nkv) head_dim values read and written once per row. One CTA per row: both halves of a
 // rotated pair sit in one thread (8 + 8 values). A thread requests its first kKeep pairs before it looks up where the
 // row belongs and keeps them in registers until the two sums are known (6144 values a row; what is beyond is read a
-// second time). 4099 rows of 32 + 2 x 8 heads of 64: 21.5 us (2.3 times 50 MB: 4.7 TB/s); reading everything twice,
+// second time). 4099 rows of 32 + 2 x 8 heads of 128: 21.5 us for 101 MB, 4.7 TB/s; reading everything twice,
 // behind the lookup, took 32. One row: 3.1 us, the lookup's and the row's latency.
 #include "bp_common.cuh"
 
@@ -253,7 +253,7 @@ extern "C" int bp_paged_append(const void* qkv, long long ldqkv, const void* q_n
   if (page_size < 8 || page_size > 256 || (page_size & (page_size - 1)) != 0)
     return fail(BP_ERR_UNSUPPORTED, "page_size must be a power of two from 8 to 256 (got %d)", page_size);
   if (rows == 0 || seqs == 0) return BP_OK;
-  if (qkv == nullptr || pages == nullptr || q_start == nullptr || kv_len == nullptr || k_pages == nullptr ||
+  if (qkv == nullptr || (pages == nullptr && max_pages > 0) || q_start == nullptr || kv_len == nullptr || k_pages == nullptr ||
       v_pages == nullptr || q_out == nullptr || (cos_t == nullptr) != (sin_t == nullptr) ||
       (q_norm_w == nullptr) != (k_norm_w == nullptr))
     return fail(BP_ERR_INVALID_ARGUMENT, "a pointer is NULL (cos_t / sin_t and the norm weights: both or neither)");

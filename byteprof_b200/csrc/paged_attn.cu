@@ -15,8 +15,8 @@
 // does 16 rows for the price of one here; 16 rows at HBM speed need a tenth of what mma.sync can do, so tcgen05 has
 // nothing to add. P is rounded to bf16 for the second product (its relative error, 2^-8 at most, averages out over
 // the keys; the sum l adds the unrounded fp32 values).
-// 64 streams of up to 8192 keys, 16 heads of 128: 186 us for 1.13 GB, 6.1 TB/s, where registers filled straight from global
-// memory, one unit ahead, took 225; 5 drafted tokens over 30001 keys 51 us (4.9 TB/s), one token over 4096 10.4 (latency:
+// 64 streams of up to 8192 keys, 32 heads of 128 over 8: 186 us for 1.13 GB, 6.1 TB/s, where registers filled straight from global
+// memory, one unit ahead, took 225; 5 drafted tokens over 30001 keys 51 us (4.9 TB/s), one token over 1025 10.4 (latency:
 // the cut, one trip through the ring, the join).
 #include <cudaTypedefs.h>
 
@@ -67,6 +67,8 @@ __device__ __forceinline__ FewUnits few_units(const PagedArgs& a, const PagedSeq
 // How many kv heads the warps of a CTA take side by side over the same keys (the other warps take other keys). A key's
 // heads lie next to each other, so 4 at a time read 1 KB of DRAM in one go instead of 256 bytes here and the rest some
 // other time (head_dim 128); with too few units for that, the heads go to CTAs of their own. `one`: units at one head per CTA.
+// Measured with 1, 2 and 4 heads: 64 streams of up to 8192 keys (117 G units) 192, 189 and 180 us; 5 tokens over 30001 keys
+// (25 G) 49, 57 and 70; one token over 1025 (1 G) 9.4, 10.3 and 11.9.
 __device__ __forceinline__ int heads_per_cta(const PagedArgs& a, long long one) {
   if (a.nkv % 4 == 0 && one >= 64LL * a.G) return 4;
   if (a.nkv % 2 == 0 && one >= 32LL * a.G) return 2;
@@ -595,7 +597,7 @@ extern "C" int bp_paged_attention(const void* q, long long ldq, const void* k_pa
     return fail(BP_ERR_UNSUPPORTED, "the cache holds at most 2^31 positions (got %d pages of %d)", num_pages, page_size);
   if (rows == 0 || seqs == 0) return BP_OK;
   if (num_pages < 1) return fail(BP_ERR_INVALID_ARGUMENT, "a cache of no pages");
-  if (q == nullptr || pages == nullptr || q_start == nullptr || kv_len == nullptr || k_pages == nullptr ||
+  if (q == nullptr || (pages == nullptr && max_pages > 0) || q_start == nullptr || kv_len == nullptr || k_pages == nullptr ||
       v_pages == nullptr || out == nullptr)
     return fail(BP_ERR_INVALID_ARGUMENT, "a pointer argument is NULL");
   if (ldq < static_cast<long long>(nh) * head_dim || ldo < static_cast<long long>(nh) * head_dim || ld_pages < max_pages)

@@ -181,3 +181,11 @@ def test_captured_and_replayed_with_new_inputs():
         x.copy_(torch.randn(100, 512, generator=g, device="cuda"))
         graph.replay()
         assert torch.equal(y, int8_linear(x, wq, ws))
+
+
+def test_a_result_of_more_than_32_bits():
+    m, n, k = 40003, 65600, 32
+    x, s, w, ws = ints(m, k, 8), scales(m, 9), ints(n, k, 10), scales(n, 11)
+    y = int8_mm(x, s, w, ws)
+    rows = torch.tensor([0, 1, 32767, 32768, m - 129, m - 1], device="cuda")
+    assert torch.equal(y[rows], int8_mm(x[rows].contiguous(), s[rows].contiguous(), w, ws))

@@ -164,3 +164,11 @@ def test_captured_and_replayed():
     graph.replay()
     for a, b in zip(got, token_logprobs(x, ids, 4)):
         assert torch.equal(a, b)
+
+
+def test_rows_more_than_32_bits_apart():
+    x = torch.empty(3, 2**31 + 64, dtype=torch.bfloat16, device="cuda")[:, :3000]
+    x.copy_(torch.randn(3, 3000, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda"))
+    ids = torch.tensor([0, 2999, 17], device="cuda")
+    for a, b in zip(token_logprobs(x, ids, 4), token_logprobs(x.contiguous(), ids, 4)):
+        assert torch.equal(a, b)

@@ -315,3 +315,38 @@ def test_no_rows_and_no_sequences():
     out = torch.full_like(q, 3.0)
     cache.attend(q, table[:0], starts[:1], kv[:0], out=out)
     assert (out == 3).all()
+
+
+@pytest.mark.parametrize("news", [[1, 2], [70, 90]])
+def test_a_table_of_no_pages_has_no_positions(news):
+    cache, q, table, starts, kv = make(news, [5, 0], 4, 2, 64, 8)
+    assert torch.isnan(cache.attend(q, table[:, :0], starts, kv)).all()
+    assert (cache.attend(q, table[:, :0], starts, kv * 0) == 0).all()
+    before = cache.k_pages.clone()
+    assert torch.isnan(cache.append(torch.ones(sum(news), 8 * 64, dtype=BF16, device="cuda"), 4, table[:, :0], starts, kv)).all()
+    assert torch.equal(cache.k_pages.view(torch.int16), before.view(torch.int16))
+
+
+@pytest.mark.parametrize("n", [1, 100])
+def test_sequences_may_share_pages(n):
+    """Three sequences continue one prefix of 64 positions (two pages), each with pages of its own behind it."""
+    cache, q, table, starts, kv = make([n] * 3, [64, 64, 64], 4, 2, 128, 32)
+    table[1:, :2] = table[0, :2]
+    check(cache.attend(q, table, starts, kv), *reference(cache, q, table, starts, kv))
+
+
+@pytest.mark.parametrize("news,befores", [([1, 2], [300, 77]), ([130, 200], [300, 77])])
+def test_a_pool_of_more_than_32_bits(news, befores):
+    """Pages whose first value is more than 2^32 elements, and 2^33 bytes, behind the pool's."""
+    small, q, table, starts, kv = make(news, befores, 8, 4, 128, 64)
+    pool = 2**32 // (64 * 4 * 128) + 64
+    big = PagedCache(*(torch.empty(pool, 64, 4, 128, dtype=BF16, device="cuda") for _ in range(2)))
+    far = torch.where(table >= 0, table + (pool - small.num_pages), table)
+    for a, b in ((big.k_pages, small.k_pages), (big.v_pages, small.v_pages)):
+        a[-small.num_pages:] = b
+    y = big.attend(q, far, starts, kv)
+    check(y, *reference(small, q, table, starts, kv))
+    qkv = torch.randn(sum(news), 16 * 128, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda").to(BF16)
+    assert torch.equal(big.append(qkv, 8, far, starts, kv), small.append(qkv, 8, table, starts, kv))
+    for a, b in ((big.k_pages, small.k_pages), (big.v_pages, small.v_pages)):
+        assert torch.equal(a[-small.num_pages:].view(torch.int16), b.view(torch.int16))

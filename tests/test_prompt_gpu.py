@@ -199,3 +199,21 @@ def test_int8_linear_module(bias):
     assert m(torch.randn(3, 256, device="cuda")).dtype == torch.float32 if bias != BF16 else True  # fp32: the dequantized product
     with pytest.raises(ValueError, match="act"):
         Int8Linear(lin, act="fp8")
+
+
+def test_apply_quantization_with_8_bit_activations():
+    """The scheme swaps the selected linears; the products are `int8_linear`'s."""
+    model = nn.Module()
+    model.model = nn.Module()
+    model.model.layers = nn.ModuleList([nn.ModuleDict({"self_attn": nn.ModuleDict({"q_proj": nn.Linear(128, 96, bias=False)}),
+                                                       "mlp": nn.ModuleDict({"down_proj": nn.Linear(256, 128, bias=False)})})])
+    model.lm_head = nn.Linear(128, 64, bias=False)
+    model.to("cuda", BF16)
+    w = model.model.layers[0]["self_attn"]["q_proj"].weight.detach().clone()
+    stats = apply_quantization(model, "blocks", "int8_w8a8")
+    q_proj = model.model.layers[0]["self_attn"]["q_proj"]
+    assert stats["n_linears"] == 2 and isinstance(model.lm_head, nn.Linear)
+    assert isinstance(q_proj, Int8Linear) and q_proj.act == "int8"
+    for rows in (1, 40, 300):
+        x = torch.randn(rows, 128, device="cuda").to(BF16)
+        assert torch.equal(q_proj(x), int8_linear(x, *quantize_rowwise_int8(w)))
