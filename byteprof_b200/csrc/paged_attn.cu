@@ -20,6 +20,8 @@
 // the cut, one trip through the ring, the join).
 #include <cudaTypedefs.h>
 
+#include <algorithm>
+
 #include "paged.cuh"
 #include "skinny_internal.h"
 #include "sm100.cuh"
@@ -463,9 +465,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   } while (w.next(a, hp));
 }
 
-// Joins the item that CTA c left unfinished: block (c, y) takes its rows y, y + kJoinY, .. (a row of 64: 4 heads of 16),
+// Joins the item that CTA c left unfinished: block (c, y) takes its rows y, y + gridDim.y, .. (a row of 64: 4 heads of 16),
 // the parts of a row dealt to its 4 warps.
-constexpr int kJoinY = 8;
+constexpr int kJoinY = 8;  // at most
 template <int HD>
 __global__ void __launch_bounds__(kMathThreads) paged_few_join_kernel(const PagedArgs a) {
   __shared__ float sm_l[kWarps];
@@ -481,7 +483,7 @@ __global__ void __launch_bounds__(kMathThreads) paged_few_join_kernel(const Page
   const int live = min(nrows, kRows);
   constexpr int kPer = HD / 32;
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
-  for (int k = blockIdx.y; k < hp * live; k += kJoinY) {
+  for (int k = blockIdx.y; k < hp * live; k += gridDim.y) {
     const int j = k / live, pr = open.z * kRows + k % live, row = j * kRows + k % live;
     float m = -INFINITY;
     for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, ml[static_cast<size_t>(2 * c + (c == c0)) * kSlotRows + row].x);
@@ -556,7 +558,7 @@ int launch_few(const PagedArgs& a, cudaStream_t s) {
   set_launch_attrs(cfg, attr);
   cudaError_t e = cudaLaunchKernelEx(&cfg, paged_few_kernel<HD>, tk, tv, a);
   if (e == cudaSuccess) {
-    cfg.gridDim = dim3(a.G, kJoinY);
+    cfg.gridDim = dim3(a.G, static_cast<unsigned>(std::min<long long>(static_cast<long long>(a.rows) * a.g, kJoinY)));
     cfg.blockDim = dim3(kMathThreads);
     cfg.dynamicSmemBytes = 0;
     e = cudaLaunchKernelEx(&cfg, paged_few_join_kernel<HD>, a);
