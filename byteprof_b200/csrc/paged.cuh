@@ -51,6 +51,18 @@ __device__ __forceinline__ float pg_ex2(float v) {
   return r;
 }
 
+// Non-negative a / b; 64-bit division is a call of some 100 instructions, and hardly any count here needs it.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
+// CTAs' equal shares of `total` units.
+__device__ __forceinline__ long long share_of(const PagedArgs& a, long long total) {
+  const long long s = quotient(total + a.G - 1, a.G);
+  return s > a.min_share ? s : a.min_share;
+}
+
 // What CTA c leaves for the join kernel: the item that starts in its share and whose parts end in CTA `last` (> c), as
 // (sequence, kv head or group of heads, tile, last); last = c: none.
 __device__ __forceinline__ void leave_split(const PagedArgs& a, int seq, int head, int tile, int last) {

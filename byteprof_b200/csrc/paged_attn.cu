@@ -60,9 +60,9 @@ struct FewUnits {
 // `hp`: kv heads per CTA (below).
 __device__ __forceinline__ FewUnits few_units(const PagedArgs& a, const PagedSeq& q, int hp) {
   FewUnits u;
-  u.tiles = static_cast<int>((static_cast<long long>(q.n) * a.g + kRows - 1) / kRows);
+  u.tiles = (q.n * a.g + kRows - 1) / kRows;  // at most 2^30 rows
   u.per = q.kv > kKeys ? (q.kv + kKeys - 1) / kKeys : 1;
-  u.all = static_cast<long long>(a.nkv / hp) * u.tiles * u.per;
+  u.all = static_cast<long long>(a.nkv >> (hp >> 1)) * u.tiles * u.per;  // (hp: 1, 2 or 4)
   return u;
 }
 
@@ -75,11 +75,6 @@ __device__ __forceinline__ int heads_per_cta(const PagedArgs& a, long long one) 
   if (a.nkv % 4 == 0 && one >= 64LL * a.G) return 4;
   if (a.nkv % 2 == 0 && one >= 32LL * a.G) return 2;
   return 1;
-}
-
-__device__ __forceinline__ long long share_of(const PagedArgs& a, long long total) {
-  const long long s = (total + a.G - 1) / a.G;
-  return s > a.min_share ? s : a.min_share;
 }
 
 constexpr int kScan = kThreads / 32;
@@ -161,8 +156,8 @@ struct FewWalk {
   long long before, u, u1;
   __device__ __forceinline__ void segment() {
     const long long rel = u - before;
-    item = static_cast<int>(rel / fu.per);
-    off = static_cast<int>(rel % fu.per);
+    item = static_cast<int>(quotient(rel, fu.per));
+    off = static_cast<int>(rel - static_cast<long long>(item) * fu.per);
     end = static_cast<int>(fu.per - off < u1 - u ? fu.per : off + (u1 - u));
   }
   __device__ __forceinline__ void start(const PagedArgs& a, const Located& at, int hp, long long first, long long last) {
@@ -219,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();  // the barriers are initialised
   const long long one = total_units(a, sm.scan);
   const int hp = heads_per_cta(a, one), step = kKeys / hp;
-  const long long total = one / hp;
+  const long long total = one >> (hp >> 1);
   const long long share = share_of(a, total), u0 = blockIdx.x * share;
   const long long u1 = u0 + share < total ? u0 + share : total;
   if (u0 >= u1) {
@@ -244,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     do {
       if (w.off == 0 && w.end < w.fu.per)
         open = make_int4(w.s, w.item / w.fu.tiles, w.item % w.fu.tiles,
-                         blockIdx.x + static_cast<int>((w.fu.per - w.end + share - 1) / share));
+                         blockIdx.x + static_cast<int>(quotient(w.fu.per - w.end + share - 1, share)));
       const int* table = a.pages + static_cast<long long>(w.s) * a.ld_pages;
       const int h = w.item / w.fu.tiles * hp + hl;
       const int s1 = w.end * hp;

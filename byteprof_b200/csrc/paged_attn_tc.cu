@@ -110,14 +110,9 @@ __device__ __forceinline__ int item_units(const PagedArgs& a, const PagedSeq& q,
 
 struct Scan {
   long long units[kScanSeqs];  // of one kv head, per sequence of the block at hand
-  long long warp_sum[kWarps], total, before;
+  long long warp_sum[kWarps], before;
   int seq;
 };
-
-__device__ __forceinline__ long long share_of(const PagedArgs& a, long long total) {
-  const long long s = (total + a.G - 1) / a.G;
-  return s > a.min_share ? s : a.min_share;
-}
 
 // A CTA's start: the sequence of its first unit, that unit's place behind the sequence's first, the units of one of its
 // kv heads, and how many units are the CTA's (0: none).
@@ -272,11 +267,7 @@ struct Walk {
     const long long rel = st.rel, head = st.head, count = st.count;
     s = st.seq;
     enter(a);
-    if ((rel | head) >> 32 == 0) {
-      h = static_cast<uint32_t>(rel) / static_cast<uint32_t>(head);
-    } else {
-      h = static_cast<int>(rel / head);
-    }
+    h = static_cast<int>(quotient(rel, head));
     long long r = rel - h * head;
     int n;
     for (tile = 0;; ++tile) {
@@ -438,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int4 open = make_int4(0, 0, 0, blockIdx.x);
       for (bool more = w.start(a, st); more && ok; more = w.next(a)) {
         if (w.off == 0 && w.rest > 0)
-          open = make_int4(w.s, w.h, w.tile, blockIdx.x + static_cast<int>((w.rest + st.share - 1) / st.share));
+          open = make_int4(w.s, w.h, w.tile, blockIdx.x + static_cast<int>(quotient(w.rest + st.share - 1, st.share)));
         const int* table = a.pages + static_cast<long long>(w.s) * a.ld_pages;
         for (int b = w.off; b < w.end && ok; ++b, ++t) {
           const int key = b * kTile + lane * rows_per;
