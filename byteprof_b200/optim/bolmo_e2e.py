@@ -344,6 +344,7 @@ class BolmoDecoder:
         if not first_patch and self.patches == 0:
             raise ValueError("the first byte of a decoder without patches has to open one")
         p, dev = self.parity, self.device
+        caches = [blk.attn.paged() for blk in self.blocks]  # raises before anything has changed
         ids = torch.tensor(prompt, dtype=torch.long).to(dev)
         # the encoder's state is committed only when the patches are known to fit
         saved = self.enc.state[0].clone() if self.patches + n > self.max_patches else None
@@ -360,12 +361,11 @@ class BolmoDecoder:
         if t:
             at = torch.tensor([i for i, o in enumerate(opened) if o], dtype=torch.long).to(dev)
             g = skinny_mm(e, self.w_patch).index_select(0, at)
-            cache = self.blocks[0].attn.paged()
-            pages = torch.arange(cache.num_pages, dtype=torch.int32, device=dev)[None]
+            pages = torch.arange(caches[0].num_pages, dtype=torch.int32, device=dev)[None]
             q_start = torch.tensor([0, t], dtype=torch.int32).to(dev)
             kv_len = torch.tensor([self.patches + t], dtype=torch.int32).to(dev)
-            for blk in self.blocks:
-                g = blk.chunk(g, blk.attn.paged(), pages, q_start, kv_len, self.cos, self.sin)
+            for blk, cache in zip(self.blocks, caches):
+                g = blk.chunk(g, cache, pages, q_start, kv_len, self.cos, self.sin)
             values = torch.cat([self.value, rmsnorm(g, self.dec_in_norm, EPS)])
             self.pos.add_(t)
             self.patches += t

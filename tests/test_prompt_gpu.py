@@ -113,11 +113,21 @@ def test_a_prompt_that_does_not_fit_changes_nothing():
         b.score([1])
 
 
+def test_a_cache_of_no_whole_pages_is_refused_and_nothing_changes():
+    ids = text(5, 11)
+    a = BolmoDecoder(**{**SMALL, "max_patches": 20})
+    b = BolmoDecoder(**{**SMALL, "max_patches": 20})
+    with pytest.raises(ValueError, match="multiple of 8"):
+        a.prefill(ids)
+    opened = [True, False, True, True, False]
+    assert torch.equal(fed(a, ids, opened), fed(b, ids, opened))
+
+
 def test_a_block_takes_packed_sequences_and_single_tokens():
     """Three prompts packed into one chunk equal the three by themselves, within the rounding of the block's bf16 output,
     and a further token each (the few-row kernels) equals the longer prompts' last rows within what 8-bit activations
-    make of it: an attention output that another order of sums moves by d (half a bf16 step of it, 2^-9 * 0.8 sigma in
-    the mean) moves its 8-bit code by a whole step s = amax / 127 (0.035 sigma at amax = 4.5) with probability d / s, so
+    make of it: an attention output that another order of sums moves by d (a bf16 rounding of it, in the mean half of its
+    largest: 2^-9 * 0.8 sigma) moves its 8-bit code by a whole step s = amax / 127 (0.035 sigma at amax = 4.5) with probability d / s, so
     the product's inputs differ by sqrt(d s) = 0.0075 sigma in the root mean square; the block's three products in a row
     make sqrt(3) of that, 0.013 sigma: 0.8 * 0.013 / 0.8 = 0.013 of the mean, under 2^-6."""
     dev = torch.device("cuda")
