@@ -24,7 +24,9 @@
 // Measured and not kept: exp2 partly as a polynomial on the FMA pipes (910 us and more), one pass over the scores with the
 // block before's maximum (907), an issuing thread per tile (1069 against 890 then), a block's columns in one unrolled
 // piece (instruction fetch: 110 us of 870), per-chunk masks (900), the next item's first scores behind this item's last
-// product (876, and 100 for the prompts).
+// product (876, and 100 for the prompts), P in columns of its own at head_dim 64 and the next scores in front of the product
+// with V (prompts 97), all 128 scores loaded at once for the maximum (848, prompts 97), the next chunk's scores loaded
+// ahead (925, prompts 104).
 #include <cudaTypedefs.h>
 
 #include "paged.cuh"
