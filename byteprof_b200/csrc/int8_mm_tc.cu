@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         tc_fence_before_sync();
         mbar_arrive_cluster(done);
       };
-      if (vec != 2) {
+      if (a.y_f32) {
         drain_rows<128>(a, src, static_cast<long long>(m0) + r, ib * kPairN + c0, s.ws[buf] + c0, s.bias[buf] + c0, vec, drained);
         continue;
       }
@@ -674,9 +674,24 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         }
         fence_async_shared();
         named_barrier_sync(2 + grp, 128);
-        if (et % 128 == 0) {
-          tma_store_2d(&ty, stage, ib * kPairN + c0 + h * 64, m0);
-          tma_store_commit();
+        const int n0 = ib * kPairN + c0 + h * 64;
+        if (vec) {
+          if (et % 128 == 0) {
+            tma_store_2d(&ty, stage, n0, m0);
+            tma_store_commit();
+          }
+          continue;
+        }
+        // Rows that TMA cannot store: a warp writes its 32 rows one after the other, 64 bytes in a row at a time (straight from
+        // registers each of 32 rows gets 2 bytes at a time: 4000 x 512 -> 50001 took 1912 us instead of 316).
+        const int rows = min(32, a.M - m0 - 32 * q), cols = a.N - n0;
+        __nv_bfloat16* y = static_cast<__nv_bfloat16*>(a.y) + static_cast<long long>(m0 + 32 * q) * a.ldy + n0;
+#pragma unroll 4
+        for (int k = 0; k < rows; ++k) {
+          const uint8_t* row = stage + (32 * q + k) * 128;
+#pragma unroll
+          for (int cc = lane; cc < 64; cc += 32)
+            if (cc < cols) y[k * a.ldy + cc] = *reinterpret_cast<const __nv_bfloat16*>(row + (((cc / 8) ^ (k & 7)) * 16) + cc % 8 * 2);
         }
       }
     }
@@ -718,12 +733,11 @@ int launch_pair(const Int8Args& a, const Part& p, cudaStream_t stream) {
   st = tc_encode_2d(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w, a.K, a.N, a.ldw, kBK, kBM, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
   if (st != BP_OK) return st;
   const int es = a.y_f32 ? 4 : 2;
-  int vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && (a.ldy * es) % 16 == 0;
+  const int vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && (a.ldy * es) % 16 == 0;
   CUtensorMap ty = ta;
   if (vec && !a.y_f32) {
     st = tc_encode_2d(&ty, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.y, a.N, a.M, a.ldy * 2, 64, kBM, CU_TENSOR_MAP_L2_PROMOTION_NONE);
     if (st != BP_OK) return st;
-    vec = 2;
   }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];

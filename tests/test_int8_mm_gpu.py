@@ -185,6 +185,19 @@ def test_captured_and_replayed_with_new_inputs():
         assert torch.equal(y, int8_linear(x, wq, ws))
 
 
+@pytest.mark.parametrize("m,n,k", [(129, 2000, 64), (300, 4097, 48), (1000, 5003, 32), (70, 3001, 256), (128, 4000, 128), (700, 1281, 4096)])
+@pytest.mark.parametrize("off", [0, 1, 2, 4])
+def test_rows_of_the_result_that_start_anywhere(m, n, k, off):
+    """Results in a buffer whose rows start at odd, 4-byte and 8-byte places, both types: the values, and nothing beside them."""
+    q, w, s, ws = ints(m, k, 30), ints(n, k, 31), scales(m, 32), scales(n, 33)
+    want = int8_mm(q, s, w, ws, out=torch.empty(m, (n + 7) // 8 * 8, device="cuda")[:, :n])
+    for dtype in (BF16, torch.float32):
+        buf = torch.full((m + 1, n + 2 * off + 3), 5.0, dtype=dtype, device="cuda")
+        int8_mm(q, s, w, ws, out=buf[:m, off:off + n])
+        assert torch.equal(buf[:m, off:off + n], want.to(dtype))
+        assert (buf[:m, :off] == 5).all() and (buf[:m, off + n:] == 5).all() and (buf[m] == 5).all()
+
+
 def test_a_result_of_more_than_32_bits():
     m, n, k = 40003, 65600, 32
     x, s, w, ws = ints(m, k, 8), scales(m, 9), ints(n, k, 10), scales(n, 11)
