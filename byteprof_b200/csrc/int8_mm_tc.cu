@@ -98,8 +98,25 @@ __device__ __forceinline__ void store1(const Int8Args& a, long long m, int n, fl
     static_cast<__nv_bfloat16*>(a.y)[m * a.ldy + n] = __float2bfloat16_rn(v);
 }
 
+// Lane l's v[k] becomes lane k's v[l].
+__device__ __forceinline__ void transpose32(float (&v)[32], int lane) {
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) {
+    const bool up = (lane & s) != 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      if (i & s) continue;
+      const float got = __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i | s], s);
+      v[i] = up ? got : v[i];
+      v[i | s] = up ? v[i | s] : got;
+    }
+  }
+}
+
 // A thread's row of a tile: kBN int32 columns of its TMEM lane -> scaled values of row m, columns n0 .. ; `drained` is
-// called once when the accumulator has been read.
+// called once when the accumulator has been read. Where the rows are not aligned, or end within 32 columns, the warp stores
+// its 32 rows one after the other, 32 columns at a time (each thread its own row, value by value: 100 x 2048 -> 8191 in
+// 40 us instead of 23).
 template <int kBN, typename F>
 __device__ __forceinline__ void drain_rows(const Int8Args& a, uint32_t src, long long m, int n0, const float* ws,
                                            const float* bias, int vec, F drained) {
@@ -109,12 +126,12 @@ __device__ __forceinline__ void drain_rows(const Int8Args& a, uint32_t src, long
     uint32_t raw[32];
     tmem_ld_32x32b_x32(src + c, raw);
     if (c + 32 == kBN) drained();
-    if (m >= a.M) continue;
     const int n = n0 + c;
-    if (vec && n + 32 <= a.N) {
-      float v[32];
+    float v[32];
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = int8_value(a, static_cast<int>(raw[j]), sx, ws[c + j], bias[c + j]);
+    for (int j = 0; j < 32; ++j) v[j] = int8_value(a, static_cast<int>(raw[j]), sx, ws[c + j], bias[c + j]);
+    if (vec && n + 32 <= a.N) {
+      if (m >= a.M) continue;
       if (a.y_f32) {
         float4* d = reinterpret_cast<float4*>(static_cast<float*>(a.y) + m * a.ldy + n);
 #pragma unroll
@@ -127,9 +144,11 @@ __device__ __forceinline__ void drain_rows(const Int8Args& a, uint32_t src, long
                             pack2(v[8 * j + 4], v[8 * j + 5]), pack2(v[8 * j + 6], v[8 * j + 7]));
       }
     } else {
+      const int lane = threadIdx.x & 31;
+      transpose32(v, lane);
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (n + j < a.N) store1(a, m, n + j, int8_value(a, static_cast<int>(raw[j]), sx, ws[c + j], bias[c + j]));
+      for (int k = 0; k < 32; ++k)
+        if (m - lane + k < a.M && n + lane < a.N) store1(a, m - lane + k, n + lane, v[k]);
     }
   }
 }
