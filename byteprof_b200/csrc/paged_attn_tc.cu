@@ -308,6 +308,9 @@ struct Walk {
   }
   // blocks [off, until(i)) of the segment are tile i's
   __device__ __forceinline__ int until(int i) const { return min(end, blocks[i]); }
+  // Blocks [off, used()) of the segment are loaded: `end`, but none of an item whose rows see nothing. A block that neither
+  // tile uses may not be in the ring: no product would hold warp 2, which clears values in it, and its slot's refill together.
+  __device__ __forceinline__ int used() const { return min(end, max(blocks[0], blocks[1])); }
 };
 
 template <int HD>
@@ -434,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (w.off == 0 && w.rest > 0)
           open = make_int4(w.s, w.h, w.tile, blockIdx.x + static_cast<int>(quotient(w.rest + st.share - 1, st.share)));
         const int* table = a.pages + static_cast<long long>(w.s) * a.ld_pages;
-        for (int b = w.off; b < w.end && ok; ++b, ++t) {
+        for (int b = w.off; b < w.used() && ok; ++b, ++t) {
           const int key = b * kTile + lane * rows_per;
           int row = none, bad = w.q.bad;
           if (lane < np && key < w.q.kv) {
@@ -533,6 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (bool on = w.start(a, st); on && ok; on = w.next(a)) {
           const int un[2] = {w.until(0), w.until(1)};
+          if (w.used() <= w.off) continue;
 #pragma unroll
           for (int i = 0; i < 2; ++i)
             if (un[i] > w.off) ok = ok && mbar_wait(&s.q_full[i], seg[i]++ & 1u, abort);
@@ -548,7 +552,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           umma_commit(&s.empty[blk & 1]);  // pair blk: the V before and this K
           for (int b = w.off; b < w.end; ++b, ++blk) {
             const bool more = b + 1 < w.end;
-            if (b >= un[0] && b >= un[1]) ok = mbar_wait(&s.full[(2 * blk + 1) & 3], (blk >> 1) & 1, abort);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               if (b < un[i] && ok) {
@@ -587,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       for (bool on = w.start(a, st); on && ok; on = w.next(a)) {
         const int un[2] = {w.until(0), w.until(1)};
-        for (int b = w.off; b < w.end && ok; ++b, ++blk) {
+        for (int b = w.off; b < w.used() && ok; ++b, ++blk) {
           ok = wait(&s.full[(2 * blk + 1) & 3], (blk >> 1) & 1);
           const int valid = w.q.kv - b * kTile;
           if (ok && valid < kTile) {
@@ -741,7 +744,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (live) reinterpret_cast<float2*>(a.part_ml)[at] = make_float2(any ? m : -INFINITY, l);
         }
         tc_fence_before_sync();
-        t0 += w.end - w.off;
+        t0 += w.used() - w.off;
       }
     }
   }
