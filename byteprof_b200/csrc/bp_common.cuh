@@ -101,10 +101,19 @@ __device__ __forceinline__ uint4 ldg_stream16(const void* ptr, uint64_t policy) 
   return r;
 }
 
-// 16-byte read-only load through L1 (small operands re-read by many warps: activations).
+// 16-byte read-only load through L1, for constants (weights) only: the compiler may move it anywhere its address is known,
+// above pdl_wait_prior_grids too.
 __device__ __forceinline__ uint4 ldg16(const void* ptr) {
   uint4 r;
   asm("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(ptr));
+  return r;
+}
+
+// 16-byte load of data that the kernel before may have written (activations): stays behind pdl_wait_prior_grids, and not
+// through the read-only path, whose data may not change while a kernel runs (one that has started early and waits, too).
+__device__ __forceinline__ uint4 ld16(const void* ptr) {
+  uint4 r;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(ptr) : "memory");
   return r;
 }
 

@@ -46,7 +46,7 @@ struct Act;
 template <>
 struct Act<__nv_bfloat16> {
   static constexpr int kDtype = BP_DTYPE_BF16;
-  __device__ static __forceinline__ void load8(const __nv_bfloat16* p, float (&f)[8]) { unpack8(ldg16(p), f); }
+  __device__ static __forceinline__ void load8(const __nv_bfloat16* p, float (&f)[8]) { unpack8(ld16(p), f); }
   __device__ static __forceinline__ void store8(__nv_bfloat16* p, const float (&f)[8]) {
     *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
                                               pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));

@@ -54,11 +54,11 @@ __global__ void __launch_bounds__(kQThreads) quantize_rows_kernel(const __nv_bfl
 #pragma unroll
     for (int i = 0; i < kQCache; ++i) {
       const int c = tid + i * kTeam;
-      keep[i] = c < chunks ? ldg16(xr + c * 8) : make_uint4(0, 0, 0, 0);
+      keep[i] = c < chunks ? ld16(xr + c * 8) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < kQCache; ++i) m = abs_max8(keep[i], m);
-    for (int c = tid + kQCache * kTeam; c < chunks; c += kTeam) m = abs_max8(ldg16(xr + c * 8), m);
+    for (int c = tid + kQCache * kTeam; c < chunks; c += kTeam) m = abs_max8(ld16(xr + c * 8), m);
   } else {
     for (int k = tid; k < K; k += kTeam) m = max(m, __float_as_uint(__bfloat162float(xr[k])) & 0x7fffffffu);
   }
@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kQThreads) quantize_rows_kernel(const __nv_bfl
       if (c < chunks) *reinterpret_cast<uint2*>(qr + c * 8) = bad ? make_uint2(0, 0) : q8(keep[i], s, inv);
     }
     for (int c = tid + kQCache * kTeam; c < chunks; c += kTeam)
-      *reinterpret_cast<uint2*>(qr + c * 8) = bad ? make_uint2(0, 0) : q8(ldg16(xr + c * 8), s, inv);
+      *reinterpret_cast<uint2*>(qr + c * 8) = bad ? make_uint2(0, 0) : q8(ld16(xr + c * 8), s, inv);
   } else {
     for (int k = tid; k < K; k += kTeam) qr[k] = bad ? 0 : static_cast<int8_t>(q1(__bfloat162float(xr[k]), s, inv));
   }

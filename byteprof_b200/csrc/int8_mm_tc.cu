@@ -201,7 +201,7 @@ __device__ __forceinline__ void quantize_range(const Int8Args& a, const __nv_bfl
     for (int u = 0; u < kU; ++u) {
       const int i = i0 + u * n;
       row[u] = i / chunks;
-      v[u] = row[u] < a.M ? ldg16(x + row[u] * ldx + (i - row[u] * chunks) * 8) : make_uint4(0, 0, 0, 0);
+      v[u] = row[u] < a.M ? ld16(x + row[u] * ldx + (i - row[u] * chunks) * 8) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
@@ -224,7 +224,7 @@ __device__ __forceinline__ void quantize_range(const Int8Args& a, const __nv_bfl
     const float s = int8_row_scale(red[r]), inv = 1.0f / s;
     for (int i = tid; i < span; i += n) {
       const int b = i / 16, c = i % 16, k = (k0 + b) * kBK + c * 8;
-      const uint2 v = k < a.K && !bad ? q8(ldg16(x + r * ldx + k), s, inv) : make_uint2(0, 0);
+      const uint2 v = k < a.K && !bad ? q8(ld16(x + r * ldx + k), s, inv) : make_uint2(0, 0);
       *reinterpret_cast<uint2*>(dst + b * kBN * kBK + r * kBK + (((c / 2) ^ (r & 7)) * 16) + (c & 1) * 8) = v;
     }
   }

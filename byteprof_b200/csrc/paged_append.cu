@@ -137,8 +137,8 @@ __global__ void __launch_bounds__(kThreads, 7) paged_append_kernel(const AppendA
   for (int i = 0; i < kKeep; ++i) {
     const int u = tid + i * kThreads;
     if (u < all) {
-      keep[i][0] = ldg16(x + place(u));
-      keep[i][1] = ldg16(x + place(u) + apart(u));
+      keep[i][0] = ld16(x + place(u));
+      keep[i][1] = ld16(x + place(u) + apart(u));
     }
   }
   // the row's sequence: the number of sequences that end at or before it
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 7) paged_append_kernel(const AppendA
 #pragma unroll
     for (int i = 0; i < kKeep; ++i)
       if (tid + i * kThreads < all) add(tid + i * kThreads, keep[i][0], keep[i][1]);
-    for (int u = tid + kKeep * kThreads; u < nq + nk; u += kThreads) add(u, ldg16(x + place(u)), ldg16(x + place(u) + half));
+    for (int u = tid + kKeep * kThreads; u < nq + nk; u += kThreads) add(u, ld16(x + place(u)), ld16(x + place(u) + half));
     sq = __uint_as_float(static_cast<uint32_t>(sq2)) + __uint_as_float(static_cast<uint32_t>(sq2 >> 32));
     sk = __uint_as_float(static_cast<uint32_t>(sk2)) + __uint_as_float(static_cast<uint32_t>(sk2 >> 32));
 #pragma unroll
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kThreads, 7) paged_append_kernel(const AppendA
 #pragma unroll
   for (int i = 0; i < kKeep; ++i)
     if (tid + i * kThreads < all) put(tid + i * kThreads, keep[i][0], keep[i][1]);
-  for (int u = tid + kKeep * kThreads; u < all; u += kThreads) put(u, ldg16(x + place(u)), ldg16(x + place(u) + apart(u)));
+  for (int u = tid + kKeep * kThreads; u < all; u += kThreads) put(u, ld16(x + place(u)), ld16(x + place(u) + apart(u)));
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

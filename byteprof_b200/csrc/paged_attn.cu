@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int s1 = w.end * hp;
       // pages one step ahead of their use
       int key = w.off * hp * step + part * kRows + sub * box;
-      int page = lane < boxes && key < w.q.kv ? __ldg(table + (key >> a.page_log2)) : -1;
+      int page = lane < boxes && key < w.q.kv ? table[key >> a.page_log2] : -1;
       for (int b = w.off * hp; b < s1; ++b, ++n) {
         int row = none, bad = w.q.bad;
         if (key < w.q.kv && lane < boxes) {
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         bad = __reduce_min_sync(kPagedFull, bad);
         key += step;
-        page = b + 1 < s1 && lane < boxes && key < w.q.kv ? __ldg(table + (key >> a.page_log2)) : -1;
+        page = b + 1 < s1 && lane < boxes && key < w.q.kv ? table[key >> a.page_log2] : -1;
         const int st = n % kStages;
         int go = 1;
         if (lane == 0) {
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       pos[i] = ok ? w.q.pos0 + tok : -1;
 #pragma unroll
       for (int c = 0; c < HD / 32; ++c) {
-        const uint4 v = ok ? ldg16(p + 32 * c) : make_uint4(0, 0, 0, 0);
+        const uint4 v = ok ? ld16(p + 32 * c) : make_uint4(0, 0, 0, 0);
         if (i == 0) qa[c] = v; else qb[c] = v;
       }
     }

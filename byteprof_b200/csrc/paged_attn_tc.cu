@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int key = b * kTile + lane * rows_per;
           int row = none, bad = w.q.bad;
           if (lane < np && key < w.q.kv) {
-            const int page = __ldg(table + (key >> a.page_log2));
+            const int page = table[key >> a.page_log2];
             if (page >= 0 && page < a.num_pages)
               row = (page << a.page_log2) + (key & mask);
             else

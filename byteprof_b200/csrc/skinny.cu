@@ -86,7 +86,7 @@ template <int EPL>
 __device__ __forceinline__ void load_x(const __nv_bfloat16* p, float (&f)[EPL]) {
 #pragma unroll
   for (int h = 0; h < EPL / 8; ++h) {
-    const uint4 v = ldg16(p + 8 * h);
+    const uint4 v = ld16(p + 8 * h);
     f[8 * h + 0] = bf16lo(v.x); f[8 * h + 1] = bf16hi(v.x);
     f[8 * h + 2] = bf16lo(v.y); f[8 * h + 3] = bf16hi(v.y);
     f[8 * h + 4] = bf16lo(v.z); f[8 * h + 5] = bf16hi(v.z);

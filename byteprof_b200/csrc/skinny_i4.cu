@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kThreads / R) skinny_i4_kernel(const I4Args a)
       const int vecs = M * gn * (kGroup / 8);
       for (int i = threadIdx.x; i < vecs; i += kThr) {
         const int m = i / (gn * (kGroup / 8)), kv = (i - m * gn * (kGroup / 8)) * 8;
-        const uint4 v = ldg16(a.x + m * a.ldx + static_cast<long long>(gg) * kGroup + kv);
+        const uint4 v = ld16(a.x + m * a.ldx + static_cast<long long>(gg) * kGroup + kv);
         float* d = xs + m * plen + xs_index(kv);
         *reinterpret_cast<float4*>(d) = make_float4(bf16lo(v.x), bf16hi(v.x), bf16lo(v.y), bf16hi(v.y));
         *reinterpret_cast<float4*>(d + 4) = make_float4(bf16lo(v.z), bf16hi(v.z), bf16lo(v.w), bf16hi(v.w));

@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kThreads) skinny_i8x_kernel(const I8xArgs a) {
   for (int k = kb + 8 * threadIdx.x; k < ke; k += 8 * kThreads) {
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      const uint4 v = ldg16(a.x + m * a.ldx + k);
+      const uint4 v = ld16(a.x + m * a.ldx + k);
       const uint32_t wv[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int h = 0; h < 4; ++h) am[m] = max(am[m], max(wv[h] & 0x7fffu, (wv[h] >> 16) & 0x7fffu));
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kThreads) skinny_i8x_kernel(const I8xArgs a) {
   for (int j = threadIdx.x; j < M * (kc / 8); j += kThreads) {
     const int m = j / (kc / 8), c = (j - m * (kc / 8)) * 8;
     const int e = row_e[m];
-    uint4 v = ldg16(a.x + m * a.ldx + kb + c);
+    uint4 v = ld16(a.x + m * a.ldx + kb + c);
     if (e == kNonFinite) v = make_uint4(0, 0, 0, 0);
     uint32_t pl[kDigitPlanes][2];
     digitise8(v, e == kNonFinite ? 0 : e, pl);
