@@ -715,9 +715,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       }
     }
     if (et % 128 == 0) tma_store_wait<true>();
+    // The leader's commits arrive in both CTAs, in order: the peer may not end (and give up its shared memory) before the
+    // last one has reached it. Waited for here, behind the tiles, where it is due.
+    if (rank != 0 && et == 0) wait_drain(&s.mma_done, 0);
   }
   tc_fence_before_sync();
-  __syncthreads();
+  cta_teardown_barrier();
   cluster_sync_unaligned();  // the leader's MMAs have read the peer's memory, every copy has landed in both
   if (warp == 1) {
     tc_fence_after_sync();

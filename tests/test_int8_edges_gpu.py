@@ -1,0 +1,37 @@
+"""The 8-bit product at the edges of what its documentation allows. Definition and tolerances: tests/test_int8_mm_gpu.py."""
+
+import pytest
+import torch
+from test_int8_mm_gpu import check, ints, scales
+
+from byteprof_b200 import _lib
+from byteprof_b200.optim.decode_ops import token_logprobs
+from byteprof_b200.quant.int8 import int8_mm
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def test_pairs_of_ctas_one_behind_the_other_and_beside_other_kernels():
+    """Products on pairs of CTAs (more than 128 rows, enough tiles), each followed on the same SMs by kernels that lay their
+    own barriers where the pair's were, from two streams: nothing of a pair may arrive after its end."""
+    sets = []
+    for i, (m, n, k) in enumerate([(700, 5000, 256), (300, 9000, 128), (1025, 4608, 144)]):
+        q, s, w, ws = ints(m, k, 10 + i), scales(m, 20 + i), ints(n, k, 30 + i), scales(n, 40 + i, BF16)
+        y = int8_mm(q, s, w, ws)
+        check(y, q, s, w, ws)
+        sets.append(((q, s, w, ws), y))
+    logits = torch.randn(300, 30000, device="cuda").to(BF16)
+    want = token_logprobs(logits, None, 3)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for r in range(60):
+        with torch.cuda.stream(streams[r % 2]):
+            args, y = sets[r % 3]
+            got.append((int8_mm(*args), y, token_logprobs(logits, None, 3)))
+    torch.cuda.synchronize()
+    for y, ref, lp in got:
+        assert torch.equal(y, ref)
+        assert all(torch.equal(a, b) for a, b in zip(lp[1:], want[1:]))
+    assert _lib.device_errors() == 0
