@@ -124,6 +124,7 @@ __device__ __forceinline__ void drain_rows(const Int8Args& a, uint32_t src, long
 #pragma unroll 1
   for (int c = 0; c < kBN; c += 32) {
     uint32_t raw[32];
+    __syncwarp();  // (the lanes' stores below differ, and the load is the whole warp's)
     tmem_ld_32x32b_x32(src + c, raw);
     if (c + 32 == kBN) drained();
     const int n = n0 + c;
@@ -131,8 +132,9 @@ __device__ __forceinline__ void drain_rows(const Int8Args& a, uint32_t src, long
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = int8_value(a, static_cast<int>(raw[j]), sx, ws[c + j], bias[c + j]);
     if (vec && n + 32 <= a.N) {
-      if (m >= a.M) continue;
-      if (a.y_f32) {
+      if (m >= a.M) {
+        // a row past the end: nothing to store
+      } else if (a.y_f32) {
         float4* d = reinterpret_cast<float4*>(static_cast<float*>(a.y) + m * a.ldy + n);
 #pragma unroll
         for (int j = 0; j < 8; ++j) d[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
@@ -192,6 +194,7 @@ __device__ __forceinline__ void quantize_range(const Int8Args& a, const __nv_bfl
                                                float* row_scale, uint32_t* red, int tid, int n) {
   const int chunks = a.K / 8;  // K is a multiple of 8
   if (tid < 16) red[tid] = 0;
+  __syncwarp();
   named_barrier_sync(1, n);
   constexpr int kU = 8;  // loads in flight
   for (int i0 = tid; i0 - (tid & 31) < a.M * chunks; i0 += kU * n) {
@@ -215,6 +218,7 @@ __device__ __forceinline__ void quantize_range(const Int8Args& a, const __nv_bfl
       }
     }
   }
+  __syncwarp();
   named_barrier_sync(1, n);
   if (tid < a.M) row_scale[tid] = red[tid] >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : int8_row_scale(red[tid]);
   // the MMA's columns past M read what lies here and nobody reads them
@@ -228,6 +232,7 @@ __device__ __forceinline__ void quantize_range(const Int8Args& a, const __nv_bfl
       *reinterpret_cast<uint2*>(dst + b * kBN * kBK + r * kBK + (((c / 2) ^ (r & 7)) * 16) + (c & 1) * 8) = v;
     }
   }
+  __syncwarp();
   named_barrier_sync(1, n);  // row_scale is visible to the epilogue
 }
 
@@ -363,6 +368,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll 1
         for (int c = 0; c < kBN; c += 16) {
           float raw[16];
+          __syncwarp();
           tmem_ld_32x32b_x16(src + c, raw);
           if (c + 16 == kBN) {
             tc_fence_before_sync();
@@ -674,6 +680,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
         if (et % 128 == 0) tma_store_wait<false>();  // the store before has read the buffer
+        __syncwarp();
         named_barrier_sync(2 + grp, 128);
 #pragma unroll
         for (int c = 0; c < 64; c += 32) {

@@ -428,6 +428,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           *reinterpret_cast<float4*>(d + 4) = make_float4(o[8 * hh + 4][2 * r + e], o[8 * hh + 5][2 * r + e],
                                                           o[8 * hh + 6][2 * r + e], o[8 * hh + 7][2 * r + e]);
         }
+      __syncwarp();
       named_barrier_sync(1, kMathThreads);
       const int row = tid / 8, d0 = (tid % 8) * 8, r = tile * kRows + row;  // 8 threads per row, 8 dims each
       for (int j = 0; j < hp && r < nrows; ++j) {  // warps j, j + hp, .. hold parts of head j
@@ -455,6 +456,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (hh == 0 && d0 == 0) reinterpret_cast<float2*>(a.part_ml)[at_row] = make_float2(mm, ll);
         }
       }
+      __syncwarp();
       named_barrier_sync(1, kMathThreads);  // sm.o is written again
     }
   } while (w.next(a, hp));

@@ -710,6 +710,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
           for (int c = 0; c < HD; c += 32) {
             uint32_t o[32];
+            __syncwarp();  // (dead rows store nothing, and the load is the whole warp's)
             if (any)
               tmem_ld_32x32b_x32(to + c, o);
             else
@@ -733,6 +734,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
               uint32_t o[32];
+              __syncwarp();
               tmem_ld_32x32b_x32(to + c, o);
               if (live) {
 #pragma unroll
