@@ -57,6 +57,15 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
   return a / b;
 }
 
+// What is not 0 in a 16-byte piece of 8 bf16 values that holds an Inf or NaN (0 * x is 0 for every finite x).
+__device__ __forceinline__ uint32_t not_finite8(const uint4 v) {
+  const uint32_t* w = &v.x;
+  uint32_t acc = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(w[i]), "r"(0u));
+  return acc;
+}
+
 // CTAs' equal shares of `total` units.
 __device__ __forceinline__ long long share_of(const PagedArgs& a, long long total) {
   const long long s = quotient(total + a.G - 1, a.G);
@@ -68,6 +77,11 @@ __device__ __forceinline__ long long share_of(const PagedArgs& a, long long tota
 __device__ __forceinline__ void leave_split(const PagedArgs& a, int seq, int head, int tile, int last) {
   a.split[blockIdx.x] = make_int4(seq, head, tile, last);
 }
+
+// Values that some rows of a tile do not see. Their weight is 0, but 0 * Inf and 0 * NaN are not: where a block holds
+// positions behind the first that a row of the tile does not see, values that are not finite are taken as 0, and the rows that do
+// see them give NaN, as for a page that is not there. Only positions of the call's own rows can be of that kind, so this
+// costs next to nothing.
 
 // A sequence as the kernels see it: rows clipped to the call's, cached length clipped to the table's.
 struct PagedSeq {

@@ -185,6 +185,33 @@ struct FewWalk {
   }
 };
 
+// Rows `lo` and up of a warp's V tile (keys base + lo ..), by that warp: pieces that are not finite become 0, those past the
+// sequence's end too; the first key that had one (INT_MAX: none).
+template <int HD>
+__device__ __forceinline__ int hide_not_finite(uint8_t* vt, int lo, int base, int lane) {
+  constexpr int kPer = HD / 8, kU = 4;  // pieces of a row, in flight
+  int lost = 0x7fffffff;
+#pragma unroll 1
+  for (int c0 = lane; c0 < (kRows - lo) * kPer; c0 += 32 * kU) {
+    uint4 x[kU];
+    auto at = [&](int u) {
+      const int c = c0 + 32 * u, piece = c % kPer;
+      return reinterpret_cast<uint4*>(vt + (piece >> 3) * (kRows * 128) + (lo + c / kPer) * 128 + (piece & 7) * 16);
+    };
+#pragma unroll
+    for (int u = 0; u < kU; ++u) x[u] = c0 + 32 * u < (kRows - lo) * kPer ? *at(u) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+      if (not_finite8(x[u]) != 0) {
+        *at(u) = make_uint4(0, 0, 0, 0);
+        lost = min(lost, base + lo + (c0 + 32 * u) / kPer);
+      }
+  }
+  fence_async_shared();  // the slot is refilled by TMA
+  __syncwarp();
+  return __reduce_min_sync(kPagedFull, lost);
+}
+
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 2)
     paged_few_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const PagedArgs a) {
@@ -314,6 +341,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
     int bad = w.q.bad;
+    // cached positions that every row of the tile sees
+    const int all_see = static_cast<int>(max(min(w.q.pos0 + tile * kRows / a.g + 1, static_cast<long long>(w.q.kv)), 0LL));
     bool dead = false;
     for (int b = w.off * hp; b < w.end * hp; ++b, ++n) {
       const int base = b * step + part * kRows, st = n % kStages;
@@ -325,7 +354,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       bad = min(bad, sm.bad[st]);
       // piece (row, chunk) of a tile is at row * 128 + (chunk ^ (row & 7)) * 16
       const uint8_t* kt = sm.ring[st] + warp * 2 * S::kWarpTile;
-      const uint8_t* vt = kt + S::kWarpTile;
+      uint8_t* vt = sm.ring[st] + (warp * 2 + 1) * S::kWarpTile;
+      if (base + kRows > all_see) bad = min(bad, hide_not_finite<HD>(vt, max(all_see - base, 0), base, lane));
       float sc[2][4];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -380,7 +410,6 @@ __global__ void __launch_bounds__(kThreads, 2)
       const uint32_t a0 = pack2(p[0][0], p[0][1]), a1 = pack2(p[0][2], p[0][3]), a2 = pack2(p[1][0], p[1][1]),
                      a3 = pack2(p[1][2], p[1][3]);
       // values of the keys lane % 4 + {0, 4, 8, 12}, dims 64 hh + 8 perm(lane / 4) ..
-      const bool tail = base + kRows > w.q.kv;  // what lies past the end may be NaN, and p = 0 would not hide it
 #pragma unroll
       for (int hh = 0; hh < HD / 64; ++hh) {
         uint4 v[4];
@@ -388,7 +417,6 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int i = 0; i < 4; ++i) {
           const int row = c4 + 4 * i;
           v[i] = *reinterpret_cast<const uint4*>(vt + hh * (kRows * 128) + row * 128 + ((kperm ^ (row & 7)) * 16));
-          if (tail && base + row >= w.q.kv) v[i] = make_uint4(0, 0, 0, 0);
         }
         const uint32_t* w0 = &v[0].x;
         const uint32_t* w1 = &v[1].x;

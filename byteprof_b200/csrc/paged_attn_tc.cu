@@ -10,8 +10,8 @@
 //    A page that is not there is fetched from behind the pool, which TMA fills with zeros.
 //  * Warp 1 issues the MMAs of both tiles in turn: S0, S1, then per key block P0 V, S0', P1 V, S1', so that one
 //    tile's softmax runs under the other's products. S (fp32), P (bf16, over S) and O (fp32) live in TMEM.
-//  * Warp 2 waits for the V tile of the block and the K tile of the next one in the issuing thread's place, and clears V's
-//    rows behind the sequence's end.
+//  * Warp 2 waits for the V tile of the block and the K tile of the next one in the issuing thread's place, and looks
+//    through the values that some row does not see, behind the sequence's end too: what is not finite becomes 0.
 //  * Two warpgroups do the softmax, one thread per row: twice through its 128 scores in TMEM, for the maximum and for exp2
 //    and P, masked only where a row's limit lies in the block. The running maximum moves only when a score exceeds it by
 //    2^8: then O is rescaled in TMEM by the same threads, which is rare after the first block. P is rounded to bf16
@@ -306,6 +306,10 @@ struct Walk {
     }
     return false;
   }
+  // Cached positions that every row of the item sees: the first ones.
+  __device__ __forceinline__ int all_see(const PagedArgs& a) const {
+    return static_cast<int>(max(min(q.pos0 + static_cast<long long>(tile) * 2 * tile_tokens(a) + 1, static_cast<long long>(q.kv)), 0LL));
+  }
   // blocks [off, until(i)) of the segment are tile i's
   __device__ __forceinline__ int until(int i) const { return min(end, blocks[i]); }
   // Blocks [off, used()) of the segment are loaded: `end`, but none of an item whose rows see nothing. A block that neither
@@ -320,6 +324,7 @@ struct Smem {
   uint8_t kv[kSlots][kTileBytes];
   uint64_t full[kSlots], empty[2], q_full[2], q_done[2], s_full[2], p_full[2], o_done[2], mma_done;
   int bad[kBadRing];
+  int2 lost[2][2];  // per tile, for its segments in turn: (segment, first position whose value was taken out)
   uint32_t tmem_base;
   int abort;
   Scan scan;
@@ -357,6 +362,34 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// Rows `lo` and up of a V tile (keys base + lo ..), by one warp: pieces that are not finite become 0, those past the
+// sequence's end too; the first key that had one (INT_MAX: none). 32 rows a step from the step that holds `lo`: rows before it
+// are seen by all, and what is found there is right for all.
+template <int HD>
+__device__ __noinline__ int hide_not_finite(uint8_t* v, int lo, int base, int lane) {
+  constexpr int kU = 4;
+  int lost = 0x7fffffff;
+  uint4* t = reinterpret_cast<uint4*>(v) + lane;
+#pragma unroll 1
+  for (int c = (lo & ~31) * 8; c < kTile * 8 * (HD / 64); c += 32 * kU) {  // (pieces; 64 dims behind the others)
+    if (HD > 64 && c == kTile * 8) c += (lo & ~31) * 8;
+    uint32_t any = 0;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) any |= not_finite8(t[c + 32 * u]);
+    if (any == 0) continue;
+#pragma unroll 1
+    for (int u = 0; u < kU; ++u)
+      if (not_finite8(t[c + 32 * u]) != 0) {
+        t[c + 32 * u] = make_uint4(0, 0, 0, 0);
+        lost = min(lost, base + (c + lane) / 8 % kTile + 4 * u);
+      }
+  }
+  lost = __reduce_min_sync(kPagedFull, lost);
+  if (lost != 0x7fffffff) fence_async_shared();  // the product reads them
+  __syncwarp();
+  return lost;
 }
 
 constexpr int kChunk = 32;
@@ -397,6 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.p_full[i], 5);  // 4 softmax warps and warp 2
       mbar_init(&s.o_done[i], 1);
+      s.lost[i][0] = s.lost[i][1] = make_int2(-1, 0);
     }
     mbar_init(&s.mma_done, 1);
     s.abort = 0;
@@ -576,10 +610,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (warp == 2 && work) {
       // ---- the fifth arrival at p_full: V of the block and K of the next have landed. A wait costs the issuing thread
-      // some 100 clocks in which the tensor cores run dry, so it has one per product. The values past a sequence's end
-      // may be NaN, which p = 0 does not hide: they are cleared here.
+      // some 100 clocks in which the tensor cores run dry, so it has one per product. Values that a row does not see, and
+      // those past a sequence's end, may be NaN, which p = 0 does not hide: they are taken out here (paged.cuh).
       Walk w;
-      int blk = 0;
+      int blk = 0, segs[2] = {0, 0};  // blocks, and segments of each tile, so far
       uint32_t pn[2] = {0, 0};
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -589,28 +623,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         return __all_sync(kPagedFull, go != 0) != 0;
       };
       for (bool on = w.start(a, st); on && ok; on = w.next(a)) {
-        const int un[2] = {w.until(0), w.until(1)};
+        const int un[2] = {w.until(0), w.until(1)}, all_see = w.all_see(a);
         for (int b = w.off; b < w.used() && ok; ++b, ++blk) {
           ok = wait(&s.full[(2 * blk + 1) & 3], (blk >> 1) & 1);
-          const int valid = w.q.kv - b * kTile;
-          if (ok && valid < kTile) {
-            const int v0 = valid > 0 ? valid : 0;
-            for (int c = lane; c < (kTile - v0) * 8 * (HD / 64); c += 32) {
-              const int half = c / ((kTile - v0) * 8), r = c % ((kTile - v0) * 8);
-              *reinterpret_cast<uint4*>(s.kv[(2 * blk + 1) & 3] + half * kHalf + (v0 * 8 + r) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_async_shared();
-            __syncwarp();
-          }
+          int lost = 0x7fffffff;
+          if (ok && all_see < (b + 1) * kTile)
+            lost = hide_not_finite<HD>(s.kv[(2 * blk + 1) & 3], max(all_see - b * kTile, 0), b * kTile, lane);
           if (ok && b + 1 < w.end) ok = wait(&s.full[(2 * blk + 2) & 3], ((blk + 1) >> 1) & 1);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             if (b >= un[i] || !ok) continue;
             if (pn[i] > 0) ok = wait(&s.p_full[i], (pn[i] + 1) & 1u);  // the phase before is complete
             ++pn[i];
+            // With that phase the tile's softmax group is in its segment before this one at the earliest, whose place is the other.
+            if (ok && lane == 0 && lost < w.q.kv) {
+              int2& e = s.lost[i][segs[i] & 1];
+              e = make_int2(segs[i], e.x == segs[i] ? min(e.y, lost) : lost);
+            }
             if (ok && lane == 0) mbar_arrive(&s.p_full[i]);
           }
         }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) segs[i] += un[i] > w.off ? 1 : 0;
       }
     }
   } else {
@@ -698,9 +732,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) mbar_arrive(&s.p_full[i]);
           }
           if (!ok) break;
-          ok = mbar_wait(&s.o_done[i], segs++ & 1u, abort);
-          if (!__all_sync(kPagedFull, ok)) break;
+          ok = mbar_wait(&s.o_done[i], segs & 1u, abort) && mbar_wait(&s.p_full[i], static_cast<uint32_t>(n - 1) & 1u, abort);
+          if (!__all_sync(kPagedFull, ok)) break;  // (p_full, long complete, orders what warp 2 left before its arrival)
           tc_fence_after_sync();
+          const int2 lost = s.lost[i][segs & 1];
+          if (lost.x == static_cast<int>(segs)) bad = min(bad, lost.y);
+          ++segs;
         }
         if (pos >= bad) l = __int_as_float(0x7fc00000);
         const bool any = until > w.off, whole = w.off == 0 && w.end == w.per;

@@ -406,8 +406,9 @@ int bp_mlstm_commit_state(const float* c_hist, const float* n_hist, const float*
  * bp_paged_attention: out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j over the positions j <= p of the row's
  *   sequence, kv head h / (nh / nkv); q and out [rows, nh, head_dim] bf16 with row strides ldq, ldo. A row that sees
  *   nothing (a negative position) gives zeros; a row that should see a page outside [0, num_pages) or past the table
- *   gives NaN. What lies in the cache past kv_len is never used, whatever its bits are; values at visible positions
- *   must be finite. fp32 scores, maxima and sums; the weights are rounded to bf16 for the product with v.
+ *   gives NaN. What lies in the cache at positions that a row does not see (past its own, past kv_len) does not reach
+ *   it, whatever its bits are; a row that sees a key or value that is not finite is not finite itself, where it weighs
+ *   in or as a whole. fp32 scores, maxima and sums; the weights are rounded to bf16 for the product with v.
  *   workspace: scratch of the size that the next function returns, 256-byte aligned, any contents; calls that overlap in
  *   time need different ones. Splits long caches over the GPU and joins the parts in a fixed order (deterministic).
  */

@@ -32,3 +32,28 @@ def test_many_rows_of_empty_sequences_beside_long_ones(order, nh, nkv, hd):
     for _ in range(20):
         assert torch.equal(cache.attend(q, table, starts, lens), y)
     assert _lib.device_errors() == 0
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("news,befores,nh,nkv,hd,page", [
+    ([200], [100], 4, 2, 128, 16), ([333, 1, 150], [0, 700, 77], 8, 2, 64, 32), ([700], [1300], 3, 1, 128, 16),
+    ([5], [300], 8, 2, 128, 16), ([9, 1, 3], [0, 64, 500], 4, 4, 64, 8), ([17], [40], 1, 1, 128, 64), ([3], [0], 40, 5, 64, 16)])
+def test_a_value_that_is_not_finite_stays_with_the_rows_that_see_it(news, befores, nh, nkv, hd, page, value):
+    """One value of one kv head at one new position after the other: the rows before it, and the other kv heads, are as
+    without it; the rows that see it are not finite where it weighs in."""
+    cache, q, table, starts, kv = make(news, befores, nh, nkv, hd, page, seed=31)
+    want, mag = reference(cache, q, table, starts, kv)
+    g = nh // nkv
+    for s, (n, before) in enumerate(zip(news, befores)):
+        a = starts[s].item()
+        for i in sorted({0, 1, n // 3, n // 2, n - 2, n - 1} & set(range(n))):
+            p, head, dim = before + i, i % nkv, (13 * i) % hd
+            at = (table[s, p // page].item(), p % page, head, dim)
+            kept = cache.v_pages[at].clone()
+            cache.v_pages[at] = value
+            y = cache.attend(q, table, starts, kv)
+            cache.v_pages[at] = kept
+            heads = slice(head * g, (head + 1) * g)
+            assert not torch.isfinite(y[a + i:a + n, heads, dim].float()).any()
+            y[a + i:a + n, heads] = want[a + i:a + n, heads].to(BF16)
+            check(y, want, mag)

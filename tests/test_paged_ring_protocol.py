@@ -1,7 +1,8 @@
 """A model of the barrier protocol of the many-row paged attention (byteprof_b200/csrc/paged_attn_tc.cu), run on the CPU
-under random schedules: the loading warp, the issuing thread, the warp that clears the values behind a sequence's end,
+under random schedules: the loading warp, the issuing thread, the warp that looks through a block's values and clears some,
 and the two softmax groups, over a ring of two K and two V tiles. Every ring tile is tagged with the block it holds, so that a
-product over a refilled tile, or a clearing that hits another block's values, fails an assertion.
+product over a refilled tile, or a clearing that hits another block's values, fails an assertion; so does a softmax group
+that does not get what that warp found in the blocks of its segment (`lost`).
 
 A segment is (blocks, what tile 0 sees of them, what tile 1 sees). The rule that the kernel relies on: every block in the
 ring is used by at least one tile. An item that sees nothing has a block to itself (its rows are written as zeros) that no
@@ -21,7 +22,8 @@ def run(segments, seed, unused_in_ring=False, slow_clear=8):
     full = [MBar(1) for _ in range(SLOTS)]
     empty, s_full, o_done = ([MBar(1) for _ in range(2)] for _ in range(3))
     p_full = [MBar(5) for _ in range(2)]
-    ring = [None] * SLOTS
+    ring, lost = [None] * SLOTS, [[(-1, 0)] * 2 for _ in range(2)]
+    found = [[rng.random() < 0.3 for _ in range(seg[0])] for seg in segments]  # blocks with a value to take out
     events, now, last_commit = [], [0], [0]
     outputs = [[], []]  # per tile: (segment, block) of the products with V, in order
 
@@ -107,13 +109,13 @@ def run(segments, seed, unused_in_ring=False, slow_clear=8):
                 blk += 1
 
     def clearer():
-        blk, pn = 0, [0, 0]
-        for seg in segments:
+        blk, pn, segs = 0, [0, 0], [0, 0]
+        for s, seg in enumerate(segments):
             n, un = used(seg), seg[1:]
             for b in range(n):
                 slot, tag = (2 * blk + 1) & 3, ("V", blk)
                 yield from wait(full[slot], (blk >> 1) & 1)
-                if b + 1 == seg[0]:  # the sequence's end lies in the last block
+                if b + 1 == seg[0] or found[s][b]:  # the sequence's end lies in the last block
                     for _ in range(rng.randint(1, slow_clear)):
                         assert ring[slot] == tag, "another block's values are cleared"
                         yield
@@ -125,12 +127,17 @@ def run(segments, seed, unused_in_ring=False, slow_clear=8):
                         if pn[i] > 0:
                             yield from wait(p_full[i], (pn[i] + 1) & 1)
                         pn[i] += 1
+                        if found[s][b]:
+                            e = lost[i][segs[i] & 1]
+                            lost[i][segs[i] & 1] = (segs[i], min(e[1], b) if e[0] == segs[i] else b)
                         p_full[i].arrive()
                 blk += 1
+            for i in range(2):
+                segs[i] += un[i] > 0
 
     def softmax(i):
         n = segs = 0
-        for seg in segments:
+        for s, seg in enumerate(segments):
             for _ in range(seg[1 + i]):
                 yield from wait(s_full[i], n & 1)
                 for _ in range(rng.randint(0, 6)):
@@ -139,9 +146,13 @@ def run(segments, seed, unused_in_ring=False, slow_clear=8):
                 n += 1
             if seg[1 + i] > 0:
                 yield from wait(o_done[i], segs & 1)
-                segs += 1
+                yield from wait(p_full[i], (n - 1) & 1)
                 for _ in range(rng.randint(0, 10)):
                     yield
+                e = lost[i][segs & 1]
+                mine = [b for b in range(seg[1 + i]) if found[s][b]]
+                assert (e[1] if e[0] == segs else None) == (mine[0] if mine else None), "another segment's finding is read"
+                segs += 1
 
     alive = [loader(), issuer(), clearer(), softmax(0), softmax(1)]
     slow = rng.choice(alive)
