@@ -3,9 +3,10 @@ makers of inputs: tests/test_paged_gpu.py."""
 
 import pytest
 import torch
-from test_paged_gpu import check, make, reference
+from test_paged_gpu import append_reference, check, make, reference
 
 from byteprof_b200 import _lib
+from byteprof_b200.optim.decode_ops import rope_tables
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
@@ -57,3 +58,36 @@ def test_a_value_that_is_not_finite_stays_with_the_rows_that_see_it(news, before
             assert not torch.isfinite(y[a + i:a + n, heads, dim].float()).any()
             y[a + i:a + n, heads] = want[a + i:a + n, heads].to(BF16)
             check(y, want, mag)
+
+
+@pytest.mark.parametrize("news,befores,nh,nkv,hd,page", [
+    # one token per tile of 128 rows (65 to 128 heads per kv head), and the first group of two
+    ([130], [40], 71, 1, 128, 16), ([5, 90], [300, 0], 142, 2, 64, 32), ([77, 1, 40], [0, 513, 128], 128, 1, 128, 64),
+    ([60], [100], 65, 1, 64, 8), ([50, 33], [7, 200], 64, 1, 128, 16), ([9], [1500], 130, 2, 64, 64),
+    # more heads than a tile has rows: the 16-row kernel, tiles within a token and across two
+    ([1], [700], 256, 1, 128, 16), ([40, 3], [0, 250], 256, 1, 64, 32), ([20], [90], 400, 2, 128, 64), ([1, 7], [33, 0], 129, 1, 64, 8),
+    ([2], [65], 1024, 1, 128, 16), ([3, 1], [1000, 5], 1024, 4, 64, 16)])
+def test_large_head_groups(news, befores, nh, nkv, hd, page):
+    cache, q, table, starts, kv = make(news, befores, nh, nkv, hd, page, seed=nh)
+    y = cache.attend(q, table, starts, kv)
+    check(y, *reference(cache, q, table, starts, kv))
+    assert torch.equal(y, cache.attend(q, table, starts, kv))
+
+
+def test_append_with_the_most_heads():
+    """1024 query heads: what a thread keeps in registers is a fraction of the row. A sum of squares has 512 terms in each of a
+    thread's two accumulators: 2^-15 of it at most, half of that after the root, beside the usual tolerance."""
+    nh, nkv, hd, n = 1024, 4, 128, 5
+    cache, _, table, starts, kv = make([n], [30], nh, nkv, hd, 16, seed=41)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    qkv = torch.randn(n, (nh + 2 * nkv) * hd, generator=g, device="cuda").to(BF16)
+    qn = (1 + 0.1 * torch.randn(nh * hd, generator=g, device="cuda")).to(BF16)
+    kn = (1 + 0.1 * torch.randn(nkv * hd, generator=g, device="cuda")).to(BF16)
+    cos, sin = rope_tables(64, hd, 10000.0, torch.device("cuda"))
+    q = cache.append(qkv, nh, table, starts, kv, qn, kn, cos, sin)
+    pos = torch.arange(30, 30 + n, device="cuda")
+    (wq, sq), (wk, sk) = append_reference(qkv, nh, nkv, hd, pos, qn, kn, cos, sin, 1e-6)
+    at = table.long()[0, pos // 16], pos % 16
+    for y, w, s in ((q, wq, sq), (cache.k_pages[at], wk, sk)):
+        assert ((y.double() - w).abs() <= (2.0**-8 + 2.0**-16) * w.abs() + 2.0**-20 * s).all()
+    assert torch.equal(cache.v_pages[at], qkv[:, (nh + nkv) * hd:].view(n, nkv, hd))
