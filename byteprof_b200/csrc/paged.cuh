@@ -96,7 +96,10 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int s) {
   const int b0 = b > 0 ? b : 0, e0 = e < a.rows ? e : a.rows;
   r.first = b0;
   r.n = e0 > b0 ? e0 - b0 : 0;
-  const long long cap = static_cast<long long>(a.max_pages) << a.page_log2;
+  // A table may name pages again and again, so it may be longer than any cache: positions from kMaxPos on lie past it (the
+  // key counters are 32 bits and run up to a block behind the last key).
+  constexpr long long kMaxPos = 0x7fffff00;
+  const long long table = static_cast<long long>(a.max_pages) << a.page_log2, cap = table < kMaxPos ? table : kMaxPos;
   r.kv = kv < 0 ? 0 : (kv < cap ? kv : static_cast<int>(cap));
   r.bad = kv > cap ? r.kv : 0x7fffffff;
   r.pos0 = static_cast<long long>(kv) - (static_cast<long long>(e) - b) + (b0 - b);

@@ -161,7 +161,8 @@ __global__ void __launch_bounds__(kThreads, 7) paged_append_kernel(const AppendA
   }
   if (t < first) return;
   const long long pos = static_cast<long long>(len) - (end - first) + (t - first);
-  bool ok = pos >= 0 && (pos >> a.page_log2) < a.max_pages && (a.cos_t == nullptr || pos < a.max_pos);
+  constexpr long long kMaxPos = 0x7fffff00;  // as far as the attention goes (paged.cuh)
+  bool ok = pos >= 0 && pos < kMaxPos && (pos >> a.page_log2) < a.max_pages && (a.cos_t == nullptr || pos < a.max_pos);
   int page = -1;
   if (ok) page = a.pages[s * a.ld_pages + (pos >> a.page_log2)];
   ok = page >= 0 && page < a.num_pages;

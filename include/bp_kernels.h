@@ -394,7 +394,7 @@ int bp_mlstm_commit_state(const float* c_hist, const float* n_hist, const float*
  * rows q_start[s] .. q_start[s + 1] - 1 are the newest positions of sequence s, the last of them at position
  * kv_len[s] - 1 (q_start int32 [seqs + 1], nondecreasing; kv_len int32 [seqs] counts the new rows). Position p of
  * sequence s lies in page pages[s * ld_pages + p / page_size], row p % page_size; entries past a sequence's length
- * are never read. All of these are read on the device, so a captured graph serves every length. Rows at or behind
+ * are never read; positions are below 2^31 - 256 (a longer sequence is past its table). All of these are read on the device, so a captured graph serves every length. Rows at or behind
  * q_start[seqs] are left as they were. A static cache [max_pos, nkv, head_dim] is the case of consecutive pages.
  *
  * bp_paged_append: row t of qkv = q | k | v ([(nh + 2 nkv) * head_dim] bf16, row stride ldqkv) at its position p:

@@ -7,6 +7,7 @@ from test_paged_gpu import append_reference, check, make, reference
 
 from byteprof_b200 import _lib
 from byteprof_b200.optim.decode_ops import rope_tables
+from byteprof_b200.optim.paged import PagedCache
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
@@ -91,3 +92,24 @@ def test_append_with_the_most_heads():
     for y, w, s in ((q, wq, sq), (cache.k_pages[at], wk, sk)):
         assert ((y.double() - w).abs() <= (2.0**-8 + 2.0**-16) * w.abs() + 2.0**-20 * s).all()
     assert torch.equal(cache.v_pages[at], qkv[:, (nh + nkv) * hd:].view(n, nkv, hd))
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_lengths_up_to_the_end_of_32_bits(n):
+    """A table of 2^23 entries that all name one page of 256. Up to position 2^31 - 257 a row sees the same keys again and
+    again, so its result is that of the page alone (here all its values are 1: any weights give 1, up to the sums' drift); the
+    largest lengths are past the table."""
+    page = 256
+    cache = PagedCache(*(torch.ones(1, page, 1, 64, dtype=BF16, device="cuda") for _ in range(2)))
+    table = torch.zeros(1, 2**31 // page, dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    q = torch.randn(n, 1, 64, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda").to(BF16)
+    last = 2**31 - 256
+    for kv, live in ((last, n), (last + 3, max(n - 3, 0)), (2**31 - 1, 0)):
+        y = cache.attend(q, table, starts, torch.tensor([kv], dtype=torch.int32, device="cuda"))
+        assert ((y[:live].float() - 1).abs() < 2.0**-5).all() and torch.isnan(y[live:]).all()
+        kv = torch.tensor([kv], dtype=torch.int32, device="cuda")
+        own = PagedCache.zeros(1, page, 1, 64, torch.device("cuda"))
+        x = own.append(torch.ones(n, 3 * 64, dtype=BF16, device="cuda"), 1, table, starts, kv)
+        assert (x[:live] == 1).all() and torch.isnan(x[live:]).all()
+    assert _lib.device_errors() == 0
