@@ -127,6 +127,8 @@ class PagedCache:
         if need is None:
             with torch.cuda.device(dev):
                 need = int(_lib.lib().bp_paged_attention_workspace_bytes(rows, seqs, nh, self.nkv, hd))
+            if len(self._ws_bytes) >= 1024:  # a server's batches have ever new sizes
+                self._ws_bytes.clear()
             self._ws_bytes[(rows, seqs, nh, dev)] = need
         # scratch of this call alone, from torch's allocator: calls on several streams and captured graphs share none
         ws = q.new_empty(need // 2)

@@ -113,3 +113,12 @@ def test_lengths_up_to_the_end_of_32_bits(n):
         x = own.append(torch.ones(n, 3 * 64, dtype=BF16, device="cuda"), 1, table, starts, kv)
         assert (x[:live] == 1).all() and torch.isnan(x[live:]).all()
     assert _lib.device_errors() == 0
+
+
+def test_ever_new_sizes_do_not_pile_up():
+    cache, q, table, starts, kv = make([1500], [3], 2, 2, 64, 16, seed=51)
+    one = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    for rows in range(1, 1500):
+        cache.attend(q[:rows], table, one, kv)
+    assert len(cache._ws_bytes) <= 1024
+    check(cache.attend(q, table, starts, kv), *reference(cache, q, table, starts, kv))
