@@ -77,7 +77,8 @@ def _swap(model: nn.Module, name: str, make) -> None:
 def apply_quantization(model: nn.Module, target: str, scheme: str, group_size: int = 128,
                        local_scheme: str | None = None, global_scheme: str | None = None,
                        kernel: str = "default") -> dict[str, Any]:
-    """Quantize every linear selected by the target's rule; returns statistics (reference keys)."""
+    """Quantize every linear selected by the target's rule; returns statistics (reference keys). `kernel` chooses among the
+    weight-only products: int8_w8a8 linears run `int8_linear` whatever it is, and where all do, it is not reported."""
     bolmo = hasattr(model.model, "local_encoder")
     pick = should_quantize if bolmo else olmo_should_quantize
     names = [n for n, m in model.named_modules() if isinstance(m, nn.Linear) and pick(n, target)]
@@ -115,6 +116,6 @@ def apply_quantization(model: nn.Module, target: str, scheme: str, group_size: i
                              "group_size": group_size if "int4_wo" in by_scheme else None,
                              "n_linears": len(names), "gpu_mem_before_mib": before / 2**20,
                              "gpu_mem_after_mib": after / 2**20}
-    if kernel != "default":
+    if kernel != "default" and set(by_scheme) != {"int8_w8a8"}:
         stats["kernel"] = kernel
     return stats

@@ -14,7 +14,7 @@ import re
 BOLMO_TARGETS = ("none", "local", "global", "all")
 OLMO_TARGETS = ("blocks", "blocks+head")
 VALID_TARGETS = BOLMO_TARGETS + OLMO_TARGETS
-VALID_SCHEMES = ("int8_wo", "int4_wo")
+VALID_SCHEMES = ("int8_wo", "int4_wo", "int8_w8a8")
 
 _LOCAL_LAYER = r"model\.local_(?:encoder|decoder)\.layers\.\d+\."
 _LOCAL = re.compile(
