@@ -26,6 +26,8 @@ from .select import group_of, olmo_should_quantize, should_quantize
 
 
 class Int8Linear(nn.Module):
+    act = "bf16"  # modules that were saved whole before there was a choice have no attribute of their own
+
     def __init__(self, lin: nn.Linear, act: str = "bf16"):
         super().__init__()
         if act not in ("bf16", "int8"):

@@ -1,5 +1,7 @@
 """apply_quantization's statistics and Int8Linear's attributes, without a device (the swap itself runs on CPU tensors)."""
 
+import io
+
 import pytest
 import torch
 import torch.nn as nn
@@ -34,3 +36,15 @@ def test_the_statistics_name_the_kernel_that_the_linears_run(scheme, kernel, kin
 
 def test_no_linears_report_the_kernel_asked_for():
     assert apply_quantization(olmo(), "none", "int8_wo", kernel="skinny")["kernel"] == "skinny"
+
+
+def test_a_module_saved_whole_before_there_was_a_choice_of_activations_loads():
+    old = Int8Linear(nn.Linear(32, 16).to(torch.bfloat16))
+    del old.__dict__["act"]
+    buf = io.BytesIO()
+    torch.save(old, buf)
+    buf.seek(0)
+    back = torch.load(buf, weights_only=False)
+    assert back.act == "bf16" and "GEMV" in repr(back)
+    with pytest.raises(ValueError, match="CUDA"):
+        back(torch.zeros(1, 32, dtype=torch.bfloat16))
