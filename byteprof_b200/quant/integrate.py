@@ -5,7 +5,7 @@ Same API as byteprof/quant/integrate.py:22-122:
     (bp_gemv_int8), other row counts use the weights dequantized to the activation dtype with
     F.linear on the GPU (the reference's prefill path). Bias added as a separate op.
     `Int8Linear(lin, act="int8")` quantizes bf16 activations too, one scale per row, and runs the 8-bit
-    integer product for every row count (bp_int8_linear; no counterpart in the reference); scheme
+    integer product for every row count (bp_int8_linear; no gradient, no counterpart in the reference); scheme
     "int8_w8a8" of `apply_quantization` swaps it in.
   * `apply_quantization(model, target, scheme, group_size, local_scheme, global_scheme, kernel)`:
     the reference's selection rule (byteprof_b200.quant.select); kernel="skinny" swaps in
@@ -54,6 +54,8 @@ class Int8Linear(nn.Module):
             raise ValueError("Int8Linear runs on CUDA tensors only (there is no CPU path)")
         if self.act == "int8" and x2.dtype == torch.bfloat16:
             fused = self.bias if self.bias is not None and self.bias.dtype == torch.bfloat16 else None
+            if x2.stride(1) != 1 or x2.stride(0) < self.in_features:  # transposed or broadcast rows
+                x2 = x2.contiguous()
             y = int8_linear(x2.detach(), self.q, self.scale, None if fused is None else fused.detach())
             if self.bias is not None and fused is None:
                 y = y + self.bias

@@ -2,11 +2,13 @@
 
 import pytest
 import torch
+import torch.nn as nn
 from test_int8_mm_gpu import check, ints, scales
 
 from byteprof_b200 import _lib
 from byteprof_b200.optim.decode_ops import token_logprobs
 from byteprof_b200.quant.int8 import int8_mm
+from byteprof_b200.quant.integrate import Int8Linear
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
@@ -35,3 +37,15 @@ def test_pairs_of_ctas_one_behind_the_other_and_beside_other_kernels():
         assert torch.equal(y, ref)
         assert all(torch.equal(a, b) for a, b in zip(lp[1:], want[1:]))
     assert _lib.device_errors() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 2, 40, 300])
+def test_the_module_takes_any_strides(rows):
+    lin = nn.Linear(256, 96, bias=True, dtype=BF16, device="cuda")
+    m = Int8Linear(lin, act="int8")
+    x = torch.randn(256, rows, device="cuda").to(BF16)
+    assert torch.equal(m(x.t()), m(x.t().contiguous()))                        # transposed
+    wide = torch.randn(rows, 2, 512, device="cuda").to(BF16)
+    for view in (wide[..., ::2], wide[..., :256], wide[:1].expand(rows, 2, 512)[..., 3:259], wide[0, 0, :256].expand(rows, 256)):
+        y = m(view)
+        assert y.shape == (*view.shape[:-1], 96) and torch.equal(y, m(view.contiguous()))
