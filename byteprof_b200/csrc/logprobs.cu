@@ -22,8 +22,10 @@
 // values cost 27 us of 94 for 1500 rows of 100352 with 5 alternatives, since some 60 values of a row reach it.)
 //
 // Bound by the instructions of the pass (about 14 per pair of values, two of them exp2, which alone take 35 us) and by
-// memory: 1500 rows of 100352 in bf16 take 60 us (5.1 TB/s), 70 us with 5 alternatives; one row on a cluster of 8 CTAs 5.5
-// and 8.7 us. A row goes to a warp, a CTA or a cluster of up to 8 CTAs (launch), merged in a fixed order (deterministic).
+// memory: 1500 rows of 100352 in bf16 take 58 to 60 us (5.1 TB/s), 69 to 76 us with 5 alternatives; one row on a cluster of 8
+// CTAs 4.8, with 5 alternatives 8.2 and with 20 10.3 to 13 us. Where the bound says nothing (fewer values above -inf than
+// alternatives, or equal values throughout) every value is offered: one row 69 us, 1500 rows 570. A row goes to a warp, a CTA
+// or a cluster of up to 8 CTAs (launch), merged in a fixed order (deterministic).
 #include <float.h>
 
 #include "bp_common.cuh"

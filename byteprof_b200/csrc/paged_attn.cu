@@ -15,9 +15,9 @@
 // does 16 rows for the price of one here; 16 rows at HBM speed need a tenth of what mma.sync can do, so tcgen05 has
 // nothing to add. P is rounded to bf16 for the second product (its relative error, 2^-8 at most, averages out over
 // the keys; the sum l adds the unrounded fp32 values).
-// 64 streams of up to 8192 keys, 32 heads of 128 over 8: 186 us for 1.13 GB, 6.1 TB/s, where registers filled straight from global
-// memory, one unit ahead, took 225; 5 drafted tokens over 30001 keys 51 us (4.9 TB/s), one token over 1025 10.4 (latency:
-// the cut, one trip through the ring, the join).
+// 64 streams of up to 8192 keys, 32 heads of 128 over 8: 185 to 191 us for 1.13 GB, 5.9 to 6.1 TB/s, where registers filled
+// straight from global memory, one unit ahead, took 225; 5 drafted tokens over 30001 keys 51 us (4.8 TB/s), one token over
+// 1025 10.1 (latency: the cut, one trip through the ring, the join).
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -69,8 +69,8 @@ __device__ __forceinline__ FewUnits few_units(const PagedArgs& a, const PagedSeq
 // How many kv heads the warps of a CTA take side by side over the same keys (the other warps take other keys). A key's
 // heads lie next to each other, so 4 at a time read 1 KB of DRAM in one go instead of 256 bytes here and the rest some
 // other time (head_dim 128); with too few units for that, the heads go to CTAs of their own. `one`: units at one head per CTA.
-// Measured with 1, 2 and 4 heads: 64 streams of up to 8192 keys (117 G units) 192, 189 and 180 us; 5 tokens over 30001 keys
-// (25 G) 49, 57 and 70; one token over 1025 (1 G) 9.4, 10.3 and 11.9.
+// Measured with 1, 2 and 4 heads fixed: 64 streams of up to 8192 keys (117 G units) 193, 192 and 185 us; 5 tokens over 30001
+// keys (25 G) 50, 60 and 78; one token over 1025 (1 G) 9.5, 13.4 and 19.5.
 __device__ __forceinline__ int heads_per_cta(const PagedArgs& a, long long one) {
   if (a.nkv % 4 == 0 && one >= 64LL * a.G) return 4;
   if (a.nkv % 2 == 0 && one >= 32LL * a.G) return 2;
@@ -553,7 +553,9 @@ constexpr int kCtasPerSm = 2;
 // Up to 32 packed rows per sequence and kv head on average (the lengths themselves are on the device): two tiles of the
 // 16-row kernel, which then reads each key twice; the other kernel pads to 128 and takes groups of up to 128 heads.
 // 64 sequences over 2048 keys, 8 kv heads of 128: 16 packed rows take 108 us here and 223 there, 32 take 197 and 220, 40
-// take 278 and 220.
+// take 278 and 220. The rule knows the average alone, so that a call of unequal sequences goes wholly to one kernel: 63 single
+// tokens over 2048 to 8192 keys with a chunk of 449 rows over 4545 (32 heads over 8) take 429 us here, with one of 450 rows
+// 405 there, and 205 and 65 in two calls. A chunk's tiles of 16 rows each read all its keys here.
 bool few_rows(int rows, int seqs, int g) { return static_cast<long long>(rows) * g <= 32LL * seqs || g > 128; }
 
 int few_grid() { return kCtasPerSm * tc_sm_count(); }

@@ -18,16 +18,17 @@
 //    (2^-8 of each p at most), the sum adds the unrounded fp32 values.
 //
 // A block of two tiles takes 2048 clocks of MMA (head_dim 128) and 2048 of exp2, each behind the other within a tile; it
-// takes 3300 (a chunk of 4096 rows over 20480 keys, 16 heads of 128: 865 us, 874 TFLOP/s of visible keys at the power cap's
-// 1.73 GHz) to 3800 clocks (9 prompts of 6151 tokens, 32 heads of 64: 94 us), and an item about 5000 more: bound by the
+// takes 3300 (a chunk of 4096 rows over 20480 keys, 16 heads of 128: 840 to 920 us with the GPU's power cap, 874 TFLOP/s of visible
+// keys at 1.73 GHz) to 3800 clocks (9 prompts of 6151 tokens, 32 heads of 64: 94.6 us), and an item about 5000 more: bound by the
 // hand-overs between the softmax warps and the issuing thread (about 1300 clocks a block and tile), not by either unit.
 // Measured and not kept: exp2 partly as a polynomial on the FMA pipes (910 us and more), one pass over the scores with the
 // block before's maximum (907), an issuing thread per tile (1069 against 890 then), a block's columns in one unrolled
 // piece (instruction fetch: 110 us of 870), per-chunk masks (900), the next item's first scores behind this item's last
 // product (876, and 100 for the prompts), P in columns of its own at head_dim 64 and the next scores in front of the product
 // with V (prompts 97), all 128 scores loaded at once for the maximum (848, prompts 97), the next chunk's scores loaded
-// ahead (925, prompts 104), a row's softmax over two threads (894, prompts 101). The chunk's 865 us are what back-to-back
-// launches leave of the clock: one launch by itself takes 755.
+// ahead (925, prompts 104), a row's softmax over two threads (894, prompts 101). The chunk's time is what back-to-back
+// launches leave of the clock: one launch by itself takes 755. Looking for values that are not finite (warp 2) costs the prompts
+// 1.3 us and the chunk nothing, in a short rolled loop; unrolled it cost 3.6, for instruction fetch.
 #include <cudaTypedefs.h>
 
 #include "paged.cuh"
