@@ -14,7 +14,7 @@ BF16 = torch.bfloat16
 
 
 @pytest.mark.parametrize("nh,nkv,hd", [(8, 8, 128), (16, 8, 64)])
-@pytest.mark.parametrize("order", ["EERE", "EEEEEEEERR", "REEEEEEEEEEEER", "ERERERERERER"])
+@pytest.mark.parametrize("order", ["EERE", "EEEEEEEERR", "REEEEEEEEEEEER", "ERERERERERER", "E" * 20 + "RR" + "E" * 18 + "R"])
 def test_many_rows_of_empty_sequences_beside_long_ones(order, nh, nkv, hd):
     """E: 300 rows that see nothing (a slot of a captured graph without a cache), R: 300 rows over 2300 positions. Each E is
     two items for each of 8 kv heads, so that CTAs take several of them in a row and a long one behind them. No other
