@@ -560,7 +560,7 @@ constexpr int kPairN = 256;
 constexpr int kPairEpi = 256;
 constexpr int kPairThreads = 32 * kEpiWarp0 + kPairEpi;
 
-// vec: 0: y's rows are not 16-byte aligned; 1: they are (fp32); 2: bf16 through `ty`, a map of y in 64 x 128 boxes
+// vec: y's rows are 16-byte aligned, and in bf16 end at 16 bytes: stored through `ty`, a map of y in 64 x 128 boxes
 __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     int8_mm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                         const __grid_constant__ CUtensorMap ty, const Int8Args a, const Part p, const int vec) {
@@ -762,7 +762,9 @@ int launch_pair(const Int8Args& a, const Part& p, cudaStream_t stream) {
   st = tc_encode_2d(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w, a.K, a.N, a.ldw, kBK, kBM, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
   if (st != BP_OK) return st;
   const int es = a.y_f32 ? 4 : 2;
-  const int vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && (a.ldy * es) % 16 == 0;
+  // A TMA store does not end within 16 bytes: with N = 159 bf16 in rows of 160 it wrote the column behind the block, too. Such
+  // results are stored a row at a time.
+  const int vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && (a.ldy * es) % 16 == 0 && (a.y_f32 || a.N % 8 == 0);
   CUtensorMap ty = ta;
   if (vec && !a.y_f32) {
     st = tc_encode_2d(&ty, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.y, a.N, a.M, a.ldy * 2, 64, kBM, CU_TENSOR_MAP_L2_PROMOTION_NONE);

@@ -49,3 +49,17 @@ def test_the_module_takes_any_strides(rows):
     for view in (wide[..., ::2], wide[..., :256], wide[:1].expand(rows, 2, 512)[..., 3:259], wide[0, 0, :256].expand(rows, 256)):
         y = m(view)
         assert y.shape == (*view.shape[:-1], 96) and torch.equal(y, m(view.contiguous()))
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("m", [1, 20, 100, 260, 1025])
+def test_exactly_the_block_is_written(m, dtype):
+    """Every width behind a multiple of 8, in rows that are 16-byte aligned: what lies behind the block stays."""
+    k = 64
+    for n in [*range(145, 161), 2039, 2042, 2044]:
+        q, s, w, ws = ints(m, k, n), scales(m, 1), ints(n, k, 2), scales(n, 3, BF16)
+        for ld in (-(-n // 8) * 8, -(-n // 8) * 8 + 8):
+            buf = torch.full((m + 1, ld), 7.0, dtype=dtype, device="cuda")
+            y = int8_mm(q, s, w, ws, out=buf[:m, :n])
+            assert (buf[:m, n:] == 7).all() and (buf[m] == 7).all(), (n, ld)
+            check(y, q, s, w, ws)
