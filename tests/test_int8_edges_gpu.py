@@ -7,7 +7,7 @@ from test_int8_mm_gpu import check, ints, scales
 
 from byteprof_b200 import _lib
 from byteprof_b200.optim.decode_ops import token_logprobs
-from byteprof_b200.quant.int8 import int8_mm
+from byteprof_b200.quant.int8 import int8_linear, int8_mm, quantize_tokens_int8
 from byteprof_b200.quant.integrate import Int8Linear
 
 pytestmark = pytest.mark.gpu
@@ -63,3 +63,18 @@ def test_exactly_the_block_is_written(m, dtype):
             y = int8_mm(q, s, w, ws, out=buf[:m, :n])
             assert (buf[:m, n:] == 7).all() and (buf[m] == 7).all(), (n, ld)
             check(y, q, s, w, ws)
+
+
+@pytest.mark.parametrize("m", [1, 20, 100, 300])
+def test_what_lies_between_the_rows_does_not_count(m):
+    """Every K behind a multiple of 16 in rows of 16-byte steps (the tensor cores' form), with values between the rows of both
+    operands; and the bf16 rows of a fused call."""
+    for k in [*range(1, 18), 100, 113, 127, 129, 2047]:
+        ld = -(-k // 16) * 16
+        q, w = ints(m, k, k, ld=ld + 16, lo=-128), ints(150, k, 7, ld=ld, lo=-128)
+        s, ws = scales(m, 1), scales(150, 3, BF16)
+        check(int8_mm(q, s, w, ws), q, s, w, ws)
+        x = torch.randn(m, ld + 8, device="cuda").to(BF16)[:, :k]
+        q2, s2 = quantize_tokens_int8(x)
+        assert torch.equal(int8_linear(x, w, ws), int8_mm(q2, s2, w, ws))
+        check(int8_mm(q2, s2, w, ws), q2, s2, w, ws)
